@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import native
-from .native import Desk, Plane, Rng
+from .native import Cache4, Desk, Plane, Rng
 
 
 class BackendError(RuntimeError):
@@ -126,6 +126,14 @@ def make_real_plane(rows: np.ndarray, real_type: int) -> CodePlane:
     p.real_data = _ptr(rows)
     p.real_type = real_type
     return CodePlane(p, rows, np.zeros((0,), dtype=np.float32))
+
+
+@dataclass
+class Ring4:
+    """A layer's 4-bit key/value ring: its igl_cache4 and the buffers it names."""
+
+    cache: Cache4
+    buffers: list  # key codes, key gains, value codes, value gains
 
 
 class Backend:
@@ -274,6 +282,39 @@ class Backend:
                       slot_first: int, row_off: int = 0):
         self._check(self.lib.igl_cache_lay_dev(ctypes.byref(self.desk), row.ptr + row_off, width,
                                                scale, fmt, store.ptr, slot_first), "cache_lay_dev")
+
+    def cache4(self, fmt: int, cache_span: int, sink_count: int, kv_count: int, head_size: int, key_scale: float,
+               value_scale: float, key_code=None, key_gain=None, value_code=None, value_gain=None) -> Ring4:
+        """A layer's 4-bit ring (igl_cache4) over the caller's buffers, or over buffers of its own, zeroed."""
+        c = Cache4(fmt, cache_span, sink_count, kv_count, head_size, key_scale, value_scale)
+        codes = self.lib.igl_cache4_code_bytes(ctypes.byref(c))
+        gains = self.lib.igl_cache4_gain_bytes(ctypes.byref(c))
+        if not codes:
+            raise BackendError("no 4-bit ring has these dimensions")
+        buffers = [self.upload(np.zeros(n, np.uint8)) if b is None else b
+                   for b, n in ((key_code, codes), (key_gain, gains), (value_code, codes), (value_gain, gains))]
+        c.key_code, c.key_gain, c.value_code, c.value_gain = (b.ptr for b in buffers)
+        return Ring4(c, buffers)
+
+    def cache4_lay_dev(self, store: Ring4, key: DevBuf, value: DevBuf, row_stride: int, place_first: int,
+                       lane_count: int):
+        """Rows of lane_count positions into the ring, quantised."""
+        self._check(self.lib.igl_cache4_lay_dev(ctypes.byref(self.desk), ctypes.byref(store.cache), key.ptr, value.ptr,
+                                                row_stride, place_first, lane_count), "cache4_lay_dev")
+
+    def cache4_read_dev(self, store: Ring4, place_first: int, lane_count: int, key: DevBuf | None,
+                        value: DevBuf | None, row_stride: int):
+        """Rows of lane_count positions of the ring as floats; None for a side that is not wanted."""
+        self._check(self.lib.igl_cache4_read_dev(ctypes.byref(self.desk), ctypes.byref(store.cache), place_first,
+                                                 lane_count, key.ptr if key else None, value.ptr if value else None,
+                                                 row_stride), "cache4_read_dev")
+
+    def attend4_lanes_dev(self, store: Ring4, group_share: int, query: DevBuf, lane_stride: int, place_first: int,
+                          window: int, lane_count: int, score_scale: float, blend_out: DevBuf):
+        """Attention of lane_count consecutive positions over the ring."""
+        self._check(self.lib.igl_attend4_lanes_dev(ctypes.byref(self.desk), ctypes.byref(store.cache), group_share,
+                                                   query.ptr, lane_stride, place_first, window, lane_count,
+                                                   score_scale, blend_out.ptr), "attend4_lanes_dev")
 
     def sync(self):
         self._check(self.lib.igl_sync(ctypes.byref(self.desk)), "sync")

@@ -9,6 +9,7 @@
  * launched; an entry that cannot run records IGL_FAIL_SUPPORT or
  * IGL_FAIL_ARGUMENT and leaves its output unwritten.  There is no CPU path.
  */
+#include <float.h>
 #include <pthread.h>
 #include <stdlib.h>
 #include <string.h>
@@ -828,6 +829,107 @@ int igl_cache_lay_dev(igl_desk *desk, const float *row_dev, int width, float sca
   }
   return hip_check(st, igl_launch_cache_lay(row_dev, width, scale, format, store_dev, slot_first,
                                             st->stream));
+}
+
+/* ---- the 4-bit ring -------------------------------------------------------- */
+
+static int cache4_dims(const igl_cache4 *store) {
+  return store && (store->format == IGL_CACHE4_INT4 || store->format == IGL_CACHE4_E2M1) &&
+         (store->head_size == 64 || store->head_size == 128 || store->head_size == 256 ||
+          store->head_size == 512) &&
+         store->kv_count >= 1 && store->kv_count <= 65535 && store->cache_span >= 1 &&
+         store->cache_span <= INT32_MAX - 64 && store->sink_count >= 0 &&
+         store->sink_count < store->cache_span;
+}
+
+size_t igl_cache4_code_bytes(const igl_cache4 *store) {
+  if (!cache4_dims(store)) return 0;
+  return (size_t)store->cache_span * (size_t)store->kv_count * (size_t)store->head_size / 2;
+}
+
+size_t igl_cache4_gain_bytes(const igl_cache4 *store) {
+  if (!cache4_dims(store)) return 0;
+  return igl_cache4_room(store->cache_span) * (size_t)store->kv_count * (size_t)store->head_size / 32;
+}
+
+/* What every entry of the ring checks before anything is launched: the ring
+ * itself, and that `lanes` positions from `place_first` on can lie in it
+ * together with all from `oldest` on. */
+static int cache4_check(igl_desk_state *st, const igl_cache4 *store, int place_first, int lanes,
+                        long long oldest, int row_stride, long long row_floats) {
+  if (store && store->kv_count >= 1 && store->head_size >= 1 && store->cache_span >= 1 &&
+      store->head_size != 64 && store->head_size != 128 && store->head_size != 256 &&
+      store->head_size != 512) {
+    desk_fail(st, IGL_FAIL_SUPPORT);
+    return IGL_FAIL_SUPPORT;
+  }
+  if (!cache4_dims(store) || !(store->key_scale > 0.0f) || !(store->value_scale > 0.0f) ||
+      store->key_scale > FLT_MAX || store->value_scale > FLT_MAX || !store->key_code ||
+      !store->key_gain || !store->value_code || !store->value_gain ||
+      (((uintptr_t)store->key_code | (uintptr_t)store->key_gain | (uintptr_t)store->value_code |
+        (uintptr_t)store->value_gain) & 15u) ||
+      lanes < 1 || place_first < 0 || place_first > INT32_MAX - lanes ||
+      (lanes > 1 && row_stride < row_floats)) {
+    desk_fail(st, IGL_FAIL_ARGUMENT);
+    return IGL_FAIL_ARGUMENT;
+  }
+  if (oldest < store->sink_count) oldest = store->sink_count;
+  if ((long long)place_first + lanes - oldest > store->cache_span - store->sink_count) {
+    desk_fail(st, IGL_FAIL_ARGUMENT);
+    return IGL_FAIL_ARGUMENT;
+  }
+  return IGL_OKAY;
+}
+
+static int cache4_null(igl_desk_state *st) {
+  desk_fail(st, IGL_FAIL_ARGUMENT);
+  return IGL_FAIL_ARGUMENT;
+}
+
+int igl_cache4_lay_dev(igl_desk *desk, const igl_cache4 *store, const float *key_dev,
+                       const float *value_dev, int row_stride, int place_first, int lane_count) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  int code;
+  if (!st) return IGL_FAIL_STATE;
+  if (!store || !key_dev || !value_dev) return cache4_null(st);
+  if ((code = cache4_check(st, store, place_first, lane_count, place_first, row_stride,
+                           (long long)store->kv_count * store->head_size)) != IGL_OKAY)
+    return code;
+  return hip_check(st, igl_launch_cache4_lay(store, key_dev, value_dev, row_stride, place_first,
+                                             lane_count, st->stream));
+}
+
+int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first, int lane_count,
+                        float *key_dev, float *value_dev, int row_stride) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  int code;
+  if (!st) return IGL_FAIL_STATE;
+  if (!store || (!key_dev && !value_dev)) return cache4_null(st);
+  if ((code = cache4_check(st, store, place_first, lane_count, place_first, row_stride,
+                           (long long)store->kv_count * store->head_size)) != IGL_OKAY)
+    return code;
+  return hip_check(st, igl_launch_cache4_read(store, place_first, lane_count, key_dev, value_dev,
+                                              row_stride, st->stream));
+}
+
+int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_share,
+                          const float *query_dev, int lane_stride, int place_first, int window,
+                          int lane_count, float score_scale, float *blend_out_dev) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  int code;
+  if (!st) return IGL_FAIL_STATE;
+  if (!store || !query_dev || !blend_out_dev || window < 0 || group_share < 1) return cache4_null(st);
+  if (group_share > 64) {
+    desk_fail(st, IGL_FAIL_SUPPORT);
+    return IGL_FAIL_SUPPORT;
+  }
+  if ((code = cache4_check(st, store, place_first, lane_count,
+                           window > 0 ? (long long)place_first + 1 - window : 0, lane_stride,
+                           (long long)store->kv_count * store->head_size * group_share)) != IGL_OKAY)
+    return code;
+  return hip_check(st, igl_launch_attend4(store, group_share, query_dev, lane_stride, place_first,
+                                          window, lane_count, score_scale, blend_out_dev,
+                                          st->attend_dev, st->stream));
 }
 
 int igl_norm_rms_dev(igl_desk *desk, const float *in_dev, const float *gain_dev, int n, int rows,

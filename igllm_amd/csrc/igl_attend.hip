@@ -1550,3 +1550,5 @@ extern "C" float *igl_attend_fixed_ptr(int device) {
   std::lock_guard<std::mutex> hold(fixed_lock);
   return fixed_ptr[device];
 }
+
+#include "igl_attend4.h"

@@ -1,0 +1,146 @@
+// igl_cache4.h - the 4-bit key/value ring: its slots, its codes, and the
+// kernels that lay rows into it and read them back, gfx950.
+//
+// Every 32 values x of a head share a gain g, an e4m3 byte b, and a layer's
+// side a scale s:
+//     b = e4m3(amax |x| / (top s)),  level = nearest(x / (real8(b) s)),
+//     value = level real8(b) s
+// with top 7 (INT4: levels -7 .. 7, code level + 8) or 6 (E2M1).  A level has
+// at most 4 significant bits and an e4m3 value 4, so level * g is exact in
+// binary16 and fp32, and a reader rounds once, by the scale.
+//
+// Both decisions are those of real arithmetic: the quotients are formed in
+// double, where a 24-bit x over a 28-bit step (or over the 27-bit top s) lies
+// further from a border than the quotient's rounding unless it lies on it.
+#pragma once
+
+#include "igl_device.h"
+#include "igl_launch.h"
+
+namespace igl {
+
+constexpr int kCache4Group = 32;  // values that share a gain
+constexpr int kCache4Block = 64;  // slots the gain rows are padded to
+
+// real8 of a gain byte: e4m3 as the byte ring reads it (0x7F 480, no NaN).
+__device__ __forceinline__ float cache4_gain(uint32_t byte) {
+  const uint32_t h = ((byte + (byte & 0x80u)) << 7) & 0xFFFFu;  // binary16 of real8 / 256
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)h) * 256.0f;
+}
+
+// The level a code stands for.
+template <int FMT>
+__device__ __forceinline__ float cache4_level(uint32_t code) {
+  if (FMT == IGL_CACHE4_INT4) return (float)((int)code - 8);
+  const uint32_t h = ((code & 8u) << 12) | ((code & 7u) << 9);  // binary16 of level / 2^14
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)h) * 16384.0f;
+}
+
+// The slot of a position (cache4's ring with its first positions kept).
+__host__ __device__ __forceinline__ int cache4_slot(int place, int sinks, int span) {
+  return place < sinks ? place : sinks + (place - sinks) % (span - sinks);
+}
+
+// e4m3 byte of a quotient >= 0 (or infinite): nearest, ties to even, 448 at most.
+__device__ __forceinline__ uint32_t cache4_gain_byte(double q) {
+  if (!(q < 448.0)) return 0x7Eu;
+  if (q < 0.015625) return (uint32_t)__builtin_rint(q * 512.0);  // 2^-9 steps; 8 is 2^-6's byte
+  uint64_t u = __builtin_bit_cast(uint64_t, q);
+  u += 0xFFFFFFFFFFFFull + ((u >> 49) & 1u);  // to three bits of mantissa
+  return (uint32_t)(u >> 49) - (1016u << 3);
+}
+
+// The code of x over a step that is real8(b) s exactly; x NaN or step 0: zero.
+template <int FMT>
+__device__ __forceinline__ uint32_t cache4_code(float x, double step) {
+  if (!(x == x) || step == 0.0) return FMT == IGL_CACHE4_INT4 ? 8u : 0u;
+  const double q = (double)x / step;
+  if (FMT == IGL_CACHE4_INT4) {
+    double level = __builtin_rint(q);
+    if (level > 7.0) level = 7.0;
+    if (level < -7.0) level = -7.0;
+    return (uint32_t)((int)level + 8);
+  }
+  const double m = __builtin_fabs(q);
+  double level = m < 2.0 ? __builtin_rint(2.0 * m) : m < 4.0 ? 2.0 + __builtin_rint(m) : 4.0 + __builtin_rint(0.5 * m);
+  if (level > 7.0) level = 7.0;
+  const uint32_t code = (uint32_t)level;
+  return code && x < 0.0f ? code | 8u : code;
+}
+
+struct Cache4Args {
+  uint8_t *code[2];    // key, value: [span][width / 2]
+  uint8_t *gain[2];    // [width / 32][room]
+  float scale[2];
+  const float *in[2];  // rows to lay
+  float *out[2];       // rows to read, or NULL
+  long long room;      // slots a gain row holds
+  int width;           // values a row
+  int span, sinks;
+  int row_stride;
+  int place;
+  int lanes;
+};
+
+// A thread eight values, four threads a group; blockIdx.y the side.
+template <int FMT, bool VEC>
+__global__ __launch_bounds__(256) void cache4_lay_kernel(Cache4Args a) {
+  const int per = a.width / 8;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int lane = (int)(i / per);
+  if (lane >= a.lanes) return;  // whole groups: `per` is a multiple of eight
+  const int d0 = 8 * (int)(i - (long long)lane * per);
+  const int side = blockIdx.y;
+  const float *src = a.in[side] + (size_t)lane * a.row_stride + d0;
+  float x[8];
+  if (VEC) {
+    const float4_t u = *reinterpret_cast<const float4_t *>(src), v = *reinterpret_cast<const float4_t *>(src + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = u[e], x[4 + e] = v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = src[e];
+  }
+  float top = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));  // a NaN is passed over
+  top = fmaxf(top, dpp_move<0xB1>(top));
+  top = fmaxf(top, dpp_move<0x4E>(top));
+  const double scale = (double)a.scale[side];
+  const uint32_t byte = cache4_gain_byte((double)top / ((FMT == IGL_CACHE4_INT4 ? 7.0 : 6.0) * scale));
+  const double step = (double)cache4_gain(byte) * scale;
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w |= cache4_code<FMT>(x[e], step) << (4 * e);
+  const size_t slot = (size_t)cache4_slot(a.place + lane, a.sinks, a.span);
+  *reinterpret_cast<uint32_t *>(a.code[side] + slot * (size_t)(a.width / 2) + d0 / 2) = w;
+  if ((threadIdx.x & 3) == 0) a.gain[side][(size_t)(d0 / kCache4Group) * a.room + slot] = (uint8_t)byte;
+}
+
+// A thread eight values; blockIdx.y the side (one where only one is wanted).
+template <int FMT, bool VEC>
+__global__ __launch_bounds__(256) void cache4_read_kernel(Cache4Args a, int side0) {
+  const int per = a.width / 8;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int lane = (int)(i / per);
+  if (lane >= a.lanes) return;
+  const int d0 = 8 * (int)(i - (long long)lane * per);
+  const int side = side0 + blockIdx.y;
+  const size_t slot = (size_t)cache4_slot(a.place + lane, a.sinks, a.span);
+  const uint32_t w = *reinterpret_cast<const uint32_t *>(a.code[side] + slot * (size_t)(a.width / 2) + d0 / 2);
+  const float gain = cache4_gain(a.gain[side][(size_t)(d0 / kCache4Group) * a.room + slot]);
+  const float scale = a.scale[side];
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = cache4_level<FMT>((w >> (4 * e)) & 15u) * gain * scale;
+  float *dst = a.out[side] + (size_t)lane * a.row_stride + d0;
+  if (VEC) {
+    *reinterpret_cast<float4_t *>(dst) = float4_t{y[0], y[1], y[2], y[3]};
+    *reinterpret_cast<float4_t *>(dst + 4) = float4_t{y[4], y[5], y[6], y[7]};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dst[e] = y[e];
+  }
+}
+
+}  // namespace igl

@@ -5,6 +5,7 @@
 // soft_max, gelu_gate, rope_turn; app_core.c:5223-5245) plus the key/value
 // ring writer that the reference keeps outside the table (cache_lay,
 // app_core.c:11205-11236).  They read no weights; each is one small launch.
+#include "igl_cache4.h"
 #include "igl_device.h"
 
 namespace igl {
@@ -291,5 +292,76 @@ extern "C" hipError_t igl_launch_cache_lay(const float *row, int width, float sc
                                            uint8_t *store, size_t slot_first, hipStream_t stream) {
   hipLaunchKernelGGL(cache_lay_kernel, dim3((width + 255) / 256), dim3(256), 0, stream, row, width,
                      scale, fmt, store, slot_first);
+  return hipGetLastError();
+}
+
+// ---- the 4-bit ring ---------------------------------------------------------
+
+static Cache4Args cache4_args(const igl_cache4 *store, int row_stride, int place, int lanes) {
+  Cache4Args a = {};
+  a.code[0] = store->key_code;
+  a.code[1] = store->value_code;
+  a.gain[0] = store->key_gain;
+  a.gain[1] = store->value_gain;
+  a.scale[0] = store->key_scale;
+  a.scale[1] = store->value_scale;
+  a.room = (long long)igl_cache4_room(store->cache_span);
+  a.width = store->kv_count * store->head_size;
+  a.span = store->cache_span;
+  a.sinks = store->sink_count;
+  a.row_stride = row_stride;
+  a.place = place;
+  a.lanes = lanes;
+  return a;
+}
+
+static bool cache4_rows_vec(const void *p, int row_stride, int lanes) {
+  return ((uintptr_t)p & 15u) == 0 && (lanes == 1 || (row_stride & 3) == 0);
+}
+
+extern "C" hipError_t igl_launch_cache4_lay(const igl_cache4 *store, const float *key, const float *value,
+                                            int row_stride, int place_first, int lanes, hipStream_t stream) {
+  Cache4Args a = cache4_args(store, row_stride, place_first, lanes);
+  a.in[0] = key;
+  a.in[1] = value;
+  const long long blocks = ((long long)lanes * (a.width / 8) + 255) / 256;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks, 2);
+  const bool vec = cache4_rows_vec(key, row_stride, lanes) && cache4_rows_vec(value, row_stride, lanes);
+  if (store->format == IGL_CACHE4_INT4) {
+    if (vec)
+      hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_INT4, true>), grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_INT4, false>), grid, dim3(256), 0, stream, a);
+  } else {
+    if (vec)
+      hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_E2M1, true>), grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_E2M1, false>), grid, dim3(256), 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
+extern "C" hipError_t igl_launch_cache4_read(const igl_cache4 *store, int place_first, int lanes, float *key,
+                                             float *value, int row_stride, hipStream_t stream) {
+  Cache4Args a = cache4_args(store, row_stride, place_first, lanes);
+  a.out[0] = key;
+  a.out[1] = value;
+  const long long blocks = ((long long)lanes * (a.width / 8) + 255) / 256;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks, key && value ? 2 : 1);
+  const int side0 = key ? 0 : 1;
+  const bool vec = (!key || cache4_rows_vec(key, row_stride, lanes)) && (!value || cache4_rows_vec(value, row_stride, lanes));
+  if (store->format == IGL_CACHE4_INT4) {
+    if (vec)
+      hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_INT4, true>), grid, dim3(256), 0, stream, a, side0);
+    else
+      hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_INT4, false>), grid, dim3(256), 0, stream, a, side0);
+  } else {
+    if (vec)
+      hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_E2M1, true>), grid, dim3(256), 0, stream, a, side0);
+    else
+      hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_E2M1, false>), grid, dim3(256), 0, stream, a, side0);
+  }
   return hipGetLastError();
 }

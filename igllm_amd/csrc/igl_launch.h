@@ -218,6 +218,18 @@ hipError_t igl_launch_attend_prep(const uint8_t *key_store, const uint8_t *value
 size_t igl_attend_prep_work_floats(int place_bound, int window, int head_size, int lanes,
                                    int writes_row);
 
+/* The 4-bit ring (igl_cache4.h, included by igl_elem.hip; igl_attend4.h, by
+ * igl_attend.hip).  Rows, queries and blends at any 4-byte alignment; `work`
+ * holds IGL_ATTEND_FIXED_FLOATS floats. */
+static inline size_t igl_cache4_room(int cache_span) { return ((size_t)cache_span + 63) / 64 * 64; }
+hipError_t igl_launch_cache4_lay(const igl_cache4 *store, const float *key, const float *value,
+                                 int row_stride, int place_first, int lanes, hipStream_t stream);
+hipError_t igl_launch_cache4_read(const igl_cache4 *store, int place_first, int lanes, float *key,
+                                  float *value, int row_stride, hipStream_t stream);
+hipError_t igl_launch_attend4(const igl_cache4 *store, int group_share, const float *query,
+                              int lane_stride, int place_first, int window, int lanes,
+                              float score_scale, float *blend_out, float *work, hipStream_t stream);
+
 /* The desk's HIP stream, for the engine's own launches (back_hip.c). */
 void *igl_desk_stream(igl_desk *desk);
 /* Changes whenever the desk reallocates a workspace: a graph captured over

@@ -27,6 +27,8 @@ IGL_STORE_BF16 = 3
 IGL_PLANE_REAL = 1
 IGL_CACHE_E4M3 = 0
 IGL_CACHE_INT8 = 1
+IGL_CACHE4_INT4 = 0
+IGL_CACHE4_E2M1 = 1
 
 c_float_p = ctypes.POINTER(ctypes.c_float)
 c_u8_p = ctypes.POINTER(ctypes.c_uint8)
@@ -71,6 +73,16 @@ class Desk(ctypes.Structure):
         ("gelu_gate", ctypes.c_void_p),
         ("rope_turn", ctypes.c_void_p),
     ]
+
+
+class Cache4(ctypes.Structure):
+    """`igl_cache4`: a layer's 4-bit key/value ring."""
+
+    _fields_ = [(n, ctypes.c_int) for n in (
+        "format", "cache_span", "sink_count", "kv_count", "head_size")] + [
+            ("key_scale", ctypes.c_float), ("value_scale", ctypes.c_float),
+            ("key_code", ctypes.c_void_p), ("key_gain", ctypes.c_void_p),
+            ("value_code", ctypes.c_void_p), ("value_gain", ctypes.c_void_p)]
 
 
 class Rng(ctypes.Structure):
@@ -144,6 +156,11 @@ SIGNATURES = {
     "igl_scout_note": (_I, [_P, _P, _I]),
     "igl_scout_draw": (_I, [_P, _P, _I]),
     "igl_cache_lay_dev": (_I, [ctypes.POINTER(Desk), _P, _I, _F, _I, _P, _Z]),
+    "igl_cache4_code_bytes": (_Z, [ctypes.POINTER(Cache4)]),
+    "igl_cache4_gain_bytes": (_Z, [ctypes.POINTER(Cache4)]),
+    "igl_cache4_lay_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Cache4), _P, _P, _I, _I, _I]),
+    "igl_cache4_read_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Cache4), _I, _I, _P, _P, _I]),
+    "igl_attend4_lanes_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Cache4), _I, _P, _I, _I, _I, _I, _F, _P]),
     "igl_norm_rms_dev": (_I, [ctypes.POINTER(Desk), _P, _P, _I, _I, _I, _F, _P]),
     "igl_soft_max_dev": (_I, [ctypes.POINTER(Desk), _P, _I, _I, _I]),
     "igl_gelu_gate_dev": (_I, [ctypes.POINTER(Desk), _P, _P, _I]),

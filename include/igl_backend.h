@@ -234,6 +234,71 @@ int igl_attend_lanes_fixed_dev(igl_desk *desk, const uint8_t *key_store,
 int igl_cache_lay_dev(igl_desk *desk, const float *row_dev, int width, float scale, int format,
                       uint8_t *store_dev, size_t slot_first);
 
+/* ---- the 4-bit key/value ring ------------------------------------------------ */
+
+/* No counterpart in the reference, whose smallest cache is a byte a value: for
+ * contexts that a byte ring does not fit, or whose decode steps it bounds (a
+ * row takes 17/32 of the byte row's bytes).  Every 32 values of a head
+ * share a gain, an e4m3 byte g (cache_real8's values), and a layer's side has
+ * one scale, as the byte ring's: a code stands for level * g * scale. */
+typedef enum igl_cache4_format {
+  IGL_CACHE4_INT4 = 0, /* levels -8 .. 7, the code is level + 8 (7 the largest written) */
+  IGL_CACHE4_E2M1 = 1  /* sign, two exponent bits, one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6 */
+} igl_cache4_format;
+
+/* A layer's ring: device memory of the caller's, igl_cache4_code_bytes and
+ * igl_cache4_gain_bytes each, 16-byte aligned.  Codes: [cache_span][kv_count *
+ * head_size / 2], two a byte, low nibble first.  Gains: [kv_count * head_size /
+ * 32][cache_span rounded up to 64], a row for every 32 dims, so that a reader of
+ * many positions takes theirs at once.  The first `sink_count` positions keep
+ * slots 0 .. sink_count - 1; position p after them lies in slot
+ * sink_count + (p - sink_count) % (cache_span - sink_count), for sink_count 0 the
+ * byte ring's p % cache_span.  Slots that no position was laid in may hold
+ * anything.  head_size 64, 128, 256 or 512. */
+typedef struct igl_cache4 {
+  int      format;      /* igl_cache4_format */
+  int      cache_span;  /* slots */
+  int      sink_count;  /* below cache_span */
+  int      kv_count;
+  int      head_size;
+  float    key_scale;   /* positive */
+  float    value_scale;
+  uint8_t *key_code;
+  uint8_t *key_gain;
+  uint8_t *value_code;
+  uint8_t *value_gain;
+} igl_cache4;
+
+/* Bytes of one side's codes and gains (0 for dimensions no ring has). */
+size_t igl_cache4_code_bytes(const igl_cache4 *store);
+size_t igl_cache4_gain_bytes(const igl_cache4 *store);
+
+/* cache_lay for `lane_count` positions from place_first on, both sides in one
+ * launch: rows of kv_count * head_size floats, row_stride apart, into their
+ * slots.  A group's gain is the e4m3 value nearest its largest magnitude /
+ * (top * scale), top 7 or 6, 448 at most; a value's code the level nearest
+ * value / (gain * scale), both to even when halfway, decided exactly.  A NaN is
+ * stored as zero and an infinity as the largest level of the largest gain.
+ * Positions that the ring cannot hold together are refused with
+ * IGL_FAIL_ARGUMENT. */
+int igl_cache4_lay_dev(igl_desk *desk, const igl_cache4 *store, const float *key_dev,
+                       const float *value_dev, int row_stride, int place_first, int lane_count);
+/* The rows of `lane_count` positions from place_first on as floats, row_stride
+ * apart: each the product level * gain * scale, rounded once.  Either side may
+ * be NULL. */
+int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first, int lane_count,
+                        float *key_dev, float *value_dev, int row_stride);
+/* igl_attend_lanes_dev over a 4-bit ring, for any number of query heads a
+ * key/value head up to 64: lane l at position p = place_first + l sees the
+ * positions q <= p with q > p - window (window 0: every q) or q < sink_count.
+ * query_dev and blend_out_dev: [lane_count][kv_count * group_share][head_size]
+ * floats, lanes lane_stride apart.  Every lane's keys and values must already be
+ * in the ring; a ring too short to hold all that the lanes see is refused with
+ * IGL_FAIL_ARGUMENT.  A call allocates nothing, whatever its size. */
+int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_share,
+                          const float *query_dev, int lane_stride, int place_first, int window,
+                          int lane_count, float score_scale, float *blend_out_dev);
+
 int igl_norm_rms_dev(igl_desk *desk, const float *in_dev, const float *gain_dev, int n, int rows,
                      int stride, float eps, float *out_dev);
 int igl_soft_max_dev(igl_desk *desk, float *v_dev, int n, int rows, int stride);

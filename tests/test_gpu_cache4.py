@@ -1,0 +1,438 @@
+"""GPU parity of the 4-bit key/value ring: what is laid, what is read back, and
+attention over it, against the ring's definition in 64 bits (cache4_oracle).
+
+Codes and gains are whole numbers decided exactly: every byte of the ring has
+to be equal, and the bytes of other slots and of the gain rows' padding
+untouched.  A read value is one rounding of level * gain * scale: equal to the
+bit.
+
+Bar of attention, from the arithmetic: with reach = max sum |q k| score_scale
+and vmax the largest value, queries and probabilities in two binary16 terms are
+off by 2^-22 of themselves, a score's fp32 sums, scaling and exponent by fewer
+than 2^-20 reach more, so a weight by 2^-19 reach, a blend by twice that times
+vmax (weights and their sum); the blocks' sums add at most half a unit, 2^-24,
+for each of 64 + blocks steps.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+import cache4_oracle as c4
+from igllm_amd import native
+
+pytestmark = pytest.mark.gpu
+
+SCALE = 6.0 / 448.0
+
+
+class At:
+    """A device address inside a buffer."""
+
+    def __init__(self, buf, offset):
+        self.ptr = buf.ptr + offset
+
+
+def room(span):
+    return (span + 63) // 64 * 64
+
+
+def ring_bytes(rng, span, width, fmt):
+    """A ring's four buffers, every slot filled: codes of unit-variance rows, gains among e4m3's middle."""
+    out = []
+    for _ in range(2):
+        out.append(rng.integers(0, 256, size=(span, width // 2), dtype=np.uint8))
+        out.append(rng.integers(0x28, 0x50, size=(width // 32, room(span)), dtype=np.uint8))  # 1/16 .. 2
+    return out
+
+
+def open_ring(backend, fmt, span, sinks, kv, head, host, scale=SCALE):
+    bufs = [backend.upload(b) for b in host]
+    return backend.cache4(fmt, span, sinks, kv, head, scale, 0.75 * scale, *bufs)
+
+
+def close(*things):
+    for t in things:
+        for b in t.buffers if hasattr(t, "buffers") else [t]:
+            b.free()
+
+
+def rows_of(host, fmt, span, sinks, scale=SCALE):
+    def rows(side, places):
+        at = c4.slot(places, sinks, span)
+        return c4.values(c4.unpack(host[2 * side][at]), host[2 * side + 1][:, at].T, fmt, scale * (0.75 if side else 1))
+    return rows
+
+
+def special_rows(rng, lanes, width):
+    """Rows of normals with groups of everything a quotient can be."""
+    x = (rng.normal(size=(lanes, width)) * np.exp(0.5 * rng.normal(size=(1, width)))).astype(np.float32)
+    g = x.reshape(-1, 32)
+    for i, group in enumerate([
+            np.zeros(32), np.full(32, -0.0), np.full(32, np.nan), [np.nan] * 31 + [1.0], [np.inf] + [3.0] * 31,
+            [-np.inf] * 32, np.full(32, 1e30), np.full(32, 1e-30), [np.inf, np.nan] + [-1e-40] * 30,
+            np.full(32, 3e38), np.linspace(-448, 448, 32) * SCALE * 7, np.linspace(0, 1, 32) * SCALE * 7 * 2.0 ** -9,
+            np.linspace(0, 1, 32) * SCALE * 7 * 2.0 ** -10, np.linspace(-500, 500, 32) * SCALE * 8]):
+        if i < len(g):
+            g[len(g) - 1 - i] = np.asarray(group, np.float32)
+    return x
+
+
+def lay_case(backend, fmt, kv, head, sinks, span, place, lanes, pad, off, rows, scale=SCALE):
+    width = kv * head
+    host = [np.full((span, width // 2), 0xA5, np.uint8), np.full((width // 32, room(span)), 0x5A, np.uint8)] * 2
+    store = open_ring(backend, fmt, span, sinks, kv, head, host, scale)
+    stride = width + pad
+    bufs = []
+    for side in range(2):
+        x = np.zeros((lanes, stride), np.float32)
+        x[:, :width] = rows[side]
+        bufs.append(backend.alloc(x.nbytes + 16).put(x, off))
+    backend.cache4_lay_dev(store, At(bufs[0], off), At(bufs[1], off), stride, place, lanes)
+    backend.sync()
+    at = c4.slot(np.arange(place, place + lanes), sinks, span)
+    for side in range(2):
+        codes, gains = c4.quantise(rows[side], fmt, scale * (0.75 if side else 1))
+        want_c, want_g = host[0].copy(), host[1].copy()
+        want_c[at], want_g[:, at] = c4.pack(codes), gains.T
+        got_c = store.buffers[2 * side].get(np.uint8, want_c.size).reshape(want_c.shape)
+        got_g = store.buffers[2 * side + 1].get(np.uint8, want_g.size).reshape(want_g.shape)
+        assert np.array_equal(got_g, want_g), side
+        assert np.array_equal(got_c, want_c), side
+    close(store, *bufs)
+
+
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,head,sinks,span,place,lanes,pad,off", [
+    (1, 256, 4, 516, 700, 1, 0, 0),      # one decode row past the wrap
+    (1, 64, 0, 1, 5, 1, 0, 0),           # the smallest ring
+    (1, 512, 0, 700, 0, 700, 0, 0),      # a ring filled
+    (3, 128, 5, 105, 3, 102, 0, 0),      # across the sinks' end, the whole ring
+    (2, 64, 7, 60, 5000, 53, 3, 4),      # across the wrap, rows off 16-byte alignment
+    (8, 128, 0, 130, 128, 100, 4, 0),    # padded rows
+    (5, 64, 1, 9, 0, 1, 1, 12),          # one row, one sink
+])
+def test_lay_is_bit_exact(backend, fmt, kv, head, sinks, span, place, lanes, pad, off):
+    print("case lay", fmt, kv, head, sinks, span, place, lanes, pad, off, flush=True)
+    rng = np.random.default_rng(head + lanes)
+    lay_case(backend, fmt, kv, head, sinks, span, place, lanes, pad, off,
+             [special_rows(rng, lanes, kv * head) for _ in range(2)])
+
+
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("scale", [2.0 ** -6, SCALE, 1e-30, 3e-44, 1e36])
+def test_lay_next_to_every_border(backend, fmt, scale):
+    """Values at, one float below and one above halfway between levels, and group
+    peaks so near halfway between gains."""
+    print("case borders", fmt, scale, flush=True)
+    s, top = float(np.float32(0.75 * scale)), c4.TOP[fmt]  # the value side's
+    rows = []
+    half = c4.HALF[fmt]
+    mids = (half[1:] + half[:-1]) / 2
+    with np.errstate(over="ignore", under="ignore"):
+        for gain in (1, 7, 8, 9, 15, 40, 77, 119, 126):
+            step = c4.REAL8[gain] * s
+            ties = np.repeat(np.float32(mids * step), 3)
+            ties[0::3] = np.nextafter(ties[0::3], np.float32(0))
+            ties[2::3] = np.nextafter(ties[2::3], np.float32(np.inf))
+            row = np.zeros(32, np.float32)
+            row[:21] = ties * np.where(np.arange(21) % 2, -1, 1)
+            row[31] = top * step
+            rows.append(row)
+        for gain in range(126):  # peaks at the borders between gains
+            mid = np.float32((c4.REAL8[gain] + c4.REAL8[gain + 1]) / 2 * top * s)
+            for peak in (np.nextafter(mid, np.float32(0)), mid, np.nextafter(mid, np.float32(np.inf))):
+                rows.append(np.linspace(-1, 1, 32).astype(np.float32) * peak)
+    rows = np.stack(rows[:len(rows) // 2 * 2]).reshape(-1, 64)
+    rows = np.where(np.isfinite(rows), rows, 0).astype(np.float32)
+    lay_case(backend, fmt, 1, 64, 0, len(rows), 0, len(rows), 0, 0, [rows, rows], scale)
+
+
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,head,sinks,span,place,lanes,pad,off,sides", [
+    (1, 64, 3, 300, 7, 256, 0, 0, 3), (2, 256, 0, 65, 100, 65, 5, 4, 3), (3, 128, 2, 40, 1, 30, 0, 0, 1),
+    (1, 512, 0, 33, 32, 1, 0, 0, 2)])
+def test_read_is_bit_exact(backend, fmt, kv, head, sinks, span, place, lanes, pad, off, sides):
+    """Every code with every gain byte, and floats outside the rows untouched."""
+    print("case read", fmt, kv, head, lanes, sides, flush=True)
+    rng = np.random.default_rng(head + lanes)
+    width, stride = kv * head, kv * head + pad
+    host = ring_bytes(rng, span, width, fmt)
+    for side in range(2):
+        host[2 * side + 1][:] = np.arange(host[2 * side + 1].size).reshape(host[2 * side + 1].shape) % 256
+    store = open_ring(backend, fmt, span, sinks, kv, head, host)
+    fill = np.full(lanes * stride + 4, 7.0, np.float32)
+    outs = [backend.upload(fill) if sides >> side & 1 else None for side in range(2)]
+    backend.cache4_read_dev(store, place, lanes, *[At(o, off) if o else None for o in outs], stride)
+    backend.sync()
+    rows = rows_of(host, fmt, span, sinks)
+    for side, out in enumerate(outs):
+        if not out:
+            continue
+        want = fill.copy()
+        view = want[off // 4:off // 4 + lanes * stride].reshape(lanes, stride)
+        view[:, :width] = rows(side, np.arange(place, place + lanes)).astype(np.float32)
+        assert np.array_equal(out.get(np.float32, want.size), want)
+        out.free()
+    close(store)
+
+
+def attend(backend, store, share, query, place, window, score, pad=0, off=0):
+    lanes, heads = query.shape
+    stride = heads + pad
+    x = np.full((lanes, stride), np.nan, np.float32)
+    x[:, :heads] = query
+    dq = backend.alloc(x.nbytes + 16).put(x, off)
+    do = backend.alloc(x.nbytes + 16).put(np.full(lanes * stride + 4, 7.0, np.float32))
+    backend.attend4_lanes_dev(store, share, At(dq, off), stride, place, window, lanes, score, At(do, off))
+    backend.sync()
+    got = do.get(np.float32, lanes * stride + 4)
+    close(dq, do)
+    inside = np.zeros(lanes * stride + 4, bool)
+    inside[off // 4:off // 4 + lanes * stride].reshape(lanes, stride)[:, :heads] = True
+    assert np.all(got[~inside] == 7.0)
+    return got[inside].reshape(lanes, heads)
+
+
+def check(got, query, rows, share, head, place, window, sinks, score, picks=None):
+    """Sampled lanes against 64 bits; the largest error over the bar's unit."""
+    lanes = len(query)
+    picks = sorted({0, 1, lanes // 3, lanes // 2, lanes - 2, lanes - 1} & set(range(lanes))) if picks is None else picks
+    worst = 0.0
+    for lane in picks:
+        want, reach, vmax = c4.attend(rows, share, head, query[lane:lane + 1], place + lane, window, sinks, score)
+        blocks = (len(c4.seen(place + lane, window, sinks)) + 63) // 64 + 3
+        bar = vmax * (2 * reach * 2.0 ** -19 + (64 + blocks) * 2.0 ** -24)
+        err = float(np.abs(got[lane] - want[0]).max())
+        assert err <= bar, (lane, err, bar)
+        worst = max(worst, err / float(np.abs(want).max()))
+    print("worst error over the largest output", worst, flush=True)
+
+
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,share,head,sinks,span,place,window,lanes,pad,off", [
+    (1, 8, 256, 0, 1, 0, 0, 1, 0, 0),           # one position
+    (1, 8, 256, 4, 516, 5000, 512, 1, 0, 0),    # a sliding layer's step with sinks
+    (1, 8, 256, 4, 516, 2, 512, 1, 0, 0),       # before the sinks are full
+    (1, 8, 512, 0, 512, 1023, 512, 1, 0, 0),    # the whole ring, no sinks, at its wrap
+    (1, 8, 256, 0, 4096, 4095, 0, 1, 0, 0),     # a global layer
+    (1, 8, 512, 0, 9000, 8999, 0, 1, 0, 0),
+    (2, 4, 128, 70, 200, 1000, 100, 1, 0, 0),   # sinks past a block
+    (1, 1, 64, 0, 333, 332, 0, 1, 0, 0),        # one head
+    (3, 5, 64, 1, 77, 400, 70, 3, 0, 0),        # odd shares, a few lanes
+    (1, 16, 128, 0, 1000, 900, 0, 7, 3, 4),     # sixteen heads, rows off alignment
+    (1, 64, 64, 2, 300, 200, 0, 2, 0, 0),       # sixty-four heads
+    (1, 8, 512, 0, 3000, 2000, 0, 5, 0, 0),     # a block
+    (2, 7, 64, 1, 1100, 3001, 1024, 37, 0, 0),  # a short turn
+    (1, 8, 256, 4, 2600, 0, 512, 700, 0, 0),    # a prompt from the first position
+    (1, 8, 512, 0, 700, 0, 0, 600, 0, 0),
+    (2, 3, 128, 0, 130, 0, 0, 130, 2, 8),
+    (1, 12, 256, 3, 900, 3000, 300, 400, 0, 0),
+    (1, 8, 256, 0, 5000, 4500, 100, 300, 0, 0),  # a window far inside a ring that keeps all
+    (1, 8, 64, 4, 70, 30, 2, 40, 0, 0),          # a window of two
+    (1, 8, 256, 4, 70, 30, 1, 3, 0, 0),          # itself and the sinks
+    (1, 2, 512, 0, 65, 64, 65, 1, 0, 0),         # one slot of a second block
+])
+def test_attend(backend, fmt, kv, share, head, sinks, span, place, window, lanes, pad, off):
+    print("case attend", fmt, kv, share, head, sinks, span, place, window, lanes, pad, off, flush=True)
+    rng = np.random.default_rng(head + lanes + place)
+    host = ring_bytes(rng, span, kv * head, fmt)
+    store = open_ring(backend, fmt, span, sinks, kv, head, host)
+    query = rng.normal(size=(lanes, kv * share * head)).astype(np.float32)
+    score = 10.0 / np.sqrt(head)  # scores of deviation 1 to 4: the ring's values are about 1/10 to 1/3
+    got = attend(backend, store, share, query, place, window, score, pad, off)
+    check(got, query, rows_of(host, fmt, span, sinks), share, head, place, window, sinks, score)
+    close(store)
+
+
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("head,lanes", [(256, 1), (256, 9), (64, 70), (512, 40)])
+def test_slots_without_rows_count_for_nothing(backend, fmt, head, lanes):
+    """Slots that no position was laid in, and the gain rows' padding, hold the
+    largest codes and gains: lanes that do not see them are as in a clean ring."""
+    print("case unwritten", fmt, head, lanes, flush=True)
+    rng = np.random.default_rng(head)
+    span, sinks, place = 500, 4, 100
+    host = ring_bytes(rng, span, head, fmt)
+    query = rng.normal(size=(lanes, 8 * head)).astype(np.float32)
+    got = []
+    for byte in (0xFF, 0x00):
+        for b in host[0], host[2]:
+            b[place + lanes:] = byte
+        for g in host[1], host[3]:
+            g[:, place + lanes:] = 0x7F if byte else 0
+        store = open_ring(backend, fmt, span, sinks, 1, head, host)
+        got.append(attend(backend, store, 8, query, place, 0, 1.0))
+        close(store)
+    assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
+
+
+@pytest.mark.parametrize("head,lanes", [(64, 1), (256, 1), (512, 3), (256, 70)])
+def test_queries_of_any_size(backend, head, lanes):
+    """Queries far past binary16's range, up and down, and a NaN or an infinity
+    that stays in its own head."""
+    print("case query range", head, lanes, flush=True)
+    rng = np.random.default_rng(head + 1)
+    host = ring_bytes(rng, 200, head, c4.INT4)
+    store = open_ring(backend, c4.INT4, 200, 0, 1, head, host)
+    place = 200 - lanes
+    query = rng.normal(size=(lanes, 8 * head)).astype(np.float32)
+    for size in (1e30, 1e-30):
+        q = (query * np.float32(size)).astype(np.float32)
+        score = 10.0 / np.sqrt(head) / size
+        got = attend(backend, store, 8, q, place, 0, score)
+        check(got, q, rows_of(host, c4.INT4, 200, 0), 8, head, place, 0, 0, score)
+    score = 10.0 / np.sqrt(head)
+    clean = attend(backend, store, 8, query, place, 0, score)
+    query[0, 2 * head + 5] = np.nan
+    query[0, 5 * head + 1] = np.inf
+    got = attend(backend, store, 8, query, place, 0, score).reshape(lanes, 8, head)
+    assert np.all(np.isnan(got[0, [2, 5]]))
+    got[0, [2, 5]] = clean.reshape(lanes, 8, head)[0, [2, 5]]
+    assert np.array_equal(got.reshape(clean.shape), clean)
+    close(store)
+
+
+@pytest.mark.parametrize("head,lanes,span", [(256, 1, 3000), (512, 1, 3000), (128, 70, 3000), (512, 70, 600)])
+def test_a_peaked_position(backend, head, lanes, span):
+    """One position whose score lies 18 above all others and whose value is zero:
+    the blend is the sum of weights near 2^-26 of the largest, which two binary16
+    terms against one peak would lose; what the largest weight's own block loses
+    is at most its 64 positions of the rest, and 2^-24 / 2^-26 of theirs."""
+    print("case peaked", head, lanes, span, flush=True)
+    rng = np.random.default_rng(head)
+    host = ring_bytes(rng, span, head, c4.INT4)
+    host[0][:] = 0x88  # keys of zero
+    host[0][3] = 0x99  # but one
+    host[1][:] = 0x38  # gain 1
+    host[2][3] = 0x88
+    store = open_ring(backend, c4.INT4, span, 0, 1, head, host)
+    query = np.ones((lanes, 8 * head), np.float32)
+    score = 18.0 / (head * float(np.float32(SCALE)))
+    place = span - lanes
+    got = attend(backend, store, 8, query, place, 0, score)
+    want, _, _ = c4.attend(rows_of(host, c4.INT4, span, 0), 8, head, query[:1], place, 0, 0, score)
+    err = np.abs(got[0] - want[0]).max() / np.abs(want).max()
+    print("error", err)
+    assert err <= 0.07
+    close(store)
+
+
+def test_a_run_of_steps(backend):
+    """A session's layer: a prompt laid and attended in one pass, then decode
+    steps past the ring's wrap, each row laid and attended; every blend against
+    the rows in 64 bits as they were laid, and the last rows read back."""
+    print("case run", flush=True)
+    rng = np.random.default_rng(11)
+    head, share, sinks, window, fmt = 256, 8, 4, 60, c4.E2M1
+    span, prompt, steps = sinks + 100, 41, 150
+    store = backend.cache4(fmt, span, sinks, 1, head, SCALE, SCALE)
+    rows = (rng.normal(size=(2, prompt + steps, head))).astype(np.float32)
+    kept = [c4.values(*c4.quantise(rows[s], fmt, SCALE), fmt, SCALE) for s in range(2)]
+    query = rng.normal(size=(prompt + steps, share * head)).astype(np.float32)
+    dk, dv, dq = backend.upload(rows[0]), backend.upload(rows[1]), backend.upload(query)
+    do = backend.alloc(query.nbytes)
+    place = 0
+    for lanes in [prompt] + [1] * steps:
+        backend.cache4_lay_dev(store, At(dk, place * head * 4), At(dv, place * head * 4), head, place, lanes)
+        at = place * share * head * 4
+        backend.attend4_lanes_dev(store, share, At(dq, at), share * head, place, window, lanes, 1 / 16, At(do, at))
+        place += lanes
+    out = backend.alloc(50 * head * 4)
+    backend.cache4_read_dev(store, place - 50, 50, out, None, head)
+    backend.sync()
+    got = do.get(np.float32, query.size).reshape(query.shape)
+    check(got, query, lambda side, t: kept[side][t], share, head, 0, window, sinks, 1 / 16,
+          [0, 1, 5, 40, 41, 63, 64, 65, 100, 103, 104, 105, 150, 190])
+    assert np.array_equal(out.get(np.float32, 50 * head).reshape(50, head), kept[0][-50:].astype(np.float32))
+    close(store, dk, dv, dq, do, out)
+
+
+@pytest.mark.parametrize("lanes,place,head", [(1, 4000, 256), (3, 3000, 512), (100, 1900, 256), (130, 0, 512)])
+def test_recorded_and_replayed(backend, lanes, place, head):
+    """Rows laid and attended in a recording, replayed over other rows with the
+    program's own calls between: every replay equals the eager calls to the bit,
+    and no call moves the desk's workspaces, one beside a live replay included."""
+    print("case replay", lanes, place, head, flush=True)
+    rng = np.random.default_rng(lanes)
+    span = place + lanes
+    host = ring_bytes(rng, span, head, c4.INT4)
+    store = open_ring(backend, c4.INT4, span, 0, 1, head, host)
+    stride = 8 * head
+    dk, dv = backend.alloc(lanes * head * 4), backend.alloc(lanes * head * 4)
+    dq, do = backend.alloc(lanes * stride * 4), backend.alloc(lanes * stride * 4)
+    side = open_ring(backend, c4.INT4, span, 0, 1, head, host)
+    do2 = backend.alloc(lanes * stride * 4)
+    generation = backend.lib.igl_desk_generation
+    generation.argtypes, generation.restype = [ctypes.c_void_p], ctypes.c_uint
+    before = generation(ctypes.byref(backend.desk))
+
+    def step(ring, out):
+        backend.cache4_lay_dev(ring, dk, dv, head, place, lanes)
+        backend.attend4_lanes_dev(ring, 8, dq, stride, place, 0, lanes, 1 / 16, out)
+
+    backend.record_begin()
+    step(store, do)
+    replay = backend.record_end()
+    try:
+        for turn in range(4):
+            for buf, n in ((dk, head), (dv, head), (dq, stride)):
+                buf.put(rng.normal(size=(lanes, n)).astype(np.float32))
+            backend.replay_run(replay)
+            step(side, do2)
+            backend.replay_run(replay)
+            backend.sync()
+            a, b = (x.get(np.uint32, lanes * stride) for x in (do, do2))
+            assert np.array_equal(a, b), turn
+            assert np.all(np.isfinite(a.view(np.float32)))
+    finally:
+        backend.replay_free(replay)
+    assert generation(ctypes.byref(backend.desk)) == before
+    close(store, side, dk, dv, dq, do, do2)
+
+
+def test_offsets_past_32_bits(backend):
+    """A ring of more than 2^32 bytes of codes: rows past them laid, read and seen."""
+    print("case long", flush=True)
+    head, fmt, window = 512, c4.E2M1, 100
+    span = (1 << 24) + 5000
+    sizes = [span * head // 2, head // 32 * room(span)] * 2
+    bufs = [backend.alloc(n) for n in sizes]
+    store = backend.cache4(fmt, span, 0, 1, head, SCALE, SCALE, *bufs)
+    rng = np.random.default_rng(3)
+    place, lanes = (1 << 24) + 3000, 130
+    rows = rng.normal(size=(2, lanes, head)).astype(np.float32)
+    dk, dv = backend.upload(rows[0]), backend.upload(rows[1])
+    backend.cache4_lay_dev(store, dk, dv, head, place, lanes)
+    out = backend.alloc(lanes * head * 4)
+    backend.cache4_read_dev(store, place, lanes, None, out, head)
+    backend.sync()
+    kept = [c4.values(*c4.quantise(rows[s], fmt, SCALE), fmt, SCALE) for s in range(2)]
+    assert np.array_equal(out.get(np.float32, lanes * head).reshape(lanes, head), kept[1].astype(np.float32))
+    for first, n in ((lanes - 1, 1), (lanes - 21, 21)):
+        query = rng.normal(size=(n, 8 * head)).astype(np.float32)
+        got = attend(backend, store, 8, query, place + first, window, 1 / 16)
+        for lane in {0, n - 1}:
+            t = np.arange(first + lane - window + 1, first + lane + 1)
+            k, v = kept[0][t], kept[1][t]
+            s = query[lane].reshape(8, head).astype(np.float64) @ k.T / 16
+            w = np.exp(s - s.max(-1, keepdims=True))
+            want = (w @ v / w.sum(-1, keepdims=True)).reshape(-1)
+            reach = float((np.abs(query[lane].reshape(8, head)) @ np.abs(k).T).max()) / 16
+            assert np.abs(got[lane] - want).max() <= np.abs(v).max() * (2 * reach * 2.0 ** -19 + 70 * 2.0 ** -24)
+    close(store, dk, dv, out)
+
+
+def test_refusals_leave_the_outputs(backend):
+    """A refused call writes nothing and the desk goes on."""
+    print("case refused", flush=True)
+    lib, desk = backend.lib, ctypes.byref(backend.desk)
+    store = backend.cache4(c4.INT4, 100, 4, 1, 64, SCALE, SCALE)
+    out = backend.upload(np.full(8 * 64, 7.0, np.float32))
+    assert lib.igl_attend4_lanes_dev(desk, ctypes.byref(store.cache), 8, out.ptr, 512, 200, 97, 1, 1.0, out.ptr) == \
+        native.IGL_FAIL_ARGUMENT
+    assert backend.error_take() == native.IGL_FAIL_ARGUMENT
+    assert np.all(out.get(np.float32, 512) == 7.0)
+    backend.cache4_lay_dev(store, out, out, 64, 0, 1)
+    backend.sync()
+    close(store, out)

@@ -45,6 +45,8 @@
 // us for the same chunks.  A last-workgroup fold in the same kernel, after an
 // agent-scope release/acquire ticket, was slower at every chunk count tried:
 // 10.5 us at 8 chunks, over 100 us at 256.)
+#include <math.h>
+
 #include <mutex>
 
 #include "igl_backend.h"

@@ -295,10 +295,11 @@ def test_queries_of_any_size(backend, head, lanes):
 
 @pytest.mark.parametrize("head,lanes,span", [(256, 1, 3000), (512, 1, 3000), (128, 70, 3000), (512, 70, 600)])
 def test_a_peaked_position(backend, head, lanes, span):
-    """One position whose score lies 18 above all others and whose value is zero:
-    the blend is the sum of weights near 2^-26 of the largest, which two binary16
-    terms against one peak would lose; what the largest weight's own block loses
-    is at most its 64 positions of the rest, and 2^-24 / 2^-26 of theirs."""
+    """One position whose score lies 18 (26 powers of two) above all others and
+    whose value is zero: the blend is the sum of weights near 2^-26 of the
+    largest.  A block's largest weight is held as 2^8 or more, so in its own block
+    such a weight is 2^-18 or more, which binary16's smallest step, 2^-24, holds to
+    2^-7 of itself."""
     print("case peaked", head, lanes, span, flush=True)
     rng = np.random.default_rng(head)
     host = ring_bytes(rng, span, head, c4.INT4)
@@ -311,10 +312,12 @@ def test_a_peaked_position(backend, head, lanes, span):
     score = 18.0 / (head * float(np.float32(SCALE)))
     place = span - lanes
     got = attend(backend, store, 8, query, place, 0, score)
-    want, _, _ = c4.attend(rows_of(host, c4.INT4, span, 0), 8, head, query[:1], place, 0, 0, score)
-    err = np.abs(got[0] - want[0]).max() / np.abs(want).max()
-    print("error", err)
-    assert err <= 0.07
+    rows = rows_of(host, c4.INT4, span, 0)
+    want, _, _ = c4.attend(rows, 8, head, query[:1], place, 0, 0, score)
+    size, _, _ = c4.attend(lambda side, t: np.abs(rows(side, t)), 8, head, query[:1], place, 0, 0, score)
+    err = float(np.abs(got[0] - want[0]).max() / size.max())
+    print("error over the weighted sizes", err, flush=True)
+    assert err <= 2.0 ** -7
     close(store)
 
 

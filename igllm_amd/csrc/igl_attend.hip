@@ -45,8 +45,6 @@
 // us for the same chunks.  A last-workgroup fold in the same kernel, after an
 // agent-scope release/acquire ticket, was slower at every chunk count tried:
 // 10.5 us at 8 chunks, over 100 us at 256.)
-#include <math.h>
-
 #include <mutex>
 
 #include "igl_backend.h"
@@ -1552,5 +1550,3 @@ extern "C" float *igl_attend_fixed_ptr(int device) {
   std::lock_guard<std::mutex> hold(fixed_lock);
   return fixed_ptr[device];
 }
-
-#include "igl_attend4.h"

@@ -8,6 +8,9 @@
 // f the score scale, the key scale and log2 e, m a base near the peak.
 #pragma once
 
+#include <float.h>
+#include <math.h>
+
 #include "igl_cache4.h"
 
 namespace igl {
@@ -26,37 +29,41 @@ struct Attend4Args {
   int newest_slot;       // and its slot, where it lies past the sinks
   int window;
   int rows;              // lanes * share
+  uint32_t share_mul;    // row / share = row * share_mul >> share_shift
+  int share_shift;
   int key_power;         // key scale, score scale, log2 e and 256: key_part 2^key_power
   float key_part;        // in [1/2, 1), or of a score scale below zero
   float value_scale;     // times 256
-  int segments;          // of a row tile's blocks
+  int segments;          // of a row tile's blocks, each `per` of them and the last what is left
+  int per;
   float *part_out;       // [segments][kv][rows][HEAD], with more than one segment
   float *part_base;      // [segments][kv][rows]
   float *part_total;
 };
 
-// The blocks of `block` slots that hold what lanes at positions first ..
-// last see: blocks 0 .. low - 1, then mid .. mid + count - low - 1.  The visible
-// slots are the sinks' and the ring's from the oldest position to the newest,
-// cut in two where the ring wraps; the piece from slot sinks on joins the sinks.
+// The blocks of `block` slots that hold what lanes at positions first .. last
+// see: blocks 0 .. low - 1, then mid .. mid + count - low - 1.  The visible slots
+// are the sinks' and the ring's from the oldest position to the newest, cut in
+// two where the ring wraps; the piece from slot sinks on joins the sinks.
 struct Blocks4 {
   int low, mid, count;
   __host__ __device__ int at(int i) const { return i < low ? i : mid + i - low; }
 };
 
-__host__ __device__ __forceinline__ Blocks4 attend4_blocks(int block, int span, int sinks, int window, int first,
-                                                               int last) {
+__host__ __device__ inline Blocks4 attend4_blocks(int block, int first, int last, const Attend4Args &a) {
   Blocks4 b = {0, 0, 0};
-  const int kept = last < sinks ? last + 1 : sinks;
-  int oldest = window > 0 && first >= window ? first + 1 - window : 0;
-  if (oldest < sinks) oldest = sinks;
-  int low_slots = kept, mid_first = 0, mid_last = -1;
-  if (oldest <= last) {
-    mid_first = cache4_slot(oldest, sinks, span);
-    mid_last = cache4_slot(last, sinks, span);
+  int low_slots = last < a.sinks ? last + 1 : a.sinks;
+  int oldest = a.window > 0 && first >= a.window ? first + 1 - a.window : 0;
+  if (oldest < a.sinks) oldest = a.sinks;
+  int mid_first = 0, mid_last = -1;
+  if (oldest <= last) {  // all of them within a turn of the ring before the newest
+    mid_first = a.newest_slot - (a.newest - oldest);
+    if (mid_first < a.sinks) mid_first += a.span - a.sinks;
+    mid_last = a.newest_slot - (a.newest - last);
+    if (mid_last < a.sinks) mid_last += a.span - a.sinks;
     if (mid_first > mid_last) {
       low_slots = mid_last + 1;
-      mid_last = span - 1;
+      mid_last = a.span - 1;
     }
   }
   b.low = (low_slots + block - 1) / block;
@@ -67,6 +74,10 @@ __host__ __device__ __forceinline__ Blocks4 attend4_blocks(int block, int span, 
   return b;
 }
 
+// The lane of a row of a key/value head.
+__device__ __forceinline__ int attend4_lane(int row, const Attend4Args &a) {
+  return (int)(((uint64_t)(uint32_t)row * a.share_mul) >> a.share_shift);
+}
 
 // Segments a row's blocks are cut into, at most: the fold takes one a thread.
 constexpr int kAttend4Segments = 256;
@@ -158,6 +169,26 @@ __device__ __forceinline__ void value_operands(const uint32_t (&x)[8], const hal
   for (int d = 0; d < DIMS; ++d) out[d] = __builtin_bit_cast(half8_t, p[d]);
 }
 
+// The largest over groups of N neighbouring lanes, in each of them.
+template <int N>
+__device__ __forceinline__ float group_max(float v) {
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  if (N >= 16) v = fmaxf(v, dpp_move<0x140>(v));
+  if (N >= 32) {
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    v = fmaxf(a, b);
+  }
+  if (N >= 64) {
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    v = fmaxf(a, b);
+  }
+  return v;
+}
+
 // Largest and sum over the four lanes of a wave that differ by 16 and 32, the
 // same in all four: each swap of two copies leaves the partners' values side by
 // side (written out as xsum32 is).
@@ -177,196 +208,325 @@ __device__ __forceinline__ float xsum48(float v) {
   return a + b;
 }
 
-// ---- the kernel ---------------------------------------------------------------
+// LDS only: rows requested ahead stay in flight.
+__device__ __forceinline__ void attend4_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
-// Work.  A wave takes a tile of rows (a row is a lane's query head of one
-// key/value head) through blocks of 32 U slots, everything in registers:
-//   scores  S^T (slots x rows)  = K (slots x dims) . Q^T
-//   blend   O^T (dims x rows)   = V^T (dims x slots) . P^T
-// Transposed, a score's lane and register are where the blend's product wants
-// its probability: lane 16 g + n of S^T holds row n's slots 4 g + r of a
-// 16-slot tile, and of P^T row n's eight slots 8 g + e.  With slot 32 u + 8 g +
-// 2 r + b as index 4 g + r of tile 2 u + b, e is 2 r + b, and nothing crosses
-// lanes between the two products but a row's peak.  Keys are read as they lie,
-// 16 bytes of a row (one gain's dims) a lane; values eight rows a lane, whose
-// nibbles pair up by twos of rows.
-//
-// Rows keep 24 bits: queries (scaled by a power of two to their row's largest)
-// and probabilities are two binary16 terms.  A tile of up to eight rows (PAIR)
-// holds both terms in the 16 columns of one product; others take two products.
-// DW waves split a head's dims (the partial scores meet in LDS), PS waves a
-// segment's blocks (their blends meet in LDS at the end).
-//
-// A row's base m is a whole number, so every rescaling is exact; weights are
-// 2^(score - m).  It moves, to 12 below the block's peak, when the peak is not 8
-// to 14 above it: most blocks rescale nothing, a block's largest weight is in
-// [2^8, 2^15), and weights down to 2^-32 of it keep a term of binary16 (against a
-// base at the peak they end at 2^-24: one position that outweighs a block's
-// others by that much, its own value small, would take them from the blend).
-// The base stays within 58 of the largest so far, below which weights count for
-// nothing: sums stay in range.
-template <int HEAD, int FMT, int RB, bool PAIR, int DW, int PS, int U>
-struct Attend4Shape {
-  static constexpr int DH = HEAD / DW;            // dims a wave holds
-  static constexpr int KL = DH >= 128 ? DH / 128 : 1;  // key chunks of a row a lane reads
-  static constexpr int KW = DH >= 128 ? 4 : 2;    // dwords of a chunk
-  static constexpr int DPL = DH / 16;             // value dims a lane
-  static constexpr int ROWS = PAIR ? 8 : 16 * RB;
-  static constexpr int TERMS = PAIR ? 1 : 2;      // products a term pair takes
-  static constexpr int BLOCK = 32 * U;
-  static constexpr int TREE = PS > 1 ? PS / 2 * DW * (DPL * RB * 1024 + RB * 512) : 0;
-  static constexpr int SWAP = DW > 1 ? 2 * PS * DW * 2 * U * RB * 1024 : 0;
-  static constexpr int LDS = TREE > SWAP ? TREE : SWAP;
+// A buffer over the rows at a uniform address: scalar registers and a 32-bit
+// lane offset.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t attend4_rows(const uint8_t *rows) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(rows), 0, 0xFFFFFFFF, 0x00020000);
+}
+
+// Bytes to a row of a block: both factors are below 2^24.
+__device__ __forceinline__ uint32_t row_at(int row, uint32_t row_bytes) {
+  return ((uint32_t)row & 0xFFFFFFu) * (row_bytes & 0xFFFFFFu);
+}
+
+// A row's queries as two binary16 terms: times a power of two that brings the
+// row's largest, `top`, to [2^13, 2^14) (or as far up as a float reaches), so that
+// no query is too large or too small for them; the factor takes it back, and is
+// never zero, so that it leaves a hidden score's -infinity one.  A score factor
+// below zero turns the queries instead.  A NaN or an infinity stays one in its
+// terms.
+__device__ __forceinline__ float query_factor(const Attend4Args &a, float top, float &scale) {
+  int up = top > 0.0f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+  if (up > 126) up = 126;
+  scale = __builtin_amdgcn_ldexpf(a.key_part < 0.0f ? -1.0f : 1.0f, up);
+  const float factor = __builtin_amdgcn_ldexpf(fabsf(a.key_part), a.key_power - up);
+  return factor < FLT_MIN ? FLT_MIN : factor;
+}
+
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
+// Two values as two binary16 terms each, x = hi + lo to 2^-22 of itself.
+__device__ __forceinline__ void two_terms(float x, float y, half2_t &hi, half2_t &lo) {
+  hi = __builtin_convertvector((float2_t){x, y}, half2_t);
+  lo = __builtin_convertvector(((float2_t){__builtin_fmaf((float)hi[0], -1.0f, x), __builtin_fmaf((float)hi[1], -1.0f, y)}),
+                               half2_t);
+}
+
+// Eight queries in the key operands' order.
+template <int FMT>
+__device__ __forceinline__ void query_operands(const float (&x)[8], float scale, half8_t &hi, half8_t &lo) {
+  half2_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    two_terms(x[key_order<FMT>(2 * e)] * scale, x[key_order<FMT>(2 * e + 1)] * scale, h[e], l[e]);
+  hi = __builtin_bit_cast(half8_t, h);
+  lo = __builtin_bit_cast(half8_t, l);
+}
+
+// Floats from the queries' (and the blends') start to a row of a key/value head.
+__device__ __forceinline__ size_t attend4_row(int row, int kv, int head, const Attend4Args &a) {
+  const int l = attend4_lane(row, a);
+  return (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * head;
+}
+
+// A tile's rows as terms in LDS, a thread eight dims: row r at `to` + r (HEAD + 8),
+// its second term `second` halves on, its factor at factors[r].  Rows past the last
+// are the last again.
+template <int HEAD, int FMT, int ROWS, int THREADS>
+struct QueryLoad {
+  static constexpr int PIECES = HEAD / 8, ITEMS = ROWS * PIECES, PER = (ITEMS + THREADS - 1) / THREADS;
+  float x[PER][8];
+  __device__ __forceinline__ void load(const Attend4Args &a, int kv, int row0, int row_last, int tid) {
+    const bool vec = (((uintptr_t)a.query | ((size_t)a.lane_stride * 4)) & 15u) == 0;  // uniform
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int item = min(tid + THREADS * i, ITEMS - 1);
+      const float *src = a.query + attend4_row(min(row0 + item / PIECES, row_last), kv, HEAD, a) + 8 * (item % PIECES);
+      if (vec) {
+        const float4_t u = *reinterpret_cast<const float4_t *>(src), v = *reinterpret_cast<const float4_t *>(src + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = u[e], x[i][4 + e] = v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] = src[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(const Attend4Args &a, int tid, _Float16 *to, int second, float *factors) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int item = tid + THREADS * i;
+      if (ITEMS % THREADS != 0 && item >= ITEMS) break;  // whole waves
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
+      top = group_max<PIECES>(top);
+      float scale;
+      const float factor = query_factor(a, top, scale);
+      half8_t hi, lo;
+      query_operands<FMT>(x[i], scale, hi, lo);
+      const int row = item / PIECES;
+      _Float16 *at = to + row * (HEAD + 8) + 8 * (item % PIECES);
+      *reinterpret_cast<half8_t *>(at) = hi;
+      *reinterpret_cast<half8_t *>(at + second) = lo;
+      if (item % PIECES == 0) factors[row] = factor;
+    }
+  }
 };
 
-template <int HEAD, int FMT, int RB, bool PAIR, int DW, int PS, int U>
-__global__ __launch_bounds__(64 * DW * PS) void attend4_kernel(Attend4Args a) {
-  using F = Attend4Shape<HEAD, FMT, RB, PAIR, DW, PS, U>;
-  constexpr int DH = F::DH, KL = F::KL, KW = F::KW, DPL = F::DPL, ROWS = F::ROWS, TERMS = F::TERMS, BLOCK = F::BLOCK;
-  constexpr int VD = DPL >= 8 ? 8 : 4;   // dims a value step takes
-  constexpr int VW = DPL >= 8 ? DPL / 8 : 1;  // dwords of a value row a lane reads
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds4[];
+// Whether a lane at `place` sees a slot's position.
+__device__ __forceinline__ bool attend4_seen(int slot, int place, const Attend4Args &a) {
+  const int at = attend4_place(slot, a);
+  return at <= place && (a.window == 0 || at > place - a.window || at < a.sinks);
+}
+
+// Whether every lane from place_low to place_high sees all of a block past the sinks.
+__device__ __forceinline__ bool attend4_all(int slot0, int block, int place_low, int place_high, const Attend4Args &a) {
+  const int place0 = attend4_place(slot0, a);
+  return slot0 >= a.sinks && slot0 + block <= a.span && place0 <= place_low - (block - 1) &&
+         attend4_place(slot0 + block - 1, a) == place0 + block - 1 && (a.window == 0 || place0 > place_high - a.window);
+}
+
+// A row's base after a block with this peak (before its factor).
+__device__ __forceinline__ float attend4_base(float peak, float factor, float base, float &top_base) {
+  if (peak == -INFINITY) return base;
+  const float low = floorf(peak * factor) - 12.0f;
+  if (low >= base - 4.0f && low <= base + 2.0f) return base;
+  top_base = fmaxf(top_base, low);
+  return fmaxf(low, top_base - 58.0f);
+}
+
+// What is added to a score (times its factor) below a base; a row that has seen
+// nothing yet has none, and only hidden scores.
+__device__ __forceinline__ float attend4_from(float base) { return base != -INFINITY ? -base : 0.0f; }
+
+// Writes a row's dims from dim0 + (4 g + r) DPL + j of out[j][r] on: the blend, or
+// a segment's share of it (with its base and total where `stats`).  PAIR: columns
+// n and n + 8 hold a row's two terms, and each writes half of their sums.
+template <int HEAD, int DPL, bool PAIR>
+__device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&out)[DPL], float base, float total, int row,
+                                              int row_last, int seg, int kv, int dim0, bool stats, int g, int n) {
+  if (PAIR) {
+#pragma unroll
+    for (int j = 0; j < DPL; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) out[j][r] += dpp_move<0x128>(out[j][r]);
+  }
+  if (row > row_last) return;
+  const int l = attend4_lane(row, a);
+  float *dst = a.out + (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * HEAD;
+  float mul = a.value_scale;
+  bool vec = (((uintptr_t)a.out | ((size_t)a.lane_stride * 4)) & 15u) == 0;
+  if (a.segments > 1) {
+    const size_t at = ((size_t)seg * gridDim.z + kv) * a.rows + row;
+    dst = a.part_out + at * HEAD;
+    vec = true;
+    if (stats && g == 0 && (!PAIR || n < 8)) {
+      a.part_base[at] = base;
+      a.part_total[at] = total;
+    }
+  } else {
+    mul *= 1.0f / total;
+  }
+  dst += dim0 + 4 * g * DPL;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (PAIR && (r >= 2) != (n >= 8)) continue;
+#pragma unroll
+    for (int j = 0; j < DPL; j += 4) {
+      float *to = dst + r * DPL + j;
+      const float4_t o = {out[j][r] * mul, out[j + 1][r] * mul, out[j + 2][r] * mul, out[j + 3][r] * mul};
+      if (vec) {
+        *reinterpret_cast<float4_t *>(to) = o;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = o[e];
+      }
+    }
+  }
+}
+
+// ---- shared pieces ------------------------------------------------------------
+
+// ---- few rows -----------------------------------------------------------------
+
+// Steps and blocks of a few lanes.  Four waves take a block of 64 T slots, the
+// scores divided by slots (a wave T tiles of 16, every dim), the blend by dims
+// (VD ways) and then by slots (VS ways): so a wave's chain from one barrier to
+// the next is a quarter of the block's work.  Weights cross between the two
+// divisions through LDS, against a base that the four waves agree on.
+template <int HEAD, int FMT, int RB, bool PAIR, int T>
+struct Step4Shape {
+  static constexpr int KL = HEAD >= 128 ? HEAD / 128 : 1;  // key chunks of a row a lane reads
+  static constexpr int KW = HEAD >= 128 ? 4 : 2;           // dwords of a chunk
+  static constexpr int ROWS = PAIR ? 8 : 16 * RB;
+  static constexpr int TERMS = PAIR ? 1 : 2;
+  static constexpr int BLOCK = 64 * T;
+  static constexpr int VD = HEAD >= 128 ? HEAD / 128 : 1, VS = 4 / VD;
+  static constexpr int DB = HEAD / VD, DPL = DB / 16;      // a wave's dims of the blend, a lane's
+  static constexpr int UB = BLOCK / VS / 32;               // its steps of 32 slots
+  static constexpr int QP = HEAD + 8, PP = BLOCK + 8;      // pitches in halves
+  static constexpr int Q = 0;                              // [RB][TERMS][16][QP]
+  static constexpr int P = Q + RB * TERMS * 16 * QP * 2;   // [RB][TERMS][16][PP]
+  static constexpr int PEAK = P + RB * TERMS * 16 * PP * 2;  // [4][16 RB]
+  static constexpr int FACTOR = PEAK + 4 * 16 * RB * 4;    // [16 RB]
+  static constexpr int LOOP = FACTOR + 16 * RB * 4;
+  static constexpr int MERGE = (VS - 1) * VD * RB * DPL * 1024;  // the blends of waves that took other slots
+  static constexpr int LDS = LOOP > MERGE ? LOOP : MERGE;
+  static_assert(UB >= 1, "a blend step takes 32 slots");
+};
+
+template <int HEAD, int FMT, int RB, bool PAIR, int T>
+__global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
+  using F = Step4Shape<HEAD, FMT, RB, PAIR, T>;
+  constexpr int KL = F::KL, KW = F::KW, ROWS = F::ROWS, TERMS = F::TERMS, BLOCK = F::BLOCK;
+  constexpr int VD = F::VD, VS = F::VS, DB = F::DB, DPL = F::DPL, UB = F::UB, QP = F::QP, PP = F::PP;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[F::LDS];
+  _Float16 *qs = reinterpret_cast<_Float16 *>(lds + F::Q), *ws = reinterpret_cast<_Float16 *>(lds + F::P);
+  float *peaks = reinterpret_cast<float *>(lds + F::PEAK), *factors = reinterpret_cast<float *>(lds + F::FACTOR);
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int dw = DW > 1 ? wave % DW : 0, ps = wave / DW;
+  const int vd = wave % VD, vs = wave / VD;
   const int g = lane >> 4, n = lane & 15;
   const int kv = blockIdx.z, seg = blockIdx.y;
-  const int row0 = (int)(gridDim.x - 1 - blockIdx.x) * ROWS;  // a prompt's longest first
+  const int row0 = (int)blockIdx.x * ROWS;
   const int row_last = min(row0 + ROWS, a.rows) - 1;
-  const int place_low = a.place + row0 / a.share, place_high = a.place + row_last / a.share;
-  const Blocks4 blocks = attend4_blocks(BLOCK, a.span, a.sinks, a.window, place_low, place_high);
-  const int per = (blocks.count + a.segments - 1) / a.segments;
-  const int first = seg * per + ps, end = min(blocks.count, seg * per + per);
+  const int place_low = a.place + attend4_lane(row0, a), place_high = a.place + attend4_lane(row_last, a);
+  const Blocks4 blocks = attend4_blocks(BLOCK, place_low, place_high, a);
+  const int first = min(blocks.count, seg * a.per);
+  const int end = seg == a.segments - 1 ? blocks.count : min(blocks.count, first + a.per);
   const uint32_t exp16 = 0x4C004C00u;
   const uint32_t row_bytes = (uint32_t)a.kv_width / 2;
-  const size_t head_bytes = ((size_t)kv * HEAD + dw * DH) / 2;
-  const size_t gain_row = ((size_t)kv * HEAD + dw * DH) / kCache4Group;
+  const size_t head_bytes = (size_t)kv * HEAD / 2;
+  const size_t gain_row = (size_t)kv * HEAD / kCache4Group;
 
-  // ---- the rows' queries, this wave's dims
-  half8_t q[RB][TERMS][KL * KW];
-  float factor[RB];
-  int place[RB];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int row = min(row0 + 16 * rb + (PAIR ? n & 7 : n), row_last);
-    const int l = row / a.share;
-    place[rb] = a.place + l;
-    const float *src = a.query + (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * HEAD + dw * DH;
-    const bool vec = (((uintptr_t)a.query | ((size_t)a.lane_stride * 4)) & 15u) == 0;  // uniform
-    float x[KL * KW][8];
-#pragma unroll
-    for (int c = 0; c < KL; ++c)
-#pragma unroll
-      for (int s = 0; s < KW; ++s) {
-        const float *p = src + (KW == 4 ? 32 * (4 * c + g) : 16 * g) + 8 * s;
-        if (vec) {
-          const float4_t u = *reinterpret_cast<const float4_t *>(p), v = *reinterpret_cast<const float4_t *>(p + 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[KW * c + s][e] = u[e], x[KW * c + s][4 + e] = v[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[KW * c + s][e] = p[e];
-        }
-      }
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < KL * KW; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
-    top = xmax48(top);
-    // to [2^13, 2^14); an infinity or NaN stays one in its terms
-    const int up = top > 0.0f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
-    const float sign = a.key_part < 0.0f ? -1.0f : 1.0f;  // a factor below zero turns the queries
-    factor[rb] = __builtin_amdgcn_ldexpf(fabsf(a.key_part), a.key_power - up);
-#pragma unroll
-    for (int i = 0; i < KL * KW; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_amdgcn_ldexpf(x[i][key_order<FMT>(e)] * sign, up);
-        const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
-        if (PAIR) {
-          q[rb][0][i][e] = n >= 8 ? lo : hi;
-        } else {
-          q[rb][0][i][e] = hi;
-          q[rb][TERMS - 1][i][e] = lo;
-        }
-      }
-  }
-
-  // ---- what a block's rows are read into
-  uint32_t kr[2 * U][KL][KW];
-  uint32_t kg[U][KL];
-  uint32_t vr[U][8][VW];
-  uint2_t vg[U];
-  const uint32_t k_lane = (uint32_t)(2 * n) * row_bytes + (KW == 4 ? 16 : 8) * g;
-  const uint32_t v_lane = (uint32_t)(8 * g) * row_bytes + (uint32_t)(n * DPL / 2);
-  const size_t k_gain_lane = (size_t)(KW == 4 ? g : g / 2) * a.room + 2 * n;
-  const size_t v_gain_lane = (size_t)(n * DPL / kCache4Group) * a.room + 8 * g;
-  auto rows_at = [&](const uint8_t *codes, int slot0) {
-    return uniform_rows(codes + (size_t)slot0 * row_bytes + head_bytes);
-  };
+  uint32_t kr[T][KL][KW], kg[T][KL], vr[UB][8];
+  uint2_t vg[UB];
+  const uint32_t k_lane = (uint32_t)n * row_bytes + (KW == 4 ? 16 : 8) * g;
+  const uint32_t v_lane = (uint32_t)(8 * g) * row_bytes + (uint32_t)((vd * DB + n * DPL) / 2);
+  const size_t k_gain_lane = (size_t)(KW == 4 ? g : g / 2) * a.room + n;
+  const size_t v_gain_lane = (size_t)((vd * DB + n * DPL) / kCache4Group) * a.room + 8 * g;
   auto load_keys = [&](int i) {
     const int slot0 = blocks.at(i) * BLOCK;
-    const auto src = rows_at(a.key_code, slot0);
+    const auto src = attend4_rows(a.key_code + (size_t)slot0 * row_bytes + head_bytes);
     const bool whole = slot0 + BLOCK <= a.span;
 #pragma unroll
-    for (int t = 0; t < 2 * U; ++t) {
-      // slot 32 u + 2 n + b; past the ring's end its last row, which no row sees there
-      const int at = 32 * (t >> 1) + (t & 1);
-      const uint32_t off = whole ? k_lane
-                                 : (uint32_t)min(at + 2 * n, a.span - 1 - slot0) * row_bytes + (KW == 4 ? 16 : 8) * g;
+    for (int j = 0; j < T; ++j) {
+      const int at = 16 * (T * wave + j);
+      const uint32_t off = whole ? k_lane : row_at(min(at + n, a.span - 1 - slot0), row_bytes) + (KW == 4 ? 16 : 8) * g;
       const uint32_t base = whole ? (uint32_t)at * row_bytes : 0u;
 #pragma unroll
       for (int c = 0; c < KL; ++c) {
         if constexpr (KW == 4) {
           const uint4_t w = __builtin_amdgcn_raw_buffer_load_b128(src, off + 64 * c, base, 0);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) kr[t][c][s] = w[s];
+          for (int s = 0; s < 4; ++s) kr[j][c][s] = w[s];
         } else {
           const uint2_t w = __builtin_amdgcn_raw_buffer_load_b64(src, off, base, 0);
-          kr[t][c][0] = w[0];
-          kr[t][c][1] = w[1];
+          kr[j][c][0] = w[0];
+          kr[j][c][1] = w[1];
         }
       }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
+      // gain rows end on a block: past the ring's end lies their padding
 #pragma unroll
       for (int c = 0; c < KL; ++c)
-        kg[u][c] = *reinterpret_cast<const uint16_t *>(a.key_gain + (gain_row + 4 * c) * a.room + slot0 + 32 * u + k_gain_lane);
+        kg[j][c] = a.key_gain[(gain_row + 4 * c) * a.room + min(slot0 + at, (int)a.room - 16) + k_gain_lane];
+    }
   };
   auto load_values = [&](int i) {
     const int slot0 = blocks.at(i) * BLOCK;
-    const auto src = rows_at(a.value_code, slot0);
+    const auto src = attend4_rows(a.value_code + (size_t)slot0 * row_bytes + head_bytes);
     const bool whole = slot0 + BLOCK <= a.span;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < UB; ++u) {
+      const int at = 32 * (UB * vs + u);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int at = 32 * u + e;
         const uint32_t off = whole ? v_lane
-                                   : (uint32_t)min(at + 8 * g, a.span - 1 - slot0) * row_bytes + (uint32_t)(n * DPL / 2);
-        const uint32_t base = whole ? (uint32_t)at * row_bytes : 0u;
-        if constexpr (DPL == 4) {
-          vr[u][e][0] = __builtin_amdgcn_raw_buffer_load_b16(src, off, base, 0);
-        } else if constexpr (DPL == 8) {
-          vr[u][e][0] = __builtin_amdgcn_raw_buffer_load_b32(src, off, base, 0);
-        } else if constexpr (DPL == 16) {
-          const uint2_t w = __builtin_amdgcn_raw_buffer_load_b64(src, off, base, 0);
-          vr[u][e][0] = w[0];
-          vr[u][e][VW - 1] = w[1];
-        } else {
-          const uint4_t w = __builtin_amdgcn_raw_buffer_load_b128(src, off, base, 0);
-#pragma unroll
-          for (int s = 0; s < VW; ++s) vr[u][e][s] = w[s];
-        }
+                                   : row_at(min(at + 8 * g + e, a.span - 1 - slot0), row_bytes) +
+                                         (uint32_t)((vd * DB + n * DPL) / 2);
+        const uint32_t base = whole ? (uint32_t)(at + e) * row_bytes : 0u;
+        if constexpr (DPL == 4)
+          vr[u][e] = __builtin_amdgcn_raw_buffer_load_b16(src, off, base, 0);
+        else
+          vr[u][e] = __builtin_amdgcn_raw_buffer_load_b32(src, off, base, 0);
       }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      vg[u] = *reinterpret_cast<const uint2_t *>(a.value_gain + gain_row * a.room + slot0 + 32 * u + v_gain_lane);
+      vg[u] = *reinterpret_cast<const uint2_t *>(a.value_gain + gain_row * a.room + min(slot0 + at, (int)a.room - 32) +
+                                                 v_gain_lane);
+    }
   };
+
+  // ---- the rows' queries to LDS; PAIR: a row's second term in column n + 8
+  QueryLoad<HEAD, FMT, ROWS, 256> queries;
+  queries.load(a, kv, row0, row_last, tid);
+  if (first < end) {
+    load_keys(first);
+    load_values(first);
+  }
+  queries.store(a, tid, qs, (PAIR ? 8 : 16) * QP, factors);
+  attend4_barrier();
+  int place[RB];
+  float factor[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int row = 16 * rb + (PAIR ? n & 7 : n);
+    place[rb] = a.place + attend4_lane(min(row0 + row, row_last), a);
+    factor[rb] = factors[row];
+  }
+  auto query_at = [&](int rb, int m, int i) {  // key step i = KW c + w
+    const int d = KW == 4 ? 32 * (4 * (i / 4) + g) + 8 * (i % 4) : 16 * g + 8 * i;
+    return *reinterpret_cast<const half8_t *>(qs + (size_t)((rb * TERMS + m) * 16 + n) * QP + d);
+  };
+  constexpr bool KEEP = KL * KW * TERMS * RB <= 16;  // in registers through the loop
+  half8_t q[RB][TERMS][KL * KW];
+  if (KEEP) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int m = 0; m < TERMS; ++m)
+#pragma unroll
+        for (int i = 0; i < KL * KW; ++i) q[rb][m][i] = query_at(rb, m, i);
+  }
 
   float4_t out[RB][DPL];
   float base[RB], top_base[RB], total[RB];
@@ -377,113 +537,72 @@ __global__ __launch_bounds__(64 * DW * PS) void attend4_kernel(Attend4Args a) {
 #pragma unroll
     for (int j = 0; j < DPL; ++j) out[rb][j] = float4_t{0, 0, 0, 0};
   }
-  // waves that split dims walk the same blocks: they meet at each one's scores
-  if (first < end) {
-    load_keys(first);
-    load_values(first);
-  }
-  int turn = 0;
-  const int steps = DW > 1 && PS > 1 ? (end - (first - ps) + PS - 1) / PS : 0;  // of the workgroup's slowest wave
-  for (int i = first, step = 0; DW > 1 && PS > 1 ? step < steps : i < end; i += PS, ++step) {
-    const bool live = !(DW > 1 && PS > 1) || i < end;  // uniform; a wave past its blocks only meets the others
-    float4_t s[RB][2 * U];
-    if (live) {
+  for (int i = first; i < end; ++i) {
+    float4_t s[RB][T];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int t = 0; t < 2 * U; ++t) s[rb][t] = float4_t{0, 0, 0, 0};
+      for (int j = 0; j < T; ++j) s[rb][j] = float4_t{0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < KL; ++c)
+    for (int c = 0; c < KL; ++c) {
+      half2_t gain[T], off[T];
 #pragma unroll
-        for (int t = 0; t < 2 * U; ++t) {
-          const uint32_t two = kg[t >> 1][c];
-          const half2_t pair = gain_pair((two & 0xFFu) | ((two & 0xFF00u) << 8));
-          const half2_t gain = t & 1 ? half_high(pair) : half_low(pair), off = gain_offset(gain);
+      for (int j = 0; j < T; ++j) {
+        gain[j] = half_low(gain_pair(kg[j][c]));
+        off[j] = gain_offset(gain[j]);
+      }
 #pragma unroll
-          for (int w = 0; w < KW; ++w) {
-            const half8_t k = key_operand<FMT>(kr[t][c][w], gain, off, exp16);
+      for (int w = 0; w < KW; ++w) {
+        half8_t k[T];
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-              for (int m = TERMS - 1; m >= 0; --m)
-                s[rb][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rb][m][KW * c + w], s[rb][t], 0, 0, 0);
-          }
-        }
-      if (i + PS < end) load_keys(i + PS);
-    }
-    if constexpr (DW > 1) {
-      // the waves' partial scores, each in its own factor, summed in wave order
-      float4_t *room = reinterpret_cast<float4_t *>(lds4) + (size_t)turn * (PS * DW * 2 * U * RB * 64);
-      if (live) {
+        for (int j = 0; j < T; ++j) k[j] = key_operand<FMT>(kr[j][c][w], gain[j], off[j], exp16);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-          for (int t = 0; t < 2 * U; ++t) {
+          for (int m = TERMS - 1; m >= 0; --m) {
+            const half8_t op = KEEP ? q[rb][m][KW * c + w] : query_at(rb, m, KW * c + w);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[rb][t][r] *= factor[rb];
-            room[((wave * RB + rb) * 2 * U + t) * 64 + lane] = s[rb][t];
+            for (int j = 0; j < T; ++j) s[rb][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], op, s[rb][j], 0, 0, 0);
           }
       }
-      lds_barrier();
-      if (live) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-          for (int t = 0; t < 2 * U; ++t) {
-            float4_t sum = room[(((ps * DW) * RB + rb) * 2 * U + t) * 64 + lane];
-#pragma unroll
-            for (int w = 1; w < DW; ++w) sum += room[(((ps * DW + w) * RB + rb) * 2 * U + t) * 64 + lane];
-            s[rb][t] = sum;
-          }
-      }
-      turn ^= 1;
     }
-    if (!live) continue;
+    if (i + 1 < end) load_keys(i + 1);
 
-    // ---- the rows' peaks and weights
+    // ---- the block's peaks
     const int slot0 = blocks.at(i) * BLOCK;
-    const int place0 = attend4_place(slot0, a);
-    const bool all = slot0 >= a.sinks && slot0 + BLOCK <= a.span && place0 <= place_low - (BLOCK - 1) &&
-                     attend4_place(slot0 + BLOCK - 1, a) == place0 + BLOCK - 1 &&
-                     (a.window == 0 || place0 > place_high - a.window);  // uniform: every row sees every slot
-    half8_t p[RB][TERMS][U];
+    const bool all = attend4_all(slot0, BLOCK, place_low, place_high, a);  // uniform
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const float f = DW > 1 ? 1.0f : factor[rb];
       if (PAIR) {
 #pragma unroll
-        for (int t = 0; t < 2 * U; ++t)
+        for (int j = 0; j < T; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[rb][t][r] += dpp_move<0x128>(s[rb][t][r]);  // row n and n + 8
+          for (int r = 0; r < 4; ++r) s[rb][j][r] += dpp_move<0x128>(s[rb][j][r]);  // row n and n + 8
       }
-      uint32_t seen = 0xFFFFFFFFu;
       if (!all) {
-        seen = 0;
 #pragma unroll
-        for (int t = 0; t < 2 * U; ++t)
+        for (int j = 0; j < T; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int at = attend4_place(slot0 + 32 * (t >> 1) + 8 * g + 2 * r + (t & 1), a);
-            if (at <= place[rb] && (a.window == 0 || at > place[rb] - a.window || at < a.sinks)) seen |= 1u << (4 * t + r);
-          }
+          for (int r = 0; r < 4; ++r)
+            if (!attend4_seen(slot0 + 16 * (T * wave + j) + 4 * g + r, place[rb], a)) s[rb][j][r] = -INFINITY;
       }
       float peak = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < 2 * U; ++t)
+      for (int j = 0; j < T; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (all)
-            peak = fmaxf(peak, s[rb][t][r]);
-          else
-            peak = fmaxf(peak, seen >> (4 * t + r) & 1u ? s[rb][t][r] : -INFINITY);
+        for (int r = 0; r < 4; ++r) peak = fmaxf(peak, s[rb][j][r]);
       peak = xmax48(peak);
-      if (peak != -INFINITY) peak *= f;
-      const float low = floorf(peak);
-      float m = base[rb];
-      if (low != -INFINITY && !(low >= m + 8.0f && low <= m + 14.0f)) {
-        top_base[rb] = fmaxf(top_base[rb], low - 12.0f);
-        m = fmaxf(low - 12.0f, top_base[rb] - 58.0f);
-      }
+      if (g == 0) peaks[wave * 16 * RB + 16 * rb + n] = peak;
+    }
+    attend4_barrier();
+    // ---- the base, the same in every wave, and the weights
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      float peak = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) peak = fmaxf(peak, peaks[w * 16 * RB + 16 * rb + n]);
+      const float f = factor[rb];
+      const float m = attend4_base(peak, f, base[rb], top_base[rb]);
       if (__builtin_amdgcn_ballot_w64(m != base[rb])) {
         const float keep = base[rb] != -INFINITY ? __builtin_amdgcn_exp2f(base[rb] - m) : 0.0f;
         total[rb] *= keep;
@@ -493,183 +612,446 @@ __global__ __launch_bounds__(64 * DW * PS) void attend4_kernel(Attend4Args a) {
           for (int r = 0; r < 4; ++r) out[rb][j][r] *= keep;
         base[rb] = m;
       }
+      const float from = attend4_from(m);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int j = 0; j < T; ++j) {
+        half2_t hi[2], lo[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          half2_t hi, lo;
-          float w[2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int t = 2 * u + b;
-            w[b] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][t][r], f, -m));
-            if (!all) w[b] = seen >> (4 * t + r) & 1u ? w[b] : 0.0f;
-            total[rb] += w[b];
-            hi[b] = (_Float16)w[b];
-            lo[b] = (_Float16)(w[b] - (float)hi[b]);
-          }
-          if (PAIR) {
-            const half2_t mine = n >= 8 ? lo : hi;
-            p[rb][0][u][2 * r] = mine[0];
-            p[rb][0][u][2 * r + 1] = mine[1];
-          } else {
-            p[rb][0][u][2 * r] = hi[0];
-            p[rb][0][u][2 * r + 1] = hi[1];
-            p[rb][TERMS - 1][u][2 * r] = lo[0];
-            p[rb][TERMS - 1][u][2 * r + 1] = lo[1];
-          }
+        for (int r = 0; r < 4; r += 2) {
+          const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][j][r], f, from));
+          const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][j][r + 1], f, from));
+          total[rb] += w0 + w1;
+          two_terms(w0, w1, hi[r / 2], lo[r / 2]);
+          if (PAIR && n >= 8) hi[r / 2] = lo[r / 2];
         }
+        _Float16 *to = ws + (size_t)(rb * TERMS * 16 + n) * PP + 16 * (T * wave + j) + 4 * g;
+        __builtin_memcpy(__builtin_assume_aligned(to, 8), hi, sizeof(hi));
+        if (!PAIR) __builtin_memcpy(__builtin_assume_aligned(to + 16 * PP, 8), lo, sizeof(lo));
+      }
     }
-
-    // ---- the blend
+    attend4_barrier();
+    // ---- the blend of the wave's dims over its slots
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < UB; ++u) {
+      half8_t p[RB][TERMS];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int m = 0; m < TERMS; ++m)
+          p[rb][m] = *reinterpret_cast<const half8_t *>(ws + (size_t)((rb * TERMS + m) * 16 + n) * PP +
+                                                        32 * (UB * vs + u) + 8 * g);
       half2_t gain[4], off[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         gain[k] = gain_pair(__builtin_amdgcn_perm(0u, vg[u][k >> 1], k & 1 ? 0x0C030C02u : 0x0C010C00u));
         off[k] = gain_offset(gain[k]);
       }
+      half8_t op[DPL];
+      value_operands<FMT, DPL>(vr[u], gain, off, exp16, op);
 #pragma unroll
-      for (int v = 0; v < VW; ++v) {
-        uint32_t x[8];
+      for (int m = TERMS - 1; m >= 0; --m)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = vr[u][e][v];
-        half8_t op[VD];
-        value_operands<FMT, VD>(x, gain, off, exp16, op);
+        for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int d = 0; d < VD; ++d)
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-            for (int t = TERMS - 1; t >= 0; --t)
-              out[rb][VD * v + d] =
-                  __builtin_amdgcn_mfma_f32_16x16x32_f16(op[d], p[rb][t][u], out[rb][VD * v + d], 0, 0, 0);
-      }
+          for (int d = 0; d < DPL; ++d)
+            out[rb][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[d], p[rb][m], out[rb][d], 0, 0, 0);
     }
-    if (i + PS < end) load_values(i + PS);
-  }
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) total[rb] = xsum48(total[rb]);
-
-  // ---- waves that took different blocks: halves of them fold into the others
-  if constexpr (PS > 1) {
-    constexpr int SIZE = DPL * RB * 64 + RB * 32;  // float4 of a wave's blend, then its bases and totals
-#pragma unroll
-    for (int half = PS / 2; half > 0; half >>= 1) {
-      __syncthreads();
-      float4_t *room = reinterpret_cast<float4_t *>(lds4) + (size_t)((ps % half) * DW + dw) * SIZE;
-      float *stats = reinterpret_cast<float *>(room + DPL * RB * 64);
-      if (ps >= half && ps < 2 * half) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-#pragma unroll
-          for (int j = 0; j < DPL; ++j) room[(rb * DPL + j) * 64 + lane] = out[rb][j];
-          stats[128 * rb + lane] = base[rb];
-          stats[128 * rb + 64 + lane] = total[rb];
-        }
-      }
-      __syncthreads();
-      if (ps < half) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          const float theirs = stats[128 * rb + lane];
-          const float m = fmaxf(base[rb], theirs);
-          const float mine = base[rb] != -INFINITY ? __builtin_amdgcn_exp2f(base[rb] - m) : 0.0f;
-          const float part = theirs != -INFINITY ? __builtin_amdgcn_exp2f(theirs - m) : 0.0f;
-          base[rb] = m;
-          total[rb] = total[rb] * mine + stats[128 * rb + 64 + lane] * part;
-#pragma unroll
-          for (int j = 0; j < DPL; ++j) {
-            const float4_t o = room[(rb * DPL + j) * 64 + lane];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) out[rb][j][r] = out[rb][j][r] * mine + o[r] * part;
-          }
-        }
-      }
-    }
-    if (ps > 0) return;
+    if (i + 1 < end) load_values(i + 1);
   }
 
-  // ---- the rows' blends, or this segment's share of them: dims (4 g + r) DPL + j
+  // ---- the waves' totals and, of waves that took other slots, blends
+  attend4_barrier();
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    if (PAIR) {
+    total[rb] = xsum48(total[rb]);
+    if (g == 0) peaks[wave * 16 * RB + 16 * rb + n] = total[rb];
+  }
+  attend4_barrier();
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    total[rb] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) total[rb] += peaks[w * 16 * RB + 16 * rb + n];
+  }
+  if constexpr (VS > 1) {
+    attend4_barrier();
+    float4_t *room = reinterpret_cast<float4_t *>(lds) + lane;
+    if (vs > 0) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) room[((((vs - 1) * VD + vd) * RB + rb) * DPL + j) * 64] = out[rb][j];
+    }
+    attend4_barrier();
+    if (vs > 0) return;
+#pragma unroll
+    for (int w = 1; w < VS; ++w)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) out[rb][j] += room[((((w - 1) * VD + vd) * RB + rb) * DPL + j) * 64];
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+    attend4_store<HEAD, DPL, PAIR>(a, out[rb], base[rb], total[rb], row0 + 16 * rb + (PAIR ? n & 7 : n), row_last, seg, kv,
+                                   vd * DB, vd == 0, g, n);
+}
+
+// ---- many rows ----------------------------------------------------------------
+
+// Prompts.  A workgroup takes RT tiles of 16 rows through blocks of slots.  Two
+// waves share a tile's products: of 512-dim heads each takes half the dims (their
+// partial scores meet in LDS), of others half the block's slots (their blends meet
+// in LDS at the end).  Transposed, scores stay where the blend wants them: lane
+// 16 g + n of S^T (slots x rows) holds row n's slots 4 g + r of 16-slot tile b, and
+// of P^T, with slot 16 b + 4 g + r as element 4 b + r of lane group g's eight, the
+// same.
+//
+// A wave decodes its keys as it multiplies them: they lie as their operand wants
+// them, 16 bytes of a slot a lane.  Values lie across theirs, so the waves decode a
+// block's together into LDS, a block ahead, while they multiply the one before: a
+// dim's 32 slots are four 16-byte pieces, one a lane group; dim 8 d + i is row
+// i HEAD / 8 + d, its piece for g at g xor the row's bits 1 and 2, so that the eight
+// lanes that one cycle writes or reads lie in distinct banks with no padding.
+template <int HEAD, int RT>
+struct Tile4Shape {
+  static constexpr int DW = HEAD == 512 ? 2 : 1, SH = 2 / DW;
+  static constexpr int WAVES = 2 * RT, THREADS = 64 * WAVES;
+  static constexpr int BLOCK = HEAD == 512 ? 32 : 64;
+  static constexpr int DH = HEAD / DW;                     // dims a wave multiplies
+  static constexpr int KL = DH >= 128 ? DH / 128 : 1;      // key chunks of a slot a lane reads
+  static constexpr int KW = DH >= 128 ? 4 : 2;             // dwords of a chunk
+  static constexpr int DPL = DH / 16;                      // its tiles of 16 dims of the blend
+  static constexpr int VITEMS = BLOCK / 32 * 4 * HEAD / 8; // (lane group, 8 dims) of the block's 32s of slots
+  static constexpr int NV = (VITEMS + THREADS - 1) / THREADS;
+  static constexpr int V = BLOCK * HEAD * 2;               // bytes of a block's values; two of them
+  static constexpr int X = 2 * V;                          // partial scores: [WAVES][2][64] float4
+  static constexpr int LOOP = X + (DW > 1 ? WAVES * 2048 : 0);
+  static constexpr int QUERY = 2 * 16 * RT * (HEAD + 8) * 2;     // [2][16 RT][HEAD + 8] halves, before the loop
+  static constexpr int ROWS = SH * 16 * RT * HEAD * 4;           // [SH][16 RT][HEAD] floats, after it
+  static constexpr int STATS = LOOP > QUERY ? (LOOP > ROWS ? LOOP : ROWS) : (QUERY > ROWS ? QUERY : ROWS);
+  static constexpr int LDS = STATS + WAVES * 32 * 4;
+};
+
+template <int HEAD, int FMT, int RT>
+__global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a) {
+  using F = Tile4Shape<HEAD, RT>;
+  constexpr int DW = F::DW, SH = F::SH, THREADS = F::THREADS, BLOCK = F::BLOCK, DH = F::DH, KL = F::KL, KW = F::KW;
+  constexpr int KS = KL * KW, DPL = F::DPL, NV = F::NV;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds4[];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rt = wave >> 1, dw = DW > 1 ? wave & 1 : 0, sh = SH > 1 ? wave & 1 : 0;
+  const int g = lane >> 4, n = lane & 15;
+  const int kv = blockIdx.z, seg = blockIdx.y;
+  // a prompt's longest tiles first; where all run at once, two a CU, the second
+  // half starts with the shortest, so that a long one meets a short one
+  const int tiles = gridDim.x, half = tiles * (int)(gridDim.y * gridDim.z) <= 512 ? (tiles + 1) / 2 : tiles;
+  const int tile = (int)blockIdx.x < half ? tiles - 1 - (int)blockIdx.x : (int)blockIdx.x - half;
+  const int row0 = tile * 16 * RT;
+  const int row_last = min(row0 + 16 * RT, a.rows) - 1;
+  const int place_low = a.place + attend4_lane(row0, a), place_high = a.place + attend4_lane(row_last, a);
+  const Blocks4 blocks = attend4_blocks(BLOCK, place_low, place_high, a);
+  const int first = min(blocks.count, seg * a.per);
+  const int end = seg == a.segments - 1 ? blocks.count : min(blocks.count, first + a.per);
+  const uint32_t exp16 = 0x4C004C00u;
+  const uint32_t row_bytes = (uint32_t)a.kv_width / 2;
+  const size_t head_bytes = (size_t)kv * HEAD / 2;
+  const size_t gain_row = (size_t)kv * HEAD / kCache4Group;
+
+  uint32_t kr[2][KL][KW], kg[2][KL], vr[NV][8], vg[NV][2];
+  auto load_keys = [&](int i) {
+    const int slot0 = blocks.at(i) * BLOCK;
+    const int left = a.span - 1 - slot0;  // the ring's last slot, which rows past it are read from
+    const auto src = attend4_rows(a.key_code + (size_t)slot0 * row_bytes + head_bytes + dw * (DH / 2));
+    const uint8_t *gains = a.key_gain + (gain_row + dw * (DH / kCache4Group) + (KW == 4 ? g : g / 2)) * a.room + slot0;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int slot = 32 * sh + 16 * b + n;
+      const uint32_t off = row_at(min(slot, left), row_bytes) + (KW == 4 ? 16 : 8) * g;
+#pragma unroll
+      for (int c = 0; c < KL; ++c) {
+        if constexpr (KW == 4) {
+          const uint4_t w = __builtin_amdgcn_raw_buffer_load_b128(src, off + 64 * c, 0, 0);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) kr[b][c][s] = w[s];
+        } else {
+          const uint2_t w = __builtin_amdgcn_raw_buffer_load_b64(src, off, 0, 0);
+          kr[b][c][0] = w[0];
+          kr[b][c][1] = w[1];
+        }
+        kg[b][c] = gains[(size_t)(4 * c) * a.room + slot];
+      }
+    }
+  };
+  auto load_values = [&](int i) {
+    const int slot0 = blocks.at(i) * BLOCK;
+    const int left = a.span - 1 - slot0;
+    const auto src = attend4_rows(a.value_code + (size_t)slot0 * row_bytes + head_bytes);
+    const uint8_t *gains = a.value_gain + gain_row * a.room + slot0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int item = F::VITEMS % THREADS ? min(tid + THREADS * j, F::VITEMS - 1) : tid + THREADS * j;
+      const int d = item % (HEAD / 8), at = 32 * (item / (HEAD / 2)) + 4 * (item / (HEAD / 8) % 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int slot = at + 16 * (e >> 2) + (e & 3);
+        vr[j][e] = __builtin_amdgcn_raw_buffer_load_b32(src, row_at(min(slot, left), row_bytes) + 4 * d, 0, 0);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        vg[j][b] = *reinterpret_cast<const uint32_t *>(gains + (size_t)(d / 4) * a.room + at + 16 * b);
+    }
+  };
+  auto decode_values = [&](uint8_t *room) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int item = tid + THREADS * j;
+      if (F::VITEMS % THREADS && item >= F::VITEMS) break;
+      const int d = item % (HEAD / 8), of = item / (HEAD / 8) % 4, group = item / (HEAD / 2);
+      half2_t gain[4], off[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        gain[k] = gain_pair(__builtin_amdgcn_perm(0u, vg[j][k >> 1], k & 1 ? 0x0C030C02u : 0x0C010C00u));
+        off[k] = gain_offset(gain[k]);
+      }
+      half8_t op[8];
+      value_operands<FMT, 8>(vr[j], gain, off, exp16, op);
+      half8_t *to = reinterpret_cast<half8_t *>(room) + group * (HEAD * 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = i * (HEAD / 8) + d;
+        to[row * 4 + (of ^ (row >> 1 & 3))] = op[i];
+      }
+    }
+  };
+  QueryLoad<HEAD, FMT, 16 * RT, THREADS> queries;
+  queries.load(a, kv, row0, row_last, tid);
+  if (first < end) {
+    load_values(first);
+    load_keys(first);
+  }
+
+  // ---- the rows' queries: their terms through LDS, a thread eight dims, to the
+  // waves' operands
+  half8_t q[2][KS];
+  float *stats = reinterpret_cast<float *>(lds4 + F::STATS);
+  constexpr int QP = HEAD + 8;  // pitch in halves
+  _Float16 *qs = reinterpret_cast<_Float16 *>(lds4);
+  queries.store(a, tid, qs, 16 * RT * QP, stats);
+  attend4_barrier();
+  const int row = min(row0 + 16 * rt + n, row_last);
+  const int place = a.place + attend4_lane(row, a);
+  const float factor = stats[16 * rt + n];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {  // step 4 c + s is dword s of chunk 4 c + g (heads of 64: of chunk g / 2)
+      const int d = HEAD == 64 ? 16 * g + 8 * k : DH * dw + 32 * (4 * (k / 4) + g) + 8 * (k % 4);
+      q[m][k] = *reinterpret_cast<const half8_t *>(qs + m * (16 * RT * QP) + (16 * rt + n) * QP + d);
+    }
+  attend4_barrier();
+
+  float4_t out[DPL];
+  float base = -INFINITY, top_base = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (int j = 0; j < DPL; ++j) out[j] = float4_t{0, 0, 0, 0};
+  uint8_t *now = lds4, *next = lds4 + F::V;
+  if (first < end) {
+    decode_values(now);
+    load_values(min(first + 1, end - 1));
+    attend4_barrier();
+  }
+  for (int i = first; i < end; ++i) {
+    // ---- scores
+    float4_t s[2] = {float4_t{0, 0, 0, 0}, float4_t{0, 0, 0, 0}}, low[2] = {s[0], s[1]};
+#pragma unroll
+    for (int c = 0; c < KL; ++c) {
+      half2_t gain[2], off[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        gain[b] = half_low(gain_pair(kg[b][c]));
+        off[b] = gain_offset(gain[b]);
+      }
+#pragma unroll
+      for (int w = 0; w < KW; ++w)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const half8_t op = key_operand<FMT>(kr[b][c][w], gain[b], off[b], exp16);
+          low[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, q[1][KW * c + w], low[b], 0, 0, 0);
+          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, q[0][KW * c + w], s[b], 0, 0, 0);
+        }
+    }
+    load_keys(min(i + 1, end - 1));
+    s[0] += low[0];
+    s[1] += low[1];
+    if constexpr (DW > 1) {
+      float4_t *room = reinterpret_cast<float4_t *>(lds4 + F::X);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) room[(wave * 2 + b) * 64 + lane] = s[b];
+      attend4_barrier();
+#pragma unroll
+      for (int b = 0; b < 2; ++b) s[b] = room[((wave & ~1) * 2 + b) * 64 + lane] + room[((wave | 1) * 2 + b) * 64 + lane];
+    }
+    // ---- the rows' weights
+    const int slot0 = blocks.at(i) * BLOCK + 32 * sh;
+    const bool all = attend4_all(slot0, 32, place_low, place_high, a);  // uniform
+    if (!all) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!attend4_seen(slot0 + 16 * b + 4 * g + r, place, a)) s[b][r] = -INFINITY;
+    }
+    float peak = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) peak = fmaxf(peak, s[b][r]);
+    peak = xmax48(peak);
+    const float m = attend4_base(peak, factor, base, top_base);
+    if (__builtin_amdgcn_ballot_w64(m != base)) {
+      const float keep = base != -INFINITY ? __builtin_amdgcn_exp2f(base - m) : 0.0f;
+      total *= keep;
 #pragma unroll
       for (int j = 0; j < DPL; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) out[rb][j][r] += dpp_move<0x128>(out[rb][j][r]);
+        for (int r = 0; r < 4; ++r) out[j][r] *= keep;
+      base = m;
     }
-    const int row = row0 + 16 * rb + (PAIR ? n & 7 : n);
-    if (row > row_last) continue;
-    const bool split = a.segments > 1;
-    const int l = row / a.share;
-    float *dst = a.out + (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * HEAD;
-    float mul = a.value_scale;
-    bool vec = (((uintptr_t)a.out | ((size_t)a.lane_stride * 4)) & 15u) == 0;
-    if (split) {
-      const size_t at = ((size_t)seg * gridDim.z + kv) * a.rows + row;
-      dst = a.part_out + at * HEAD;
-      vec = true;
-      if (g == 0 && dw == 0 && (!PAIR || n < 8)) {
-        a.part_base[at] = base[rb];
-        a.part_total[at] = total[rb];
-      }
-    } else {
-      mul *= 1.0f / total[rb];
-    }
-    dst += dw * DH;
-    // PAIR: both halves of the columns hold the sums; each writes half of them
+    half8_t p[2];
+    {
+      half2_t hi[4], lo[4];
+      const float from = attend4_from(m);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (PAIR && (r >= 2) != (n >= 8)) continue;
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int j = 0; j < DPL; j += 4) {
-        float *to = dst + (4 * g + r) * DPL + j;
-        const float4_t o = {out[rb][j][r] * mul, out[rb][j + 1][r] * mul, out[rb][j + 2][r] * mul, out[rb][j + 3][r] * mul};
-        if (vec) {
-          *reinterpret_cast<float4_t *>(to) = o;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) to[e] = o[e];
+        for (int r = 0; r < 4; r += 2) {
+          const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], factor, from));
+          const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r + 1], factor, from));
+          total += w0 + w1;
+          two_terms(w0, w1, hi[2 * b + r / 2], lo[2 * b + r / 2]);
         }
-      }
+      p[0] = __builtin_bit_cast(half8_t, hi);
+      p[1] = __builtin_bit_cast(half8_t, lo);
     }
+    // ---- the blend: tile j is rows (j / TC) HEAD / 8 + 16 (j % TC) + .. of the wave's;
+    // and the next block's values
+    const half8_t *values = reinterpret_cast<const half8_t *>(now) + sh * (HEAD * 4);
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) {
+      constexpr int TC = DH >= 128 ? DH / 128 : 1;
+      const int at = DH >= 128 ? (j / TC) * (HEAD / 8) + dw * (DH / 8) + 16 * (j % TC) + n : 16 * j + n;
+      const half8_t op = values[at * 4 + (g ^ (at >> 1 & 3))];
+#pragma unroll
+      for (int k = 1; k >= 0; --k) out[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, p[k], out[j], 0, 0, 0);
+    }
+    decode_values(next);
+    load_values(min(i + 2, end - 1));
+    uint8_t *const was = now;
+    now = next;
+    next = was;
+    attend4_barrier();
+  }
+  total = xsum48(total);
+
+  // ---- blends through LDS, which the waves' halves of the slots meet in, to whole
+  // rows: 16-byte piece p of row r at p ^ r % 8
+  if (g == 0) {
+    stats[wave * 32 + n] = base;
+    stats[wave * 32 + 16 + n] = total;
+  }
+  attend4_barrier();
+  float mul = a.value_scale;
+  if constexpr (SH > 1) {
+    const float theirs = stats[(wave ^ 1) * 32 + n], m = fmaxf(base, theirs);
+    const float mine = base != -INFINITY ? __builtin_amdgcn_exp2f(base - m) : 0.0f;
+    const float part = theirs != -INFINITY ? __builtin_amdgcn_exp2f(theirs - m) : 0.0f;
+    base = m;
+    total = total * mine + stats[(wave ^ 1) * 32 + 16 + n] * part;
+    mul *= mine;
+  }
+  const bool split = a.segments > 1;
+  if (!split) mul *= 1.0f / total;
+  float *rows = reinterpret_cast<float *>(lds4) + sh * (16 * RT * HEAD) + (16 * rt + n) * HEAD;
+  if constexpr (DH >= 128) {
+    constexpr int TC = DH / 128;
+#pragma unroll
+    for (int t = 0; t < TC; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {  // the tiles t, t + TC, .. are its dims
+          const int piece = dw * (DH / 4) + 2 * (16 * t + 4 * g + r) + h / 4;
+          *reinterpret_cast<float4_t *>(rows + 4 * (piece ^ (n & 7))) =
+              float4_t{out[TC * h + t][r] * mul, out[TC * (h + 1) + t][r] * mul, out[TC * (h + 2) + t][r] * mul,
+                       out[TC * (h + 3) + t][r] * mul};
+        }
+  } else {
+#pragma unroll
+    for (int j = 0; j < DPL; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = 16 * j + 4 * g + r, d = 8 * (at % 8) + at / 8;
+        rows[4 * ((d / 4) ^ (n & 7)) + d % 4] = out[j][r] * mul;
+      }
+  }
+  attend4_barrier();
+  const int count = row_last - row0 + 1;
+  const bool vec = split || (((uintptr_t)a.out | ((size_t)a.lane_stride * 4)) & 15u) == 0;
+  const size_t part0 = ((size_t)seg * gridDim.z + kv) * a.rows + row0;
+  for (int i = tid; i < count * (HEAD / 4); i += THREADS) {
+    const int r = i / (HEAD / 4), piece = i % (HEAD / 4);
+    const float *from = reinterpret_cast<const float *>(lds4) + r * HEAD + 4 * (piece ^ (r & 7));
+    float4_t o = *reinterpret_cast<const float4_t *>(from);
+    if (SH > 1) o += *reinterpret_cast<const float4_t *>(from + 16 * RT * HEAD);
+    float *to = (split ? a.part_out + (part0 + r) * HEAD : a.out + attend4_row(row0 + r, kv, HEAD, a)) + 4 * piece;
+    if (vec) {
+      *reinterpret_cast<float4_t *>(to) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e] = o[e];
+    }
+  }
+  if (split && g == 0 && dw == 0 && sh == 0 && 16 * rt + n < count) {
+    a.part_base[part0 + 16 * rt + n] = base;
+    a.part_total[part0 + 16 * rt + n] = total;
   }
 }
 
 // Folds the segments of a row: a workgroup a row and DIMS of its dims, thread
-// (c, s) of four dims c and the segments s, s + SL, ...  Every segment's base
-// and total go through LDS as its weight and weighted total.
+// (c, s) of four dims c and the segments s, s + SL, ...  Thread t finds segment
+// t's weight; the blends are requested before.
 template <int DIMS>
 __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int head_size) {
   constexpr int COLS = DIMS / 4, SL = 256 / COLS;
-  __shared__ float weight[kAttend4Segments];
-  __shared__ float share[kAttend4Segments];
+  constexpr int AHEAD = 4;
+  __shared__ float weight[kAttend4Segments], red[8];
   __shared__ float4_t part[SL][COLS];
   const int tid = threadIdx.x, c = tid % COLS, sl = tid / COLS;
+  const int wave = tid >> 6;
   const int row = blockIdx.x, kv = blockIdx.y, kv_count = gridDim.y;
   const size_t step = (size_t)kv_count * a.rows, at = (size_t)kv * a.rows + row;
   const int d0 = blockIdx.z * DIMS + 4 * c;
-  constexpr int AHEAD = 4;
+  const float mine = tid < a.segments ? a.part_base[at + tid * step] : -INFINITY;
+  const float sum = tid < a.segments ? a.part_total[at + tid * step] : 0.0f;
   float4_t first[AHEAD];
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) {
     const int s = min(sl + i * SL, a.segments - 1);
     first[i] = *reinterpret_cast<const float4_t *>(a.part_out + (at + s * step) * head_size + d0);
   }
-  // base of segment tid (there are no more than 256)
-  const float mine = tid < a.segments ? a.part_base[at + tid * step] : -INFINITY;
-  const float sum = tid < a.segments ? a.part_total[at + tid * step] : 0.0f;
-  share[tid] = mine;
-  __syncthreads();
-  float m = -INFINITY;
-  for (int s = 0; s < a.segments; ++s) m = fmaxf(m, share[s]);
+  const float top = group_max<64>(mine);
+  if ((tid & 63) == 0) red[wave] = top;
+  attend4_barrier();
+  const float m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float w = mine != -INFINITY ? __builtin_amdgcn_exp2f(mine - m) : 0.0f;
-  __syncthreads();
   weight[tid] = w;
-  share[tid] = w * sum;
-  __syncthreads();
+  const float part_total = wave_sum_to_last(w * sum);
+  if ((tid & 63) == 63) red[4 + wave] = part_total;
+  attend4_barrier();
   float4_t acc = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) {
@@ -679,14 +1061,19 @@ __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int he
   for (int s = sl + AHEAD * SL; s < a.segments; s += SL)
     acc += *reinterpret_cast<const float4_t *>(a.part_out + (at + s * step) * head_size + d0) * weight[s];
   part[sl][c] = acc;
-  __syncthreads();
+  // the slices by halves, in the same order every time
+#pragma unroll
+  for (int half = SL / 2; half > 0; half >>= 1) {
+    attend4_barrier();
+    if (sl < half) {
+      acc += part[sl + half][c];
+      part[sl][c] = acc;
+    }
+  }
   if (sl) return;
-  float total = 0.0f;
-  for (int s = 0; s < a.segments; ++s) total += share[s];
-  for (int s = 1; s < SL; ++s) acc += part[s][c];
-  const int l = row / a.share;
+  const float mul = 1.0f / (red[4] + red[5] + red[6] + red[7]);
+  const int l = attend4_lane(row, a);
   float *to = a.out + (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * head_size + d0;
-  const float mul = 1.0f / total;
 #pragma unroll
   for (int e = 0; e < 4; ++e) to[e] = acc[e] * mul;
 }
@@ -695,53 +1082,60 @@ __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int he
 
 using namespace igl;
 
-// Which form a launch takes.
+constexpr int kTile4 = 2;  // tiles of 16 rows a workgroup of attend4_tile_kernel takes
+
+// Which form a launch takes: tiles of up to eight rows, or sixteen, on
+// attend4_step_kernel, or of 32 on attend4_tile_kernel.
 struct Attend4Plan {
-  int pair, rb, dw, ps;  // attend4_kernel's
-  int tiles, segments;
+  int step, pair, block;
+  int tiles;
 };
 
-static Attend4Plan attend4_plan(int head, int span, int sinks, int kv_count, int share, int place, int window, int lanes) {
-  Attend4Plan p = {0, 1, 1, 4, 1, 1};
-  const long long rows = (long long)lanes * share;
-  const long long tiles32 = (rows + 31) / 32;
-  if (rows <= 8) {
-    p.pair = 1;
-  } else if (tiles32 * kv_count >= 256) {
-    p.rb = 2;
-    p.ps = 1;
-    p.dw = head == 512 ? 2 : 1;
-  } else if (head == 512) {
-    p.dw = 2;
-    p.ps = 2;
+static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
+  Attend4Plan p = {1, 0, 64, 1};
+  p.pair = a.rows <= 8;
+  p.step = a.rows <= 320;
+  p.block = !p.step && head == 512 ? 32 : p.step && head < 256 ? 128 : 64;
+  const int each = !p.step ? 16 * kTile4 : p.pair ? 8 : 16;
+  p.tiles = (int)(((long long)a.rows + each - 1) / each);
+  // the most blocks of a tile: without a window the last one's, else as many as
+  // any alignment of its span and the sinks' can touch
+  int blocks = attend4_blocks(p.block, a.place, a.newest, a).count;
+  if (a.window > 0) {
+    const long long reach = (long long)a.window + (each + a.share - 2) / a.share;
+    const long long most = (reach + p.block - 2) / p.block + 1 + (a.sinks + p.block - 1) / p.block + 1;
+    if (most < blocks) blocks = (int)most;
   }
-  const int each = p.pair ? 8 : 16 * p.rb;
-  p.tiles = (int)((rows + each - 1) / each);
-  // a tile's blocks, the last one's
-  const int first = place + (int)(((long long)(p.tiles - 1) * each) / share), last = place + lanes - 1;
-  const int blocks = attend4_blocks(64, span, sinks, window, first, last).count;
-  long long s = p.ps == 1 ? 1 : 256 / ((long long)p.tiles * kv_count);
-  const long long room = (long long)IGL_ATTEND_FIXED_FLOATS / (rows * kv_count * (head + 2));
-  if (s > (blocks + p.ps - 1) / p.ps) s = (blocks + p.ps - 1) / p.ps;
+  long long s = 512 / ((long long)p.tiles * kv_count);
+  const long long room = (long long)IGL_ATTEND_FIXED_FLOATS / ((long long)a.rows * kv_count * (head + 2));
+  if (s > blocks) s = blocks;
   if (s > room) s = room;
   if (s > kAttend4Segments) s = kAttend4Segments;
   if (s < 1) s = 1;
-  p.segments = (int)s;
+  a.per = (int)((blocks + s - 1) / s);
+  a.segments = (blocks + a.per - 1) / a.per;
   return p;
 }
 
-template <int HEAD, int FMT, int RB, bool PAIR, int DW, int PS, int U>
+template <int HEAD, int FMT>
 static hipError_t attend4_launch(const Attend4Args &a, const Attend4Plan &p, int kv_count, hipStream_t stream) {
-  constexpr int size = Attend4Shape<HEAD, FMT, RB, PAIR, DW, PS, U>::LDS;
-  const void *kernel = reinterpret_cast<const void *>(&attend4_kernel<HEAD, FMT, RB, PAIR, DW, PS, U>);
-  if (size > 65536) {  // granted once a device; granting again changes nothing
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, size);
-    if (e != hipSuccess) return e;
+  constexpr int T = HEAD >= 256 ? 1 : 2;
+  const dim3 grid(p.tiles, a.segments, kv_count);
+  if (!p.step) {
+    constexpr int RT = kTile4, size = Tile4Shape<HEAD, RT>::LDS;
+    if (size > 65536) {  // granting it again changes nothing
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&attend4_tile_kernel<HEAD, FMT, RT>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, size);
+      if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((attend4_tile_kernel<HEAD, FMT, RT>), grid, dim3(128 * RT), (size_t)size, stream, a);
+  } else if (p.pair) {
+    hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, 1, true, T>), grid, dim3(256), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, 1, false, T>), grid, dim3(256), 0, stream, a);
   }
-  const dim3 grid(p.tiles, p.segments, kv_count);
-  hipLaunchKernelGGL((attend4_kernel<HEAD, FMT, RB, PAIR, DW, PS, U>), grid, dim3(64 * DW * PS), (size_t)size, stream, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.segments == 1) return e;
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.segments == 1) return e;
   const int dims = a.rows <= 64 ? 16 : 64;
   const dim3 fgrid(a.rows, kv_count, HEAD / dims);
   if (dims == 16)
@@ -751,19 +1145,11 @@ static hipError_t attend4_launch(const Attend4Args &a, const Attend4Plan &p, int
   return hipGetLastError();
 }
 
-template <int HEAD, int FMT>
-static hipError_t attend4_launch_head(const Attend4Args &a, const Attend4Plan &p, int kv_count, hipStream_t stream) {
-  constexpr int DW = HEAD == 512 ? 2 : 1;
-  if (p.pair) return attend4_launch<HEAD, FMT, 1, true, 1, 4, 2>(a, p, kv_count, stream);
-  if (p.rb == 2) return attend4_launch<HEAD, FMT, 2, false, DW, 1, 2>(a, p, kv_count, stream);
-  return attend4_launch<HEAD, FMT, 1, false, DW, 4 / DW, 2>(a, p, kv_count, stream);
-}
-
 template <int HEAD>
 static hipError_t attend4_launch_format(const Attend4Args &a, const Attend4Plan &p, int format, int kv_count,
                                         hipStream_t stream) {
-  if (format == IGL_CACHE4_INT4) return attend4_launch_head<HEAD, IGL_CACHE4_INT4>(a, p, kv_count, stream);
-  return attend4_launch_head<HEAD, IGL_CACHE4_E2M1>(a, p, kv_count, stream);
+  if (format == IGL_CACHE4_INT4) return attend4_launch<HEAD, IGL_CACHE4_INT4>(a, p, kv_count, stream);
+  return attend4_launch<HEAD, IGL_CACHE4_E2M1>(a, p, kv_count, stream);
 }
 
 extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_share, const float *query, int lane_stride,
@@ -772,8 +1158,6 @@ extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_shar
   Attend4Args a = {};
   const long long rows = (long long)lanes * group_share;
   if (rows > 0x7FFFFFFF - 64) return hipErrorInvalidValue;
-  const Attend4Plan p = attend4_plan(store->head_size, store->cache_span, store->sink_count, store->kv_count, group_share,
-                                     place_first, window, lanes);
   a.key_code = store->key_code;
   a.key_gain = store->key_gain;
   a.value_code = store->value_code;
@@ -791,14 +1175,18 @@ extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_shar
   a.newest_slot = a.newest < a.sinks ? -1 : cache4_slot(a.newest, a.sinks, a.span);
   a.window = window;
   a.rows = (int)rows;
+  // rows below 2^31: a multiplier that is less than share / 2^shift too large, 2^shift >= 2^31 share
+  a.share_shift = 31;
+  while ((1 << (a.share_shift - 31)) < group_share) ++a.share_shift;
+  a.share_mul = (uint32_t)(((1ull << a.share_shift) + group_share - 1) / group_share);
   // log2 e, and the 256 that a gain is divided by
   const double factor = (double)store->key_scale * score_scale * 1.4426950408889634 * 256.0;
   a.key_part = (float)frexp(factor, &a.key_power);
   a.value_scale = store->value_scale * 256.0f;
-  a.segments = p.segments;
+  const Attend4Plan p = attend4_plan(a, store->head_size, store->kv_count);
   a.part_out = work;
-  a.part_base = work + (size_t)p.segments * store->kv_count * rows * store->head_size;
-  a.part_total = a.part_base + (size_t)p.segments * store->kv_count * rows;
+  a.part_base = work + (size_t)a.segments * store->kv_count * rows * store->head_size;
+  a.part_total = a.part_base + (size_t)a.segments * store->kv_count * rows;
   switch (store->head_size) {
     case 64: return attend4_launch_format<64>(a, p, store->format, store->kv_count, stream);
     case 128: return attend4_launch_format<128>(a, p, store->format, store->kv_count, stream);

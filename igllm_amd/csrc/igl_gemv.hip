@@ -3413,3 +3413,6 @@ extern "C" hipError_t igl_launch_gemv_zero(const igl_code_view *v, const int8_t 
   }
   return hipSuccess;
 }
+
+// The 4-bit ring's attention: in this translation unit for its matrix results in VGPRs.
+#include "igl_attend4.h"

@@ -47,11 +47,12 @@ struct Attend4Args {
 // two where the ring wraps; the piece from slot sinks on joins the sinks.
 struct Blocks4 {
   int low, mid, count;
+  int low_ahead, mid_ahead;  // a ring slot's position less the slot, in the two runs
   __host__ __device__ int at(int i) const { return i < low ? i : mid + i - low; }
 };
 
 __host__ __device__ inline Blocks4 attend4_blocks(int block, int first, int last, const Attend4Args &a) {
-  Blocks4 b = {0, 0, 0};
+  Blocks4 b = {0, 0, 0, 0, 0};
   int low_slots = last < a.sinks ? last + 1 : a.sinks;
   int oldest = a.window > 0 && first >= a.window ? first + 1 - a.window : 0;
   if (oldest < a.sinks) oldest = a.sinks;
@@ -71,6 +72,9 @@ __host__ __device__ inline Blocks4 attend4_blocks(int block, int first, int last
   if (b.mid < b.low) b.mid = b.low;
   const int end = mid_last < 0 ? 0 : mid_last / block + 1;
   b.count = b.low + (end > b.mid ? end - b.mid : 0);
+  // slots past the newest position's hold a turn before
+  b.low_ahead = a.newest - a.newest_slot;
+  b.mid_ahead = b.low_ahead - (mid_first > a.newest_slot ? a.span - a.sinks : 0);
   return b;
 }
 
@@ -100,9 +104,19 @@ __device__ __forceinline__ half2_t gain_pair(uint32_t x) { return as_half2((x + 
 __device__ __forceinline__ half2_t half_low(half2_t x) { return __builtin_shufflevector(x, x, 0, 0); }
 __device__ __forceinline__ half2_t half_high(half2_t x) { return __builtin_shufflevector(x, x, 1, 1); }
 
-// What turns 16 + c into (c - 8) g with one fma: -24 g, exact (g has four
-// significant bits).  E2M1 codes are levels as they are decoded.
-__device__ __forceinline__ half2_t gain_offset(half2_t g) { return g * half2_t{(_Float16)-24.0f, (_Float16)-24.0f}; }
+// Nibbles I of both halves of a dword as 64 + c: moved to bits 4 .. 7 of the
+// halves, where they count whole numbers under binary16's exponent of 64.
+constexpr uint32_t kNibble64 = 0x54005400u;
+
+template <int I>
+__device__ __forceinline__ half2_t nibble_pair64(uint32_t d, uint32_t exp64) {
+  const uint32_t moved = I == 0 ? d << 4 : d >> (I == 0 ? 0 : 4 * I - 4);
+  return as_half2(and_or_b32(moved, 0x00F000F0u, exp64));
+}
+
+// What turns 64 + c into (c - 8) g with one fma: -72 g, exact (72 and g have four
+// significant bits each).  E2M1 codes are levels as they are decoded.
+__device__ __forceinline__ half2_t gain_offset(half2_t g) { return g * half2_t{(_Float16)-72.0f, (_Float16)-72.0f}; }
 
 // Element e of a key operand of eight dims is dim key_order<FMT>(e) of them: a
 // dword's nibbles i and i + 4 lie 16 bits apart, the halves of one register; a
@@ -114,13 +128,13 @@ __host__ __device__ constexpr int key_order(int e) {
 
 // Eight codes of one row, times their gain (both halves of g; h its offset).
 template <int FMT>
-__device__ __forceinline__ half8_t key_operand(uint32_t w, half2_t g, half2_t h, uint32_t exp16) {
+__device__ __forceinline__ half8_t key_operand(uint32_t w, half2_t g, half2_t h, uint32_t exp64) {
   half2_t p[4];
   if (FMT == IGL_CACHE4_INT4) {
-    p[0] = __builtin_elementwise_fma(nibble_pair16<0>(w, exp16), g, h);
-    p[1] = __builtin_elementwise_fma(nibble_pair16<1>(w, exp16), g, h);
-    p[2] = __builtin_elementwise_fma(nibble_pair16<2>(w, exp16), g, h);
-    p[3] = __builtin_elementwise_fma(nibble_pair16<3>(w, exp16), g, h);
+    p[0] = __builtin_elementwise_fma(nibble_pair64<0>(w, exp64), g, h);
+    p[1] = __builtin_elementwise_fma(nibble_pair64<1>(w, exp64), g, h);
+    p[2] = __builtin_elementwise_fma(nibble_pair64<2>(w, exp64), g, h);
+    p[3] = __builtin_elementwise_fma(nibble_pair64<3>(w, exp64), g, h);
   } else {
     p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0) * g;
     p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1) * g;
@@ -135,7 +149,7 @@ __device__ __forceinline__ half8_t key_operand(uint32_t w, half2_t g, half2_t h,
 // offsets).
 template <int FMT, int DIMS>
 __device__ __forceinline__ void value_operands(const uint32_t (&x)[8], const half2_t (&g)[4], const half2_t (&h)[4],
-                                               uint32_t exp16, half8_t (&out)[DIMS]) {
+                                               uint32_t exp64, half8_t (&out)[DIMS]) {
   half2_t p[DIMS][4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -144,10 +158,10 @@ __device__ __forceinline__ void value_operands(const uint32_t (&x)[8], const hal
 #pragma unroll
       for (int half = 0; half < DIMS / 4; ++half) {
         const uint32_t t = __builtin_amdgcn_perm(b, a, half ? 0x07060302u : 0x05040100u);
-        p[4 * half + 0][q] = __builtin_elementwise_fma(nibble_pair16<0>(t, exp16), g[q], h[q]);
-        p[4 * half + 1][q] = __builtin_elementwise_fma(nibble_pair16<1>(t, exp16), g[q], h[q]);
-        p[4 * half + 2][q] = __builtin_elementwise_fma(nibble_pair16<2>(t, exp16), g[q], h[q]);
-        p[4 * half + 3][q] = __builtin_elementwise_fma(nibble_pair16<3>(t, exp16), g[q], h[q]);
+        p[4 * half + 0][q] = __builtin_elementwise_fma(nibble_pair64<0>(t, exp64), g[q], h[q]);
+        p[4 * half + 1][q] = __builtin_elementwise_fma(nibble_pair64<1>(t, exp64), g[q], h[q]);
+        p[4 * half + 2][q] = __builtin_elementwise_fma(nibble_pair64<2>(t, exp64), g[q], h[q]);
+        p[4 * half + 3][q] = __builtin_elementwise_fma(nibble_pair64<3>(t, exp64), g[q], h[q]);
       }
     } else {
       // bytes of both rows' nibbles: of the even dims, and of the odd ones
@@ -242,6 +256,8 @@ __device__ __forceinline__ float query_factor(const Attend4Args &a, float top, f
 }
 
 typedef float float2_t __attribute__((ext_vector_type(2)));
+// Four floats at any address of a float: rows need no alignment.
+typedef float float4a_t __attribute__((ext_vector_type(4), aligned(4)));
 
 // Two values as two binary16 terms each, x = hi + lo to 2^-22 of itself.
 __device__ __forceinline__ void two_terms(float x, float y, half2_t &hi, half2_t &lo) {
@@ -275,19 +291,13 @@ struct QueryLoad {
   static constexpr int PIECES = HEAD / 8, ITEMS = ROWS * PIECES, PER = (ITEMS + THREADS - 1) / THREADS;
   float x[PER][8];
   __device__ __forceinline__ void load(const Attend4Args &a, int kv, int row0, int row_last, int tid) {
-    const bool vec = (((uintptr_t)a.query | ((size_t)a.lane_stride * 4)) & 15u) == 0;  // uniform
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int item = min(tid + THREADS * i, ITEMS - 1);
       const float *src = a.query + attend4_row(min(row0 + item / PIECES, row_last), kv, HEAD, a) + 8 * (item % PIECES);
-      if (vec) {
-        const float4_t u = *reinterpret_cast<const float4_t *>(src), v = *reinterpret_cast<const float4_t *>(src + 4);
+      const float4_t u = *reinterpret_cast<const float4a_t *>(src), v = *reinterpret_cast<const float4a_t *>(src + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][e] = u[e], x[i][4 + e] = v[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = src[e];
-      }
+      for (int e = 0; e < 4; ++e) x[i][e] = u[e], x[i][4 + e] = v[e];
     }
   }
   __device__ __forceinline__ void store(const Attend4Args &a, int tid, _Float16 *to, int second, float *factors) {
@@ -318,11 +328,14 @@ __device__ __forceinline__ bool attend4_seen(int slot, int place, const Attend4A
   return at <= place && (a.window == 0 || at > place - a.window || at < a.sinks);
 }
 
-// Whether every lane from place_low to place_high sees all of a block past the sinks.
-__device__ __forceinline__ bool attend4_all(int slot0, int block, int place_low, int place_high, const Attend4Args &a) {
-  const int place0 = attend4_place(slot0, a);
-  return slot0 >= a.sinks && slot0 + block <= a.span && place0 <= place_low - (block - 1) &&
-         attend4_place(slot0 + block - 1, a) == place0 + block - 1 && (a.window == 0 || place0 > place_high - a.window);
+// Whether every lane from place_low to place_high sees all of a run's `count` slots
+// from slot0 on: all past the sinks, and from the oldest position that the last
+// lane sees to the first lane's own (a slot of another turn would lie outside).
+__device__ __forceinline__ bool attend4_all(int slot0, int count, int ahead, int place_low, int place_high,
+                                            const Attend4Args &a) {
+  const int place0 = slot0 + ahead;
+  return slot0 >= a.sinks && slot0 <= a.span - count && place0 <= place_low - (count - 1) &&
+         (a.window == 0 || place0 > place_high - a.window);
 }
 
 // A row's base after a block with this peak (before its factor).
@@ -354,11 +367,9 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
   const int l = attend4_lane(row, a);
   float *dst = a.out + (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * HEAD;
   float mul = a.value_scale;
-  bool vec = (((uintptr_t)a.out | ((size_t)a.lane_stride * 4)) & 15u) == 0;
   if (a.segments > 1) {
     const size_t at = ((size_t)seg * gridDim.z + kv) * a.rows + row;
     dst = a.part_out + at * HEAD;
-    vec = true;
     if (stats && g == 0 && (!PAIR || n < 8)) {
       a.part_base[at] = base;
       a.part_total[at] = total;
@@ -372,14 +383,8 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
     if (PAIR && (r >= 2) != (n >= 8)) continue;
 #pragma unroll
     for (int j = 0; j < DPL; j += 4) {
-      float *to = dst + r * DPL + j;
-      const float4_t o = {out[j][r] * mul, out[j + 1][r] * mul, out[j + 2][r] * mul, out[j + 3][r] * mul};
-      if (vec) {
-        *reinterpret_cast<float4_t *>(to) = o;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) to[e] = o[e];
-      }
+      *reinterpret_cast<float4a_t *>(dst + r * DPL + j) =
+          float4_t{out[j][r] * mul, out[j + 1][r] * mul, out[j + 2][r] * mul, out[j + 3][r] * mul};
     }
   }
 }
@@ -435,7 +440,7 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
   const Blocks4 blocks = attend4_blocks(BLOCK, place_low, place_high, a);
   const int first = min(blocks.count, seg * a.per);
   const int end = seg == a.segments - 1 ? blocks.count : min(blocks.count, first + a.per);
-  const uint32_t exp16 = 0x4C004C00u;
+  const uint32_t exp64 = kNibble64;
   const uint32_t row_bytes = (uint32_t)a.kv_width / 2;
   const size_t head_bytes = (size_t)kv * HEAD / 2;
   const size_t gain_row = (size_t)kv * HEAD / kCache4Group;
@@ -555,7 +560,7 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
       for (int w = 0; w < KW; ++w) {
         half8_t k[T];
 #pragma unroll
-        for (int j = 0; j < T; ++j) k[j] = key_operand<FMT>(kr[j][c][w], gain[j], off[j], exp16);
+        for (int j = 0; j < T; ++j) k[j] = key_operand<FMT>(kr[j][c][w], gain[j], off[j], exp64);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -570,7 +575,8 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
 
     // ---- the block's peaks
     const int slot0 = blocks.at(i) * BLOCK;
-    const bool all = attend4_all(slot0, BLOCK, place_low, place_high, a);  // uniform
+    const bool all =
+        attend4_all(slot0, BLOCK, i < blocks.low ? blocks.low_ahead : blocks.mid_ahead, place_low, place_high, a);  // uniform
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       if (PAIR) {
@@ -647,7 +653,7 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
         off[k] = gain_offset(gain[k]);
       }
       half8_t op[DPL];
-      value_operands<FMT, DPL>(vr[u], gain, off, exp16, op);
+      value_operands<FMT, DPL>(vr[u], gain, off, exp64, op);
 #pragma unroll
       for (int m = TERMS - 1; m >= 0; --m)
 #pragma unroll
@@ -756,7 +762,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
   const Blocks4 blocks = attend4_blocks(BLOCK, place_low, place_high, a);
   const int first = min(blocks.count, seg * a.per);
   const int end = seg == a.segments - 1 ? blocks.count : min(blocks.count, first + a.per);
-  const uint32_t exp16 = 0x4C004C00u;
+  const uint32_t exp64 = kNibble64;
   const uint32_t row_bytes = (uint32_t)a.kv_width / 2;
   const size_t head_bytes = (size_t)kv * HEAD / 2;
   const size_t gain_row = (size_t)kv * HEAD / kCache4Group;
@@ -818,7 +824,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
         off[k] = gain_offset(gain[k]);
       }
       half8_t op[8];
-      value_operands<FMT, 8>(vr[j], gain, off, exp16, op);
+      value_operands<FMT, 8>(vr[j], gain, off, exp64, op);
       half8_t *to = reinterpret_cast<half8_t *>(room) + group * (HEAD * 4);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -879,7 +885,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
       for (int w = 0; w < KW; ++w)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const half8_t op = key_operand<FMT>(kr[b][c][w], gain[b], off[b], exp16);
+          const half8_t op = key_operand<FMT>(kr[b][c][w], gain[b], off[b], exp64);
           low[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, q[1][KW * c + w], low[b], 0, 0, 0);
           s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, q[0][KW * c + w], s[b], 0, 0, 0);
         }
@@ -897,7 +903,8 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
     }
     // ---- the rows' weights
     const int slot0 = blocks.at(i) * BLOCK + 32 * sh;
-    const bool all = attend4_all(slot0, 32, place_low, place_high, a);  // uniform
+    const bool all =
+        attend4_all(slot0, 32, i < blocks.low ? blocks.low_ahead : blocks.mid_ahead, place_low, place_high, a);  // uniform
     if (!all) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -1000,7 +1007,6 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
   }
   attend4_barrier();
   const int count = row_last - row0 + 1;
-  const bool vec = split || (((uintptr_t)a.out | ((size_t)a.lane_stride * 4)) & 15u) == 0;
   const size_t part0 = ((size_t)seg * gridDim.z + kv) * a.rows + row0;
   for (int i = tid; i < count * (HEAD / 4); i += THREADS) {
     const int r = i / (HEAD / 4), piece = i % (HEAD / 4);
@@ -1008,12 +1014,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
     float4_t o = *reinterpret_cast<const float4_t *>(from);
     if (SH > 1) o += *reinterpret_cast<const float4_t *>(from + 16 * RT * HEAD);
     float *to = (split ? a.part_out + (part0 + r) * HEAD : a.out + attend4_row(row0 + r, kv, HEAD, a)) + 4 * piece;
-    if (vec) {
-      *reinterpret_cast<float4_t *>(to) = o;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) to[e] = o[e];
-    }
+    *reinterpret_cast<float4a_t *>(to) = o;
   }
   if (split && g == 0 && dw == 0 && sh == 0 && 16 * rt + n < count) {
     a.part_base[part0 + 16 * rt + n] = base;
@@ -1072,10 +1073,7 @@ __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int he
   }
   if (sl) return;
   const float mul = 1.0f / (red[4] + red[5] + red[6] + red[7]);
-  const int l = attend4_lane(row, a);
-  float *to = a.out + (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * head_size + d0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) to[e] = acc[e] * mul;
+  *reinterpret_cast<float4a_t *>(a.out + attend4_row(row, kv, head_size, a) + d0) = acc * mul;
 }
 
 }  // namespace igl

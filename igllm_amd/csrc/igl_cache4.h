@@ -50,22 +50,47 @@ __device__ __forceinline__ uint32_t cache4_gain_byte(double q) {
   return (uint32_t)(u >> 49) - (1016u << 3);
 }
 
-// The code of x over a step that is real8(b) s exactly; x NaN or step 0: zero.
+// The level index of |q| = |x| / step, in single precision or exactly: INT4 q
+// itself; E2M1 2 q below 2, 2 + q below 4, 4 + q / 2 from there (its tables' steps
+// are 1/2, 1 and 2), to the nearest whole number, ties to even.
+template <int FMT, typename F>
+__device__ __forceinline__ F cache4_index(F q) {
+  if (FMT == IGL_CACHE4_INT4) return q;
+  return q < (F)2 ? (F)2 * q : q < (F)4 ? (F)2 + q : (F)4 + (F)0.5 * q;
+}
+
+// What decides a group's codes: its step, real8(b) s, and in single precision the
+// step's reciprocal (0 where a float does not hold it in full: then every code is
+// decided exactly).
+struct Cache4Step {
+  double step;
+  float inverse;
+};
+
+__device__ __forceinline__ Cache4Step cache4_step(double step) {
+  const bool held = step > 1e-30 && step < 1e30;
+  return Cache4Step{step, held ? 1.0f / (float)step : 0.0f};
+}
+
+// The code of x; x NaN or step 0: zero.  The single-precision index is off by less
+// than 2^-20 of itself, at most 14 where it counts, so it decides unless it lies
+// within 2^-15 of halfway; there the exact quotient does.
 template <int FMT>
-__device__ __forceinline__ uint32_t cache4_code(float x, double step) {
-  if (!(x == x) || step == 0.0) return FMT == IGL_CACHE4_INT4 ? 8u : 0u;
-  const double q = (double)x / step;
-  if (FMT == IGL_CACHE4_INT4) {
-    double level = __builtin_rint(q);
-    if (level > 7.0) level = 7.0;
-    if (level < -7.0) level = -7.0;
-    return (uint32_t)((int)level + 8);
+__device__ __forceinline__ uint32_t cache4_code(float x, const Cache4Step &t) {
+  const float m = fabsf(x);
+  const float at = cache4_index<FMT>(m * t.inverse);
+  float index = __builtin_rintf(at);
+  if (!(fabsf(at - index) < 0.5f - 3.1e-5f) || t.inverse == 0.0f) {  // and a NaN, an infinity, a number past 2^23
+    if (at <= 16.0f || t.inverse == 0.0f) {
+      double exact = t.step > 0.0 ? cache4_index<FMT, double>((double)m / t.step) : 0.0;
+      exact = __builtin_rint(exact);
+      index = exact < 7.0 ? (float)exact : 7.0f;
+    }
   }
-  const double m = __builtin_fabs(q);
-  double level = m < 2.0 ? __builtin_rint(2.0 * m) : m < 4.0 ? 2.0 + __builtin_rint(m) : 4.0 + __builtin_rint(0.5 * m);
-  if (level > 7.0) level = 7.0;
-  const uint32_t code = (uint32_t)level;
-  return code && x < 0.0f ? code | 8u : code;
+  if (!(index <= 7.0f)) index = 7.0f;
+  const uint32_t level = m == m ? (uint32_t)index : 0u;
+  if (FMT == IGL_CACHE4_INT4) return x < 0.0f ? 8u - level : 8u + level;
+  return level && x < 0.0f ? level | 8u : level;
 }
 
 struct Cache4Args {
@@ -108,7 +133,7 @@ __global__ __launch_bounds__(256) void cache4_lay_kernel(Cache4Args a) {
   top = fmaxf(top, dpp_move<0x4E>(top));
   const double scale = (double)a.scale[side];
   const uint32_t byte = cache4_gain_byte((double)top / ((FMT == IGL_CACHE4_INT4 ? 7.0 : 6.0) * scale));
-  const double step = (double)cache4_gain(byte) * scale;
+  const Cache4Step step = cache4_step((double)cache4_gain(byte) * scale);
   uint32_t w = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) w |= cache4_code<FMT>(x[e], step) << (4 * e);

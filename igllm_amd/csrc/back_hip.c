@@ -72,6 +72,7 @@ struct igl_desk_state {
   /* partials of the attention's wide launches (igl_attend_wide):
    * IGL_ATTEND_FIXED_FLOATS floats, held from open to close */
   float *attend_dev;
+  float *attend4_dev; /* partials of the 4-bit ring's attention: IGL_ATTEND4_FLOATS floats, as long */
   float *quant_dev;   /* plane_lift: the activations on the plane's entry grid */
   size_t quant_floats;
   /* plane_lift's prefill on the grid: widened codes, unit gains, level sums,
@@ -929,7 +930,7 @@ int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_sha
     return code;
   return hip_check(st, igl_launch_attend4(store, group_share, query_dev, lane_stride, place_first,
                                           window, lane_count, score_scale, blend_out_dev,
-                                          st->attend_dev, st->stream));
+                                          st->attend4_dev, st->stream));
 }
 
 int igl_norm_rms_dev(igl_desk *desk, const float *in_dev, const float *gain_dev, int n, int rows,
@@ -1169,7 +1170,8 @@ int igl_back_open(igl_desk *desk, int device_index, int sum_limit, int col_limit
       hipMalloc((void **)&st->act_dev, (size_t)st->lane_limit * st->col_limit * sizeof(float)) != hipSuccess ||
       hipHostMalloc((void **)&st->act_pin, (size_t)st->lane_limit * st->col_limit * sizeof(float),
                     hipHostMallocDefault) != hipSuccess ||
-      hipMalloc((void **)&st->attend_dev, IGL_ATTEND_FIXED_FLOATS * sizeof(float)) != hipSuccess) {
+      hipMalloc((void **)&st->attend_dev, IGL_ATTEND_FIXED_FLOATS * sizeof(float)) != hipSuccess ||
+      hipMalloc((void **)&st->attend4_dev, IGL_ATTEND4_FLOATS * sizeof(float)) != hipSuccess) {
     desk->state = st;
     igl_back_close(desk);
     return IGL_FAIL_DEVICE;
@@ -1197,6 +1199,7 @@ void igl_back_close(igl_desk *desk) {
   if (st->part_dev) (void)hipFree(st->part_dev);
   if (st->work_dev) (void)hipFree(st->work_dev);
   if (st->attend_dev) (void)hipFree(st->attend_dev);
+  if (st->attend4_dev) (void)hipFree(st->attend4_dev);
   if (st->quant_dev) (void)hipFree(st->quant_dev);
   if (st->wide_dev) (void)hipFree(st->wide_dev);
   if (st->ones_dev) (void)hipFree(st->ones_dev);

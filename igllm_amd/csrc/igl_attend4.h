@@ -36,8 +36,9 @@ struct Attend4Args {
   float value_scale;     // times 256
   int segments;          // of a row tile's blocks, each `per` of them and the last what is left
   int per;
-  float *part_out;       // [segments][kv][rows][HEAD], with more than one segment
-  float *part_base;      // [segments][kv][rows]
+  int part_row0;         // first row whose blocks are cut
+  float *part_out;       // [segments][kv][rows - part_row0][HEAD], with more than one segment
+  float *part_base;      // [segments][kv][rows - part_row0]
   float *part_total;
 };
 
@@ -201,6 +202,33 @@ __device__ __forceinline__ float group_max(float v) {
     v = fmaxf(a, b);
   }
   return v;
+}
+
+// The same for four dims, one half (`high`, uniform) of eight rows' dwords.
+template <int FMT>
+__device__ __forceinline__ void value_operands_half(const uint32_t (&x)[8], bool high, const half2_t (&g)[4],
+                                                    const half2_t (&h)[4], uint32_t exp64, half8_t (&out)[4]) {
+  const uint32_t pick = high ? 0x07060302u : 0x05040100u;
+  half2_t p[4][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t t = __builtin_amdgcn_perm(x[2 * q + 1], x[2 * q], pick);  // the rows' four codes each
+    if (FMT == IGL_CACHE4_INT4) {
+      p[0][q] = __builtin_elementwise_fma(nibble_pair64<0>(t, exp64), g[q], h[q]);
+      p[1][q] = __builtin_elementwise_fma(nibble_pair64<1>(t, exp64), g[q], h[q]);
+      p[2][q] = __builtin_elementwise_fma(nibble_pair64<2>(t, exp64), g[q], h[q]);
+      p[3][q] = __builtin_elementwise_fma(nibble_pair64<3>(t, exp64), g[q], h[q]);
+    } else {
+      const uint32_t even = (t & 0x0F0Fu) | ((t >> 12) & 0xF0F0u);         // bytes of both rows: dims 0, 2
+      const uint32_t odd = ((t >> 4) & 0x0F0Fu) | ((t >> 16) & 0xF0F0u);   // and 1, 3
+      p[0][q] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(even, 1.0f, 0) * g[q];
+      p[1][q] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(odd, 1.0f, 0) * g[q];
+      p[2][q] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(even, 1.0f, 1) * g[q];
+      p[3][q] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(odd, 1.0f, 1) * g[q];
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < 4; ++d) out[d] = __builtin_bit_cast(half8_t, p[d]);
 }
 
 // Largest and sum over the four lanes of a wave that differ by 16 and 32, the
@@ -705,45 +733,49 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
 
 // ---- many rows ----------------------------------------------------------------
 
-// Prompts.  A workgroup takes RT tiles of 16 rows through blocks of slots.  Two
-// waves share a tile's products: of 512-dim heads each takes half the dims (their
-// partial scores meet in LDS), of others half the block's slots (their blends meet
-// in LDS at the end).  Transposed, scores stay where the blend wants them: lane
-// 16 g + n of S^T (slots x rows) holds row n's slots 4 g + r of 16-slot tile b, and
-// of P^T, with slot 16 b + 4 g + r as element 4 b + r of lane group g's eight, the
-// same.
+// Prompts.  A workgroup of eight waves takes four tiles of 16 rows through blocks
+// of slots, whose codes its waves decode together into LDS as binary16 operands,
+// once for all its rows and a block ahead of the products.  Two waves share a
+// tile's products: of 512-dim heads each takes half the dims (their partial scores
+// meet in LDS), of others half the block's slots (their blends meet in LDS at the
+// end).  Transposed, scores stay where the blend wants them: lane 16 g + n of S^T
+// (slots x rows) holds row n's slots 4 g + r of 16-slot tile b, and of P^T, with slot
+// 16 b + 4 g + r as element 4 b + r of lane group g's eight, the same.
 //
-// A wave decodes its keys as it multiplies them: they lie as their operand wants
-// them, 16 bytes of a slot a lane.  Values lie across theirs, so the waves decode a
-// block's together into LDS, a block ahead, while they multiply the one before: a
-// dim's 32 slots are four 16-byte pieces, one a lane group; dim 8 d + i is row
-// i HEAD / 8 + d, its piece for g at g xor the row's bits 1 and 2, so that the eight
-// lanes that one cycle writes or reads lie in distinct banks with no padding.
-template <int HEAD, int RT>
+// A wave decodes the next block while it multiplies this one's keys: an item of 32
+// dims of a key and one of four dims of a lane group's eight slots of values a
+// thread, in straight code that the scheduler is told to lay between the products.
+//
+// LDS.  Keys: a slot's dims in 16-byte pieces, piece s of chunk c (dims 32 c + 8 s ..
+// + 7, a dword of codes) at s HEAD / 32 + c, xor the slot's low bits.  Values: a dim's
+// 32 slots in four pieces, one a lane group; dim 8 d + i is row i HEAD / 8 + d, its
+// piece for g at g xor the row's bits 1 and 2.  So the eight lanes that one cycle
+// writes or reads lie in distinct banks, with no padding.
+template <int HEAD>
 struct Tile4Shape {
+  static constexpr int RT = 4, WAVES = 8;
   static constexpr int DW = HEAD == 512 ? 2 : 1, SH = 2 / DW;
-  static constexpr int WAVES = 2 * RT, THREADS = 64 * WAVES;
   static constexpr int BLOCK = HEAD == 512 ? 32 : 64;
   static constexpr int DH = HEAD / DW;                     // dims a wave multiplies
-  static constexpr int KL = DH >= 128 ? DH / 128 : 1;      // key chunks of a slot a lane reads
-  static constexpr int KW = DH >= 128 ? 4 : 2;             // dwords of a chunk
+  static constexpr int KS = DH / 32;                       // its key steps
   static constexpr int DPL = DH / 16;                      // its tiles of 16 dims of the blend
+  static constexpr int KITEMS = BLOCK * HEAD / 32;         // chunks of 32 dims, a thread each: all or half of the 512
   static constexpr int VITEMS = BLOCK / 32 * 4 * HEAD / 8; // (lane group, 8 dims) of the block's 32s of slots
-  static constexpr int NV = (VITEMS + THREADS - 1) / THREADS;
-  static constexpr int V = BLOCK * HEAD * 2;               // bytes of a block's values; two of them
-  static constexpr int X = 2 * V;                          // partial scores: [WAVES][2][64] float4
+  static constexpr int V = BLOCK * HEAD * 2;               // bytes of a block's keys, and of its values
+  static constexpr int X = 4 * V;                          // partial scores: [WAVES][2][64] float4
   static constexpr int LOOP = X + (DW > 1 ? WAVES * 2048 : 0);
   static constexpr int QUERY = 2 * 16 * RT * (HEAD + 8) * 2;     // [2][16 RT][HEAD + 8] halves, before the loop
   static constexpr int ROWS = SH * 16 * RT * HEAD * 4;           // [SH][16 RT][HEAD] floats, after it
   static constexpr int STATS = LOOP > QUERY ? (LOOP > ROWS ? LOOP : ROWS) : (QUERY > ROWS ? QUERY : ROWS);
   static constexpr int LDS = STATS + WAVES * 32 * 4;
+  static_assert(KITEMS <= 512 && VITEMS <= 256, "an item of each a thread");
 };
 
-template <int HEAD, int FMT, int RT>
-__global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a) {
-  using F = Tile4Shape<HEAD, RT>;
-  constexpr int DW = F::DW, SH = F::SH, THREADS = F::THREADS, BLOCK = F::BLOCK, DH = F::DH, KL = F::KL, KW = F::KW;
-  constexpr int KS = KL * KW, DPL = F::DPL, NV = F::NV;
+template <int HEAD, int FMT>
+__global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
+  using F = Tile4Shape<HEAD>;
+  constexpr int RT = F::RT, DW = F::DW, SH = F::SH, THREADS = 512, BLOCK = F::BLOCK, DH = F::DH, KS = F::KS;
+  constexpr int DPL = F::DPL;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds4[];
 
   const int tid = threadIdx.x;
@@ -752,93 +784,78 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
   const int rt = wave >> 1, dw = DW > 1 ? wave & 1 : 0, sh = SH > 1 ? wave & 1 : 0;
   const int g = lane >> 4, n = lane & 15;
   const int kv = blockIdx.z, seg = blockIdx.y;
-  // a prompt's longest tiles first; where all run at once, two a CU, the second
-  // half starts with the shortest, so that a long one meets a short one
-  const int tiles = gridDim.x, half = tiles * (int)(gridDim.y * gridDim.z) <= 512 ? (tiles + 1) / 2 : tiles;
-  const int tile = (int)blockIdx.x < half ? tiles - 1 - (int)blockIdx.x : (int)blockIdx.x - half;
-  const int row0 = tile * 16 * RT;
+  const int row0 = (int)(gridDim.x - 1 - blockIdx.x) * 16 * RT;  // a prompt's longest first
   const int row_last = min(row0 + 16 * RT, a.rows) - 1;
+  const bool split = a.segments > 1 && row0 >= a.part_row0;
+  if (seg > 0 && !split) return;
   const int place_low = a.place + attend4_lane(row0, a), place_high = a.place + attend4_lane(row_last, a);
   const Blocks4 blocks = attend4_blocks(BLOCK, place_low, place_high, a);
   const int first = min(blocks.count, seg * a.per);
-  const int end = seg == a.segments - 1 ? blocks.count : min(blocks.count, first + a.per);
+  const int end = !split || seg == a.segments - 1 ? blocks.count : min(blocks.count, first + a.per);
   const uint32_t exp64 = kNibble64;
   const uint32_t row_bytes = (uint32_t)a.kv_width / 2;
   const size_t head_bytes = (size_t)kv * HEAD / 2;
   const size_t gain_row = (size_t)kv * HEAD / kCache4Group;
 
-  uint32_t kr[2][KL][KW], kg[2][KL], vr[NV][8], vg[NV][2];
-  auto load_keys = [&](int i) {
+  // ---- a thread's items of a block: where there are fewer than threads, two write
+  // the same
+  const int k_item = tid % F::KITEMS, k_slot = k_item / (HEAD / 32), k_chunk = k_item % (HEAD / 32);
+  const int v_item = (tid & 255) % F::VITEMS, v_dims = v_item % (HEAD / 8), v_of = v_item / (HEAD / 8) % 4;
+  const int v_group = v_item / (HEAD / 2), v_slot = 32 * v_group + 4 * v_of;
+  const bool v_high = wave >= 4;  // which four of the eight dims
+  uint4_t kr;
+  uint32_t kg, vr[8], vg[2];
+  const uint8_t *const k_gain = a.key_gain + (gain_row + k_chunk) * a.room + k_slot;
+  const uint8_t *const v_gain = a.value_gain + (gain_row + v_dims / 4) * a.room + v_slot;
+  const uint32_t k_lane = row_at(k_slot, row_bytes) + 16 * k_chunk, v_lane = row_at(v_slot, row_bytes) + 4 * v_dims;
+  auto load = [&](int i) {
     const int slot0 = blocks.at(i) * BLOCK;
-    const int left = a.span - 1 - slot0;  // the ring's last slot, which rows past it are read from
-    const auto src = attend4_rows(a.key_code + (size_t)slot0 * row_bytes + head_bytes + dw * (DH / 2));
-    const uint8_t *gains = a.key_gain + (gain_row + dw * (DH / kCache4Group) + (KW == 4 ? g : g / 2)) * a.room + slot0;
+    const auto keys = attend4_rows(a.key_code + (size_t)slot0 * row_bytes + head_bytes);
+    const auto values = attend4_rows(a.value_code + (size_t)slot0 * row_bytes + head_bytes);
+    if (slot0 + BLOCK <= a.span) {  // uniform: rows at scalar distances
+      kr = __builtin_amdgcn_raw_buffer_load_b128(keys, k_lane, 0, 0);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int slot = 32 * sh + 16 * b + n;
-      const uint32_t off = row_at(min(slot, left), row_bytes) + (KW == 4 ? 16 : 8) * g;
-#pragma unroll
-      for (int c = 0; c < KL; ++c) {
-        if constexpr (KW == 4) {
-          const uint4_t w = __builtin_amdgcn_raw_buffer_load_b128(src, off + 64 * c, 0, 0);
-#pragma unroll
-          for (int s = 0; s < 4; ++s) kr[b][c][s] = w[s];
-        } else {
-          const uint2_t w = __builtin_amdgcn_raw_buffer_load_b64(src, off, 0, 0);
-          kr[b][c][0] = w[0];
-          kr[b][c][1] = w[1];
-        }
-        kg[b][c] = gains[(size_t)(4 * c) * a.room + slot];
-      }
-    }
-  };
-  auto load_values = [&](int i) {
-    const int slot0 = blocks.at(i) * BLOCK;
-    const int left = a.span - 1 - slot0;
-    const auto src = attend4_rows(a.value_code + (size_t)slot0 * row_bytes + head_bytes);
-    const uint8_t *gains = a.value_gain + gain_row * a.room + slot0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int item = F::VITEMS % THREADS ? min(tid + THREADS * j, F::VITEMS - 1) : tid + THREADS * j;
-      const int d = item % (HEAD / 8), at = 32 * (item / (HEAD / 2)) + 4 * (item / (HEAD / 8) % 4);
+      for (int e = 0; e < 8; ++e)
+        vr[e] = __builtin_amdgcn_raw_buffer_load_b32(values, v_lane, (16 * (e >> 2) + (e & 3)) * row_bytes, 0);
+    } else {
+      const int left = a.span - 1 - slot0;  // rows past the ring's last slot are read from it
+      kr = __builtin_amdgcn_raw_buffer_load_b128(keys, row_at(min(k_slot, left), row_bytes) + 16 * k_chunk, 0, 0);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int slot = at + 16 * (e >> 2) + (e & 3);
-        vr[j][e] = __builtin_amdgcn_raw_buffer_load_b32(src, row_at(min(slot, left), row_bytes) + 4 * d, 0, 0);
+        const int slot = v_slot + 16 * (e >> 2) + (e & 3);
+        vr[e] = __builtin_amdgcn_raw_buffer_load_b32(values, row_at(min(slot, left), row_bytes) + 4 * v_dims, 0, 0);
       }
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-        vg[j][b] = *reinterpret_cast<const uint32_t *>(gains + (size_t)(d / 4) * a.room + at + 16 * b);
     }
+    kg = k_gain[slot0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) vg[b] = *reinterpret_cast<const uint32_t *>(v_gain + slot0 + 16 * b);
   };
-  auto decode_values = [&](uint8_t *room) {
+  auto decode = [&](uint8_t *room) {
+    {
+      const half2_t gain = half_low(gain_pair(kg)), off = gain_offset(gain);
+      half8_t *to = reinterpret_cast<half8_t *>(room) + k_slot * (HEAD / 8);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int item = tid + THREADS * j;
-      if (F::VITEMS % THREADS && item >= F::VITEMS) break;
-      const int d = item % (HEAD / 8), of = item / (HEAD / 8) % 4, group = item / (HEAD / 2);
-      half2_t gain[4], off[4];
+      for (int s = 0; s < 4; ++s)
+        to[(s * (HEAD / 32) + k_chunk) ^ (k_slot & 7)] = key_operand<FMT>(kr[s], gain, off, exp64);
+    }
+    half2_t gain[4], off[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        gain[k] = gain_pair(__builtin_amdgcn_perm(0u, vg[j][k >> 1], k & 1 ? 0x0C030C02u : 0x0C010C00u));
-        off[k] = gain_offset(gain[k]);
-      }
-      half8_t op[8];
-      value_operands<FMT, 8>(vr[j], gain, off, exp64, op);
-      half8_t *to = reinterpret_cast<half8_t *>(room) + group * (HEAD * 4);
+    for (int k = 0; k < 4; ++k) {
+      gain[k] = gain_pair(__builtin_amdgcn_perm(0u, vg[k >> 1], k & 1 ? 0x0C030C02u : 0x0C010C00u));
+      off[k] = gain_offset(gain[k]);
+    }
+    half8_t op[4];
+    value_operands_half<FMT>(vr, v_high, gain, off, exp64, op);
+    half8_t *to = reinterpret_cast<half8_t *>(room + F::V) + v_group * (HEAD * 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = i * (HEAD / 8) + d;
-        to[row * 4 + (of ^ (row >> 1 & 3))] = op[i];
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int row = (i + (v_high ? 4 : 0)) * (HEAD / 8) + v_dims;
+      to[row * 4 + (v_of ^ (row >> 1 & 3))] = op[i];
     }
   };
   QueryLoad<HEAD, FMT, 16 * RT, THREADS> queries;
   queries.load(a, kv, row0, row_last, tid);
-  if (first < end) {
-    load_values(first);
-    load_keys(first);
-  }
+  if (first < end) load(first);
 
   // ---- the rows' queries: their terms through LDS, a thread eight dims, to the
   // waves' operands
@@ -864,33 +881,39 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
   float base = -INFINITY, top_base = -INFINITY, total = 0.0f;
 #pragma unroll
   for (int j = 0; j < DPL; ++j) out[j] = float4_t{0, 0, 0, 0};
-  uint8_t *now = lds4, *next = lds4 + F::V;
+  uint8_t *now = lds4, *next = lds4 + 2 * F::V;
   if (first < end) {
-    decode_values(now);
-    load_values(min(first + 1, end - 1));
+    decode(now);
+    load(min(first + 1, end - 1));
     attend4_barrier();
   }
   for (int i = first; i < end; ++i) {
-    // ---- scores
+    // ---- scores, and the next block's operands
+    const half8_t *keys = reinterpret_cast<const half8_t *>(now) + 32 * sh * (HEAD / 8);
     float4_t s[2] = {float4_t{0, 0, 0, 0}, float4_t{0, 0, 0, 0}}, low[2] = {s[0], s[1]};
 #pragma unroll
-    for (int c = 0; c < KL; ++c) {
-      half2_t gain[2], off[2];
+    for (int k = 0; k < KS; ++k) {
+      const int piece = HEAD == 64 ? (2 * (g & 1) + k) * 2 + (g >> 1)
+                                   : (k % 4) * (HEAD / 32) + (DH / 32) * dw + 4 * (k / 4) + g;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        gain[b] = half_low(gain_pair(kg[b][c]));
-        off[b] = gain_offset(gain[b]);
+        const int slot = 16 * b + n;
+        const half8_t op = keys[slot * (HEAD / 8) + (piece ^ (slot & 7))];
+        low[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, q[1][k], low[b], 0, 0, 0);
+        s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, q[0][k], s[b], 0, 0, 0);
       }
-#pragma unroll
-      for (int w = 0; w < KW; ++w)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const half8_t op = key_operand<FMT>(kr[b][c][w], gain[b], off[b], exp64);
-          low[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, q[1][KW * c + w], low[b], 0, 0, 0);
-          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, q[0][KW * c + w], s[b], 0, 0, 0);
-        }
     }
-    load_keys(min(i + 1, end - 1));
+    decode(next);
+    // two products, the next one's operand, and their share of the decoding
+    __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+    for (int k = 0; k < 2 * KS; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 128 / (2 * KS), 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (k % (KS / 4 > 0 ? KS / 4 : 1) == 0) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+    }
+    load(min(i + 2, end - 1));
     s[0] += low[0];
     s[1] += low[1];
     if constexpr (DW > 1) {
@@ -944,9 +967,8 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
       p[0] = __builtin_bit_cast(half8_t, hi);
       p[1] = __builtin_bit_cast(half8_t, lo);
     }
-    // ---- the blend: tile j is rows (j / TC) HEAD / 8 + 16 (j % TC) + .. of the wave's;
-    // and the next block's values
-    const half8_t *values = reinterpret_cast<const half8_t *>(now) + sh * (HEAD * 4);
+    // ---- the blend: tile j is rows (j / TC) HEAD / 8 + 16 (j % TC) + .. of the wave's
+    const half8_t *values = reinterpret_cast<const half8_t *>(now + F::V) + sh * (HEAD * 4);
 #pragma unroll
     for (int j = 0; j < DPL; ++j) {
       constexpr int TC = DH >= 128 ? DH / 128 : 1;
@@ -955,8 +977,12 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
 #pragma unroll
       for (int k = 1; k >= 0; --k) out[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, p[k], out[j], 0, 0, 0);
     }
-    decode_values(next);
-    load_values(min(i + 2, end - 1));
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+    }
     uint8_t *const was = now;
     now = next;
     next = was;
@@ -980,7 +1006,6 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
     total = total * mine + stats[(wave ^ 1) * 32 + 16 + n] * part;
     mul *= mine;
   }
-  const bool split = a.segments > 1;
   if (!split) mul *= 1.0f / total;
   float *rows = reinterpret_cast<float *>(lds4) + sh * (16 * RT * HEAD) + (16 * rt + n) * HEAD;
   if constexpr (DH >= 128) {
@@ -1007,7 +1032,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attend4_tile_kernel(Attend4Args a
   }
   attend4_barrier();
   const int count = row_last - row0 + 1;
-  const size_t part0 = ((size_t)seg * gridDim.z + kv) * a.rows + row0;
+  const size_t part0 = ((size_t)seg * gridDim.z + kv) * (a.rows - a.part_row0) + (row0 - a.part_row0);
   for (int i = tid; i < count * (HEAD / 4); i += THREADS) {
     const int r = i / (HEAD / 4), piece = i % (HEAD / 4);
     const float *from = reinterpret_cast<const float *>(lds4) + r * HEAD + 4 * (piece ^ (r & 7));
@@ -1033,8 +1058,8 @@ __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int he
   __shared__ float4_t part[SL][COLS];
   const int tid = threadIdx.x, c = tid % COLS, sl = tid / COLS;
   const int wave = tid >> 6;
-  const int row = blockIdx.x, kv = blockIdx.y, kv_count = gridDim.y;
-  const size_t step = (size_t)kv_count * a.rows, at = (size_t)kv * a.rows + row;
+  const int row = a.part_row0 + (int)blockIdx.x, kv = blockIdx.y, kv_count = gridDim.y;
+  const size_t step = (size_t)kv_count * gridDim.x, at = (size_t)kv * gridDim.x + blockIdx.x;
   const int d0 = blockIdx.z * DIMS + 4 * c;
   const float mine = tid < a.segments ? a.part_base[at + tid * step] : -INFINITY;
   const float sum = tid < a.segments ? a.part_total[at + tid * step] : 0.0f;
@@ -1080,10 +1105,8 @@ __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int he
 
 using namespace igl;
 
-constexpr int kTile4 = 2;  // tiles of 16 rows a workgroup of attend4_tile_kernel takes
-
 // Which form a launch takes: tiles of up to eight rows, or sixteen, on
-// attend4_step_kernel, or of 32 on attend4_tile_kernel.
+// attend4_step_kernel, or of 64 on attend4_tile_kernel.
 struct Attend4Plan {
   int step, pair, block;
   int tiles;
@@ -1094,24 +1117,53 @@ static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
   p.pair = a.rows <= 8;
   p.step = a.rows <= 320;
   p.block = !p.step && head == 512 ? 32 : p.step && head < 256 ? 128 : 64;
-  const int each = !p.step ? 16 * kTile4 : p.pair ? 8 : 16;
+  const int each = !p.step ? 64 : p.pair ? 8 : 16;
   p.tiles = (int)(((long long)a.rows + each - 1) / each);
-  // the most blocks of a tile: without a window the last one's, else as many as
-  // any alignment of its span and the sinks' can touch
-  int blocks = attend4_blocks(p.block, a.place, a.newest, a).count;
+  // a tile's blocks, and the most of any: without a window the last one's, else as
+  // many as any alignment of its span and the sinks' can touch
+  auto tile_blocks = [&](int t) {
+    const int low = t * each, high = a.rows - low < each ? a.rows - 1 : low + each - 1;
+    return attend4_blocks(p.block, a.place + low / a.share, a.place + high / a.share, a).count;
+  };
+  int blocks = tile_blocks(p.tiles - 1);
+  long long all = (long long)blocks * p.tiles;
   if (a.window > 0) {
     const long long reach = (long long)a.window + (each + a.share - 2) / a.share;
     const long long most = (reach + p.block - 2) / p.block + 1 + (a.sinks + p.block - 1) / p.block + 1;
-    if (most < blocks) blocks = (int)most;
+    const int whole = attend4_blocks(p.block, a.place, a.newest, a).count;
+    blocks = most < whole ? (int)most : whole;
+    all = (long long)blocks * p.tiles;
+  } else if (!p.step) {
+    all = 0;
+    for (int t = 0; t < p.tiles; ++t) all += tile_blocks(t);
   }
-  long long s = 512 / ((long long)p.tiles * kv_count);
-  const long long room = (long long)IGL_ATTEND_FIXED_FLOATS / ((long long)a.rows * kv_count * (head + 2));
-  if (s > blocks) s = blocks;
-  if (s > room) s = room;
-  if (s > kAttend4Segments) s = kAttend4Segments;
-  if (s < 1) s = 1;
-  a.per = (int)((blocks + s - 1) / s);
-  a.segments = (blocks + a.per - 1) / a.per;
+  // as many segments as fill the card (two step workgroups a CU, one of the tiles'),
+  // within the workspace; of the tiles without a window only the rows of more
+  // blocks than a share
+  const long long at_once = p.step ? 512 : 256;
+  long long per = (all * kv_count + at_once - 1) / at_once;
+  a.part_row0 = 0;
+  for (;;) {
+    if (per < (blocks + kAttend4Segments - 1) / kAttend4Segments) per = (blocks + kAttend4Segments - 1) / kAttend4Segments;
+    if (per < 1) per = 1;
+    if (per > blocks) per = blocks;
+    a.per = (int)per;
+    a.segments = (int)((blocks + per - 1) / per);
+    if (a.segments == 1) break;
+    if (!p.step && a.window == 0) {
+      int low = 0, high = p.tiles - 1;  // the first tile of more blocks than `per`
+      while (low < high) {
+        const int mid = (low + high) / 2;
+        if (tile_blocks(mid) > per)
+          high = mid;
+        else
+          low = mid + 1;
+      }
+      a.part_row0 = low * each;
+    }
+    if ((long long)a.segments * kv_count * (a.rows - a.part_row0) * (head + 2) <= (long long)IGL_ATTEND4_FLOATS) break;
+    per += (per + 7) / 8;
+  }
   return p;
 }
 
@@ -1120,13 +1172,13 @@ static hipError_t attend4_launch(const Attend4Args &a, const Attend4Plan &p, int
   constexpr int T = HEAD >= 256 ? 1 : 2;
   const dim3 grid(p.tiles, a.segments, kv_count);
   if (!p.step) {
-    constexpr int RT = kTile4, size = Tile4Shape<HEAD, RT>::LDS;
+    constexpr int size = Tile4Shape<HEAD>::LDS;
     if (size > 65536) {  // granting it again changes nothing
-      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&attend4_tile_kernel<HEAD, FMT, RT>),
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&attend4_tile_kernel<HEAD, FMT>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, size);
       if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((attend4_tile_kernel<HEAD, FMT, RT>), grid, dim3(128 * RT), (size_t)size, stream, a);
+    hipLaunchKernelGGL((attend4_tile_kernel<HEAD, FMT>), grid, dim3(512), (size_t)size, stream, a);
   } else if (p.pair) {
     hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, 1, true, T>), grid, dim3(256), 0, stream, a);
   } else {
@@ -1134,12 +1186,14 @@ static hipError_t attend4_launch(const Attend4Args &a, const Attend4Plan &p, int
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.segments == 1) return e;
-  const int dims = a.rows <= 64 ? 16 : 64;
-  const dim3 fgrid(a.rows, kv_count, HEAD / dims);
+  const int rows = a.rows - a.part_row0, dims = rows <= 64 ? 16 : rows <= 1024 ? 64 : HEAD;
+  const dim3 fgrid(rows, kv_count, HEAD / dims);
   if (dims == 16)
     hipLaunchKernelGGL((attend4_fold_kernel<16>), fgrid, dim3(256), 0, stream, a, HEAD);
-  else
+  else if (dims == 64)
     hipLaunchKernelGGL((attend4_fold_kernel<64>), fgrid, dim3(256), 0, stream, a, HEAD);
+  else
+    hipLaunchKernelGGL((attend4_fold_kernel<HEAD>), fgrid, dim3(256), 0, stream, a, HEAD);
   return hipGetLastError();
 }
 
@@ -1183,8 +1237,9 @@ extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_shar
   a.value_scale = store->value_scale * 256.0f;
   const Attend4Plan p = attend4_plan(a, store->head_size, store->kv_count);
   a.part_out = work;
-  a.part_base = work + (size_t)a.segments * store->kv_count * rows * store->head_size;
-  a.part_total = a.part_base + (size_t)a.segments * store->kv_count * rows;
+  const size_t parts = (size_t)a.segments * store->kv_count * (size_t)(a.rows - a.part_row0);
+  a.part_base = work + parts * store->head_size;
+  a.part_total = a.part_base + parts;
   switch (store->head_size) {
     case 64: return attend4_launch_format<64>(a, p, store->format, store->kv_count, stream);
     case 128: return attend4_launch_format<128>(a, p, store->format, store->kv_count, stream);

@@ -44,7 +44,7 @@ hipError_t W(igl_launch_attend4)(const igl_cache4 *s, int share, const float *qu
   check_ring(w, s);
   check_range(w, "query", query, rows);
   check_range(w, "blend", blend, rows);
-  check_range(w, "work", work, IGL_ATTEND_FIXED_FLOATS * sizeof(float));
+  check_range(w, "work", work, IGL_ATTEND4_FLOATS * sizeof(float));
   return R(igl_launch_attend4)(s, share, query, lane_stride, place_first, window, lanes, score_scale, blend, work,
                                stream);
 }

@@ -417,8 +417,6 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
   }
 }
 
-// ---- shared pieces ------------------------------------------------------------
-
 // ---- few rows -----------------------------------------------------------------
 
 // Steps and blocks of a few lanes.  Four waves take a block of 64 T slots, the
@@ -426,30 +424,30 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
 // (VD ways) and then by slots (VS ways): so a wave's chain from one barrier to
 // the next is a quarter of the block's work.  Weights cross between the two
 // divisions through LDS, against a base that the four waves agree on.
-template <int HEAD, int FMT, int RB, bool PAIR, int T>
+template <int HEAD, bool PAIR, int T>
 struct Step4Shape {
   static constexpr int KL = HEAD >= 128 ? HEAD / 128 : 1;  // key chunks of a row a lane reads
   static constexpr int KW = HEAD >= 128 ? 4 : 2;           // dwords of a chunk
-  static constexpr int ROWS = PAIR ? 8 : 16 * RB;
+  static constexpr int ROWS = PAIR ? 8 : 16;
   static constexpr int TERMS = PAIR ? 1 : 2;
   static constexpr int BLOCK = 64 * T;
   static constexpr int VD = HEAD >= 128 ? HEAD / 128 : 1, VS = 4 / VD;
   static constexpr int DB = HEAD / VD, DPL = DB / 16;      // a wave's dims of the blend, a lane's
   static constexpr int UB = BLOCK / VS / 32;               // its steps of 32 slots
   static constexpr int QP = HEAD + 8, PP = BLOCK + 8;      // pitches in halves
-  static constexpr int Q = 0;                              // [RB][TERMS][16][QP]
-  static constexpr int P = Q + RB * TERMS * 16 * QP * 2;   // [RB][TERMS][16][PP]
-  static constexpr int PEAK = P + RB * TERMS * 16 * PP * 2;  // [4][16 RB]
-  static constexpr int FACTOR = PEAK + 4 * 16 * RB * 4;    // [16 RB]
-  static constexpr int LOOP = FACTOR + 16 * RB * 4;
-  static constexpr int MERGE = (VS - 1) * VD * RB * DPL * 1024;  // the blends of waves that took other slots
+  static constexpr int Q = 0;                              // [TERMS][16][QP]
+  static constexpr int P = Q + TERMS * 16 * QP * 2;        // [TERMS][16][PP]
+  static constexpr int PEAK = P + TERMS * 16 * PP * 2;     // [4][16]
+  static constexpr int FACTOR = PEAK + 4 * 16 * 4;         // [16]
+  static constexpr int LOOP = FACTOR + 16 * 4;
+  static constexpr int MERGE = (VS - 1) * VD * DPL * 1024;  // the blends of waves that took other slots
   static constexpr int LDS = LOOP > MERGE ? LOOP : MERGE;
   static_assert(UB >= 1, "a blend step takes 32 slots");
 };
 
-template <int HEAD, int FMT, int RB, bool PAIR, int T>
+template <int HEAD, int FMT, bool PAIR, int T>
 __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
-  using F = Step4Shape<HEAD, FMT, RB, PAIR, T>;
+  using F = Step4Shape<HEAD, PAIR, T>;
   constexpr int KL = F::KL, KW = F::KW, ROWS = F::ROWS, TERMS = F::TERMS, BLOCK = F::BLOCK;
   constexpr int VD = F::VD, VS = F::VS, DB = F::DB, DPL = F::DPL, UB = F::UB, QP = F::QP, PP = F::PP;
   __shared__ __attribute__((aligned(16))) uint8_t lds[F::LDS];
@@ -538,44 +536,30 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
   }
   queries.store(a, tid, qs, (PAIR ? 8 : 16) * QP, factors);
   attend4_barrier();
-  int place[RB];
-  float factor[RB];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int row = 16 * rb + (PAIR ? n & 7 : n);
-    place[rb] = a.place + attend4_lane(min(row0 + row, row_last), a);
-    factor[rb] = factors[row];
-  }
-  auto query_at = [&](int rb, int m, int i) {  // key step i = KW c + w
+  const int row = PAIR ? n & 7 : n;
+  const int place = a.place + attend4_lane(min(row0 + row, row_last), a);
+  const float factor = factors[row];
+  auto query_at = [&](int m, int i) {  // key step i = KW c + w
     const int d = KW == 4 ? 32 * (4 * (i / 4) + g) + 8 * (i % 4) : 16 * g + 8 * i;
-    return *reinterpret_cast<const half8_t *>(qs + (size_t)((rb * TERMS + m) * 16 + n) * QP + d);
+    return *reinterpret_cast<const half8_t *>(qs + (size_t)(m * 16 + n) * QP + d);
   };
-  constexpr bool KEEP = KL * KW * TERMS * RB <= 16;  // in registers through the loop
-  half8_t q[RB][TERMS][KL * KW];
+  constexpr bool KEEP = KL * KW * TERMS <= 16;  // in registers through the loop
+  half8_t q[TERMS][KL * KW];
   if (KEEP) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int m = 0; m < TERMS; ++m)
 #pragma unroll
-      for (int m = 0; m < TERMS; ++m)
-#pragma unroll
-        for (int i = 0; i < KL * KW; ++i) q[rb][m][i] = query_at(rb, m, i);
+      for (int i = 0; i < KL * KW; ++i) q[m][i] = query_at(m, i);
   }
 
-  float4_t out[RB][DPL];
-  float base[RB], top_base[RB], total[RB];
+  float4_t out[DPL];
+  float base = -INFINITY, top_base = -INFINITY, total = 0.0f;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    base[rb] = top_base[rb] = -INFINITY;
-    total[rb] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < DPL; ++j) out[rb][j] = float4_t{0, 0, 0, 0};
-  }
+  for (int j = 0; j < DPL; ++j) out[j] = float4_t{0, 0, 0, 0};
   for (int i = first; i < end; ++i) {
-    float4_t s[RB][T];
+    float4_t s[T];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-      for (int j = 0; j < T; ++j) s[rb][j] = float4_t{0, 0, 0, 0};
+    for (int j = 0; j < T; ++j) s[j] = float4_t{0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < KL; ++c) {
       half2_t gain[T], off[T];
@@ -590,13 +574,11 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
 #pragma unroll
         for (int j = 0; j < T; ++j) k[j] = key_operand<FMT>(kr[j][c][w], gain[j], off[j], exp64);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
+        for (int m = TERMS - 1; m >= 0; --m) {
+          const half8_t op = KEEP ? q[m][KW * c + w] : query_at(m, KW * c + w);
 #pragma unroll
-          for (int m = TERMS - 1; m >= 0; --m) {
-            const half8_t op = KEEP ? q[rb][m][KW * c + w] : query_at(rb, m, KW * c + w);
-#pragma unroll
-            for (int j = 0; j < T; ++j) s[rb][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], op, s[rb][j], 0, 0, 0);
-          }
+          for (int j = 0; j < T; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j], op, s[j], 0, 0, 0);
+        }
       }
     }
     if (i + 1 < end) load_keys(i + 1);
@@ -605,75 +587,65 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
     const int slot0 = blocks.at(i) * BLOCK;
     const bool all =
         attend4_all(slot0, BLOCK, i < blocks.low ? blocks.low_ahead : blocks.mid_ahead, place_low, place_high, a);  // uniform
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      if (PAIR) {
-#pragma unroll
-        for (int j = 0; j < T; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[rb][j][r] += dpp_move<0x128>(s[rb][j][r]);  // row n and n + 8
-      }
-      if (!all) {
-#pragma unroll
-        for (int j = 0; j < T; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!attend4_seen(slot0 + 16 * (T * wave + j) + 4 * g + r, place[rb], a)) s[rb][j][r] = -INFINITY;
-      }
-      float peak = -INFINITY;
+    if (PAIR) {
 #pragma unroll
       for (int j = 0; j < T; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) peak = fmaxf(peak, s[rb][j][r]);
-      peak = xmax48(peak);
-      if (g == 0) peaks[wave * 16 * RB + 16 * rb + n] = peak;
+        for (int r = 0; r < 4; ++r) s[j][r] += dpp_move<0x128>(s[j][r]);  // row n and n + 8
     }
+    if (!all) {
+#pragma unroll
+      for (int j = 0; j < T; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!attend4_seen(slot0 + 16 * (T * wave + j) + 4 * g + r, place, a)) s[j][r] = -INFINITY;
+    }
+    float peak = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) peak = fmaxf(peak, s[j][r]);
+    peak = xmax48(peak);
+    if (g == 0) peaks[wave * 16 + n] = peak;
     attend4_barrier();
     // ---- the base, the same in every wave, and the weights
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      float peak = -INFINITY;
+    for (int w = 0; w < 4; ++w) peak = fmaxf(peak, peaks[w * 16 + n]);
+    const float m = attend4_base(peak, factor, base, top_base);
+    if (__builtin_amdgcn_ballot_w64(m != base)) {
+      const float keep = base != -INFINITY ? __builtin_amdgcn_exp2f(base - m) : 0.0f;
+      total *= keep;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) peak = fmaxf(peak, peaks[w * 16 * RB + 16 * rb + n]);
-      const float f = factor[rb];
-      const float m = attend4_base(peak, f, base[rb], top_base[rb]);
-      if (__builtin_amdgcn_ballot_w64(m != base[rb])) {
-        const float keep = base[rb] != -INFINITY ? __builtin_amdgcn_exp2f(base[rb] - m) : 0.0f;
-        total[rb] *= keep;
+      for (int j = 0; j < DPL; ++j)
 #pragma unroll
-        for (int j = 0; j < DPL; ++j)
+        for (int r = 0; r < 4; ++r) out[j][r] *= keep;
+      base = m;
+    }
+    const float from = attend4_from(m);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) out[rb][j][r] *= keep;
-        base[rb] = m;
+    for (int j = 0; j < T; ++j) {
+      half2_t hi[2], lo[2];
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], factor, from));
+        const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r + 1], factor, from));
+        total += w0 + w1;
+        two_terms(w0, w1, hi[r / 2], lo[r / 2]);
+        if (PAIR && n >= 8) hi[r / 2] = lo[r / 2];
       }
-      const float from = attend4_from(m);
-#pragma unroll
-      for (int j = 0; j < T; ++j) {
-        half2_t hi[2], lo[2];
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][j][r], f, from));
-          const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][j][r + 1], f, from));
-          total[rb] += w0 + w1;
-          two_terms(w0, w1, hi[r / 2], lo[r / 2]);
-          if (PAIR && n >= 8) hi[r / 2] = lo[r / 2];
-        }
-        _Float16 *to = ws + (size_t)(rb * TERMS * 16 + n) * PP + 16 * (T * wave + j) + 4 * g;
-        __builtin_memcpy(__builtin_assume_aligned(to, 8), hi, sizeof(hi));
-        if (!PAIR) __builtin_memcpy(__builtin_assume_aligned(to + 16 * PP, 8), lo, sizeof(lo));
-      }
+      _Float16 *to = ws + n * PP + 16 * (T * wave + j) + 4 * g;
+      __builtin_memcpy(__builtin_assume_aligned(to, 8), hi, sizeof(hi));
+      if (!PAIR) __builtin_memcpy(__builtin_assume_aligned(to + 16 * PP, 8), lo, sizeof(lo));
     }
     attend4_barrier();
     // ---- the blend of the wave's dims over its slots
 #pragma unroll
     for (int u = 0; u < UB; ++u) {
-      half8_t p[RB][TERMS];
+      half8_t p[TERMS];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int m = 0; m < TERMS; ++m)
-          p[rb][m] = *reinterpret_cast<const half8_t *>(ws + (size_t)((rb * TERMS + m) * 16 + n) * PP +
-                                                        32 * (UB * vs + u) + 8 * g);
+      for (int m = 0; m < TERMS; ++m)
+        p[m] = *reinterpret_cast<const half8_t *>(ws + (size_t)(m * 16 + n) * PP +
+                                                      32 * (UB * vs + u) + 8 * g);
       half2_t gain[4], off[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -685,50 +657,35 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
 #pragma unroll
       for (int m = TERMS - 1; m >= 0; --m)
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-          for (int d = 0; d < DPL; ++d)
-            out[rb][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[d], p[rb][m], out[rb][d], 0, 0, 0);
+        for (int d = 0; d < DPL; ++d)
+          out[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[d], p[m], out[d], 0, 0, 0);
     }
     if (i + 1 < end) load_values(i + 1);
   }
 
   // ---- the waves' totals and, of waves that took other slots, blends
   attend4_barrier();
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    total[rb] = xsum48(total[rb]);
-    if (g == 0) peaks[wave * 16 * RB + 16 * rb + n] = total[rb];
-  }
+  total = xsum48(total);
+  if (g == 0) peaks[wave * 16 + n] = total;
   attend4_barrier();
+  total = 0.0f;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    total[rb] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) total[rb] += peaks[w * 16 * RB + 16 * rb + n];
-  }
+  for (int w = 0; w < 4; ++w) total += peaks[w * 16 + n];
   if constexpr (VS > 1) {
     attend4_barrier();
     float4_t *room = reinterpret_cast<float4_t *>(lds) + lane;
     if (vs > 0) {
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int j = 0; j < DPL; ++j) room[((((vs - 1) * VD + vd) * RB + rb) * DPL + j) * 64] = out[rb][j];
+      for (int j = 0; j < DPL; ++j) room[(((vs - 1) * VD + vd) * DPL + j) * 64] = out[j];
     }
     attend4_barrier();
     if (vs > 0) return;
 #pragma unroll
     for (int w = 1; w < VS; ++w)
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int j = 0; j < DPL; ++j) out[rb][j] += room[((((w - 1) * VD + vd) * RB + rb) * DPL + j) * 64];
+      for (int j = 0; j < DPL; ++j) out[j] += room[(((w - 1) * VD + vd) * DPL + j) * 64];
   }
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
-    attend4_store<HEAD, DPL, PAIR>(a, out[rb], base[rb], total[rb], row0 + 16 * rb + (PAIR ? n & 7 : n), row_last, seg, kv,
-                                   vd * DB, vd == 0, g, n);
+  attend4_store<HEAD, DPL, PAIR>(a, out, base, total, row0 + row, row_last, seg, kv, vd * DB, vd == 0, g, n);
 }
 
 // ---- many rows ----------------------------------------------------------------
@@ -775,7 +732,7 @@ template <int HEAD, int FMT>
 __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
   using F = Tile4Shape<HEAD>;
   constexpr int RT = F::RT, DW = F::DW, SH = F::SH, THREADS = 512, BLOCK = F::BLOCK, DH = F::DH, KS = F::KS;
-  constexpr int DPL = F::DPL;
+  constexpr int DPL = F::DPL, TC = DH / 128;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds4[];
 
   const int tid = threadIdx.x;
@@ -871,8 +828,8 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {  // step 4 c + s is dword s of chunk 4 c + g (heads of 64: of chunk g / 2)
-      const int d = HEAD == 64 ? 16 * g + 8 * k : DH * dw + 32 * (4 * (k / 4) + g) + 8 * (k % 4);
+    for (int k = 0; k < KS; ++k) {  // step 4 c + s is dword s of chunk 4 c + g
+      const int d = DH * dw + 32 * (4 * (k / 4) + g) + 8 * (k % 4);
       q[m][k] = *reinterpret_cast<const half8_t *>(qs + m * (16 * RT * QP) + (16 * rt + n) * QP + d);
     }
   attend4_barrier();
@@ -893,8 +850,7 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
     float4_t s[2] = {float4_t{0, 0, 0, 0}, float4_t{0, 0, 0, 0}}, low[2] = {s[0], s[1]};
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const int piece = HEAD == 64 ? (2 * (g & 1) + k) * 2 + (g >> 1)
-                                   : (k % 4) * (HEAD / 32) + (DH / 32) * dw + 4 * (k / 4) + g;
+      const int piece = (k % 4) * (HEAD / 32) + (DH / 32) * dw + 4 * (k / 4) + g;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const int slot = 16 * b + n;
@@ -911,7 +867,7 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
       __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
       __builtin_amdgcn_sched_group_barrier(0x002, 128 / (2 * KS), 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      if (k % (KS / 4 > 0 ? KS / 4 : 1) == 0) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+      if (k % (KS / 4) == 0) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
     }
     load(min(i + 2, end - 1));
     s[0] += low[0];
@@ -971,8 +927,7 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
     const half8_t *values = reinterpret_cast<const half8_t *>(now + F::V) + sh * (HEAD * 4);
 #pragma unroll
     for (int j = 0; j < DPL; ++j) {
-      constexpr int TC = DH >= 128 ? DH / 128 : 1;
-      const int at = DH >= 128 ? (j / TC) * (HEAD / 8) + dw * (DH / 8) + 16 * (j % TC) + n : 16 * j + n;
+      const int at = (j / TC) * (HEAD / 8) + dw * (DH / 8) + 16 * (j % TC) + n;
       const half8_t op = values[at * 4 + (g ^ (at >> 1 & 3))];
 #pragma unroll
       for (int k = 1; k >= 0; --k) out[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, p[k], out[j], 0, 0, 0);
@@ -1008,28 +963,17 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
   }
   if (!split) mul *= 1.0f / total;
   float *rows = reinterpret_cast<float *>(lds4) + sh * (16 * RT * HEAD) + (16 * rt + n) * HEAD;
-  if constexpr (DH >= 128) {
-    constexpr int TC = DH / 128;
 #pragma unroll
-    for (int t = 0; t < TC; ++t)
+  for (int t = 0; t < TC; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int h = 0; h < 8; h += 4) {  // the tiles t, t + TC, .. are its dims
-          const int piece = dw * (DH / 4) + 2 * (16 * t + 4 * g + r) + h / 4;
-          *reinterpret_cast<float4_t *>(rows + 4 * (piece ^ (n & 7))) =
-              float4_t{out[TC * h + t][r] * mul, out[TC * (h + 1) + t][r] * mul, out[TC * (h + 2) + t][r] * mul,
-                       out[TC * (h + 3) + t][r] * mul};
-        }
-  } else {
-#pragma unroll
-    for (int j = 0; j < DPL; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = 16 * j + 4 * g + r, d = 8 * (at % 8) + at / 8;
-        rows[4 * ((d / 4) ^ (n & 7)) + d % 4] = out[j][r] * mul;
+      for (int h = 0; h < 8; h += 4) {  // the tiles t, t + TC, .. are its dims
+        const int piece = dw * (DH / 4) + 2 * (16 * t + 4 * g + r) + h / 4;
+        *reinterpret_cast<float4_t *>(rows + 4 * (piece ^ (n & 7))) =
+            float4_t{out[TC * h + t][r] * mul, out[TC * (h + 1) + t][r] * mul, out[TC * (h + 2) + t][r] * mul,
+                     out[TC * (h + 3) + t][r] * mul};
       }
-  }
   attend4_barrier();
   const int count = row_last - row0 + 1;
   const size_t part0 = ((size_t)seg * gridDim.z + kv) * (a.rows - a.part_row0) + (row0 - a.part_row0);
@@ -1105,63 +1049,106 @@ __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int he
 
 using namespace igl;
 
-// Which form a launch takes: tiles of up to eight rows, or sixteen, on
-// attend4_step_kernel, or of 64 on attend4_tile_kernel.
+// How a launch is cut: tiles of up to eight rows (`pair`) or sixteen on
+// attend4_step_kernel, or of 64 on attend4_tile_kernel; blocks of `block` slots.
 struct Attend4Plan {
-  int step, pair, block;
-  int tiles;
+  bool step, pair, deep;
+  int block, each, tiles;  // rows a tile
+  int blocks;              // of the tile with most, or a bound of it
+  long long all;           // of all tiles
 };
 
-static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
-  Attend4Plan p = {1, 0, 64, 1};
-  p.pair = a.rows <= 8;
-  p.step = a.rows <= 320;
-  p.block = !p.step && head == 512 ? 32 : p.step && head < 256 ? 128 : 64;
-  const int each = !p.step ? 64 : p.pair ? 8 : 16;
-  p.tiles = (int)(((long long)a.rows + each - 1) / each);
-  // a tile's blocks, and the most of any: without a window the last one's, else as
-  // many as any alignment of its span and the sinks' can touch
-  auto tile_blocks = [&](int t) {
-    const int low = t * each, high = a.rows - low < each ? a.rows - 1 : low + each - 1;
-    return attend4_blocks(p.block, a.place + low / a.share, a.place + high / a.share, a).count;
-  };
-  int blocks = tile_blocks(p.tiles - 1);
-  long long all = (long long)blocks * p.tiles;
+// Counts a form's blocks.  Without a window the last tile has most; with one, as
+// many as any alignment of a tile's span and the sinks' can touch.
+static int attend4_tile_blocks(const Attend4Plan &p, int tile, const Attend4Args &a) {
+  const int low = tile * p.each, high = a.rows - low < p.each ? a.rows - 1 : low + p.each - 1;
+  return attend4_blocks(p.block, a.place + low / a.share, a.place + high / a.share, a).count;
+}
+
+static void attend4_count(Attend4Plan &p, const Attend4Args &a) {
+  p.tiles = (int)(((long long)a.rows + p.each - 1) / p.each);
+  p.blocks = attend4_tile_blocks(p, p.tiles - 1, a);
+  p.all = (long long)p.blocks * p.tiles;
   if (a.window > 0) {
-    const long long reach = (long long)a.window + (each + a.share - 2) / a.share;
+    const long long reach = (long long)a.window + (p.each + a.share - 2) / a.share;
     const long long most = (reach + p.block - 2) / p.block + 1 + (a.sinks + p.block - 1) / p.block + 1;
     const int whole = attend4_blocks(p.block, a.place, a.newest, a).count;
-    blocks = most < whole ? (int)most : whole;
-    all = (long long)blocks * p.tiles;
-  } else if (!p.step) {
-    all = 0;
-    for (int t = 0; t < p.tiles; ++t) all += tile_blocks(t);
+    p.blocks = most < whole ? (int)most : whole;
+    p.all = (long long)p.blocks * p.tiles;
+  } else if (p.tiles > 1) {  // between the first tile's and the last's, evenly
+    p.all = ((long long)attend4_tile_blocks(p, 0, a) + p.blocks) * p.tiles / 2;
   }
-  // as many segments as fill the card (two step workgroups a CU, one of the tiles'),
-  // within the workspace; of the tiles without a window only the rows of more
-  // blocks than a share
-  const long long at_once = p.step ? 512 : 256;
-  long long per = (all * kv_count + at_once - 1) / at_once;
+}
+
+static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
+  const long long cus = 256;
+  Attend4Plan p = {};
+  // Tiles of 64 rows, where they give every CU more than six blocks of 64 slots:
+  // 2047 lanes of a 512 window, 256-dim heads, 36 us (step form 49), of 512-dim heads
+  // 64 (76), a prompt of as many 62 + 10 (100) and 122 + 12 (168), 100 lanes at 15000
+  // 40 + 6 (53 + 6); but 1000 lanes, 4.6 blocks, 27 + 10 (25).  64-dim heads decode so
+  // little that they never do: 45 + 10 (37).
+  p.block = head == 512 ? 32 : 64;
+  p.each = 64;
+  p.step = true;
+  if (a.rows > 48 && head >= 128) {
+    attend4_count(p, a);
+    p.step = p.all * kv_count * p.block <= 6 * 64 * cus;
+  }
+  if (p.step) {
+    p.pair = a.rows <= 8;
+    p.each = p.pair ? 8 : 16;
+    p.block = head < 256 ? 128 : 64;
+    // Twice the slots between barriers where every workgroup still has two such
+    // blocks: 131072 positions of eight 128-dim heads 40.5 -> 35.6 us, of two 64-dim
+    // 11.0 -> 9.8, 40000 of eight the same.  Not of wide heads, whose rows already
+    // fill the registers: two 512-dim heads 32.9 -> 42.8.
+    p.deep = p.pair && head < 256 &&
+             (long long)attend4_blocks(2 * p.block, a.place, a.newest, a).count * kv_count >= 2 * 2 * cus;
+    p.block <<= p.deep;
+    attend4_count(p, a);
+  }
+
+  // Segments: as many as fill the card, two step workgroups a CU (each taken for the
+  // longest: a cut of all rows costs a fold) or one of the tiles'.
+  const auto floats = [&](long long segments) { return segments * kv_count * (a.rows - a.part_row0) * (head + 2); };
+  const int per_least = (p.blocks + kAttend4Segments - 1) / kAttend4Segments;
+  const long long at_once = p.step ? 2 * cus : cus;
+  long long per = ((p.step ? (long long)p.blocks * p.tiles : p.all) * kv_count + at_once - 1) / at_once;
   a.part_row0 = 0;
+  if (!p.step && (a.window > 0 || 4 * attend4_tile_blocks(p, 0, a) > 3 * p.blocks)) {
+    // Tiles alike: the cheapest number of whole turns of the card, a workgroup's start
+    // and end taken for one block and a share of 2^20 partial floats for another
+    // (160 lanes at 15000, 512-dim heads: 13 segments of 20 tiles, two turns, 165 us;
+    // 12, one turn, 117).
+    double least = 0.0;
+    for (int n = 1; n <= p.blocks && n <= kAttend4Segments; ++n) {
+      const long long size = (p.blocks + n - 1) / n, used = (p.blocks + size - 1) / size;
+      if (used > 1 && floats(used) > (long long)IGL_ATTEND4_FLOATS) break;
+      const double cost = (double)((used * p.tiles * kv_count + cus - 1) / cus) * (double)(size + 1) +
+                          (used > 1 ? 1.0 + (double)floats(used) / (1 << 20) : 0.0);
+      if (n == 1 || cost < least) least = cost, per = size;
+    }
+  }
   for (;;) {
-    if (per < (blocks + kAttend4Segments - 1) / kAttend4Segments) per = (blocks + kAttend4Segments - 1) / kAttend4Segments;
+    if (per < per_least) per = per_least;
     if (per < 1) per = 1;
-    if (per > blocks) per = blocks;
+    if (per > p.blocks) per = p.blocks;
     a.per = (int)per;
-    a.segments = (int)((blocks + per - 1) / per);
+    a.segments = (int)((p.blocks + per - 1) / per);
     if (a.segments == 1) break;
-    if (!p.step && a.window == 0) {
-      int low = 0, high = p.tiles - 1;  // the first tile of more blocks than `per`
+    if (!p.step && a.window == 0) {  // only the rows of more blocks than a share
+      int low = 0, high = p.tiles - 1;  // the first tile of more
       while (low < high) {
         const int mid = (low + high) / 2;
-        if (tile_blocks(mid) > per)
+        if (attend4_tile_blocks(p, mid, a) > per)
           high = mid;
         else
           low = mid + 1;
       }
-      a.part_row0 = low * each;
+      a.part_row0 = low * p.each;
     }
-    if ((long long)a.segments * kv_count * (a.rows - a.part_row0) * (head + 2) <= (long long)IGL_ATTEND4_FLOATS) break;
+    if (floats(a.segments) <= (long long)IGL_ATTEND4_FLOATS) break;
     per += (per + 7) / 8;
   }
   return p;
@@ -1172,17 +1159,21 @@ static hipError_t attend4_launch(const Attend4Args &a, const Attend4Plan &p, int
   constexpr int T = HEAD >= 256 ? 1 : 2;
   const dim3 grid(p.tiles, a.segments, kv_count);
   if (!p.step) {
-    constexpr int size = Tile4Shape<HEAD>::LDS;
-    if (size > 65536) {  // granting it again changes nothing
+    if constexpr (HEAD >= 128) {
+      constexpr int size = Tile4Shape<HEAD>::LDS;
+      static_assert(size > 65536 && size <= 163840, "a granted size");
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&attend4_tile_kernel<HEAD, FMT>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, size);
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, size);  // again: no change
       if (e != hipSuccess) return e;
+      hipLaunchKernelGGL((attend4_tile_kernel<HEAD, FMT>), grid, dim3(512), (size_t)size, stream, a);
     }
-    hipLaunchKernelGGL((attend4_tile_kernel<HEAD, FMT>), grid, dim3(512), (size_t)size, stream, a);
+  } else if (p.deep) {
+    if constexpr (HEAD < 256)
+      hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, 2 * T>), grid, dim3(256), 0, stream, a);
   } else if (p.pair) {
-    hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, 1, true, T>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, T>), grid, dim3(256), 0, stream, a);
   } else {
-    hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, 1, false, T>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, false, T>), grid, dim3(256), 0, stream, a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.segments == 1) return e;

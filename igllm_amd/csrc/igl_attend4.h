@@ -80,15 +80,16 @@ __host__ __device__ inline Blocks4 attend4_blocks(int block, int first, int last
 }
 
 // The lane of a row of a key/value head.
-__device__ __forceinline__ int attend4_lane(int row, const Attend4Args &a) {
+__host__ __device__ __forceinline__ int attend4_lane(int row, const Attend4Args &a) {
   return (int)(((uint64_t)(uint32_t)row * a.share_mul) >> a.share_shift);
 }
 
 // Segments a row's blocks are cut into, at most: the fold takes one a thread.
 constexpr int kAttend4Segments = 256;
 
-// The position whose row a slot holds once `newest` is laid; INT_MAX: none.
-__device__ __forceinline__ int attend4_place(int slot, const Attend4Args &a) {
+// The position whose row a slot holds once `newest` is laid, INT_MAX for none; a
+// first position is its slot's before it is laid too.
+__host__ __device__ __forceinline__ int attend4_place(int slot, const Attend4Args &a) {
   int back = a.newest_slot - slot;
   if (back < 0) back += a.span - a.sinks;
   int place = a.newest - back;
@@ -351,7 +352,7 @@ struct QueryLoad {
 };
 
 // Whether a lane at `place` sees a slot's position.
-__device__ __forceinline__ bool attend4_seen(int slot, int place, const Attend4Args &a) {
+__host__ __device__ __forceinline__ bool attend4_seen(int slot, int place, const Attend4Args &a) {
   const int at = attend4_place(slot, a);
   return at <= place && (a.window == 0 || at > place - a.window || at < a.sinks);
 }
@@ -359,8 +360,8 @@ __device__ __forceinline__ bool attend4_seen(int slot, int place, const Attend4A
 // Whether every lane from place_low to place_high sees all of a run's `count` slots
 // from slot0 on: all past the sinks, and from the oldest position that the last
 // lane sees to the first lane's own (a slot of another turn would lie outside).
-__device__ __forceinline__ bool attend4_all(int slot0, int count, int ahead, int place_low, int place_high,
-                                            const Attend4Args &a) {
+__host__ __device__ __forceinline__ bool attend4_all(int slot0, int count, int ahead, int place_low, int place_high,
+                                                     const Attend4Args &a) {
   const int place0 = slot0 + ahead;
   return slot0 >= a.sinks && slot0 <= a.span - count && place0 <= place_low - (count - 1) &&
          (a.window == 0 || place0 > place_high - a.window);
@@ -1195,12 +1196,9 @@ static hipError_t attend4_launch_format(const Attend4Args &a, const Attend4Plan 
   return attend4_launch<HEAD, IGL_CACHE4_E2M1>(a, p, kv_count, stream);
 }
 
-extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_share, const float *query, int lane_stride,
-                                         int place_first, int window, int lanes, float score_scale, float *blend_out,
-                                         float *work, hipStream_t stream) {
+static Attend4Args attend4_args(const igl_cache4 *store, int group_share, const float *query, int lane_stride,
+                                int place_first, int window, int lanes, float score_scale, float *blend_out) {
   Attend4Args a = {};
-  const long long rows = (long long)lanes * group_share;
-  if (rows > 0x7FFFFFFF - 64) return hipErrorInvalidValue;
   a.key_code = store->key_code;
   a.key_gain = store->key_gain;
   a.value_code = store->value_code;
@@ -1217,7 +1215,7 @@ extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_shar
   a.newest = place_first + lanes - 1;
   a.newest_slot = a.newest < a.sinks ? -1 : cache4_slot(a.newest, a.sinks, a.span);
   a.window = window;
-  a.rows = (int)rows;
+  a.rows = lanes * group_share;
   // rows below 2^31: a multiplier that is less than share / 2^shift too large, 2^shift >= 2^31 share
   a.share_shift = 31;
   while ((1 << (a.share_shift - 31)) < group_share) ++a.share_shift;
@@ -1226,9 +1224,18 @@ extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_shar
   const double factor = (double)store->key_scale * score_scale * 1.4426950408889634 * 256.0;
   a.key_part = (float)frexp(factor, &a.key_power);
   a.value_scale = store->value_scale * 256.0f;
+  return a;
+}
+
+extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_share, const float *query, int lane_stride,
+                                         int place_first, int window, int lanes, float score_scale, float *blend_out,
+                                         float *work, hipStream_t stream) {
+  if ((long long)lanes * group_share >= 1 << 28) return hipErrorInvalidValue;  // a grid has fewer than 2^32 threads
+  Attend4Args a =
+      attend4_args(store, group_share, query, lane_stride, place_first, window, lanes, score_scale, blend_out);
   const Attend4Plan p = attend4_plan(a, store->head_size, store->kv_count);
-  a.part_out = work;
   const size_t parts = (size_t)a.segments * store->kv_count * (size_t)(a.rows - a.part_row0);
+  a.part_out = work;
   a.part_base = work + parts * store->head_size;
   a.part_total = a.part_base + parts;
   switch (store->head_size) {

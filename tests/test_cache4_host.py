@@ -181,6 +181,40 @@ def test_launches_stay_inside_their_buffers(host, head, kv, share):
     assert host.launches()[1] == 0
 
 
+PLANS = [  # head, kv, span, sinks, share, place, window, lanes
+    (64, 1, 1, 0, 1, 0, 0, 1), (64, 1, 1, 0, 64, 9, 1, 1), (128, 2, 65, 0, 3, 0, 0, 65), (256, 1, 516, 4, 8, 700, 512, 1),
+    (256, 1, 2600, 4, 8, 0, 512, 2047), (512, 1, 2047, 0, 4, 0, 0, 2047), (512, 1, 16384, 0, 8, 15000, 0, 160),
+    (512, 1, 16384, 0, 8, 8000, 0, 300), (128, 8, 131072, 0, 4, 131071, 0, 1), (512, 4, 40000, 1, 8, 39990, 0, 10),
+    (128, 16, 5000, 0, 8, 0, 0, 5000), (512, 16, 3000, 5, 8, 900, 700, 2000), (64, 8, 300, 299, 2, 0, 0, 300),
+    (256, 1, 100000, 17, 1, 99000, 50000, 17), (128, 1, 700, 0, 64, 5000, 300, 400), (256, 2, 65, 64, 2, 900, 1, 1),
+]
+
+
+def random_plans(count=400):
+    rng = np.random.default_rng(11)
+    for _ in range(count):
+        head, kv, share = int(rng.choice([64, 128, 256, 512])), int(rng.choice([1, 2, 3, 8])), int(rng.integers(1, 65))
+        span = int(2 ** rng.uniform(0, 12.5))
+        sinks = int(rng.integers(0, min(span, 1 + int(2 ** rng.uniform(0, 8)))))
+        ring = span - sinks
+        lanes = int(min(2 ** rng.uniform(0, 11), ring))
+        if rng.random() < 0.5:  # everything there is
+            place, window = int(rng.integers(0, span - lanes + 1)), 0
+        else:
+            window = int(rng.integers(1, ring - lanes + 2))
+            place = int(2 ** rng.uniform(0, 24)) - 1
+        yield head, kv, span, sinks, share, place, window, lanes
+
+
+def test_every_plan_covers_what_its_rows_see(lib):
+    """The attention's tiles, blocks, segments, masks and partials, by counting:
+    each slot a lane sees lies in one block of one segment, no block is taken for
+    wholly visible that is not, and the partials fit their room."""
+    lib.plan4_check.restype, lib.plan4_check.argtypes = ctypes.c_int, [ctypes.c_int] * 8
+    for plan in PLANS + list(random_plans()):
+        assert lib.plan4_check(*plan) == 0, plan
+
+
 def test_oracle_agrees_with_itself():
     """What is stored stands for the nearest value there is: every level of every
     gain is stored as itself, and no other code of the chosen gain is nearer."""

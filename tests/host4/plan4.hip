@@ -70,3 +70,17 @@ extern "C" int plan4_check(int head, int kv, int span, int sinks, int share, int
   }
   return 0;
 }
+
+// The form a call takes: 0 tiles of 64 rows, 1 of sixteen, 2 of eight, 3 the same
+// in deep blocks; plus 4 times its segments.
+extern "C" int plan4_form(int head, int kv, int span, int sinks, int share, int place, int window, int lanes) {
+  igl_cache4 store = {};
+  store.cache_span = span;
+  store.sink_count = sinks;
+  store.kv_count = kv;
+  store.head_size = head;
+  store.key_scale = store.value_scale = 1.0f;
+  Attend4Args a = attend4_args(&store, share, nullptr, 0, place, window, lanes, 1.0f, nullptr);
+  const Attend4Plan p = attend4_plan(a, head, kv);
+  return (p.deep ? 3 : p.pair ? 2 : p.step ? 1 : 0) + 4 * a.segments;
+}

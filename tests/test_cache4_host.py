@@ -215,6 +215,20 @@ def test_every_plan_covers_what_its_rows_see(lib):
         assert lib.plan4_check(*plan) == 0, plan
 
 
+@pytest.mark.parametrize("form,segments,plan", [
+    (2, 9, (256, 1, 516, 4, 8, 5000, 512, 1)),      # eight rows
+    (3, 53, (64, 8, 40000, 0, 1, 39999, 0, 1)),     # in deep blocks
+    (1, 126, (512, 1, 16384, 0, 8, 16000, 0, 5)),   # sixteen
+    (1, 1, (256, 1, 2600, 4, 8, 0, 512, 1000)),     # too few blocks for tiles
+    (0, 1, (256, 1, 2600, 4, 8, 0, 512, 2047)),     # tiles of 64
+    (0, 12, (512, 1, 16384, 0, 8, 15000, 0, 160)),  # one turn of the card
+    (1, 1, (64, 1, 2047, 0, 8, 0, 0, 2047)),        # 64-dim heads have none
+])
+def test_forms(lib, form, segments, plan):
+    got = lib.plan4_form(*plan)
+    assert (got % 4, got // 4) == (form, segments)
+
+
 def test_oracle_agrees_with_itself():
     """What is stored stands for the nearest value there is: every level of every
     gain is stored as itself, and no other code of the chosen gain is nearer."""

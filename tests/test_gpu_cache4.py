@@ -232,6 +232,18 @@ def check(got, query, rows, share, head, place, window, sinks, score, picks=None
     (1, 8, 64, 4, 70, 30, 2, 40, 0, 0),          # a window of two
     (1, 8, 256, 4, 70, 30, 1, 3, 0, 0),          # itself and the sinks
     (1, 2, 512, 0, 65, 64, 65, 1, 0, 0),         # one slot of a second block
+    (8, 1, 64, 0, 40000, 39999, 0, 1, 0, 0),     # deep blocks
+    (8, 1, 128, 9, 41000, 90000, 40900, 1, 0, 0),  # across the wrap
+    (1, 64, 128, 5, 300, 290, 0, 9, 4, 4),       # steps of many rows
+    # tiles of 64 rows
+    (16, 4, 128, 0, 700, 440, 0, 250, 0, 0),     # as many blocks each
+    (8, 8, 256, 5, 560, 3000, 300, 250, 4, 4),   # windows across the wrap, rows off alignment
+    (4, 16, 512, 3, 720, 9000, 450, 250, 0, 0),
+    (2, 8, 128, 3, 6500, 9000, 6400, 60, 0, 0),  # segments of every tile, the last one short
+    (2, 8, 512, 0, 4400, 4310, 0, 90, 0, 0),
+    (2, 8, 256, 0, 1100, 0, 0, 1100, 0, 0),      # a prompt, its long tiles cut
+    (1, 8, 512, 7, 1500, 0, 0, 1400, 0, 0),
+    (4, 7, 256, 70, 1170, 2000, 600, 500, 0, 0),  # odd shares, sinks past a block
 ])
 def test_attend(backend, fmt, kv, share, head, sinks, span, place, window, lanes, pad, off):
     print("case attend", fmt, kv, share, head, sinks, span, place, window, lanes, pad, off, flush=True)
@@ -243,6 +255,70 @@ def test_attend(backend, fmt, kv, share, head, sinks, span, place, window, lanes
     got = attend(backend, store, share, query, place, window, score, pad, off)
     check(got, query, rows_of(host, fmt, span, sinks), share, head, place, window, sinks, score)
     close(store)
+
+
+FORMS = [(1, 8, 128, 1, 400), (1, 8, 512, 7, 400), (16, 8, 128, 130, 600), (8, 8, 256, 260, 700), (8, 16, 512, 130, 500)]
+
+
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,share,head,lanes,span", FORMS)
+@pytest.mark.parametrize("low,high,scale", [(0, 8, 16.0), (0, 256, 2.0 ** -9), (0x78, 0x80, 2.0 ** -13)])
+def test_gains_of_every_size(backend, fmt, kv, share, head, lanes, span, low, high, scale):
+    """Gains below e4m3's normal numbers, any byte (signs too), the largest."""
+    print("case gains", fmt, kv, share, head, lanes, low, flush=True)
+    rng = np.random.default_rng(low + head)
+    host = ring_bytes(rng, span, kv * head, fmt)
+    for side in (1, 3):
+        host[side][:] = rng.integers(low, high, size=host[side].shape, dtype=np.uint8)
+    place = span - lanes
+    store = backend.cache4(fmt, span, 0, kv, head, scale, 0.75 * scale, *(backend.upload(b) for b in host))
+    query = rng.normal(size=(lanes, kv * share * head)).astype(np.float32)
+    score = 1.0 / np.sqrt(head)
+    got = attend(backend, store, share, query, place, 0, score)
+    check(got, query, rows_of(host, fmt, span, 0, scale), share, head, place, 0, 0, score, [0, lanes - 1])
+    close(store)
+
+
+@pytest.mark.parametrize("kv,share,head,lanes,span", FORMS)
+@pytest.mark.parametrize("score", [0.0, -0.7, 1e-38, -1e-30])
+def test_score_scales(backend, kv, share, head, lanes, span, score):
+    """No scale at all (the mean of what is seen), one below zero, and the least."""
+    print("case score", kv, share, head, lanes, score, flush=True)
+    rng = np.random.default_rng(head)
+    host = ring_bytes(rng, span, kv * head, c4.E2M1)
+    place = span - lanes
+    store = open_ring(backend, c4.E2M1, span, 0, kv, head, host)
+    query = rng.normal(size=(lanes, kv * share * head)).astype(np.float32)
+    got = attend(backend, store, share, query, place, 0, score)
+    check(got, query, rows_of(host, c4.E2M1, span, 0), share, head, place, 0, 0, score, [0, lanes - 1])
+    close(store)
+
+
+@pytest.mark.parametrize("kv,share,head,lanes,span", FORMS)
+def test_calls_on_two_desks(backend, kv, share, head, lanes, span):
+    """Two desks, each on its stream and with its own workspace, at once: what each
+    gives alone, to the bit, call after call."""
+    from igllm_amd.backend import Backend
+    print("case two desks", kv, share, head, lanes, flush=True)
+    rng = np.random.default_rng(head)
+    host = ring_bytes(rng, span, kv * head, c4.INT4)
+    place, stride = span - lanes, kv * share * head
+    query = [rng.normal(size=(lanes, stride)).astype(np.float32) for _ in range(2)]
+    other = Backend()
+    desks = [backend, other]
+    stores = [open_ring(d, c4.INT4, span, 0, kv, head, host) for d in desks]
+    want = [attend(d, s, share, q, place, 0, 0.1) for d, s, q in zip(desks, stores, query)]
+    dq = [d.upload(q) for d, q in zip(desks, query)]
+    do = [[d.alloc(q.nbytes) for _ in range(6)] for d, q in zip(desks, query)]
+    for turn in range(6):
+        for i, d in enumerate(desks):
+            d.attend4_lanes_dev(stores[i], share, dq[i], stride, place, 0, lanes, 0.1, do[i][turn])
+    for i, d in enumerate(desks):
+        d.sync()
+        for out in do[i]:
+            assert np.array_equal(out.get(np.float32, want[i].size).reshape(want[i].shape), want[i])
+        close(stores[i], dq[i], *do[i])
+    other.close()
 
 
 @pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
@@ -351,7 +427,8 @@ def test_a_run_of_steps(backend):
     close(store, dk, dv, dq, do, out)
 
 
-@pytest.mark.parametrize("lanes,place,head", [(1, 4000, 256), (3, 3000, 512), (100, 1900, 256), (130, 0, 512)])
+@pytest.mark.parametrize("lanes,place,head", [(1, 4000, 256), (3, 3000, 512), (100, 1900, 256), (130, 0, 512),
+                                              (200, 9000, 256), (1500, 0, 512)])
 def test_recorded_and_replayed(backend, lanes, place, head):
     """Rows laid and attended in a recording, replayed over other rows with the
     program's own calls between: every replay equals the eager calls to the bit,
@@ -392,6 +469,31 @@ def test_recorded_and_replayed(backend, lanes, place, head):
         backend.replay_free(replay)
     assert generation(ctypes.byref(backend.desk)) == before
     close(store, side, dk, dv, dq, do, do2)
+
+
+@pytest.mark.parametrize("kv,share,head,lanes,span", FORMS[2:])
+def test_tiles_beside_slots_without_rows(backend, kv, share, head, lanes, span):
+    """Tiles of 64 rows: slots that no position was laid in, and a NaN in a query,
+    touch no other row."""
+    print("case tiles unwritten", kv, share, head, lanes, flush=True)
+    rng = np.random.default_rng(head)
+    held = span - 70
+    host = ring_bytes(rng, span, kv * head, c4.INT4)
+    query = rng.normal(size=(lanes, kv * share * head)).astype(np.float32)
+    bad = (3 * share + 1) * head
+    got = []
+    for byte in (0xFF, 0x00):
+        for b in host[0], host[2]:
+            b[held:] = byte
+        for g in host[1], host[3]:
+            g[:, held:] = 0x7F if byte else 0
+        store = open_ring(backend, c4.INT4, span, 0, kv, head, host)
+        got.append(attend(backend, store, share, query, held - lanes, 0, 0.1))
+        close(store)
+        query[5, bad] = np.nan  # the second time
+    assert np.all(np.isnan(got[1][5, bad:bad + head]))
+    got[1][5, bad:bad + head] = got[0][5, bad:bad + head]
+    assert np.array_equal(got[0], got[1])
 
 
 def test_offsets_past_32_bits(backend):

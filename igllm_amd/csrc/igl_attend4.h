@@ -285,8 +285,6 @@ __device__ __forceinline__ float query_factor(const Attend4Args &a, float top, f
 }
 
 typedef float float2_t __attribute__((ext_vector_type(2)));
-// Four floats at any address of a float: rows need no alignment.
-typedef float float4a_t __attribute__((ext_vector_type(4), aligned(4)));
 
 // Two values as two binary16 terms each, x = hi + lo to 2^-22 of itself.
 __device__ __forceinline__ void two_terms(float x, float y, half2_t &hi, half2_t &lo) {

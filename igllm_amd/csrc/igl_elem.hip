@@ -315,8 +315,10 @@ static Cache4Args cache4_args(const igl_cache4 *store, int row_stride, int place
   return a;
 }
 
-static bool cache4_rows_vec(const void *p, int row_stride, int lanes) {
-  return ((uintptr_t)p & 15u) == 0 && (lanes == 1 || (row_stride & 3) == 0);
+// Workgroups of eight values a thread; 0: more than a grid has, 2^32 threads.
+static unsigned cache4_groups(const Cache4Args &a) {
+  const long long groups = ((long long)a.lanes * (a.width / 8) + 255) / 256;
+  return groups < 1 << 24 ? (unsigned)groups : 0;
 }
 
 extern "C" hipError_t igl_launch_cache4_lay(const igl_cache4 *store, const float *key, const float *value,
@@ -324,21 +326,12 @@ extern "C" hipError_t igl_launch_cache4_lay(const igl_cache4 *store, const float
   Cache4Args a = cache4_args(store, row_stride, place_first, lanes);
   a.in[0] = key;
   a.in[1] = value;
-  const long long blocks = ((long long)lanes * (a.width / 8) + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks, 2);
-  const bool vec = cache4_rows_vec(key, row_stride, lanes) && cache4_rows_vec(value, row_stride, lanes);
-  if (store->format == IGL_CACHE4_INT4) {
-    if (vec)
-      hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_INT4, true>), grid, dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_INT4, false>), grid, dim3(256), 0, stream, a);
-  } else {
-    if (vec)
-      hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_E2M1, true>), grid, dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_E2M1, false>), grid, dim3(256), 0, stream, a);
-  }
+  const dim3 grid(cache4_groups(a), 2);
+  if (!grid.x) return hipErrorInvalidValue;
+  if (store->format == IGL_CACHE4_INT4)
+    hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_INT4>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_E2M1>), grid, dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -347,21 +340,12 @@ extern "C" hipError_t igl_launch_cache4_read(const igl_cache4 *store, int place_
   Cache4Args a = cache4_args(store, row_stride, place_first, lanes);
   a.out[0] = key;
   a.out[1] = value;
-  const long long blocks = ((long long)lanes * (a.width / 8) + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks, key && value ? 2 : 1);
+  const dim3 grid(cache4_groups(a), key && value ? 2 : 1);
   const int side0 = key ? 0 : 1;
-  const bool vec = (!key || cache4_rows_vec(key, row_stride, lanes)) && (!value || cache4_rows_vec(value, row_stride, lanes));
-  if (store->format == IGL_CACHE4_INT4) {
-    if (vec)
-      hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_INT4, true>), grid, dim3(256), 0, stream, a, side0);
-    else
-      hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_INT4, false>), grid, dim3(256), 0, stream, a, side0);
-  } else {
-    if (vec)
-      hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_E2M1, true>), grid, dim3(256), 0, stream, a, side0);
-    else
-      hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_E2M1, false>), grid, dim3(256), 0, stream, a, side0);
-  }
+  if (!grid.x) return hipErrorInvalidValue;
+  if (store->format == IGL_CACHE4_INT4)
+    hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_INT4>), grid, dim3(256), 0, stream, a, side0);
+  else
+    hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_E2M1>), grid, dim3(256), 0, stream, a, side0);
   return hipGetLastError();
 }

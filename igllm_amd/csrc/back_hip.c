@@ -920,7 +920,7 @@ int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_sha
   int code;
   if (!st) return IGL_FAIL_STATE;
   if (!store || !query_dev || !blend_out_dev || window < 0 || group_share < 1) return cache4_null(st);
-  if (group_share > 64) {
+  if (group_share > 64 || (long long)lane_count * group_share >= 1 << 28) {
     desk_fail(st, IGL_FAIL_SUPPORT);
     return IGL_FAIL_SUPPORT;
   }

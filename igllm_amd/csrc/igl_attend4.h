@@ -6,6 +6,21 @@
 // or t < sinks):
 //     o = sum_t 2^(f q . k_t - m) v_t / sum_t 2^(f q . k_t - m),
 // f the score scale, the key scale and log2 e, m a base near the peak.
+//
+// On the matrix cores, in binary16 with fp32 sums.  A key or value is level * gain:
+// eight significant bits at most, exact in binary16 with the gain over 256 (their
+// scales are multiplied in afterwards).  Queries and weights are two binary16 terms
+// each, high and low, 2^-22 of themselves: one term would leave 2^-11, two products
+// leave blends as near their 64-bit value as fp32 sums do (3e-7 measured).  Products
+// are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane that decodes
+// codes holds a row's eight dims, or a dim's eight rows, as one operand, and a query
+// row's scores lie along lanes as its weights are wanted.
+//
+// A row's base is a whole number about twelve below the block's peak, moved only
+// where a peak leaves it by a few: most blocks rescale nothing, a block's largest
+// weight is 2^8 to 2^15, and its small ones are held down to binary16's last step,
+// 2^-24.  It follows peaks down too, to 58 below the highest, so that positions far
+// below others keep what fp32 sums keep of them.
 #pragma once
 
 #include <float.h>
@@ -422,7 +437,15 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
 // scores divided by slots (a wave T tiles of 16, every dim), the blend by dims
 // (VD ways) and then by slots (VS ways): so a wave's chain from one barrier to
 // the next is a quarter of the block's work.  Weights cross between the two
-// divisions through LDS, against a base that the four waves agree on.
+// divisions through LDS, against a base that the four waves agree on.  The next
+// block's codes are on their way while this one's are used.  Up to eight rows
+// (PAIR) put both terms of a row into the sixteen columns of one product.
+//
+// A short context is bound by its chain, about 1.5 us a block, so it is cut over as
+// many workgroups as it has blocks: a 512 window of 256-dim heads 5.6 us and 3.7 for
+// the fold (one wave a block took 16.9 in all), 16384 positions 6.2 + 3.6.  A long
+// one is bound by its bytes and their decoding (16 us of vector issue a CU and 3 of
+// matrix): 131072 positions of eight 128-dim heads, 143 MB, in 35.4 us, 4.0 TB/s.
 template <int HEAD, bool PAIR, int T>
 struct Step4Shape {
   static constexpr int KL = HEAD >= 128 ? HEAD / 128 : 1;  // key chunks of a row a lane reads
@@ -701,6 +724,12 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
 // A wave decodes the next block while it multiplies this one's keys: an item of 32
 // dims of a key and one of four dims of a lane group's eight slots of values a
 // thread, in straight code that the scheduler is told to lay between the products.
+// Blends leave through LDS as whole rows (scattered dwords were 4 us of a window's 41).
+//
+// Bound by issue: vector work, half of it decoding, and products take turns on a SIMD,
+// 164k of 207k cycles for 2047 lanes of 512-dim heads, 124 us, 34 GFLOP before the
+// second terms; of a 512 window of 256-dim heads 36 us.  Two waves a SIMD is what 250
+// registers leave; 64 rows a workgroup halve the decoding of 32 (156 and 41 us).
 //
 // LDS.  Keys: a slot's dims in 16-byte pieces, piece s of chunk c (dims 32 c + 8 s ..
 // + 7, a dword of codes) at s HEAD / 32 + c, xor the slot's low bits.  Values: a dim's
@@ -992,7 +1021,11 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
 
 // Folds the segments of a row: a workgroup a row and DIMS of its dims, thread
 // (c, s) of four dims c and the segments s, s + SL, ...  Thread t finds segment
-// t's weight; the blends are requested before.
+// t's weight; the blends are requested before.  Segments are added in the same
+// order every time.  Few rows are cut by dims to fill the card, bound by the chain
+// of three loads (3.6 us at 9 and at 256 segments); many rows are taken whole, so
+// that statistics are read once (7928 rows of two segments, 512 dims, 12 us, 4.1
+// TB/s; by 64 dims 60).
 template <int DIMS>
 __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int head_size) {
   constexpr int COLS = DIMS / 4, SL = 256 / COLS;
@@ -1228,7 +1261,7 @@ static Attend4Args attend4_args(const igl_cache4 *store, int group_share, const 
 extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_share, const float *query, int lane_stride,
                                          int place_first, int window, int lanes, float score_scale, float *blend_out,
                                          float *work, hipStream_t stream) {
-  if ((long long)lanes * group_share >= 1 << 28) return hipErrorInvalidValue;  // a grid has fewer than 2^32 threads
+  // rows fewer than 2^28, so that a grid has fewer than 2^32 threads
   Attend4Args a =
       attend4_args(store, group_share, query, lane_stride, place_first, window, lanes, score_scale, blend_out);
   const Attend4Plan p = attend4_plan(a, store->head_size, store->kv_count);

@@ -294,7 +294,9 @@ int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first
  * query_dev and blend_out_dev: [lane_count][kv_count * group_share][head_size]
  * floats, lanes lane_stride apart.  Every lane's keys and values must already be
  * in the ring; a ring too short to hold all that the lanes see is refused with
- * IGL_FAIL_ARGUMENT.  A call allocates nothing, whatever its size. */
+ * IGL_FAIL_ARGUMENT, lane_count * group_share of 2^28 and more with
+ * IGL_FAIL_SUPPORT.  A call allocates nothing, whatever its size: its partials lie
+ * in 48 MiB that the desk holds from its opening. */
 int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_share,
                           const float *query_dev, int lane_stride, int place_first, int window,
                           int lane_count, float score_scale, float *blend_out_dev);

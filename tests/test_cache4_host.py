@@ -145,6 +145,7 @@ def test_bad_calls_are_refused(host):
         assert call() == ARG
         assert host.take() == ARG
     assert host.attend(c, 65, room, 65 * 256, 0, 0, 1, room) == SUPPORT and host.take() == SUPPORT
+    assert host.attend(c, 64, room, 64 * 256, 0, 1, 1 << 22, room) == SUPPORT and host.take() == SUPPORT
     assert host.launches() == before
     assert host.lib.igl_cache4_lay_dev(None, ctypes.byref(c), room, room, 256, 0, 1) == native.IGL_FAIL_STATE
     assert host.lib.igl_cache4_read_dev(None, ctypes.byref(c), 0, 1, room, room, 256) == native.IGL_FAIL_STATE

@@ -48,7 +48,7 @@ struct Attend4Args {
   int share_shift;
   int key_power;         // key scale, score scale, log2 e and 256: key_part 2^key_power
   float key_part;        // in [1/2, 1), or of a score scale below zero
-  float value_scale;     // times 256
+  float value_scale;
   int segments;          // of a row tile's blocks, each `per` of them and the last what is left
   int per;
   int part_row0;         // first row whose blocks are cut
@@ -296,7 +296,7 @@ __device__ __forceinline__ float query_factor(const Attend4Args &a, float top, f
   if (up > 126) up = 126;
   scale = __builtin_amdgcn_ldexpf(a.key_part < 0.0f ? -1.0f : 1.0f, up);
   const float factor = __builtin_amdgcn_ldexpf(fabsf(a.key_part), a.key_power - up);
-  return factor < FLT_MIN ? FLT_MIN : factor;
+  return factor < FLT_MIN ? FLT_MIN : factor > FLT_MAX ? FLT_MAX : factor;  // nor too large for a score of zero
 }
 
 typedef float float2_t __attribute__((ext_vector_type(2)));
@@ -408,7 +408,7 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
   if (row > row_last) return;
   const int l = attend4_lane(row, a);
   float *dst = a.out + (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * HEAD;
-  float mul = a.value_scale;
+  float mul = 1.0f;
   if (a.segments > 1) {
     const size_t at = ((size_t)seg * gridDim.z + kv) * a.rows + row;
     dst = a.part_out + at * HEAD;
@@ -417,7 +417,7 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
       a.part_total[at] = total;
     }
   } else {
-    mul *= 1.0f / total;
+    mul = a.value_scale * (256.0f / total);  // the 256 that a gain is divided by
   }
   dst += dim0 + 4 * g * DPL;
 #pragma unroll
@@ -980,7 +980,7 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
     stats[wave * 32 + 16 + n] = total;
   }
   attend4_barrier();
-  float mul = a.value_scale;
+  float mul = 1.0f;
   if constexpr (SH > 1) {
     const float theirs = stats[(wave ^ 1) * 32 + n], m = fmaxf(base, theirs);
     const float mine = base != -INFINITY ? __builtin_amdgcn_exp2f(base - m) : 0.0f;
@@ -989,7 +989,7 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
     total = total * mine + stats[(wave ^ 1) * 32 + 16 + n] * part;
     mul *= mine;
   }
-  if (!split) mul *= 1.0f / total;
+  if (!split) mul *= a.value_scale * (256.0f / total);
   float *rows = reinterpret_cast<float *>(lds4) + sh * (16 * RT * HEAD) + (16 * rt + n) * HEAD;
 #pragma unroll
   for (int t = 0; t < TC; ++t)
@@ -1073,7 +1073,7 @@ __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int he
     }
   }
   if (sl) return;
-  const float mul = 1.0f / (red[4] + red[5] + red[6] + red[7]);
+  const float mul = a.value_scale * (256.0f / (red[4] + red[5] + red[6] + red[7]));
   *reinterpret_cast<float4a_t *>(a.out + attend4_row(row, kv, head_size, a) + d0) = acc * mul;
 }
 
@@ -1254,7 +1254,7 @@ static Attend4Args attend4_args(const igl_cache4 *store, int group_share, const 
   // log2 e, and the 256 that a gain is divided by
   const double factor = (double)store->key_scale * score_scale * 1.4426950408889634 * 256.0;
   a.key_part = (float)frexp(factor, &a.key_power);
-  a.value_scale = store->value_scale * 256.0f;
+  a.value_scale = store->value_scale;
   return a;
 }
 

@@ -295,6 +295,27 @@ def test_score_scales(backend, kv, share, head, lanes, span, score):
 
 
 @pytest.mark.parametrize("kv,share,head,lanes,span", FORMS)
+@pytest.mark.parametrize("scale", [2.0 ** 121, 2.0 ** -100])
+def test_scales_near_a_floats_ends(backend, kv, share, head, lanes, span, scale):
+    """Layers' scales that a float just holds, the largest value below its end; and
+    queries of zero beside a factor that no float holds, which see the mean."""
+    print("case ends", kv, share, head, lanes, scale, flush=True)
+    rng = np.random.default_rng(head)
+    host = ring_bytes(rng, span, kv * head, c4.INT4)
+    place = span - lanes
+    store = open_ring(backend, c4.INT4, span, 0, kv, head, host, scale)
+    query = rng.normal(size=(lanes, kv * share * head)).astype(np.float32)
+    score = float(np.float32(10.0 / np.sqrt(head) * SCALE / scale))
+    rows = rows_of(host, c4.INT4, span, 0, scale)
+    got = attend(backend, store, share, query, place, 0, score)
+    check(got, query, rows, share, head, place, 0, 0, score, [0, lanes - 1])
+    query[:] = 0.0
+    got = attend(backend, store, share, query, place, 0, 1e30)
+    check(got, query, rows, share, head, place, 0, 0, 1e30, [0, lanes - 1])
+    close(store)
+
+
+@pytest.mark.parametrize("kv,share,head,lanes,span", FORMS)
 def test_calls_on_two_desks(backend, kv, share, head, lanes, span):
     """Two desks, each on its stream and with its own workspace, at once: what each
     gives alone, to the bit, call after call."""

@@ -445,7 +445,8 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
 // many workgroups as it has blocks: a 512 window of 256-dim heads 5.6 us and 3.7 for
 // the fold (one wave a block took 16.9 in all), 16384 positions 6.2 + 3.6.  A long
 // one is bound by its bytes and their decoding (16 us of vector issue a CU and 3 of
-// matrix): 131072 positions of eight 128-dim heads, 143 MB, in 35.4 us, 4.0 TB/s.
+// matrix): 131072 positions of eight 128-dim heads, 143 MB, in 35.4 us, 4.0 TB/s
+// (out of caches 39, 3.7).
 template <int HEAD, bool PAIR, int T>
 struct Step4Shape {
   static constexpr int KL = HEAD >= 128 ? HEAD / 128 : 1;  // key chunks of a row a lane reads
@@ -1131,13 +1132,14 @@ static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
     p.pair = a.rows <= 8;
     p.each = p.pair ? 8 : 16;
     p.block = head < 256 ? 128 : 64;
-    // Twice the slots between barriers where every workgroup still has two such
-    // blocks: 131072 positions of eight 128-dim heads 40.5 -> 35.6 us, of two 64-dim
-    // 11.0 -> 9.8, 40000 of eight the same.  Not of wide heads, whose rows already
-    // fill the registers: two 512-dim heads 32.9 -> 42.8.
+    // Four times the slots between barriers, and on their way, where every workgroup
+    // still has two such blocks: 131072 positions of eight 128-dim heads 40.5 -> 35.4 us
+    // in caches, as by twice the slots, but with the fold 43.7 out of them for 46.1;
+    // 65536 22.3 -> 19.8.  Not of wide heads, whose rows already fill the registers:
+    // two 512-dim heads by twice the slots 32.9 -> 42.8.
     p.deep = p.pair && head < 256 &&
-             (long long)attend4_blocks(2 * p.block, a.place, a.newest, a).count * kv_count >= 2 * 2 * cus;
-    p.block <<= p.deep;
+             (long long)attend4_blocks(4 * p.block, a.place, a.newest, a).count * kv_count >= 2 * 2 * cus;
+    if (p.deep) p.block *= 4;
     attend4_count(p, a);
   }
 
@@ -1201,7 +1203,7 @@ static hipError_t attend4_launch(const Attend4Args &a, const Attend4Plan &p, int
     }
   } else if (p.deep) {
     if constexpr (HEAD < 256)
-      hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, 2 * T>), grid, dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, 4 * T>), grid, dim3(256), 0, stream, a);
   } else if (p.pair) {
     hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, T>), grid, dim3(256), 0, stream, a);
   } else {

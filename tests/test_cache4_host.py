@@ -218,7 +218,8 @@ def test_every_plan_covers_what_its_rows_see(lib):
 
 @pytest.mark.parametrize("form,segments,plan", [
     (2, 9, (256, 1, 516, 4, 8, 5000, 512, 1)),      # eight rows
-    (3, 53, (64, 8, 40000, 0, 1, 39999, 0, 1)),     # in deep blocks
+    (3, 27, (64, 16, 40000, 0, 1, 39999, 0, 1)),    # in deep blocks
+    (2, 63, (64, 8, 40000, 0, 1, 39999, 0, 1)),     # of which each workgroup would have one
     (1, 126, (512, 1, 16384, 0, 8, 16000, 0, 5)),   # sixteen
     (1, 1, (256, 1, 2600, 4, 8, 0, 512, 1000)),     # too few blocks for tiles
     (0, 1, (256, 1, 2600, 4, 8, 0, 512, 2047)),     # tiles of 64

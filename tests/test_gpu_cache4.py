@@ -232,8 +232,10 @@ def check(got, query, rows, share, head, place, window, sinks, score, picks=None
     (1, 8, 64, 4, 70, 30, 2, 40, 0, 0),          # a window of two
     (1, 8, 256, 4, 70, 30, 1, 3, 0, 0),          # itself and the sinks
     (1, 2, 512, 0, 65, 64, 65, 1, 0, 0),         # one slot of a second block
-    (8, 1, 64, 0, 40000, 39999, 0, 1, 0, 0),     # deep blocks
+    (8, 1, 64, 0, 40000, 39999, 0, 1, 0, 0),     # long steps
     (8, 1, 128, 9, 41000, 90000, 40900, 1, 0, 0),  # across the wrap
+    (16, 1, 64, 0, 40000, 39999, 0, 1, 0, 0),    # in deep blocks
+    (16, 1, 128, 9, 41000, 90000, 40900, 1, 0, 0),
     (1, 64, 128, 5, 300, 290, 0, 9, 4, 4),       # steps of many rows
     # tiles of 64 rows
     (16, 4, 128, 0, 700, 440, 0, 250, 0, 0),     # as many blocks each

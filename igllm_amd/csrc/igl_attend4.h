@@ -1150,6 +1150,14 @@ static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
   const long long at_once = p.step ? 2 * cus : cus;
   long long per = ((p.step ? (long long)p.blocks * p.tiles : p.all) * kv_count + at_once - 1) / at_once;
   a.part_row0 = 0;
+  // One step workgroup a CU where it then has four blocks at most and partials are
+  // many and wide: five lanes at 16000, 512-dim heads 16.4 + 4.7 -> 16.2 + 4.1 us,
+  // eight 17.7 + 6.2 -> 18.7 + 4.4, five of four 256-dim at 4000 11.8 -> 10.3; but of
+  // 64-dim heads 6.0 -> 6.7, and twelve lanes, six blocks, 22.6 + 5.0 -> 24.2 + 4.0.
+  if (p.step && !p.pair && head >= 256) {
+    const long long one = ((long long)p.blocks * p.tiles * kv_count + cus - 1) / cus;
+    if (one <= 4) per = one;
+  }
   if (!p.step && (a.window > 0 || 4 * attend4_tile_blocks(p, 0, a) > 3 * p.blocks)) {
     // Tiles alike: the cheapest number of whole turns of the card, a workgroup's start
     // and end taken for one block and a share of 2^20 partial floats for another

@@ -220,7 +220,8 @@ def test_every_plan_covers_what_its_rows_see(lib):
     (2, 9, (256, 1, 516, 4, 8, 5000, 512, 1)),      # eight rows
     (3, 27, (64, 16, 40000, 0, 1, 39999, 0, 1)),    # in deep blocks
     (2, 63, (64, 8, 40000, 0, 1, 39999, 0, 1)),     # of which each workgroup would have one
-    (1, 126, (512, 1, 16384, 0, 8, 16000, 0, 5)),   # sixteen
+    (1, 84, (512, 1, 16384, 0, 8, 16000, 0, 5)),    # sixteen, one workgroup a CU
+    (1, 79, (512, 1, 16384, 0, 8, 15000, 0, 12)),   # two
     (1, 1, (256, 1, 2600, 4, 8, 0, 512, 1000)),     # too few blocks for tiles
     (0, 1, (256, 1, 2600, 4, 8, 0, 512, 2047)),     # tiles of 64
     (0, 12, (512, 1, 16384, 0, 8, 15000, 0, 160)),  # one turn of the card

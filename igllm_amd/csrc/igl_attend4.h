@@ -408,7 +408,7 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
   if (row > row_last) return;
   const int l = attend4_lane(row, a);
   float *dst = a.out + (size_t)l * a.lane_stride + ((size_t)kv * a.share + (row - l * a.share)) * HEAD;
-  float mul = 1.0f;
+  float mul = 1.0f, scale = 1.0f;
   if (a.segments > 1) {
     const size_t at = ((size_t)seg * gridDim.z + kv) * a.rows + row;
     dst = a.part_out + at * HEAD;
@@ -417,7 +417,10 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
       a.part_total[at] = total;
     }
   } else {
-    mul = a.value_scale * (256.0f / total);  // the 256 that a gain is divided by
+    // the 256 that a gain is divided by; the scale apart, as a total may be past 2^70
+    // and a float not hold their product
+    mul = 256.0f / total;
+    scale = a.value_scale;
   }
   dst += dim0 + 4 * g * DPL;
 #pragma unroll
@@ -426,7 +429,8 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
 #pragma unroll
     for (int j = 0; j < DPL; j += 4) {
       *reinterpret_cast<float4a_t *>(dst + r * DPL + j) =
-          float4_t{out[j][r] * mul, out[j + 1][r] * mul, out[j + 2][r] * mul, out[j + 3][r] * mul};
+          float4_t{out[j][r] * mul * scale, out[j + 1][r] * mul * scale, out[j + 2][r] * mul * scale,
+                   out[j + 3][r] * mul * scale};
     }
   }
 }
@@ -990,7 +994,8 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
     total = total * mine + stats[(wave ^ 1) * 32 + 16 + n] * part;
     mul *= mine;
   }
-  if (!split) mul *= a.value_scale * (256.0f / total);
+  if (!split) mul *= 256.0f / total;  // the value scale after it, as attend4_store has them
+  const float scale = split ? 1.0f : a.value_scale;
   float *rows = reinterpret_cast<float *>(lds4) + sh * (16 * RT * HEAD) + (16 * rt + n) * HEAD;
 #pragma unroll
   for (int t = 0; t < TC; ++t)
@@ -1012,7 +1017,7 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
     float4_t o = *reinterpret_cast<const float4_t *>(from);
     if (SH > 1) o += *reinterpret_cast<const float4_t *>(from + 16 * RT * HEAD);
     float *to = (split ? a.part_out + (part0 + r) * HEAD : a.out + attend4_row(row0 + r, kv, HEAD, a)) + 4 * piece;
-    *reinterpret_cast<float4a_t *>(to) = o;
+    *reinterpret_cast<float4a_t *>(to) = o * scale;
   }
   if (split && g == 0 && dw == 0 && sh == 0 && 16 * rt + n < count) {
     a.part_base[part0 + 16 * rt + n] = base;
@@ -1074,8 +1079,8 @@ __global__ __launch_bounds__(256) void attend4_fold_kernel(Attend4Args a, int he
     }
   }
   if (sl) return;
-  const float mul = a.value_scale * (256.0f / (red[4] + red[5] + red[6] + red[7]));
-  *reinterpret_cast<float4a_t *>(a.out + attend4_row(row, kv, head_size, a) + d0) = acc * mul;
+  const float mul = 256.0f / (red[4] + red[5] + red[6] + red[7]);
+  *reinterpret_cast<float4a_t *>(a.out + attend4_row(row, kv, head_size, a) + d0) = acc * mul * a.value_scale;
 }
 
 }  // namespace igl

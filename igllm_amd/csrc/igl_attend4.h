@@ -18,9 +18,12 @@
 //
 // A row's base is a whole number about twelve below the block's peak, moved only
 // where a peak leaves it by a few: most blocks rescale nothing, a block's largest
-// weight is 2^8 to 2^15, and its small ones are held down to binary16's last step,
-// 2^-24.  It follows peaks down too, to 58 below the highest, so that positions far
-// below others keep what fp32 sums keep of them.
+// weight is 2^8 to 2^15, and its small ones are held to half of binary16's last
+// step, 2^-25.  That is 2^-33 of the largest: of a weight 26 powers of two below it
+// in its own block 2^-7 is left, of one 33 below nothing, in other blocks 2^-22.  A
+// third term would hold them, for half as many products again.  Bases follow peaks
+// down too, to 58 below the highest, so that positions far below others keep what
+// fp32 sums keep of them.
 #pragma once
 
 #include <float.h>

@@ -296,7 +296,10 @@ int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first
  * in the ring; a ring too short to hold all that the lanes see is refused with
  * IGL_FAIL_ARGUMENT, lane_count * group_share of 2^28 and more with
  * IGL_FAIL_SUPPORT.  A call allocates nothing, whatever its size: its partials lie
- * in 48 MiB that the desk holds from its opening. */
+ * in 48 MiB that the desk holds from its opening.  Weights are held to
+ * 2^-22 of themselves, or to 2^-33 of the largest among the 32 to 512 slots taken
+ * with them if that is more: a blend that is small beside the row's values, as of a
+ * first position that has nearly all the weight and no value, is as exact as that. */
 int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_share,
                           const float *query_dev, int lane_stride, int place_first, int window,
                           int lane_count, float score_scale, float *blend_out_dev);

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import cache4_oracle as c4
-from test_gpu_cache4 import SCALE, attend, check, close, open_ring, ring_bytes
+from test_gpu_cache4 import SCALE, attend, check, close, open_ring, ring_bytes, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -45,4 +45,36 @@ def test_value_scales_under_falling_peaks(backend, kv, share, head, sinks, span,
         return c4.values(c4.unpack(host[2 * side][at]), host[2 * side + 1][:, at].T, c4.INT4, scales[side])
 
     check(got, query, rows, share, head, place, window, sinks, score)
+    close(store)
+
+
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,share,head,span", [(16, 1, 64, 40000), (16, 1, 128, 40000), (8, 4, 128, 65600)])
+def test_a_peaked_position_of_long_blocks(backend, fmt, kv, share, head, span):
+    """A position of zero value 26 powers of two above zero, all others' scores within
+    `near` powers of it, in blocks of 512 slots, and values in its own block alone:
+    weights are held to half of binary16's smallest step, 2^-25, beside one of 2^8 or
+    more, so the others, 2^(-18 - near) at least, to 2^(near - 7) of themselves."""
+    print("case peaked long", fmt, kv, share, head, span, flush=True)
+    rng = np.random.default_rng(head)
+    host = ring_bytes(rng, span, kv * head, fmt)
+    zero = 0x88 if fmt == c4.INT4 else 0x00
+    host[0][3] = 0x99 if fmt == c4.INT4 else 0x22  # level 1
+    host[1][:] = 0x08 if fmt == c4.INT4 else 0x10  # 2^-6 and 2^-5: others' scores are near zero
+    host[1][:, 3] = 0x38
+    host[2][3] = host[2][512:] = zero
+    store = open_ring(backend, fmt, span, 0, kv, head, host)
+    query = np.ones((1, kv * share * head), np.float32)
+    score = 18.0 / (head * float(np.float32(SCALE)))
+    got = attend(backend, store, share, query, span - 1, 0, score).reshape(kv, share, head)
+    rows = rows_of(host, fmt, span, 0)
+    s = rows(0, np.arange(span)).reshape(span, kv, head).sum(-1) * score
+    near = np.abs(np.delete(s, 3, 0)).max() / np.log(2.0)
+    w = np.exp(s)
+    v = rows(1, np.arange(512)).reshape(512, kv, head)
+    err = np.abs(got - (w[:512, :, None] * v).sum(0)[:, None] / w.sum(0)[:, None, None]).max()
+    size = ((w[:512, :, None] * np.abs(v)).sum(0) / w.sum(0)[:, None]).max()
+    print("near", near, "error over the weighted sizes", err / size, flush=True)
+    assert near < 4.0
+    assert err <= 2.0 ** (near - 7) * size
     close(store)

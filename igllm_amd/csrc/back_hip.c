@@ -839,7 +839,7 @@ static int cache4_dims(const igl_cache4 *store) {
          (store->head_size == 64 || store->head_size == 128 || store->head_size == 256 ||
           store->head_size == 512) &&
          store->kv_count >= 1 && store->kv_count <= 65535 && store->cache_span >= 1 &&
-         store->cache_span <= INT32_MAX - 256 && store->sink_count >= 0 &&
+         store->cache_span <= IGL_CACHE4_SPAN_MOST && store->sink_count >= 0 &&
          store->sink_count < store->cache_span;
 }
 

@@ -473,6 +473,7 @@ struct Step4Shape {
   static constexpr int MERGE = (VS - 1) * VD * DPL * 1024;  // the blends of waves that took other slots
   static constexpr int LDS = LOOP > MERGE ? LOOP : MERGE;
   static_assert(UB >= 1, "a blend step takes 32 slots");
+  static_assert(BLOCK <= IGL_ATTEND4_BLOCK_MOST, "slots are counted to a block's end");
 };
 
 template <int HEAD, int FMT, bool PAIR, int T>
@@ -510,7 +511,7 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
   auto load_keys = [&](int i) {
     const int slot0 = blocks.at(i) * BLOCK;
     const auto src = attend4_rows(a.key_code + (size_t)slot0 * row_bytes + head_bytes);
-    const bool whole = slot0 + BLOCK <= a.span;
+    const bool whole = slot0 <= a.span - BLOCK;
 #pragma unroll
     for (int j = 0; j < T; ++j) {
       const int at = 16 * (T * wave + j);
@@ -537,7 +538,7 @@ __global__ __launch_bounds__(256) void attend4_step_kernel(Attend4Args a) {
   auto load_values = [&](int i) {
     const int slot0 = blocks.at(i) * BLOCK;
     const auto src = attend4_rows(a.value_code + (size_t)slot0 * row_bytes + head_bytes);
-    const bool whole = slot0 + BLOCK <= a.span;
+    const bool whole = slot0 <= a.span - BLOCK;
 #pragma unroll
     for (int u = 0; u < UB; ++u) {
       const int at = 32 * (UB * vs + u);
@@ -805,7 +806,7 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
     const int slot0 = blocks.at(i) * BLOCK;
     const auto keys = attend4_rows(a.key_code + (size_t)slot0 * row_bytes + head_bytes);
     const auto values = attend4_rows(a.value_code + (size_t)slot0 * row_bytes + head_bytes);
-    if (slot0 + BLOCK <= a.span) {  // uniform: rows at scalar distances
+    if (slot0 <= a.span - BLOCK) {  // uniform: rows at scalar distances
       kr = __builtin_amdgcn_raw_buffer_load_b128(keys, k_lane, 0, 0);
 #pragma unroll
       for (int e = 0; e < 8; ++e)

@@ -222,6 +222,9 @@ size_t igl_attend_prep_work_floats(int place_bound, int window, int head_size, i
  * igl_gemv.hip).  Rows, queries and blends at any 4-byte alignment; `work`
  * holds IGL_ATTEND4_FLOATS floats. */
 #define IGL_ATTEND4_FLOATS (3u << 22)
+/* The attention counts slots to the end of a ring's last block in ints. */
+#define IGL_ATTEND4_BLOCK_MOST 512
+#define IGL_CACHE4_SPAN_MOST (INT32_MAX - IGL_ATTEND4_BLOCK_MOST)
 static inline size_t igl_cache4_room(int cache_span) { return ((size_t)cache_span + 63) / 64 * 64; }
 hipError_t igl_launch_cache4_lay(const igl_cache4 *store, const float *key, const float *value,
                                  int row_stride, int place_first, int lanes, hipStream_t stream);

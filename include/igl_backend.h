@@ -257,7 +257,7 @@ typedef enum igl_cache4_format {
  * anything.  head_size 64, 128, 256 or 512. */
 typedef struct igl_cache4 {
   int      format;      /* igl_cache4_format */
-  int      cache_span;  /* slots */
+  int      cache_span;  /* slots, below 2^31 - 512 */
   int      sink_count;  /* below cache_span */
   int      kv_count;
   int      head_size;

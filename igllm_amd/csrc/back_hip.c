@@ -882,6 +882,20 @@ static int cache4_check(igl_desk_state *st, const igl_cache4 *store, int place_f
   return IGL_OKAY;
 }
 
+/* Rows that laying or reading takes in one launch. */
+static int cache4_rows_check(igl_desk_state *st, const igl_cache4 *store, int place_first,
+                             int lanes, int row_stride) {
+  const int code =
+      cache4_check(st, store, place_first, lanes, place_first, row_stride,
+                   (long long)store->kv_count * store->head_size);
+  if (code != IGL_OKAY) return code;
+  if (igl_cache4_groups(store->kv_count * store->head_size, lanes) > IGL_CACHE4_GROUPS_MOST) {
+    desk_fail(st, IGL_FAIL_SUPPORT);
+    return IGL_FAIL_SUPPORT;
+  }
+  return IGL_OKAY;
+}
+
 static int cache4_null(igl_desk_state *st) {
   desk_fail(st, IGL_FAIL_ARGUMENT);
   return IGL_FAIL_ARGUMENT;
@@ -893,8 +907,7 @@ int igl_cache4_lay_dev(igl_desk *desk, const igl_cache4 *store, const float *key
   int code;
   if (!st) return IGL_FAIL_STATE;
   if (!store || !key_dev || !value_dev) return cache4_null(st);
-  if ((code = cache4_check(st, store, place_first, lane_count, place_first, row_stride,
-                           (long long)store->kv_count * store->head_size)) != IGL_OKAY)
+  if ((code = cache4_rows_check(st, store, place_first, lane_count, row_stride)) != IGL_OKAY)
     return code;
   return hip_check(st, igl_launch_cache4_lay(store, key_dev, value_dev, row_stride, place_first,
                                              lane_count, st->stream));
@@ -906,8 +919,7 @@ int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first
   int code;
   if (!st) return IGL_FAIL_STATE;
   if (!store || (!key_dev && !value_dev)) return cache4_null(st);
-  if ((code = cache4_check(st, store, place_first, lane_count, place_first, row_stride,
-                           (long long)store->kv_count * store->head_size)) != IGL_OKAY)
+  if ((code = cache4_rows_check(st, store, place_first, lane_count, row_stride)) != IGL_OKAY)
     return code;
   return hip_check(st, igl_launch_cache4_read(store, place_first, lane_count, key_dev, value_dev,
                                               row_stride, st->stream));
@@ -920,7 +932,7 @@ int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_sha
   int code;
   if (!st) return IGL_FAIL_STATE;
   if (!store || !query_dev || !blend_out_dev || window < 0 || group_share < 1) return cache4_null(st);
-  if (group_share > 64 || (long long)lane_count * group_share >= 1 << 28) {
+  if (group_share > 64 || (long long)lane_count * group_share > IGL_ATTEND4_ROWS_MOST) {
     desk_fail(st, IGL_FAIL_SUPPORT);
     return IGL_FAIL_SUPPORT;
   }

@@ -1280,7 +1280,6 @@ static Attend4Args attend4_args(const igl_cache4 *store, int group_share, const 
 extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_share, const float *query, int lane_stride,
                                          int place_first, int window, int lanes, float score_scale, float *blend_out,
                                          float *work, hipStream_t stream) {
-  // rows fewer than 2^28, so that a grid has fewer than 2^32 threads
   Attend4Args a =
       attend4_args(store, group_share, query, lane_stride, place_first, window, lanes, score_scale, blend_out);
   const Attend4Plan p = attend4_plan(a, store->head_size, store->kv_count);

@@ -315,19 +315,12 @@ static Cache4Args cache4_args(const igl_cache4 *store, int row_stride, int place
   return a;
 }
 
-// Workgroups of eight values a thread; 0: more than a grid has, 2^32 threads.
-static unsigned cache4_groups(const Cache4Args &a) {
-  const long long groups = ((long long)a.lanes * (a.width / 8) + 255) / 256;
-  return groups < 1 << 24 ? (unsigned)groups : 0;
-}
-
 extern "C" hipError_t igl_launch_cache4_lay(const igl_cache4 *store, const float *key, const float *value,
                                             int row_stride, int place_first, int lanes, hipStream_t stream) {
   Cache4Args a = cache4_args(store, row_stride, place_first, lanes);
   a.in[0] = key;
   a.in[1] = value;
-  const dim3 grid(cache4_groups(a), 2);
-  if (!grid.x) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)igl_cache4_groups(a.width, lanes), 2);
   if (store->format == IGL_CACHE4_INT4)
     hipLaunchKernelGGL((cache4_lay_kernel<IGL_CACHE4_INT4>), grid, dim3(256), 0, stream, a);
   else
@@ -340,9 +333,8 @@ extern "C" hipError_t igl_launch_cache4_read(const igl_cache4 *store, int place_
   Cache4Args a = cache4_args(store, row_stride, place_first, lanes);
   a.out[0] = key;
   a.out[1] = value;
-  const dim3 grid(cache4_groups(a), key && value ? 2 : 1);
+  const dim3 grid((unsigned)igl_cache4_groups(a.width, lanes), key && value ? 2 : 1);
   const int side0 = key ? 0 : 1;
-  if (!grid.x) return hipErrorInvalidValue;
   if (store->format == IGL_CACHE4_INT4)
     hipLaunchKernelGGL((cache4_read_kernel<IGL_CACHE4_INT4>), grid, dim3(256), 0, stream, a, side0);
   else

@@ -225,6 +225,13 @@ size_t igl_attend_prep_work_floats(int place_bound, int window, int head_size, i
 /* The attention counts slots to the end of a ring's last block in ints. */
 #define IGL_ATTEND4_BLOCK_MOST 512
 #define IGL_CACHE4_SPAN_MOST (INT32_MAX - IGL_ATTEND4_BLOCK_MOST)
+/* A grid has fewer than 2^32 threads: the attention takes 256 for every 16 rows (query
+ * heads times lanes), laying and reading one for every eight values. */
+#define IGL_ATTEND4_ROWS_MOST ((1 << 28) - 16)
+static inline long long igl_cache4_groups(int width, int lanes) {
+  return ((long long)lanes * (width / 8) + 255) / 256;
+}
+#define IGL_CACHE4_GROUPS_MOST ((1 << 24) - 1)
 static inline size_t igl_cache4_room(int cache_span) { return ((size_t)cache_span + 63) / 64 * 64; }
 hipError_t igl_launch_cache4_lay(const igl_cache4 *store, const float *key, const float *value,
                                  int row_stride, int place_first, int lanes, hipStream_t stream);

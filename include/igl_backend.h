@@ -280,12 +280,12 @@ size_t igl_cache4_gain_bytes(const igl_cache4 *store);
  * value / (gain * scale), both to even when halfway, decided exactly.  A NaN is
  * stored as zero and an infinity as the largest level of the largest gain.
  * Positions that the ring cannot hold together are refused with
- * IGL_FAIL_ARGUMENT. */
+ * IGL_FAIL_ARGUMENT, more than 2^35 - 2^11 values a side with IGL_FAIL_SUPPORT. */
 int igl_cache4_lay_dev(igl_desk *desk, const igl_cache4 *store, const float *key_dev,
                        const float *value_dev, int row_stride, int place_first, int lane_count);
 /* The rows of `lane_count` positions from place_first on as floats, row_stride
  * apart: each the product level * gain * scale, rounded once.  Either side may
- * be NULL. */
+ * be NULL; limits as igl_cache4_lay_dev's. */
 int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first, int lane_count,
                         float *key_dev, float *value_dev, int row_stride);
 /* igl_attend_lanes_dev over a 4-bit ring, for any number of query heads a
@@ -294,7 +294,7 @@ int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first
  * query_dev and blend_out_dev: [lane_count][kv_count * group_share][head_size]
  * floats, lanes lane_stride apart.  Every lane's keys and values must already be
  * in the ring; a ring too short to hold all that the lanes see is refused with
- * IGL_FAIL_ARGUMENT, lane_count * group_share of 2^28 and more with
+ * IGL_FAIL_ARGUMENT, lane_count * group_share past 2^28 - 16 with
  * IGL_FAIL_SUPPORT.  A call allocates nothing, whatever its size: its partials lie
  * in 48 MiB that the desk holds from its opening.  Weights are held to
  * 2^-22 of themselves, or to 2^-33 of the largest among the 32 to 512 slots taken

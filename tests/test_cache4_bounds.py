@@ -32,3 +32,40 @@ def test_the_longest_rings_blocks_end_below_an_int(lib):  # noqa: F811
     lib.plan4_form.restype, lib.plan4_form.argtypes = ctypes.c_int, [ctypes.c_int] * 8
     assert lib.plan4_form(64, 1, low, 0, 1, low - 1, 0, 1) % 4 == 3  # blocks of 512
     assert (low - 1) // 512 * 512 + 512 <= INT_MAX
+
+
+def test_launches_of_too_many_threads_are_refused_before(lib, tmp_path):  # noqa: F811
+    """A grid has fewer than 2^32 threads: rows of 32 dims and more are laid and read by
+    a thread every eight values, attended by 256 every sixteen rows.  The last call
+    that fits is launched, the next refused as unsupported, neither as the device's
+    failure.  The pointers are no memory; nothing on the host follows them."""
+    import os
+    import shutil
+    import test_cache4_host as t
+
+    so = shutil.copy(os.path.join(t.HERE, "host4", "_build", "libhost4.so"), tmp_path / "libhost4.so")
+    own = ctypes.CDLL(str(so))  # its own counts: the stand-in notes that these buffers are none
+    for name, (res, args) in native.SIGNATURES.items():
+        getattr(own, name).restype, getattr(own, name).argtypes = res, args
+    own.audit_report.restype, own.audit_report.argtypes = ctypes.c_long, [ctypes.POINTER(ctypes.c_long)] * 2
+    host = Host(own)
+    at = 1 << 40
+    for head, kv in ((64, 1), (512, 1), (128, 3)):
+        c = native.Cache4(0, INT_MAX - 4096, 0, kv, head, 1.0, 1.0, at, at, at, at)
+        width = kv * head
+        most = ((1 << 24) - 1) * 256 // (width // 8)  # rows
+        for lanes, code in ((most, native.IGL_OKAY), (most + 1, native.IGL_FAIL_SUPPORT)):
+            before = host.launches()[0]
+            assert host.lay(c, at, at, width, 0, lanes) == code
+            assert host.take() == code
+            assert host.read(c, 0, lanes, at, at, width) == code
+            assert host.take() == code
+            assert host.launches()[0] - before == (2 if code == native.IGL_OKAY else 0)
+    c = native.Cache4(0, INT_MAX - 4096, 0, 1, 64, 1.0, 1.0, at, at, at, at)
+    for share, lanes, code in ((16, (1 << 24) - 1, native.IGL_OKAY), (1, (1 << 28) - 16, native.IGL_OKAY),
+                               (1, (1 << 28) - 15, native.IGL_FAIL_SUPPORT), (3, 89478481, native.IGL_FAIL_SUPPORT)):
+        before = host.launches()[0]
+        assert host.attend(c, share, at, 64 * share, 0, 0, lanes, at) == code, (share, lanes)
+        assert host.take() == code
+        assert (host.launches()[0] > before) == (code == native.IGL_OKAY)
+        assert ((lanes * share + 15) // 16 * 256 < 1 << 32) == (code == native.IGL_OKAY)

@@ -293,8 +293,9 @@ int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first
  * positions q <= p with q > p - window (window 0: every q) or q < sink_count.
  * query_dev and blend_out_dev: [lane_count][kv_count * group_share][head_size]
  * floats, lanes lane_stride apart.  Every lane's keys and values must already be
- * in the ring; a ring too short to hold all that the lanes see is refused with
- * IGL_FAIL_ARGUMENT, lane_count * group_share past 2^28 - 16 with
+ * in the ring; a ring too short to hold all that the lanes see (with a window, and
+ * past it, one of fewer than sink_count + window + lane_count - 1 slots) is refused
+ * with IGL_FAIL_ARGUMENT, lane_count * group_share past 2^28 - 16 with
  * IGL_FAIL_SUPPORT.  A call allocates nothing, whatever its size: its partials lie
  * in 48 MiB that the desk holds from its opening.  Weights are held to
  * 2^-22 of themselves, or to 2^-33 of the largest among the 32 to 512 slots taken

@@ -69,3 +69,22 @@ def test_launches_of_too_many_threads_are_refused_before(lib, tmp_path):  # noqa
         assert host.take() == code
         assert (host.launches()[0] > before) == (code == native.IGL_OKAY)
         assert ((lanes * share + 15) // 16 * 256 < 1 << 32) == (code == native.IGL_OKAY)
+
+
+@pytest.mark.parametrize("window,sinks,lanes", [(512, 4, 1), (512, 4, 5), (60, 0, 16), (1, 3, 1)])
+def test_a_session_on_the_shortest_ring_of_a_window(host, window, sinks, lanes):
+    """sink_count + window + lanes - 1 slots carry a session of blocks of `lanes` as far
+    as it goes; with one less it ends where the ring wraps."""
+    for span, ends in ((sinks + window + lanes - 1, False), (sinks + window + lanes - 2, True)):
+        if span <= sinks:
+            continue
+        c = host.ring(1, span, sinks, 1, 256)
+        rows, heads = host.alloc(lanes * 256 * 4), host.alloc(lanes * 2048 * 4)
+        codes = []
+        for place in range(0, 3 * (span + lanes), lanes):
+            assert host.lay(c, rows, rows, 256, place, lanes) == native.IGL_OKAY
+            codes.append(host.attend(c, 8, heads, 2048, place, window, lanes, heads))
+            host.take()
+        assert (native.IGL_FAIL_ARGUMENT in codes) == ends
+        assert codes[0] == native.IGL_OKAY and (codes[-1] == native.IGL_OKAY) != ends
+    assert host.launches()[1] == 0

@@ -72,7 +72,7 @@ struct igl_desk_state {
   /* partials of the attention's wide launches (igl_attend_wide):
    * IGL_ATTEND_FIXED_FLOATS floats, held from open to close */
   float *attend_dev;
-  float *attend4_dev; /* partials of the 4-bit ring's attention: IGL_ATTEND4_FLOATS floats, as long */
+  float *attend4_dev; /* of the 4-bit ring's: IGL_ATTEND4_FLOATS floats, as long, or NULL */
   float *quant_dev;   /* plane_lift: the activations on the plane's entry grid */
   size_t quant_floats;
   /* plane_lift's prefill on the grid: widened codes, unit gains, level sums,
@@ -1182,11 +1182,16 @@ int igl_back_open(igl_desk *desk, int device_index, int sum_limit, int col_limit
       hipMalloc((void **)&st->act_dev, (size_t)st->lane_limit * st->col_limit * sizeof(float)) != hipSuccess ||
       hipHostMalloc((void **)&st->act_pin, (size_t)st->lane_limit * st->col_limit * sizeof(float),
                     hipHostMallocDefault) != hipSuccess ||
-      hipMalloc((void **)&st->attend_dev, IGL_ATTEND_FIXED_FLOATS * sizeof(float)) != hipSuccess ||
-      hipMalloc((void **)&st->attend4_dev, IGL_ATTEND4_FLOATS * sizeof(float)) != hipSuccess) {
+      hipMalloc((void **)&st->attend_dev, IGL_ATTEND_FIXED_FLOATS * sizeof(float)) != hipSuccess) {
     desk->state = st;
     igl_back_close(desk);
     return IGL_FAIL_DEVICE;
+  }
+  /* a desk whose device has no room for these opens all the same: attention over the
+   * 4-bit ring then keeps no partials, every row in one segment */
+  if (hipMalloc((void **)&st->attend4_dev, IGL_ATTEND4_FLOATS * sizeof(float)) != hipSuccess) {
+    st->attend4_dev = NULL;
+    (void)hipGetLastError();
   }
   desk->state = st;
   desk->name_text = "hip/gfx950";

@@ -1122,7 +1122,8 @@ static void attend4_count(Attend4Plan &p, const Attend4Args &a) {
   }
 }
 
-static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
+// `room`: floats there are for partials.
+static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count, long long room = IGL_ATTEND4_FLOATS) {
   const long long cus = 256;
   Attend4Plan p = {};
   // Tiles of 64 rows, where they give every CU more than six blocks of 64 slots:
@@ -1175,7 +1176,7 @@ static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
     double least = 0.0;
     for (int n = 1; n <= p.blocks && n <= kAttend4Segments; ++n) {
       const long long size = (p.blocks + n - 1) / n, used = (p.blocks + size - 1) / size;
-      if (used > 1 && floats(used) > (long long)IGL_ATTEND4_FLOATS) break;
+      if (used > 1 && floats(used) > room) break;
       const double cost = (double)((used * p.tiles * kv_count + cus - 1) / cus) * (double)(size + 1) +
                           (used > 1 ? 1.0 + (double)floats(used) / (1 << 20) : 0.0);
       if (n == 1 || cost < least) least = cost, per = size;
@@ -1199,7 +1200,7 @@ static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count) {
       }
       a.part_row0 = low * p.each;
     }
-    if (floats(a.segments) <= (long long)IGL_ATTEND4_FLOATS) break;
+    if (floats(a.segments) <= room) break;
     per += (per + 7) / 8;
   }
   return p;
@@ -1282,11 +1283,13 @@ extern "C" hipError_t igl_launch_attend4(const igl_cache4 *store, int group_shar
                                          float *work, hipStream_t stream) {
   Attend4Args a =
       attend4_args(store, group_share, query, lane_stride, place_first, window, lanes, score_scale, blend_out);
-  const Attend4Plan p = attend4_plan(a, store->head_size, store->kv_count);
-  const size_t parts = (size_t)a.segments * store->kv_count * (size_t)(a.rows - a.part_row0);
-  a.part_out = work;
-  a.part_base = work + parts * store->head_size;
-  a.part_total = a.part_base + parts;
+  const Attend4Plan p = attend4_plan(a, store->head_size, store->kv_count, work ? IGL_ATTEND4_FLOATS : 0);
+  if (a.segments > 1) {
+    const size_t parts = (size_t)a.segments * store->kv_count * (size_t)(a.rows - a.part_row0);
+    a.part_out = work;
+    a.part_base = work + parts * store->head_size;
+    a.part_total = a.part_base + parts;
+  }
   switch (store->head_size) {
     case 64: return attend4_launch_format<64>(a, p, store->format, store->kv_count, stream);
     case 128: return attend4_launch_format<128>(a, p, store->format, store->kv_count, stream);

@@ -220,7 +220,7 @@ size_t igl_attend_prep_work_floats(int place_bound, int window, int head_size, i
 
 /* The 4-bit ring (igl_cache4.h, included by igl_elem.hip; igl_attend4.h, by
  * igl_gemv.hip).  Rows, queries and blends at any 4-byte alignment; `work`
- * holds IGL_ATTEND4_FLOATS floats. */
+ * holds IGL_ATTEND4_FLOATS floats, or is NULL: then no row's blocks are cut. */
 #define IGL_ATTEND4_FLOATS (3u << 22)
 /* The attention counts slots to the end of a ring's last block in ints. */
 #define IGL_ATTEND4_BLOCK_MOST 512

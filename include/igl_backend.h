@@ -297,7 +297,8 @@ int igl_cache4_read_dev(igl_desk *desk, const igl_cache4 *store, int place_first
  * past it, one of fewer than sink_count + window + lane_count - 1 slots) is refused
  * with IGL_FAIL_ARGUMENT, lane_count * group_share past 2^28 - 16 with
  * IGL_FAIL_SUPPORT.  A call allocates nothing, whatever its size: its partials lie
- * in 48 MiB that the desk holds from its opening.  Weights are held to
+ * in 48 MiB that the desk holds from its opening (where the device had not that much
+ * left, it keeps none, and long contexts take longer).  Weights are held to
  * 2^-22 of themselves, or to 2^-33 of the largest among the 32 to 512 slots taken
  * with them if that is more: a blend that is small beside the row's values, as of a
  * first position that has nearly all the weight and no value, is as exact as that. */

@@ -88,3 +88,34 @@ def test_a_session_on_the_shortest_ring_of_a_window(host, window, sinks, lanes):
         assert (native.IGL_FAIL_ARGUMENT in codes) == ends
         assert codes[0] == native.IGL_OKAY and (codes[-1] == native.IGL_OKAY) != ends
     assert host.launches()[1] == 0
+
+
+def test_a_desk_without_room_for_partials_opens(lib):  # noqa: F811
+    """Where the device has no 48 MiB left a desk opens as before there were any, and
+    attention over the ring runs in one launch, without partials.  In a process of
+    its own, whose memory is bounded; the stand-in notes the missing buffer, which the
+    launch does not use."""
+    import subprocess
+    import sys
+    import test_cache4_host as t
+
+    script = r"""
+import ctypes, resource, sys
+sys.path.insert(0, sys.argv[1]); sys.path.insert(0, sys.argv[2])
+import test_cache4_host as t
+from igllm_amd import native
+lib = ctypes.CDLL(t.os.path.join(t.HERE, "host4", "_build", "libhost4.so"))
+for name, (res, args) in native.SIGNATURES.items():
+    getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
+lib.audit_report.restype, lib.audit_report.argtypes = ctypes.c_long, [ctypes.POINTER(ctypes.c_long)] * 2
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (32 << 20),) * 2)
+host = t.Host(lib)
+c = host.ring(0, 16384)
+room = host.alloc(8 * 256 * 4)
+before = host.launches()[0]
+assert host.attend(c, 8, room, 2048, 16383, 0, 1, room) == native.IGL_OKAY
+print("launches", host.launches()[0] - before)
+"""
+    r = subprocess.run([sys.executable, "-c", script, t.HERE, t.os.path.dirname(t.HERE)], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "launches 1\n", (r.stdout, r.stderr[-1500:])

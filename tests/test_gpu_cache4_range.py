@@ -1,5 +1,7 @@
 """GPU attention over the 4-bit ring at the ends of its numbers: scales, scores
 and weights far from one another, against 64 bits."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -78,3 +80,30 @@ def test_a_peaked_position_of_long_blocks(backend, fmt, kv, share, head, span):
     assert near < 4.0
     assert err <= 2.0 ** (near - 7) * size
     close(store)
+
+
+@pytest.mark.parametrize("kv,share,head,sinks,span,place,window,lanes", [
+    (1, 8, 256, 0, 4096, 4095, 0, 1), (16, 1, 64, 0, 40000, 39999, 0, 1), (1, 8, 512, 0, 3000, 2000, 0, 5),
+    (2, 8, 128, 3, 6500, 9000, 6400, 60), (1, 8, 512, 7, 1500, 0, 0, 1400)])
+def test_launches_without_room_for_partials(backend, kv, share, head, sinks, span, place, window, lanes):
+    """What a desk without partials launches: every row's blocks in one segment."""
+    print("case no partials", kv, share, head, span, lanes, flush=True)
+    rng = np.random.default_rng(head + lanes)
+    host = ring_bytes(rng, span, kv * head, c4.E2M1)
+    store = open_ring(backend, c4.E2M1, span, sinks, kv, head, host)
+    stride = kv * share * head
+    query = rng.normal(size=(lanes, stride)).astype(np.float32)
+    score = 10.0 / np.sqrt(head)
+    dq, do = backend.upload(query), backend.alloc(query.nbytes)
+    stream = backend.lib.igl_desk_stream
+    stream.restype, stream.argtypes = ctypes.c_void_p, [ctypes.c_void_p]
+    launch = backend.lib.igl_launch_attend4
+    launch.restype = ctypes.c_int
+    launch.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p] + [ctypes.c_int] * 4 + [
+        ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    assert launch(ctypes.byref(store.cache), share, dq.ptr, stride, place, window, lanes, score, do.ptr, None,
+                  stream(ctypes.byref(backend.desk))) == 0
+    backend.sync()
+    got = do.get(np.float32, query.size).reshape(query.shape)
+    check(got, query, rows_of(host, c4.E2M1, span, sinks), share, head, place, window, sinks, score)
+    close(store, dq, do)

@@ -479,7 +479,7 @@ struct Step4Shape {
 };
 
 template <int HEAD, int FMT, bool PAIR, int T>
-__global__ __launch_bounds__(256, T > 2 ? 2 : 1) void attend4_step_kernel(Attend4Args a) {
+__global__ __launch_bounds__(256, T > 4 ? 2 : 1) void attend4_step_kernel(Attend4Args a) {
   using F = Step4Shape<HEAD, PAIR, T>;
   constexpr int KL = F::KL, KW = F::KW, ROWS = F::ROWS, TERMS = F::TERMS, BLOCK = F::BLOCK;
   constexpr int VD = F::VD, VS = F::VS, DB = F::DB, DPL = F::DPL, UB = F::UB, QP = F::QP, PP = F::PP;
@@ -1096,7 +1096,8 @@ using namespace igl;
 // How a launch is cut: tiles of up to eight rows (`pair`) or sixteen on
 // attend4_step_kernel, or of 64 on attend4_tile_kernel; blocks of `block` slots.
 struct Attend4Plan {
-  bool step, pair, deep;
+  bool step, pair;
+  int deep;                // times the slots of a step's block, 2 or 4, or 0
   int block, each, tiles;  // rows a tile
   int blocks;              // of the tile with most, or a bound of it
   long long all;           // of all tiles
@@ -1145,13 +1146,32 @@ static Attend4Plan attend4_plan(Attend4Args &a, int head, int kv_count, long lon
     p.each = p.pair ? 8 : 16;
     p.block = head < 256 ? 128 : 64;
     // Four times the slots between barriers, and on their way, where every workgroup
-    // still has two such blocks: 131072 positions of eight 128-dim heads 40.5 -> 35.4 us
-    // in caches, as by twice the slots, but with the fold 43.7 out of them for 46.1;
-    // 65536 22.3 -> 19.8.  Not of wide heads, whose rows already fill the registers:
-    // two 512-dim heads by twice the slots 32.9 -> 42.8.
-    p.deep = p.pair && head < 256 &&
-             (long long)attend4_blocks(4 * p.block, a.place, a.newest, a).count * kv_count >= 2 * 2 * cus;
-    if (p.deep) p.block *= 4;
+    // still has two such blocks: 131072 positions of eight 128-dim heads in caches 40.7 ->
+    // 34.6 us (35.9 by twice), int4's 44.2 -> 37.4 (39.3); out of them 50.2 -> 40.7 and
+    // 51.2 -> 44.2; and no more than an eighth more slots than in small blocks, by which
+    // it waits for its last: 200000 of eight 77.8 -> 73.2 (3584 for 3200), but 40000 of
+    // sixteen 28.4 -> 35.0 (25.3 by twice), 66000 of eight 29.7 -> 34.4, 105000 35.9 ->
+    // 41.5.  Of 64-dim heads a fifth: 200000 61.0 -> 46.0, but 80000 of eight 27.4 -> 29.8,
+    // 40000 of sixteen 24.0 -> 29.7 (20.0 by twice), 66000 25.7 -> 28.6.  Else twice the
+    // slots, where it has two of those and no more slots than in small blocks: 131072 of
+    // two 64-dim heads 12.4 -> 10.0 us (int4) and 10.8 -> 9.6, 128-dim 15.6 -> 13.8 and
+    // 15.0 -> 13.2, 32768 of eight 15.2 -> 13.6 and 14.6 -> 12.9, 80000 30.9 -> 29.8; but
+    // 33000, 768 slots for 640, 19.0 -> 20.2.  Not of wide heads, whose rows already fill
+    // the registers: two 512-dim heads by twice the slots 32.9 -> 42.8.
+    if (p.pair && head < 256) {
+      const auto blocks = [&](int times) {
+        return (long long)attend4_blocks(times * p.block, a.place, a.newest, a).count * kv_count;
+      };
+      const auto slots = [&](int times) {  // of a workgroup, in small blocks
+        return (blocks(times) + 2 * cus - 1) / (2 * cus) * times;
+      };
+      const int part = head == 64 ? 5 : 8;
+      if (blocks(4) >= 2 * 2 * cus && slots(4) * part <= slots(1) * (part + 1))
+        p.deep = 4;
+      else if (blocks(2) >= 2 * 2 * cus && slots(2) <= slots(1))
+        p.deep = 2;
+      if (p.deep) p.block *= p.deep;
+    }
     attend4_count(p, a);
   }
 
@@ -1222,8 +1242,12 @@ static hipError_t attend4_launch(const Attend4Args &a, const Attend4Plan &p, int
       hipLaunchKernelGGL((attend4_tile_kernel<HEAD, FMT>), grid, dim3(512), (size_t)size, stream, a);
     }
   } else if (p.deep) {
-    if constexpr (HEAD < 256)
-      hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, 4 * T>), grid, dim3(256), 0, stream, a);
+    if constexpr (HEAD < 256) {
+      if (p.deep == 4)
+        hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, 4 * T>), grid, dim3(256), 0, stream, a);
+      else
+        hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, 2 * T>), grid, dim3(256), 0, stream, a);
+    }
   } else if (p.pair) {
     hipLaunchKernelGGL((attend4_step_kernel<HEAD, FMT, true, T>), grid, dim3(256), 0, stream, a);
   } else {

@@ -119,3 +119,28 @@ print("launches", host.launches()[0] - before)
 """
     r = subprocess.run([sys.executable, "-c", script, t.HERE, t.os.path.dirname(t.HERE)], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout == "launches 1\n", (r.stdout, r.stderr[-1500:])
+
+
+@pytest.mark.parametrize("form,plan", [
+    (3, (64, 2, 131072, 0, 8, 131071, 0, 1)), (3, (128, 2, 131072, 0, 4, 131071, 0, 1)),
+    (3, (128, 8, 32768, 0, 4, 32767, 0, 1)), (3, (64, 8, 32768, 0, 1, 90000, 32768, 1)),
+    (3, (128, 8, 131072, 0, 4, 131071, 0, 1)), (3, (128, 8, 200000, 0, 4, 199999, 0, 1)),
+    (2, (64, 8, 40000, 0, 1, 39999, 0, 1)),   # a workgroup would have more slots
+    (2, (128, 8, 66000, 0, 4, 65999, 0, 1)), (2, (64, 8, 66000, 0, 4, 65999, 0, 1)),
+    (2, (128, 8, 105000, 0, 4, 104999, 0, 1)),
+    (2, (128, 2, 65536, 0, 4, 65535, 0, 1)),  # or one block
+    (2, (256, 8, 65536, 0, 8, 65535, 0, 1))])  # wide heads fill the registers
+def test_steps_over_long_contexts_take_longer_blocks(lib, form, plan):  # noqa: F811
+    """Twice the slots a block where four times leave a workgroup fewer than two blocks
+    or cut unevenly, small blocks where both do."""
+    lib.plan4_form.restype, lib.plan4_form.argtypes = ctypes.c_int, [ctypes.c_int] * 8
+    lib.plan4_check.restype, lib.plan4_check.argtypes = ctypes.c_int, [ctypes.c_int] * 8
+    assert lib.plan4_form(*plan) % 4 == form
+    assert lib.plan4_check(*plan) == 0
+
+
+def test_sixteen_heads_at_40000_take_blocks_between(lib):  # noqa: F811
+    """32 segments of five blocks of 256 slots, not 27 of three of 512."""
+    lib.plan4_form.restype, lib.plan4_form.argtypes = ctypes.c_int, [ctypes.c_int] * 8
+    got = lib.plan4_form(128, 16, 40000, 0, 4, 39999, 0, 1)
+    assert (got % 4, got // 4) == (3, 32)

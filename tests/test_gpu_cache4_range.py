@@ -107,3 +107,20 @@ def test_launches_without_room_for_partials(backend, kv, share, head, sinks, spa
     got = do.get(np.float32, query.size).reshape(query.shape)
     check(got, query, rows_of(host, c4.E2M1, span, sinks), share, head, place, window, sinks, score)
     close(store, dq, do)
+
+
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,share,head,sinks,span,place,window", [
+    (2, 8, 64, 0, 131072, 131071, 0), (2, 4, 128, 0, 131072, 131071, 0), (8, 4, 128, 4, 45004, 90000, 45000),
+    (8, 1, 64, 3, 45000, 44999, 0), (16, 1, 128, 9, 41000, 90000, 40900)])
+def test_steps_in_blocks_between(backend, fmt, kv, share, head, sinks, span, place, window):
+    """Steps in blocks of 256 slots: long contexts of few heads, and the wrap."""
+    print("case between", fmt, kv, share, head, span, place, flush=True)
+    rng = np.random.default_rng(head + kv)
+    host = ring_bytes(rng, span, kv * head, fmt)
+    store = open_ring(backend, fmt, span, sinks, kv, head, host)
+    query = rng.normal(size=(1, kv * share * head)).astype(np.float32)
+    score = 10.0 / np.sqrt(head)
+    got = attend(backend, store, share, query, place, window, score)
+    check(got, query, rows_of(host, fmt, span, sinks), share, head, place, window, sinks, score)
+    close(store)

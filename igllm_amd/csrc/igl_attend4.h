@@ -454,8 +454,9 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
 // one is bound by its bytes and their decoding (16 us of vector issue a CU and 3 of
 // matrix): 131072 positions of eight 128-dim heads, 143 MB, in 35.4 us, 4.0 TB/s
 // (out of caches 39, 3.7).  Blocks of 512 slots fill the registers of a wave of two a
-// SIMD, which the kernel asks for: one register more of int4's halved the workgroups
+// SIMD, which 128-dim heads' ask for: one register more of int4's halved the workgroups
 // a CU, and the same in int4 took 52 us where 37.4 do (e2m1 34.6, in caches both).
+// 64-dim heads' have them anyhow, and asking took 0.4 us of 29.
 template <int HEAD, bool PAIR, int T>
 struct Step4Shape {
   static constexpr int KL = HEAD >= 128 ? HEAD / 128 : 1;  // key chunks of a row a lane reads
@@ -479,7 +480,7 @@ struct Step4Shape {
 };
 
 template <int HEAD, int FMT, bool PAIR, int T>
-__global__ __launch_bounds__(256, T > 4 ? 2 : 1) void attend4_step_kernel(Attend4Args a) {
+__global__ __launch_bounds__(256, T > 4 && HEAD > 64 ? 2 : 1) void attend4_step_kernel(Attend4Args a) {
   using F = Step4Shape<HEAD, PAIR, T>;
   constexpr int KL = F::KL, KW = F::KW, ROWS = F::ROWS, TERMS = F::TERMS, BLOCK = F::BLOCK;
   constexpr int VD = F::VD, VS = F::VS, DB = F::DB, DPL = F::DPL, UB = F::UB, QP = F::QP, PP = F::PP;

@@ -1,0 +1,147 @@
+"""Both binary16 terms of the queries and of the weights of attention over the
+4-bit ring, and every row of its prompts, against 64 bits.
+
+Rows that random inputs leave within a bar are here made to err alike: every query
+(or every weight) is 1 + 7/16 2^-10, whose first term, 1, is 4.3e-4 too small, so
+that a blend without second terms is off by 1.8e-4 and more of its values.
+
+The bars, counting roundings of 2^-24: a row's blend and its total each take at most
+a sum every sixteen of the slots that a workgroup walks, `walked`, 256 segments and
+64 more, (walked / 8 + 640) 2^-24 together; the scores' own roundings 2 reach 2^-19
+as in the ring's other tests.
+"""
+import numpy as np
+import pytest
+
+import cache4_oracle as c4
+from test_gpu_cache4 import SCALE, attend, close, open_ring, ring_bytes, rows_of
+
+SIZE = 1.0 + 7.0 / 16 * 2.0 ** -10
+
+CASES = [  # kv, share, head, sinks, span, place, window, lanes
+    (1, 8, 256, 4, 516, 5000, 512, 1), (2, 8, 64, 0, 700, 699, 0, 1),             # eight rows
+    (2, 8, 64, 0, 131072, 131071, 0, 1), (8, 4, 128, 0, 32768, 32767, 0, 1),      # in blocks of 256
+    (16, 1, 64, 0, 40000, 39999, 0, 1), (8, 4, 128, 0, 65536, 65535, 0, 1),       # of 512
+    (1, 16, 128, 0, 1000, 900, 0, 7), (1, 8, 512, 0, 3000, 2000, 0, 5),           # sixteen rows
+    (1, 8, 64, 0, 2047, 0, 0, 2047),
+    (16, 4, 128, 0, 700, 440, 0, 250), (8, 8, 256, 5, 560, 3000, 300, 250),       # tiles
+    (4, 16, 512, 3, 720, 9000, 450, 250), (2, 8, 512, 0, 4400, 4310, 0, 90), (1, 8, 512, 7, 1500, 0, 0, 1400)]
+
+
+def sums_bar(seen):
+    return (min(seen, 4400) / 8 + 640) * 2.0 ** -24
+
+
+def seen_slots(sinks, span, place, window, lanes):
+    """Slots each lane sees, and whether the slot is an even one, as [lanes] counts."""
+    even, odd = np.zeros(lanes), np.zeros(lanes)
+    for lane in range(lanes):
+        at = c4.slot(c4.seen(place + lane, window, sinks), sinks, span)
+        even[lane] = np.count_nonzero(at % 2 == 0)
+        odd[lane] = len(at) - even[lane]
+    return even, odd
+
+
+def two_kinds(even, odd, score):
+    """The blend of values 1 at score `score` and -1 at -`score`, in 64 bits."""
+    up, down = even * np.exp(score), odd * np.exp(-score)
+    return (up - down) / (up + down)
+
+
+def test_blends_without_second_terms_pass_no_bar():
+    """The mistake planted here, in 64 bits and binary16: what the bars below are for."""
+    assert float(np.float16(SIZE)) == 1.0
+    for kv, share, head, sinks, span, place, window, lanes in CASES:
+        even, odd = seen_slots(sinks, span, place, window, min(lanes, 3))
+        for n in even + odd:
+            assert abs(float(np.float16(SIZE)) / SIZE - 1.0) > sums_bar(n)  # weights, of equal values
+        err = np.abs(two_kinds(even, odd, 1.0 / SIZE) - two_kinds(even, odd, 1.0))
+        for e, n, least in zip(err, even + odd, np.minimum(even, odd)):
+            assert e > 2 * 2.0 ** -19 + sums_bar(n) or least < 0.4 * n  # queries, of a row that sees both kinds
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,share,head,sinks,span,place,window,lanes", CASES)
+def test_weights_keep_their_second_term(backend, fmt, kv, share, head, sinks, span, place, window, lanes):
+    """All scores log SIZE, so all weights SIZE times a power of two; all values one."""
+    print("case weights", fmt, kv, share, head, span, place, lanes, flush=True)
+    host = ring_bytes(np.random.default_rng(0), span, kv * head, fmt)
+    for side in range(2):
+        host[2 * side][:] = 0x99 if fmt == c4.INT4 else 0x22  # level 1
+        host[2 * side + 1][:] = 0x38                          # gain 1
+    store = open_ring(backend, fmt, span, sinks, kv, head, host)
+    query = np.ones((lanes, kv * share * head), np.float32)
+    score = np.log(SIZE) / (head * float(np.float32(SCALE)))
+    got = attend(backend, store, share, query, place, window, score)
+    want = float(np.float32(0.75 * SCALE))
+    err = np.abs(got / want - 1.0).max(1)
+    print("error", err.max(), flush=True)
+    for lane in range(lanes):
+        n = len(c4.seen(place + lane, window, sinks))
+        assert err[lane] <= sums_bar(n), (lane, err[lane])
+    close(store)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,share,head,sinks,span,place,window,lanes", CASES)
+def test_queries_keep_their_second_term(backend, fmt, kv, share, head, sinks, span, place, window, lanes):
+    """Queries of SIZE; even slots at score 1 with value 1, odd ones at -1 with -1."""
+    print("case queries", fmt, kv, share, head, span, place, lanes, flush=True)
+    host = ring_bytes(np.random.default_rng(0), span, kv * head, fmt)
+    for side in range(2):
+        host[2 * side][0::2] = 0x99 if fmt == c4.INT4 else 0x22
+        host[2 * side][1::2] = 0x77 if fmt == c4.INT4 else 0xAA  # level -1
+        host[2 * side + 1][:] = 0x38
+    store = open_ring(backend, fmt, span, sinks, kv, head, host)
+    query = np.full((lanes, kv * share * head), SIZE, np.float32)
+    score = float(np.float32(1.0 / (head * SIZE * float(np.float32(SCALE)))))
+    got = attend(backend, store, share, query, place, window, score) / float(np.float32(0.75 * SCALE))
+    even, odd = seen_slots(sinks, span, place, window, lanes)
+    want = two_kinds(even, odd, score * head * SIZE * float(np.float32(SCALE)))
+    err = np.abs(got - want[:, None]).max(1)
+    print("error", err.max(), flush=True)
+    for lane in range(lanes):
+        assert err[lane] <= 2 * 2.0 ** -19 + sums_bar(even[lane] + odd[lane]), (lane, err[lane])
+    close(store)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
+@pytest.mark.parametrize("kv,share,head,sinks,span,place,window,lanes", [
+    (2, 5, 64, 3, 900, 0, 0, 900), (2, 8, 256, 0, 700, 0, 0, 700), (1, 8, 512, 7, 1500, 0, 0, 900),
+    (4, 16, 512, 3, 720, 9000, 450, 250), (8, 8, 256, 5, 560, 3000, 300, 250), (1, 8, 256, 4, 1700, 0, 512, 1100),
+    (16, 4, 128, 0, 700, 440, 0, 250), (2, 3, 128, 0, 400, 0, 0, 400)])
+def test_every_row_of_a_prompt(backend, fmt, kv, share, head, sinks, span, place, window, lanes):
+    """Every lane of every head, each against its own bar."""
+    print("case rows", fmt, kv, share, head, span, place, lanes, flush=True)
+    rng = np.random.default_rng(head + lanes)
+    host = ring_bytes(rng, span, kv * head, fmt)
+    store = open_ring(backend, fmt, span, sinks, kv, head, host)
+    query = rng.normal(size=(lanes, kv * share * head)).astype(np.float32)
+    score = 10.0 / np.sqrt(head)
+    got = attend(backend, store, share, query, place, window, score).reshape(lanes, kv, share, head)
+    lane = place + np.arange(lanes)[:, None]
+    t = np.arange(max(0, place + 1 - window) if window else 0, place + lanes)
+    t = np.concatenate([np.arange(min(sinks, t[0])), t])
+    hide = t > lane
+    if window:
+        hide |= (t <= lane - window) & (t >= sinks)
+    rows = rows_of(host, fmt, span, sinks)
+    key, value = (rows(side, t).reshape(-1, kv, head) for side in range(2))
+    bar = (64 + (len(t) + 63) // 64 + 3) * 2.0 ** -24
+    worst = 0.0
+    for j in range(kv):
+        for h in range(share):
+            q = query.reshape(lanes, kv, share, head)[:, j, h].astype(np.float64)
+            s = np.where(hide, -np.inf, q @ key[:, j].T * score)
+            w = np.exp(s - s.max(1, keepdims=True))
+            want = w @ value[:, j] / w.sum(1, keepdims=True)
+            reach = np.where(hide, 0.0, np.abs(q) @ np.abs(key[:, j]).T * score).max(1)
+            err = np.abs(got[:, j, h] - want).max(1)
+            over = err / (np.abs(value).max() * (2 * reach * 2.0 ** -19 + bar))
+            worst = max(worst, float(over.max()))
+            assert np.all(over <= 1.0), (j, h, int(over.argmax()))
+    print("largest part of its bar", worst, flush=True)
+    close(store)

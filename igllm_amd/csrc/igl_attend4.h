@@ -50,7 +50,7 @@ struct Attend4Args {
   uint32_t share_mul;    // row / share = row * share_mul >> share_shift
   int share_shift;
   int key_power;         // key scale, score scale, log2 e and 256: key_part 2^key_power
-  float key_part;        // in [1/2, 1), or of a score scale below zero
+  float key_part;        // in [1/2, 1), or of a score scale below zero, or NaN
   float value_scale;
   int segments;          // of a row tile's blocks, each `per` of them and the last what is left
   int per;
@@ -1300,7 +1300,7 @@ static Attend4Args attend4_args(const igl_cache4 *store, int group_share, const 
   a.share_mul = (uint32_t)(((1ull << a.share_shift) + group_share - 1) / group_share);
   // log2 e, and the 256 that a gain is divided by
   const double factor = (double)store->key_scale * score_scale * 1.4426950408889634 * 256.0;
-  a.key_part = (float)frexp(factor, &a.key_power);
+  a.key_part = isfinite(factor) ? (float)frexp(factor, &a.key_power) : NAN;
   a.value_scale = store->value_scale;
   return a;
 }

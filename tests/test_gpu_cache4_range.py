@@ -124,3 +124,18 @@ def test_steps_in_blocks_between(backend, fmt, kv, share, head, sinks, span, pla
     got = attend(backend, store, share, query, place, window, score)
     check(got, query, rows_of(host, fmt, span, sinks), share, head, place, window, sinks, score)
     close(store)
+
+
+@pytest.mark.parametrize("kv,share,head,lanes,span", [(1, 8, 128, 1, 400), (1, 8, 512, 7, 400), (16, 1, 64, 1, 40000),
+                                                      (8, 8, 256, 260, 700), (8, 16, 512, 130, 500)])
+@pytest.mark.parametrize("score", [np.inf, -np.inf, np.nan])
+def test_score_scales_that_are_no_numbers(backend, kv, share, head, lanes, span, score):
+    """Infinite scores differ by no number: no blend is one, of queries of zero either."""
+    print("case no score", kv, share, head, lanes, score, flush=True)
+    rng = np.random.default_rng(head)
+    host = ring_bytes(rng, span, kv * head, c4.INT4)
+    store = open_ring(backend, c4.INT4, span, 0, kv, head, host)
+    query = rng.normal(size=(lanes, kv * share * head)).astype(np.float32)
+    query[0] = 0.0
+    assert np.all(np.isnan(attend(backend, store, share, query, span - lanes, 0, score)))
+    close(store)

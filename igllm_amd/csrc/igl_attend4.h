@@ -288,18 +288,22 @@ __device__ __forceinline__ uint32_t row_at(int row, uint32_t row_bytes) {
   return ((uint32_t)row & 0xFFFFFFu) * (row_bytes & 0xFFFFFFu);
 }
 
-// A row's queries as two binary16 terms: times a power of two that brings the
-// row's largest, `top`, to [2^13, 2^14) (or as far up as a float reaches), so that
-// no query is too large or too small for them; the factor takes it back, and is
-// never zero, so that it leaves a hidden score's -infinity one.  A score factor
-// below zero turns the queries instead.  A NaN or an infinity stays one in its
-// terms.
+// A row's queries as two binary16 terms: times the score factor's significand and a
+// power of two that brings the row's largest, `top`, to [2^12, 2^14) (or as far up as a
+// float reaches, then without the significand), so that no query is too large or too
+// small for them.  The power of two that is left is the scores' factor: their products
+// with it are exact, so that a base lies below a peak by what it should however large
+// scores are.  It is never zero, so that it leaves a hidden score's -infinity one.  A
+// score factor below zero turns the queries instead.  A NaN or an infinity stays one
+// in its terms.
 __device__ __forceinline__ float query_factor(const Attend4Args &a, float top, float &scale) {
-  int up = top > 0.0f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
-  if (up > 126) up = 126;
-  scale = __builtin_amdgcn_ldexpf(a.key_part < 0.0f ? -1.0f : 1.0f, up);
-  const float factor = __builtin_amdgcn_ldexpf(fabsf(a.key_part), a.key_power - up);
-  return factor < FLT_MIN ? FLT_MIN : factor > FLT_MAX ? FLT_MAX : factor;  // nor too large for a score of zero
+  const int want = top > 0.0f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+  const int up = want > 126 ? 126 : want;
+  const bool apart = want > 126 || a.key_part == 0.0f;
+  const float part = fabsf(a.key_part);
+  scale = __builtin_amdgcn_ldexpf(__builtin_copysignf(apart ? 1.0f : part, a.key_part), up);
+  const float factor = __builtin_amdgcn_ldexpf(apart ? part : 1.0f, a.key_power - up);
+  return factor < FLT_MIN ? FLT_MIN : factor > 0x1p127f ? 0x1p127f : factor;  // nor too large for a score of zero
 }
 
 typedef float float2_t __attribute__((ext_vector_type(2)));
@@ -386,7 +390,8 @@ __host__ __device__ __forceinline__ bool attend4_all(int slot0, int count, int a
 // A row's base after a block with this peak (before its factor).
 __device__ __forceinline__ float attend4_base(float peak, float factor, float base, float &top_base) {
   if (peak == -INFINITY) return base;
-  const float low = floorf(peak * factor) - 12.0f;
+  const float at = peak * factor;
+  const float low = fabsf(at) < 0x1p23f ? floorf(at) - 12.0f : at;  // where a float holds whole numbers
   if (low >= base - 4.0f && low <= base + 2.0f) return base;
   top_base = fmaxf(top_base, low);
   return fmaxf(low, top_base - 58.0f);

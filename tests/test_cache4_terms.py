@@ -17,6 +17,8 @@ import cache4_oracle as c4
 from test_gpu_cache4 import SCALE, attend, close, open_ring, ring_bytes, rows_of
 
 SIZE = 1.0 + 7.0 / 16 * 2.0 ** -10
+NEAR = SIZE * np.log(2.0)  # scores of the queries' test: their factor is then a power of two, and no
+# part of it can be taken into the queries that would round otherwise
 
 CASES = [  # kv, share, head, sinks, span, place, window, lanes
     (1, 8, 256, 4, 516, 5000, 512, 1), (2, 8, 64, 0, 700, 699, 0, 1),             # eight rows
@@ -55,7 +57,7 @@ def test_blends_without_second_terms_pass_no_bar():
         even, odd = seen_slots(sinks, span, place, window, min(lanes, 3))
         for n in even + odd:
             assert abs(float(np.float16(SIZE)) / SIZE - 1.0) > sums_bar(n)  # weights, of equal values
-        err = np.abs(two_kinds(even, odd, 1.0 / SIZE) - two_kinds(even, odd, 1.0))
+        err = np.abs(two_kinds(even, odd, NEAR / SIZE) - two_kinds(even, odd, NEAR))
         for e, n, least in zip(err, even + odd, np.minimum(even, odd)):
             assert e > 2 * 2.0 ** -19 + sums_bar(n) or least < 0.4 * n  # queries, of a row that sees both kinds
 
@@ -87,7 +89,7 @@ def test_weights_keep_their_second_term(backend, fmt, kv, share, head, sinks, sp
 @pytest.mark.parametrize("fmt", [c4.INT4, c4.E2M1])
 @pytest.mark.parametrize("kv,share,head,sinks,span,place,window,lanes", CASES)
 def test_queries_keep_their_second_term(backend, fmt, kv, share, head, sinks, span, place, window, lanes):
-    """Queries of SIZE; even slots at score 1 with value 1, odd ones at -1 with -1."""
+    """Queries of SIZE; even slots at score NEAR with value 1, odd ones at -NEAR with -1."""
     print("case queries", fmt, kv, share, head, span, place, lanes, flush=True)
     host = ring_bytes(np.random.default_rng(0), span, kv * head, fmt)
     for side in range(2):
@@ -96,7 +98,7 @@ def test_queries_keep_their_second_term(backend, fmt, kv, share, head, sinks, sp
         host[2 * side + 1][:] = 0x38
     store = open_ring(backend, fmt, span, sinks, kv, head, host)
     query = np.full((lanes, kv * share * head), SIZE, np.float32)
-    score = float(np.float32(1.0 / (head * SIZE * float(np.float32(SCALE)))))
+    score = float(np.float32(np.log(2.0) / (head * float(np.float32(SCALE)))))
     got = attend(backend, store, share, query, place, window, score) / float(np.float32(0.75 * SCALE))
     even, odd = seen_slots(sinks, span, place, window, lanes)
     want = two_kinds(even, odd, score * head * SIZE * float(np.float32(SCALE)))

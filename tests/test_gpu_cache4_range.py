@@ -139,3 +139,34 @@ def test_score_scales_that_are_no_numbers(backend, kv, share, head, lanes, span,
     query[0] = 0.0
     assert np.all(np.isnan(attend(backend, store, share, query, span - lanes, 0, score)))
     close(store)
+
+
+@pytest.mark.parametrize("kv,share,head,sinks,span,place,window,lanes", [
+    (1, 8, 128, 0, 400, 399, 0, 1), (16, 1, 64, 0, 40000, 39999, 0, 1), (2, 8, 64, 0, 131072, 131071, 0, 1),
+    (1, 8, 512, 0, 3000, 2000, 0, 5), (1, 8, 64, 0, 700, 0, 0, 600), (8, 8, 256, 5, 560, 3000, 300, 250),
+    (8, 16, 512, 0, 500, 370, 0, 130), (2, 8, 128, 3, 6500, 9000, 6400, 60)])
+@pytest.mark.parametrize("power", [20, 24, 27, 33, 60, 110])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_apart(backend, kv, share, head, sinks, span, place, window, lanes, power, sign):
+    """Scores of zero and of 1.3 times 2^power, positive or negative, in powers of two: a
+    row sees the mean of the higher ones' values, however coarse a float is there."""
+    print("case far", kv, share, head, span, lanes, power, sign, flush=True)
+    rng = np.random.default_rng(head + power)
+    host = ring_bytes(rng, span, kv * head, c4.E2M1)
+    host[0][:] = 0x00
+    host[0][5::90] = 0x22  # level 1
+    host[1][:] = 0x38
+    store = open_ring(backend, c4.E2M1, span, sinks, kv, head, host)
+    query = np.ones((lanes, kv * share * head), np.float32)
+    query[:] *= 1.0 + rng.integers(0, 64, size=(lanes, 1)).astype(np.float32) / 64
+    score = sign * 1.3 * 2.0 ** power * np.log(2.0) / (head * float(np.float32(SCALE)))
+    got = attend(backend, store, share, query, place, window, score).reshape(lanes, kv, share, head)
+    rows = rows_of(host, c4.E2M1, span, sinks)
+    for lane in sorted({0, lanes // 2, lanes - 1}):
+        t = c4.seen(place + lane, window, sinks)
+        far = c4.slot(t, sinks, span) % 90 == 5
+        high = far if sign > 0 and far.any() else ~far if sign < 0 and not far.all() else np.ones(len(t), bool)
+        v = rows(1, t[high]).reshape(-1, kv, head)
+        err = np.abs(got[lane] - v.mean(0)[:, None]).max()
+        assert err <= np.abs(v).max() * (64 + (len(t) + 63) // 64 + 3) * 2.0 ** -24, (lane, err)
+    close(store)

@@ -390,9 +390,9 @@ __host__ __device__ __forceinline__ bool attend4_all(int slot0, int count, int a
 // A row's base after a block with this peak (before its factor).
 __device__ __forceinline__ float attend4_base(float peak, float factor, float base, float &top_base) {
   if (peak == -INFINITY) return base;
-  const float at = peak * factor;
+  const float at = peak * factor, above = at - base;
+  if (above >= 8.0f && above < 15.0f) return base;
   const float low = fabsf(at) < 0x1p23f ? floorf(at) - 12.0f : at;  // where a float holds whole numbers
-  if (low >= base - 4.0f && low <= base + 2.0f) return base;
   top_base = fmaxf(top_base, low);
   return fmaxf(low, top_base - 58.0f);
 }

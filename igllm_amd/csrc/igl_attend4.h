@@ -387,11 +387,16 @@ __host__ __device__ __forceinline__ bool attend4_all(int slot0, int count, int a
          (a.window == 0 || place0 > place_high - a.window);
 }
 
-// A row's base after a block with this peak (before its factor).
+// Whether a row's base stays after a block with this peak (before its factor).
+__device__ __forceinline__ bool attend4_stays(float peak, float factor, float base) {
+  const float above = peak * factor - base;
+  return (above >= 8.0f && above < 15.0f) || peak == -INFINITY;
+}
+
+// The row's base after such a block.
 __device__ __forceinline__ float attend4_base(float peak, float factor, float base, float &top_base) {
-  if (peak == -INFINITY) return base;
-  const float at = peak * factor, above = at - base;
-  if (above >= 8.0f && above < 15.0f) return base;
+  if (attend4_stays(peak, factor, base)) return base;
+  const float at = peak * factor;
   const float low = fabsf(at) < 0x1p23f ? floorf(at) - 12.0f : at;  // where a float holds whole numbers
   top_base = fmaxf(top_base, low);
   return fmaxf(low, top_base - 58.0f);
@@ -650,8 +655,8 @@ __global__ __launch_bounds__(256, T > 4 && HEAD > 64 ? 2 : 1) void attend4_step_
     // ---- the base, the same in every wave, and the weights
 #pragma unroll
     for (int w = 0; w < 4; ++w) peak = fmaxf(peak, peaks[w * 16 + n]);
-    const float m = attend4_base(peak, factor, base, top_base);
-    if (__builtin_amdgcn_ballot_w64(m != base)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!attend4_stays(peak, factor, base)) != 0, 0)) {
+      const float m = attend4_base(peak, factor, base, top_base);
       const float keep = base != -INFINITY ? __builtin_amdgcn_exp2f(base - m) : 0.0f;
       total *= keep;
 #pragma unroll
@@ -660,7 +665,7 @@ __global__ __launch_bounds__(256, T > 4 && HEAD > 64 ? 2 : 1) void attend4_step_
         for (int r = 0; r < 4; ++r) out[j][r] *= keep;
       base = m;
     }
-    const float from = attend4_from(m);
+    const float from = attend4_from(base);
 #pragma unroll
     for (int j = 0; j < T; ++j) {
       half2_t hi[2], lo[2];
@@ -942,8 +947,8 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) peak = fmaxf(peak, s[b][r]);
     peak = xmax48(peak);
-    const float m = attend4_base(peak, factor, base, top_base);
-    if (__builtin_amdgcn_ballot_w64(m != base)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!attend4_stays(peak, factor, base)) != 0, 0)) {
+      const float m = attend4_base(peak, factor, base, top_base);
       const float keep = base != -INFINITY ? __builtin_amdgcn_exp2f(base - m) : 0.0f;
       total *= keep;
 #pragma unroll
@@ -955,7 +960,7 @@ __global__ __launch_bounds__(512, 2) void attend4_tile_kernel(Attend4Args a) {
     half8_t p[2];
     {
       half2_t hi[4], lo[4];
-      const float from = attend4_from(m);
+      const float from = attend4_from(base);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll

@@ -51,6 +51,6 @@ def test_two_workgroups_a_cu(kernels):
     for name, k in kernels.items():
         if "attend4_step" in name or "attend4_tile" in name:
             assert k["vgpr_count"] <= 256, (name, k)
-            assert k.get("vgpr_spill_count", 0) <= 1, (name, k)
+            assert k["private_segment_fixed_size"] <= 32, (name, k)  # a few words of 512-slot steps
         if "attend4_step" in name:
             assert 2 * k["group_segment_fixed_size"] <= 160 << 10, (name, k)

@@ -11,7 +11,7 @@
 // eight significant bits at most, exact in binary16 with the gain over 256 (their
 // scales are multiplied in afterwards).  Queries and weights are two binary16 terms
 // each, high and low, 2^-22 of themselves: one term would leave 2^-11, two products
-// leave blends as near their 64-bit value as fp32 sums do (3e-7 measured).  Products
+// leave blends as near their 64-bit value as fp32 sums do (2.7e-7 to 5.5e-7 of them).  Products
 // are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane that decodes
 // codes holds a row's eight dims, or a dim's eight rows, as one operand, and a query
 // row's scores lie along lanes as its weights are wanted.
@@ -24,6 +24,9 @@
 // third term would hold them, for half as many products again.  Bases follow peaks
 // down too, to 58 below the highest, so that positions far below others keep what
 // fp32 sums keep of them.
+//
+// Times below are of runs of some ten launches, before the card's clocks have risen:
+// after some hundred, what computes takes a tenth less.
 #pragma once
 
 #include <float.h>
@@ -203,26 +206,6 @@ __device__ __forceinline__ void value_operands(const uint32_t (&x)[8], const hal
   for (int d = 0; d < DIMS; ++d) out[d] = __builtin_bit_cast(half8_t, p[d]);
 }
 
-// The largest over groups of N neighbouring lanes, in each of them.
-template <int N>
-__device__ __forceinline__ float group_max(float v) {
-  v = fmaxf(v, dpp_move<0xB1>(v));
-  v = fmaxf(v, dpp_move<0x4E>(v));
-  v = fmaxf(v, dpp_move<0x141>(v));
-  if (N >= 16) v = fmaxf(v, dpp_move<0x140>(v));
-  if (N >= 32) {
-    float a = v, b = v;
-    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-    v = fmaxf(a, b);
-  }
-  if (N >= 64) {
-    float a = v, b = v;
-    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-    v = fmaxf(a, b);
-  }
-  return v;
-}
-
 // The same for four dims, one half (`high`, uniform) of eight rows' dwords.
 template <int FMT>
 __device__ __forceinline__ void value_operands_half(const uint32_t (&x)[8], bool high, const half2_t (&g)[4],
@@ -248,6 +231,26 @@ __device__ __forceinline__ void value_operands_half(const uint32_t (&x)[8], bool
   }
 #pragma unroll
   for (int d = 0; d < 4; ++d) out[d] = __builtin_bit_cast(half8_t, p[d]);
+}
+
+// The largest over groups of N neighbouring lanes, in each of them.
+template <int N>
+__device__ __forceinline__ float group_max(float v) {
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  if (N >= 16) v = fmaxf(v, dpp_move<0x140>(v));
+  if (N >= 32) {
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    v = fmaxf(a, b);
+  }
+  if (N >= 64) {
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    v = fmaxf(a, b);
+  }
+  return v;
 }
 
 // Largest and sum over the four lanes of a wave that differ by 16 and 32, the
@@ -462,8 +465,8 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
 // many workgroups as it has blocks: a 512 window of 256-dim heads 5.6 us and 3.7 for
 // the fold (one wave a block took 16.9 in all), 16384 positions 6.2 + 3.6.  A long
 // one is bound by its bytes and their decoding (16 us of vector issue a CU and 3 of
-// matrix): 131072 positions of eight 128-dim heads, 143 MB, in 35.4 us, 4.0 TB/s
-// (out of caches 39, 3.7).  Blocks of 512 slots fill the registers of a wave of two a
+// matrix): 131072 positions of eight 128-dim heads, 143 MB, in 34.4 us, 4.1 TB/s
+// (out of caches 41, 3.5; int4's 37.6 and 45).  Blocks of 512 slots fill the registers of a wave of two a
 // SIMD, which 128-dim heads' ask for: one register more of int4's halved the workgroups
 // a CU, and the same in int4 took 52 us where 37.4 do (e2m1 34.6, in caches both).
 // 64-dim heads' have them anyhow, and asking took 0.4 us of 29.
@@ -748,10 +751,13 @@ __global__ __launch_bounds__(256, T > 4 && HEAD > 64 ? 2 : 1) void attend4_step_
 // thread, in straight code that the scheduler is told to lay between the products.
 // Blends leave through LDS as whole rows (scattered dwords were 4 us of a window's 41).
 //
-// Bound by issue: vector work, half of it decoding, and products take turns on a SIMD,
-// 164k of 207k cycles for 2047 lanes of 512-dim heads, 124 us, 34 GFLOP before the
-// second terms; of a 512 window of 256-dim heads 36 us.  Two waves a SIMD is what 250
-// registers leave; 64 rows a workgroup halve the decoding of 32 (156 and 41 us).
+// 2047 lanes of 512-dim heads 121 us, 34 GFLOP before the second terms; of a 512 window
+// of 256-dim heads 36 us.  No unit is full: of 207k busy cycles a CU vector work, half
+// of it decoding, issues in 100k a SIMD, products in 67k, LDS serves in 81k.  A block's
+// scores, exchange, weights and blend follow one another, and two waves a SIMD, which
+// is what 250 registers leave, cover for each other only in part: a wave waits for data
+// or barriers in a third of its cycles and for its turn to issue in three tenths.  64
+// rows a workgroup halve the decoding of 32 (156 and 41 us).
 //
 // LDS.  Keys: a slot's dims in 16-byte pieces, piece s of chunk c (dims 32 c + 8 s ..
 // + 7, a dword of codes) at s HEAD / 32 + c, xor the slot's low bits.  Values: a dim's

@@ -11,10 +11,10 @@
 // eight significant bits at most, exact in binary16 with the gain over 256 (their
 // scales are multiplied in afterwards).  Queries and weights are two binary16 terms
 // each, high and low, 2^-22 of themselves: one term would leave 2^-11, two products
-// leave blends as near their 64-bit value as fp32 sums do (2.7e-7 to 5.5e-7 of them).  Products
-// are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane that decodes
-// codes holds a row's eight dims, or a dim's eight rows, as one operand, and a query
-// row's scores lie along lanes as its weights are wanted.
+// leave blends as near their 64-bit value as fp32 sums do (2.7e-7 to 5.5e-7 of them).
+// Products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane that
+// decodes codes holds a row's eight dims, or a dim's eight rows, as one operand, and a
+// query row's scores lie along lanes as its weights are wanted.
 //
 // A row's base is a whole number about twelve below the block's peak, moved only
 // where a peak leaves it by a few: most blocks rescale nothing, a block's largest
@@ -466,10 +466,11 @@ __device__ __forceinline__ void attend4_store(const Attend4Args &a, float4_t (&o
 // the fold (one wave a block took 16.9 in all), 16384 positions 6.2 + 3.6.  A long
 // one is bound by its bytes and their decoding (16 us of vector issue a CU and 3 of
 // matrix): 131072 positions of eight 128-dim heads, 143 MB, in 34.4 us, 4.1 TB/s
-// (out of caches 41, 3.5; int4's 37.6 and 45).  Blocks of 512 slots fill the registers of a wave of two a
-// SIMD, which 128-dim heads' ask for: one register more of int4's halved the workgroups
-// a CU, and the same in int4 took 52 us where 37.4 do (e2m1 34.6, in caches both).
-// 64-dim heads' have them anyhow, and asking took 0.4 us of 29.
+// (out of caches 41, 3.5; int4's 37.6 and 45).
+//
+// Blocks of 512 slots fill the registers of a wave of two a SIMD, which those of
+// 128-dim heads ask for: one register more of int4's halved the workgroups a CU, 52 us
+// for 37.6.  Those of 64-dim heads have them anyhow, and asking took 0.4 us of 29.
 template <int HEAD, bool PAIR, int T>
 struct Step4Shape {
   static constexpr int KL = HEAD >= 128 ? HEAD / 128 : 1;  // key chunks of a row a lane reads

@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import native
-from .native import Cache4, Desk, Plane, Rng
+from .native import Cache4, Desk, Experts, Mx4, Plane, Rng, Route
 
 
 class BackendError(RuntimeError):
@@ -134,6 +134,22 @@ class Ring4:
 
     cache: Cache4
     buffers: list  # key codes, key gains, value codes, value gains
+
+
+@dataclass
+class Mx4Rows:
+    """Microscaled 4-bit rows: their igl_mx4 and the buffers it names."""
+
+    rows: Mx4
+    buffers: list  # codes, scales
+
+
+@dataclass
+class ExpertSet:
+    """A layer's experts: their igl_experts and the rows it names."""
+
+    experts: Experts
+    sheets: list  # gate_up, down
 
 
 class Backend:
@@ -315,6 +331,59 @@ class Backend:
         self._check(self.lib.igl_attend4_lanes_dev(ctypes.byref(self.desk), ctypes.byref(store.cache), group_share,
                                                    query.ptr, lane_stride, place_first, window, lane_count,
                                                    score_scale, blend_out.ptr), "attend4_lanes_dev")
+
+    def mx4(self, rows: int, cols: int, code=None, scale=None, code_stride: int = 0, scale_stride: int = 0) -> Mx4Rows:
+        """Microscaled rows (igl_mx4) over the caller's buffers, or over buffers of its own, zeroed; strides in
+        bytes, 0: rows one behind the other."""
+        if rows < 1 or cols < 32 or cols % 32:
+            raise BackendError("no microscaled rows have these dimensions")
+        code_stride, scale_stride = code_stride or cols // 2, scale_stride or cols // 32
+        buffers = [self.upload(np.zeros(n, np.uint8)) if b is None else b
+                   for b, n in ((code, rows * code_stride), (scale, rows * scale_stride))]
+        return Mx4Rows(Mx4(rows, cols, buffers[0].ptr, code_stride, buffers[1].ptr, scale_stride), buffers)
+
+    def mx4_lay_dev(self, store: Mx4Rows, row_first: int, row_count: int, src: DevBuf, src_type: int, src_stride: int):
+        """Rows of floats into microscaled rows."""
+        self._check(self.lib.igl_mx4_lay_dev(ctypes.byref(self.desk), ctypes.byref(store.rows), row_first, row_count,
+                                             src.ptr, src_type, src_stride), "mx4_lay_dev")
+
+    def mx4_read_dev(self, store: Mx4Rows, row_first: int, row_count: int, dst: DevBuf, dst_type: int,
+                     dst_stride: int):
+        """Microscaled rows as floats."""
+        self._check(self.lib.igl_mx4_read_dev(ctypes.byref(self.desk), ctypes.byref(store.rows), row_first, row_count,
+                                              dst.ptr, dst_type, dst_stride), "mx4_read_dev")
+
+    def mx4_mat_mat_dev(self, sheet: Mx4Rows, act: DevBuf, act_type: int, act_stride: int, lanes: int, out: DevBuf,
+                        out_type: int, out_stride: int):
+        """A microscaled sheet times lanes of floats."""
+        self._check(self.lib.igl_mx4_mat_mat_dev(ctypes.byref(self.desk), ctypes.byref(sheet.rows), act.ptr, act_type,
+                                                 act_stride, lanes, out.ptr, out_type, out_stride), "mx4_mat_mat_dev")
+
+    def mx4_mat_mx4_dev(self, sheet: Mx4Rows, act: Mx4Rows, lane_first: int, lanes: int, out: DevBuf, out_type: int,
+                        out_stride: int):
+        """A microscaled sheet times lanes that are microscaled rows."""
+        self._check(self.lib.igl_mx4_mat_mx4_dev(ctypes.byref(self.desk), ctypes.byref(sheet.rows),
+                                                 ctypes.byref(act.rows), lane_first, lanes, out.ptr, out_type,
+                                                 out_stride), "mx4_mat_mx4_dev")
+
+    def route_dev(self, rule: Route, logits: DevBuf, logit_stride: int, lanes: int, bias: DevBuf | None,
+                  gain: DevBuf | None, pick: DevBuf, weight: DevBuf):
+        """The experts of every lane and their weights."""
+        self._check(self.lib.igl_route_dev(ctypes.byref(self.desk), ctypes.byref(rule), logits.ptr, logit_stride, lanes,
+                                           bias.ptr if bias else None, gain.ptr if gain else None, pick.ptr,
+                                           weight.ptr), "route_dev")
+
+    def experts(self, gate_up: Mx4Rows, down: Mx4Rows, expert_count: int, hidden: int, inner: int,
+                gate: int = native.IGL_GATE_GELU) -> ExpertSet:
+        """A layer's experts (igl_experts) over their microscaled weights."""
+        return ExpertSet(Experts(expert_count, hidden, inner, gate, gate_up.rows, down.rows), [gate_up, down])
+
+    def experts_dev(self, experts: ExpertSet, act: DevBuf, act_type: int, act_stride: int, lanes: int, pick: DevBuf,
+                    weight: DevBuf, top: int, out: DevBuf, out_type: int, out_stride: int):
+        """The experts' feed-forward blocks of every lane, by its picks and weights."""
+        self._check(self.lib.igl_experts_dev(ctypes.byref(self.desk), ctypes.byref(experts.experts), act.ptr, act_type,
+                                             act_stride, lanes, pick.ptr, weight.ptr, top, out.ptr, out_type,
+                                             out_stride), "experts_dev")
 
     def sync(self):
         self._check(self.lib.igl_sync(ctypes.byref(self.desk)), "sync")

@@ -91,6 +91,9 @@ struct igl_desk_state {
   /* the GEMM's binary16 copy of its activations */
   float *gemm_dev;
   size_t gemm_floats;
+  /* microscaled products: the lanes' terms; the experts' places and rows */
+  float *mx4_dev;
+  size_t mx4_floats;
   /* a recording in progress on the stream, and replays not yet freed (both
    * freeze the scratch above: a replay keeps the addresses it recorded) */
   int recording;
@@ -945,6 +948,145 @@ int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_sha
                                           st->attend4_dev, st->stream));
 }
 
+/* ---- microscaled rows, and experts ----------------------------------------- */
+
+static int fail(igl_desk_state *st, int code) {
+  desk_fail(st, code);
+  return code;
+}
+
+static int mx4_real(int type) { return type == IGL_STORE_F32 || type == IGL_STORE_BF16; }
+
+/* Rows of a type, `stride` values apart, at an alignment their type has. */
+static int mx4_rows_good(const void *rows, int type, int stride, int count, int width) {
+  return rows && mx4_real(type) && ((uintptr_t)rows & (type == IGL_STORE_F32 ? 3u : 1u)) == 0 &&
+         (count == 1 || stride >= width);
+}
+
+static int mx4_good(const igl_mx4 *s) {
+  return s && s->row_count >= 1 && s->col_count >= 32 && s->col_count % 32 == 0 && s->code && s->scale &&
+         ((uintptr_t)s->code & 15u) == 0 && s->code_stride % 16 == 0 &&
+         s->code_stride >= (size_t)s->col_count / 2 && s->scale_stride >= (size_t)s->col_count / 32;
+}
+
+static int mx4_span_good(const igl_mx4 *s, int first, int count) {
+  return mx4_good(s) && first >= 0 && count >= 1 && first <= s->row_count - count;
+}
+
+/* What laying and reading check before anything is launched. */
+static int mx4_rows_check(igl_desk_state *st, const igl_mx4 *store, int row_first, int row_count, const void *rows,
+                          int type, int stride) {
+  if (store && rows && !mx4_real(type)) return fail(st, IGL_FAIL_SUPPORT);
+  if (!mx4_span_good(store, row_first, row_count) || !mx4_rows_good(rows, type, stride, row_count, store->col_count))
+    return fail(st, IGL_FAIL_ARGUMENT);
+  if (igl_mx4_groups(store->col_count, row_count) > IGL_MX4_GROUPS_MOST) return fail(st, IGL_FAIL_SUPPORT);
+  return IGL_OKAY;
+}
+
+int igl_mx4_lay_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row_count, const void *src_dev,
+                    int src_type, int src_stride) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  int code;
+  if (!st) return IGL_FAIL_STATE;
+  if ((code = mx4_rows_check(st, store, row_first, row_count, src_dev, src_type, src_stride)) != IGL_OKAY) return code;
+  return hip_check(st, igl_launch_mx4_lay(store, row_first, row_count, src_dev, src_type == IGL_STORE_BF16, src_stride,
+                                          st->stream));
+}
+
+int igl_mx4_read_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row_count, void *dst_dev, int dst_type,
+                     int dst_stride) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  int code;
+  if (!st) return IGL_FAIL_STATE;
+  if ((code = mx4_rows_check(st, store, row_first, row_count, dst_dev, dst_type, dst_stride)) != IGL_OKAY) return code;
+  return hip_check(st, igl_launch_mx4_read(store, row_first, row_count, dst_dev, dst_type == IGL_STORE_BF16, dst_stride,
+                                           st->stream));
+}
+
+/* Room in the workspace of microscaled products. */
+static int mx4_room(igl_desk_state *st, size_t bytes) {
+  return grow_dev(st, &st->mx4_dev, &st->mx4_floats, (bytes + 3) / 4);
+}
+
+int igl_mx4_mat_mat_dev(igl_desk *desk, const igl_mx4 *sheet, const void *act_dev, int act_type, int act_stride,
+                        int lane_count, void *out_dev, int out_type, int out_stride) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  int code;
+  if (!st) return IGL_FAIL_STATE;
+  if (sheet && act_dev && out_dev && (!mx4_real(act_type) || !mx4_real(out_type))) return fail(st, IGL_FAIL_SUPPORT);
+  if (!mx4_good(sheet) || lane_count < 1 || !mx4_rows_good(act_dev, act_type, act_stride, lane_count, sheet->col_count) ||
+      !mx4_rows_good(out_dev, out_type, out_stride, lane_count, sheet->row_count))
+    return fail(st, IGL_FAIL_ARGUMENT);
+  if (lane_count > IGL_MX4_LANES_MOST || igl_mx4_groups(sheet->col_count, lane_count) > IGL_MX4_GROUPS_MOST)
+    return fail(st, IGL_FAIL_SUPPORT);
+  if ((code = mx4_room(st, igl_mx4_work_bytes(sheet->row_count, sheet->col_count, lane_count,
+                                              act_type == IGL_STORE_BF16))) != IGL_OKAY)
+    return code;
+  return hip_check(st, igl_launch_mx4_mat_mat(sheet, act_dev, act_type == IGL_STORE_BF16, act_stride, lane_count,
+                                              out_dev, out_type == IGL_STORE_BF16, out_stride, st->mx4_dev,
+                                              st->stream));
+}
+
+int igl_mx4_mat_mx4_dev(igl_desk *desk, const igl_mx4 *sheet, const igl_mx4 *act, int lane_first, int lane_count,
+                        void *out_dev, int out_type, int out_stride) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  if (!st) return IGL_FAIL_STATE;
+  if (sheet && act && out_dev && !mx4_real(out_type)) return fail(st, IGL_FAIL_SUPPORT);
+  if (!mx4_good(sheet) || !mx4_span_good(act, lane_first, lane_count) || act->col_count != sheet->col_count ||
+      !mx4_rows_good(out_dev, out_type, out_stride, lane_count, sheet->row_count))
+    return fail(st, IGL_FAIL_ARGUMENT);
+  if (lane_count > IGL_MX4_LANES_MOST) return fail(st, IGL_FAIL_SUPPORT);
+  return hip_check(st, igl_launch_mx4_mat_mx4(sheet, act, lane_first, lane_count, out_dev, out_type == IGL_STORE_BF16,
+                                              out_stride, st->stream));
+}
+
+int igl_route_dev(igl_desk *desk, const igl_route *rule, const float *logit_dev, int logit_stride, int lane_count,
+                  const float *bias_dev, const float *gain_dev, int32_t *pick_dev, float *weight_dev) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  if (!st) return IGL_FAIL_STATE;
+  if (!rule || !logit_dev || !pick_dev || !weight_dev || lane_count < 1 || rule->expert_count < 1 || rule->top < 1 ||
+      rule->top > rule->expert_count || (lane_count > 1 && logit_stride < rule->expert_count) ||
+      (rule->score != IGL_ROUTE_SOFTMAX && rule->score != IGL_ROUTE_SIGMOID) || rule->group_count < 1 ||
+      rule->expert_count % rule->group_count != 0 || rule->group_top < 1 || rule->group_top > rule->group_count ||
+      rule->group_best < 1 || rule->group_best > 2 || !(rule->gain_scale >= -FLT_MAX && rule->gain_scale <= FLT_MAX) ||
+      (((uintptr_t)logit_dev | (uintptr_t)bias_dev | (uintptr_t)gain_dev | (uintptr_t)pick_dev |
+        (uintptr_t)weight_dev) & 3u))
+    return fail(st, IGL_FAIL_ARGUMENT);
+  if (rule->expert_count > 1024 || rule->top > 64 || rule->group_count > 64 || lane_count > IGL_ROUTE_LANES_MOST)
+    return fail(st, IGL_FAIL_SUPPORT);
+  return hip_check(st, igl_launch_route(rule, logit_dev, logit_stride, lane_count, bias_dev, gain_dev, pick_dev,
+                                        weight_dev, st->stream));
+}
+
+int igl_experts_dev(igl_desk *desk, const igl_experts *experts, const void *act_dev, int act_type, int act_stride,
+                    int lane_count, const int32_t *pick_dev, const float *weight_dev, int top, void *out_dev,
+                    int out_type, int out_stride) {
+  igl_desk_state *st = desk ? desk->state : NULL;
+  const igl_experts *x = experts;
+  int code;
+  if (!st) return IGL_FAIL_STATE;
+  if (x && act_dev && out_dev && (!mx4_real(act_type) || !mx4_real(out_type))) return fail(st, IGL_FAIL_SUPPORT);
+  if (!x || x->expert_count < 1 || x->hidden < 32 || x->inner < 32 || !mx4_good(&x->gate_up) || !mx4_good(&x->down) ||
+      x->gate_up.col_count != x->hidden || x->down.col_count != x->inner ||
+      (long long)x->expert_count * 2 * x->inner != x->gate_up.row_count ||
+      (long long)x->expert_count * x->hidden != x->down.row_count ||
+      (x->gate != IGL_GATE_GELU && x->gate != IGL_GATE_SILU) || lane_count < 1 || top < 1 || !pick_dev || !weight_dev ||
+      (((uintptr_t)pick_dev | (uintptr_t)weight_dev) & 3u) ||
+      !mx4_rows_good(act_dev, act_type, act_stride, lane_count, x->hidden) ||
+      !mx4_rows_good(out_dev, out_type, out_stride, lane_count, x->hidden))
+    return fail(st, IGL_FAIL_ARGUMENT);
+  if (x->expert_count > 1024 || top > 64 ||
+      (long long)lane_count * top / 16 + x->expert_count > 65535 ||
+      igl_mx4_groups(x->hidden, lane_count * top) > IGL_MX4_GROUPS_MOST / 8 ||
+      igl_mx4_groups(x->inner, lane_count * top) > IGL_MX4_GROUPS_MOST / 8)
+    return fail(st, IGL_FAIL_SUPPORT);
+  if ((code = mx4_room(st, igl_experts_work_bytes(x, lane_count, top, act_type == IGL_STORE_BF16))) != IGL_OKAY)
+    return code;
+  return hip_check(st, igl_launch_experts(x, act_dev, act_type == IGL_STORE_BF16, act_stride, lane_count, pick_dev,
+                                          weight_dev, top, out_dev, out_type == IGL_STORE_BF16, out_stride,
+                                          st->mx4_dev, st->stream));
+}
+
 int igl_norm_rms_dev(igl_desk *desk, const float *in_dev, const float *gain_dev, int n, int rows,
                      int stride, float eps, float *out_dev) {
   igl_desk_state *st = desk ? desk->state : NULL;
@@ -1224,6 +1366,7 @@ void igl_back_close(igl_desk *desk) {
   if (st->prod_dev) (void)hipFree(st->prod_dev);
   if (st->elem_dev) (void)hipFree(st->elem_dev);
   if (st->gemm_dev) (void)hipFree(st->gemm_dev);
+  if (st->mx4_dev) (void)hipFree(st->mx4_dev);
   if (st->mark[0]) (void)hipEventDestroy(st->mark[0]);
   if (st->mark[1]) (void)hipEventDestroy(st->mark[1]);
   if (st->stream) (void)hipStreamDestroy(st->stream);

@@ -7,6 +7,7 @@
 // app_core.c:11205-11236).  They read no weights; each is one small launch.
 #include "igl_cache4.h"
 #include "igl_device.h"
+#include "igl_route.h"
 
 namespace igl {
 

@@ -31,6 +31,7 @@
 // partials that level_close_kernel adds (exactly, in any order) and closes.
 #include "igl_device.h"
 #include "igl_launch.h"
+#include "igl_mx4.h"
 
 namespace igl {
 

@@ -241,6 +241,34 @@ hipError_t igl_launch_attend4(const igl_cache4 *store, int group_share, const fl
                               int lane_stride, int place_first, int window, int lanes,
                               float score_scale, float *blend_out, float *work, hipStream_t stream);
 
+/* Microscaled rows and the experts that have such weights (igl_mx4.h, included by
+ * igl_gemm_level.hip), and the choice of experts (igl_route.h, by igl_elem.hip).  A
+ * thread for every eight values of rows (igl_mx4_groups workgroups), a tile of
+ * lanes a row of workgroups. */
+static inline long long igl_mx4_groups(int cols, int rows) {
+  return ((long long)rows * (cols / 8) + 255) / 256;
+}
+#define IGL_MX4_GROUPS_MOST ((1 << 24) - 1)
+#define IGL_MX4_LANES_MOST (65535 * 16)
+#define IGL_ROUTE_LANES_MOST ((1 << 26) - 64)
+hipError_t igl_launch_mx4_lay(const igl_mx4 *store, int row_first, int rows, const void *src, int bf16,
+                              int src_stride, hipStream_t stream);
+hipError_t igl_launch_mx4_read(const igl_mx4 *store, int row_first, int rows, void *dst, int bf16,
+                               int dst_stride, hipStream_t stream);
+size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int act_bf16);
+hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *act, int act_bf16, int act_stride,
+                                  int lanes, void *out, int out_bf16, int out_stride, void *work,
+                                  hipStream_t stream);
+hipError_t igl_launch_mx4_mat_mx4(const igl_mx4 *sheet, const igl_mx4 *act, int lane_first, int lanes,
+                                  void *out, int out_bf16, int out_stride, hipStream_t stream);
+size_t igl_experts_work_bytes(const igl_experts *x, int lanes, int top, int act_bf16);
+hipError_t igl_launch_experts(const igl_experts *x, const void *act, int act_bf16, int act_stride,
+                              int lanes, const int32_t *pick, const float *weight, int top, void *out,
+                              int out_bf16, int out_stride, void *work, hipStream_t stream);
+hipError_t igl_launch_route(const igl_route *rule, const float *logits, int logit_stride, int lanes,
+                            const float *bias, const float *gain, int32_t *pick, float *weight,
+                            hipStream_t stream);
+
 /* The desk's HIP stream, for the engine's own launches (back_hip.c). */
 void *igl_desk_stream(igl_desk *desk);
 /* Changes whenever the desk reallocates a workspace: a graph captured over

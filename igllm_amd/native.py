@@ -29,6 +29,10 @@ IGL_CACHE_E4M3 = 0
 IGL_CACHE_INT8 = 1
 IGL_CACHE4_INT4 = 0
 IGL_CACHE4_E2M1 = 1
+IGL_ROUTE_SOFTMAX = 0
+IGL_ROUTE_SIGMOID = 1
+IGL_GATE_GELU = 0
+IGL_GATE_SILU = 1
 
 c_float_p = ctypes.POINTER(ctypes.c_float)
 c_u8_p = ctypes.POINTER(ctypes.c_uint8)
@@ -83,6 +87,28 @@ class Cache4(ctypes.Structure):
             ("key_scale", ctypes.c_float), ("value_scale", ctypes.c_float),
             ("key_code", ctypes.c_void_p), ("key_gain", ctypes.c_void_p),
             ("value_code", ctypes.c_void_p), ("value_gain", ctypes.c_void_p)]
+
+
+class Mx4(ctypes.Structure):
+    """`igl_mx4`: microscaled 4-bit rows in device memory."""
+
+    _fields_ = [("row_count", ctypes.c_int), ("col_count", ctypes.c_int), ("code", ctypes.c_void_p),
+                ("code_stride", ctypes.c_size_t), ("scale", ctypes.c_void_p), ("scale_stride", ctypes.c_size_t)]
+
+
+class Route(ctypes.Structure):
+    """`igl_route`: how a lane's experts are chosen."""
+
+    _fields_ = [(n, ctypes.c_int) for n in (
+        "expert_count", "top", "score", "group_count", "group_top", "group_best", "renorm")] + [
+            ("gain_scale", ctypes.c_float)]
+
+
+class Experts(ctypes.Structure):
+    """`igl_experts`: a layer's experts with microscaled weights."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("expert_count", "hidden", "inner", "gate")] + [
+        ("gate_up", Mx4), ("down", Mx4)]
 
 
 class Rng(ctypes.Structure):
@@ -161,6 +187,12 @@ SIGNATURES = {
     "igl_cache4_lay_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Cache4), _P, _P, _I, _I, _I]),
     "igl_cache4_read_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Cache4), _I, _I, _P, _P, _I]),
     "igl_attend4_lanes_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Cache4), _I, _P, _I, _I, _I, _I, _F, _P]),
+    "igl_mx4_lay_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Mx4), _I, _I, _P, _I, _I]),
+    "igl_mx4_read_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Mx4), _I, _I, _P, _I, _I]),
+    "igl_mx4_mat_mat_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Mx4), _P, _I, _I, _I, _P, _I, _I]),
+    "igl_mx4_mat_mx4_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Mx4), ctypes.POINTER(Mx4), _I, _I, _P, _I, _I]),
+    "igl_route_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Route), _P, _I, _I, _P, _P, _P, _P]),
+    "igl_experts_dev": (_I, [ctypes.POINTER(Desk), ctypes.POINTER(Experts), _P, _I, _I, _I, _P, _P, _I, _P, _I, _I]),
     "igl_norm_rms_dev": (_I, [ctypes.POINTER(Desk), _P, _P, _I, _I, _I, _F, _P]),
     "igl_soft_max_dev": (_I, [ctypes.POINTER(Desk), _P, _I, _I, _I]),
     "igl_gelu_gate_dev": (_I, [ctypes.POINTER(Desk), _P, _P, _I]),

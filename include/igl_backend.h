@@ -306,6 +306,98 @@ int igl_attend4_lanes_dev(igl_desk *desk, const igl_cache4 *store, int group_sha
                           const float *query_dev, int lane_stride, int place_first, int window,
                           int lane_count, float score_scale, float *blend_out_dev);
 
+/* ---- microscaled 4-bit rows -------------------------------------------------- */
+
+/* No counterpart in the reference: weights, or activations, as e2m1 codes with a
+ * power of two for every 32 (the MX form).  A code has a sign, two bits of
+ * exponent and one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives; a
+ * scale byte b stands for 2^(b - 127), 255 for a NaN.  Rows lie in device memory
+ * of the caller's: codes two a byte, low nibble first, code_stride bytes apart (16-
+ * byte aligned, a multiple of 16), scale bytes one a group, scale_stride apart. */
+typedef struct igl_mx4 {
+  int      row_count;
+  int      col_count;    /* a multiple of 32 */
+  uint8_t *code;
+  size_t   code_stride;  /* col_count / 2 at least */
+  uint8_t *scale;
+  size_t   scale_stride; /* col_count / 32 at least */
+} igl_mx4;
+
+/* Rows of floats (IGL_STORE_F32 or IGL_STORE_BF16, src_stride values apart) into
+ * rows row_first .. + row_count - 1: a group's power of two is two below its largest
+ * magnitude's (2^-127 at least), a value's code the nearest level, ties to the even
+ * code, 6 at most.  A group with an infinity or a NaN gets scale 255 and codes 0. */
+int igl_mx4_lay_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row_count,
+                    const void *src_dev, int src_type, int src_stride);
+/* Rows as floats again: level * 2^(b - 127), exactly but where F32 or BF16 has no
+ * such small number. */
+int igl_mx4_read_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row_count,
+                     void *dst_dev, int dst_type, int dst_stride);
+/* igl_mat_mat_dev for a microscaled sheet: out[m] = sheet x[m], lanes of act_type to
+ * lanes of out_type (F32 or BF16), sums in 32 bits.  F32 lanes are taken to 2^-24
+ * and BF16 lanes to 2^-14 of the largest of their 32 values (a bf16 output has 2^-8);
+ * neither finer than 2^-130 and 2^-120.  A lane with an infinity or a NaN has NaN
+ * outputs.  Lanes are cut into terms in the desk's workspace, which grows
+ * to lanes * col_count * 4 bytes (2.5 for BF16): call it once before recording. */
+int igl_mx4_mat_mat_dev(igl_desk *desk, const igl_mx4 *sheet, const void *act_dev, int act_type,
+                        int act_stride, int lane_count, void *out_dev, int out_type,
+                        int out_stride);
+/* The same for lanes that are microscaled rows, act's lane_first .. + lane_count - 1;
+ * no workspace. */
+int igl_mx4_mat_mx4_dev(igl_desk *desk, const igl_mx4 *sheet, const igl_mx4 *act, int lane_first,
+                        int lane_count, void *out_dev, int out_type, int out_stride);
+
+/* ---- experts ------------------------------------------------------------------- */
+
+/* The router's scores and the gate of the experts of the reference's graph
+ * (app_core.c:11582-11635), and the forms other models take. */
+typedef enum igl_route_score { IGL_ROUTE_SOFTMAX = 0, IGL_ROUTE_SIGMOID = 1 } igl_route_score;
+typedef enum igl_gate { IGL_GATE_GELU = 0, IGL_GATE_SILU = 1 } igl_gate;
+
+typedef struct igl_route {
+  int   expert_count; /* 1 .. 1024 */
+  int   top;          /* experts a lane takes, 64 at most */
+  int   score;        /* igl_route_score */
+  int   group_count;  /* groups of neighbouring experts, 64 at most; 1: none */
+  int   group_top;    /* groups that stay */
+  int   group_best;   /* a group's score: its largest choice (1) or its two largest's sum (2) */
+  int   renorm;       /* the weights of a lane over their sum */
+  float gain_scale;   /* times every weight */
+} igl_route;
+
+/* The experts of every lane and their weights, pick_dev and weight_dev
+ * [lane_count][top], from router logits [lane_count][logit_stride]: scores s =
+ * softmax or sigmoid; choices s + bias_dev[e] (bias_dev may be NULL); with groups only
+ * the group_top groups of the largest group scores stay; the `top` largest choices in
+ * falling order, the lowest index first where equal.  A weight is the chosen s (over
+ * the sum of the lane's with renorm; zero where that is zero), times gain_scale and
+ * gain_dev[e] (may be NULL).  Choices are formed and compared in 64 bits.  An expert
+ * whose logit is minus infinity or a NaN, or whose choice is, is never chosen; a lane
+ * with too few has -1 and weight 0 in the places left over.  A logit of plus infinity
+ * counts as the largest float. */
+int igl_route_dev(igl_desk *desk, const igl_route *rule, const float *logit_dev, int logit_stride,
+                  int lane_count, const float *bias_dev, const float *gain_dev, int32_t *pick_dev,
+                  float *weight_dev);
+
+/* A layer's experts with microscaled weights. */
+typedef struct igl_experts {
+  int     expert_count;
+  int     hidden;   /* a multiple of 32 */
+  int     inner;    /* a multiple of 32 */
+  int     gate;     /* igl_gate */
+  igl_mx4 gate_up;  /* [expert_count * 2 * inner] rows of hidden: an expert's gate rows, then its up rows */
+  igl_mx4 down;     /* [expert_count * hidden] rows of inner */
+} igl_experts;
+
+/* out[m] = sum_j weight[m][j] down_e(gate(gate_e x[m]) * up_e x[m]), e = pick[m][j], j
+ * in rising order: igl_route_dev's picks and weights, [lane_count][top].  A pick
+ * outside 0 .. expert_count - 1 takes no expert; a lane without one is zero.  Lanes and
+ * their precision as igl_mx4_mat_mat_dev's.  The desk's workspace grows with the
+ * call's size: call it once before recording. */
+int igl_experts_dev(igl_desk *desk, const igl_experts *experts, const void *act_dev, int act_type,
+                    int act_stride, int lane_count, const int32_t *pick_dev,
+                    const float *weight_dev, int top, void *out_dev, int out_type, int out_stride);
+
 int igl_norm_rms_dev(igl_desk *desk, const float *in_dev, const float *gain_dev, int n, int rows,
                      int stride, float eps, float *out_dev);
 int igl_soft_max_dev(igl_desk *desk, float *v_dev, int n, int rows, int stride);

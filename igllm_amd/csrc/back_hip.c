@@ -969,6 +969,9 @@ static int mx4_good(const igl_mx4 *s) {
          s->code_stride >= (size_t)s->col_count / 2 && s->scale_stride >= (size_t)s->col_count / 32;
 }
 
+/* Kernels count a wave's rows (128) in 32 bits. */
+static int mx4_wide(const igl_mx4 *s) { return s->code_stride > (size_t)1 << 24; }
+
 static int mx4_span_good(const igl_mx4 *s, int first, int count) {
   return mx4_good(s) && first >= 0 && count >= 1 && first <= s->row_count - count;
 }
@@ -1017,10 +1020,10 @@ int igl_mx4_mat_mat_dev(igl_desk *desk, const igl_mx4 *sheet, const void *act_de
   if (!mx4_good(sheet) || lane_count < 1 || !mx4_rows_good(act_dev, act_type, act_stride, lane_count, sheet->col_count) ||
       !mx4_rows_good(out_dev, out_type, out_stride, lane_count, sheet->row_count))
     return fail(st, IGL_FAIL_ARGUMENT);
-  if (lane_count > IGL_MX4_LANES_MOST || igl_mx4_groups(sheet->col_count, lane_count) > IGL_MX4_GROUPS_MOST)
+  if (mx4_wide(sheet) || lane_count > IGL_MX4_LANES_MOST || igl_mx4_groups(sheet->col_count, lane_count) > IGL_MX4_GROUPS_MOST)
     return fail(st, IGL_FAIL_SUPPORT);
   if ((code = mx4_room(st, igl_mx4_work_bytes(sheet->row_count, sheet->col_count, lane_count,
-                                              act_type == IGL_STORE_BF16))) != IGL_OKAY)
+                                              act_type == IGL_STORE_BF16 ? 3 : 5))) != IGL_OKAY)
     return code;
   return hip_check(st, igl_launch_mx4_mat_mat(sheet, act_dev, act_type == IGL_STORE_BF16, act_stride, lane_count,
                                               out_dev, out_type == IGL_STORE_BF16, out_stride, st->mx4_dev,
@@ -1030,14 +1033,17 @@ int igl_mx4_mat_mat_dev(igl_desk *desk, const igl_mx4 *sheet, const void *act_de
 int igl_mx4_mat_mx4_dev(igl_desk *desk, const igl_mx4 *sheet, const igl_mx4 *act, int lane_first, int lane_count,
                         void *out_dev, int out_type, int out_stride) {
   igl_desk_state *st = desk ? desk->state : NULL;
+  int code;
   if (!st) return IGL_FAIL_STATE;
   if (sheet && act && out_dev && !mx4_real(out_type)) return fail(st, IGL_FAIL_SUPPORT);
   if (!mx4_good(sheet) || !mx4_span_good(act, lane_first, lane_count) || act->col_count != sheet->col_count ||
       !mx4_rows_good(out_dev, out_type, out_stride, lane_count, sheet->row_count))
     return fail(st, IGL_FAIL_ARGUMENT);
-  if (lane_count > IGL_MX4_LANES_MOST) return fail(st, IGL_FAIL_SUPPORT);
+  if (mx4_wide(sheet) || mx4_wide(act) || lane_count > IGL_MX4_LANES_MOST) return fail(st, IGL_FAIL_SUPPORT);
+  if ((code = mx4_room(st, igl_mx4_work_bytes(sheet->row_count, sheet->col_count, lane_count, 0))) != IGL_OKAY)
+    return code;
   return hip_check(st, igl_launch_mx4_mat_mx4(sheet, act, lane_first, lane_count, out_dev, out_type == IGL_STORE_BF16,
-                                              out_stride, st->stream));
+                                              out_stride, st->mx4_dev, st->stream));
 }
 
 int igl_route_dev(igl_desk *desk, const igl_route *rule, const float *logit_dev, int logit_stride, int lane_count,
@@ -1075,7 +1081,7 @@ int igl_experts_dev(igl_desk *desk, const igl_experts *experts, const void *act_
       !mx4_rows_good(act_dev, act_type, act_stride, lane_count, x->hidden) ||
       !mx4_rows_good(out_dev, out_type, out_stride, lane_count, x->hidden))
     return fail(st, IGL_FAIL_ARGUMENT);
-  if (x->expert_count > 1024 || top > 64 ||
+  if (x->expert_count > 1024 || top > 64 || mx4_wide(&x->gate_up) || mx4_wide(&x->down) ||
       (long long)lane_count * top / 16 + x->expert_count > 65535 ||
       igl_mx4_groups(x->hidden, lane_count * top) > IGL_MX4_GROUPS_MOST / 8 ||
       igl_mx4_groups(x->inner, lane_count * top) > IGL_MX4_GROUPS_MOST / 8)

@@ -255,12 +255,13 @@ hipError_t igl_launch_mx4_lay(const igl_mx4 *store, int row_first, int rows, con
                               int src_stride, hipStream_t stream);
 hipError_t igl_launch_mx4_read(const igl_mx4 *store, int row_first, int rows, void *dst, int bf16,
                                int dst_stride, hipStream_t stream);
-size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int act_bf16);
+/* terms: 5 and 3 for lanes of floats and bf16, 0 for microscaled ones. */
+size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int terms);
 hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *act, int act_bf16, int act_stride,
                                   int lanes, void *out, int out_bf16, int out_stride, void *work,
                                   hipStream_t stream);
 hipError_t igl_launch_mx4_mat_mx4(const igl_mx4 *sheet, const igl_mx4 *act, int lane_first, int lanes,
-                                  void *out, int out_bf16, int out_stride, hipStream_t stream);
+                                  void *out, int out_bf16, int out_stride, void *work, hipStream_t stream);
 size_t igl_experts_work_bytes(const igl_experts *x, int lanes, int top, int act_bf16);
 hipError_t igl_launch_experts(const igl_experts *x, const void *act, int act_bf16, int act_stride,
                               int lanes, const int32_t *pick, const float *weight, int top, void *out,

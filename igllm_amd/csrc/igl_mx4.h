@@ -32,6 +32,10 @@ typedef float float32_t __attribute__((ext_vector_type(32)));
 
 constexpr int kMx4Group = 32;
 
+// A step of a product is four groups of a row, one for each sixteen lanes of a wave
+// (its parts); two steps are a cache line of codes, and steps are taken in pairs.
+__host__ __device__ constexpr int mx4_steps(int groups) { return (groups + 7) / 8 * 2; }
+
 // ---- rows ---------------------------------------------------------------------
 
 struct __attribute__((packed)) Mx4Quad {
@@ -45,9 +49,7 @@ __device__ __forceinline__ float bf16_float(uint16_t b) { return __builtin_bit_c
 
 // bf16 of a float, nearest, ties to even; a NaN stays one.
 __device__ __forceinline__ uint16_t float_bf16(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+  return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
 }
 
 // Eight values of a row, at any alignment that their type allows.
@@ -150,21 +152,24 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(const uint8_t *code, size
 
 // ---- lanes of floats as terms ---------------------------------------------------
 
-// A group of a lane in T terms: six dwords a term, then the scale bytes of the first
-// four (s, s - 5, ..), and of the fifth; whole chunks of sixteen bytes.
+// Four groups of a lane (a step of a product) in T terms of six dwords: the first four
+// dwords of every term and group (64 bytes a term), then the last two (32 bytes a
+// term), then the scales as if a term's last two: the bytes of the first four terms (s,
+// s - 5, ..) and of the fifth.  An operand is then sixteen bytes and eight, each read
+// in place, and a step of a lane is one block.
 template <int T>
 struct TermForm {
-  static constexpr int kDwords = T == 5 ? 32 : 20;
-  static constexpr int kBytes = 4 * kDwords;
-  static constexpr int kScale = 6 * T;  // the dword of the scales
-  static_assert(6 * T + (T + 3) / 4 <= kDwords, "room");
+  static constexpr int kStep = T * 96 + 32;  // bytes: 320, 512
+  static constexpr int kChunks = kStep / 64; // of sixteen bytes a group
+  static constexpr int low(int t, int part) { return 64 * t + 16 * part; }
+  static constexpr int high(int t, int part) { return 64 * T + 32 * t + 8 * part; }
 };
 
 // The terms of a group.  s is 20 at least, so that s - 5 j stays a byte (five terms
 // then end at 2^-130, three at 2^-120); an infinity or a NaN makes the scale a NaN, so that
 // every output of its lane is one.
 template <int T>
-__device__ __forceinline__ void mx4_terms(float (&x)[32], uint32_t (&rec)[TermForm<T>::kDwords]) {
+__device__ __forceinline__ void mx4_terms(float (&x)[32], uint8_t *step, int part) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 32; ++i) top = max(top, abs_bits(x[i]));
@@ -183,7 +188,10 @@ __device__ __forceinline__ void mx4_terms(float (&x)[32], uint32_t (&rec)[TermFo
     }
     const uint6_t w = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, 1.0f);
 #pragma unroll
-    for (int i = 0; i < 6; ++i) rec[6 * t + i] = w[i];
+    for (int i = 0; i < 1; ++i) {
+      *reinterpret_cast<uint4_t *>(step + TermForm<T>::low(t, part)) = uint4_t{w[0], w[1], w[2], w[3]};
+      *reinterpret_cast<uint2_t *>(step + TermForm<T>::high(t, part)) = uint2_t{w[4], w[5]};
+    }
     if (t + 1 < T) {
       const float32_t back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, 32.0f);
 #pragma unroll
@@ -191,42 +199,53 @@ __device__ __forceinline__ void mx4_terms(float (&x)[32], uint32_t (&rec)[TermFo
     }
   }
   if (none) s = 255;
-  rec[TermForm<T>::kScale] = (uint32_t)s * 0x01010101u - 0x0F0A0500u;
-  if (T == 5) rec[TermForm<T>::kScale + 1] = (uint32_t)(s - 20);
-#pragma unroll
-  for (int i = TermForm<T>::kScale + (T + 3) / 4; i < TermForm<T>::kDwords; ++i) rec[i] = 0;
+  *reinterpret_cast<uint2_t *>(step + TermForm<T>::high(T, part)) =
+      uint2_t{(uint32_t)s * 0x01010101u - 0x0F0A0500u, (uint32_t)(s - 20)};
 }
 
-// The operand of term t of a record, and its scale.
+// The operand of term t of a group, and its scales.
 template <int T>
-__device__ __forceinline__ int8v_t term_operand(const uint32_t (&rec)[TermForm<T>::kDwords], int t) {
-  return int8v_t{(int)rec[6 * t],     (int)rec[6 * t + 1], (int)rec[6 * t + 2], (int)rec[6 * t + 3],
-                 (int)rec[6 * t + 4], (int)rec[6 * t + 5], 0,                   0};
+__device__ __forceinline__ int8v_t term_operand(const uint8_t *step, int t, int part) {
+  const uint4_t a = *reinterpret_cast<const uint4_t *>(step + TermForm<T>::low(t, part));
+  const uint2_t b = *reinterpret_cast<const uint2_t *>(step + TermForm<T>::high(t, part));
+  return int8v_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], 0, 0};
 }
 
-// A thread a group: lanes of floats to records [lane][groups].
+template <int T>
+__device__ __forceinline__ uint2_t term_scales(const uint8_t *step, int part) {
+  return *reinterpret_cast<const uint2_t *>(step + TermForm<T>::high(T, part));
+}
+
+// Steps lie by step, then by lane, so that sixteen lanes of a product are one block.
+template <int T>
+__device__ __forceinline__ size_t term_at(size_t lane, int step, size_t lanes) {
+  return ((size_t)step * lanes + lane) * TermForm<T>::kStep;
+}
+
+// A thread for group id of the lanes' groups: floats to its terms.
 template <int T, bool BF16>
-__global__ __launch_bounds__(256) void mx4_terms_kernel(const void *act, long long act_stride, int groups, int lanes,
-                                                        uint32_t *terms) {
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long lane = id / groups;
-  const int g = (int)(id - lane * groups);
+__device__ __forceinline__ void mx4_terms_group(const void *act, long long act_stride, int groups, int lanes,
+                                                uint8_t *terms, long long id) {
+  const int padded = 4 * mx4_steps(groups);
+  const long long lane = id / padded;
+  const int g = (int)(id - lane * padded);
   if (lane >= lanes) return;
   const void *row = static_cast<const uint8_t *>(act) + (size_t)lane * (size_t)act_stride * (BF16 ? 2 : 4);
   float x[32];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    float part[8];
-    mx4_load8<BF16>(row, 32 * (size_t)g + 8 * e, part);
+    float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};  // groups behind the last are zeros
+    if (g < groups) mx4_load8<BF16>(row, 32 * (size_t)g + 8 * e, part);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[8 * e + i] = part[i];
   }
-  uint32_t rec[TermForm<T>::kDwords];
-  mx4_terms<T>(x, rec);
-  uint4_t *dst = reinterpret_cast<uint4_t *>(terms + (size_t)id * TermForm<T>::kDwords);
-#pragma unroll
-  for (int i = 0; i < TermForm<T>::kDwords / 4; ++i)
-    dst[i] = uint4_t{rec[4 * i], rec[4 * i + 1], rec[4 * i + 2], rec[4 * i + 3]};
+  mx4_terms<T>(x, terms + term_at<T>((size_t)lane, g >> 2, (size_t)lanes), g & 3);
+}
+
+template <int T, bool BF16>
+__global__ __launch_bounds__(256) void mx4_terms_kernel(const void *act, long long act_stride, int groups, int lanes,
+                                                        uint8_t *terms) {
+  mx4_terms_group<T, BF16>(act, act_stride, groups, lanes, terms, (long long)blockIdx.x * 256 + threadIdx.x);
 }
 
 // ---- the product ------------------------------------------------------------------
@@ -249,14 +268,18 @@ struct Mx4Tile {
 struct Mx4Args {
   Mx4View w;
   int rows, groups;         // rows of a sheet (an expert's), groups of a row
-  const uint32_t *terms;    // records [lane][groups], lanes of floats
+  const uint8_t *terms;     // of term_lanes lanes of floats
+  int term_lanes;
   Mx4View act;              // or microscaled lanes
   int lanes;
   // grouped: the tiles, how many there are, and the lane of every place (NULL: the place)
   const Mx4Tile *tiles;
   const int *tile_count;
   const int *lane_of;
-  void *out;                // [lane or place][out_stride]
+  const uint8_t *row_scales;    // packed (mx4_prepare_kernel), for the tile kernel
+  const uint32_t *lane_scales;
+  void *out;                // [lane or place][out_stride]; the experts' gate: terms of out_stride places
+  int silu;                 // the experts' gate
   long long out_stride;
 };
 
@@ -292,25 +315,21 @@ __global__ __launch_bounds__(256) void mx4_wave_kernel(Mx4Args g) {
   const int place = first + min(at, count - 1);
   const size_t from = (size_t)(g.lane_of ? g.lane_of[place] : place);
   float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int g0 = 0; g0 < g.groups; g0 += 4) {
+  const int steps = mx4_steps(g.groups);
+  for (int s = 0; s < steps; ++s) {
     int ws, as;
-    const int8v_t w = mx4_group(g.w, row, g0 + part, g.groups, ws);
+    const int8v_t w = mx4_group(g.w, row, 4 * s + part, g.groups, ws);
     if constexpr (T == 0) {
-      const int8v_t a = mx4_group(g.act, from, g0 + part, g.groups, as);
+      const int8v_t a = mx4_group(g.act, from, 4 * s + part, g.groups, as);
       acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 4, 4, 0, ws, 0, as);
     } else {
-      uint32_t rec[TermForm<T>::kDwords];
-      const uint4_t *src = reinterpret_cast<const uint4_t *>(
-          g.terms + (from * (size_t)g.groups + (size_t)min(g0 + part, g.groups - 1)) * TermForm<T>::kDwords);
-#pragma unroll
-      for (int i = 0; i < TermForm<T>::kDwords / 4; ++i) {
-        const uint4_t c = g0 + part < g.groups ? src[i] : uint4_t{0, 0, 0, 0};
-        rec[4 * i] = c[0], rec[4 * i + 1] = c[1], rec[4 * i + 2] = c[2], rec[4 * i + 3] = c[3];
-      }
+      const uint8_t *step = g.terms + term_at<T>(from, s, (size_t)g.term_lanes);
+      const uint2_t scales = term_scales<T>(step, part);
 #pragma unroll
       for (int t = 0; t < T; ++t) {
-        as = t < 4 ? (int)(rec[TermForm<T>::kScale] >> (8 * t)) : (int)rec[TermForm<T>::kScale + 1];
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, term_operand<T>(rec, t), acc, 4, 2, 0, ws, 0, as);
+        as = t < 4 ? (int)(scales[0] >> (8 * t)) : (int)scales[1];
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, term_operand<T>(step, t, part), acc, 4, 2, 0, ws,
+                                                               0, as);
       }
     }
   }
@@ -328,12 +347,17 @@ __global__ __launch_bounds__(256) void mx4_wave_kernel(Mx4Args g) {
   }
 }
 
-// ---- the experts' feed-forward ------------------------------------------------------
+// silu(x) = x / (1 + e^-x)
+__device__ __forceinline__ float silu_near(float x) {
+  if (!(x > -87.0f)) return x * 0.0f;
+  return x / (1.0f + exp_near(x > 87.0f ? -87.0f : -x));
+}
 
-// Places: the slots (lane, choice) in the order of their experts.  One workgroup
-// counts them, sets every expert's range and tiles, and lists the slots; a slot whose
-// expert is none (out of range) has no place.
-constexpr int kPlaceThreads = 1024;
+// ---- experts' places ----------------------------------------------------------------
+
+// Places: the slots (lane, choice) in the order of their experts; tiles: pieces of an
+// expert's places.  A slot whose expert is none (out of range) has no place.
+constexpr int kExpertsMost = 1024;
 
 struct PlaceArgs {
   const int32_t *pick;
@@ -342,54 +366,458 @@ struct PlaceArgs {
   int *place_of;                  // [slots] place of a slot, or -1
   Mx4Tile *tiles;
   int *tile_count;
-  int *count;                     // [experts] scratch
 };
 
-__global__ __launch_bounds__(kPlaceThreads) void expert_place_kernel(PlaceArgs a) {
-  for (int e = threadIdx.x; e < a.experts; e += kPlaceThreads) a.count[e] = 0;
+// One workgroup of 256: counts, running sums of places and tiles over the experts (four a
+// thread), then the slots' numbers.  Which place of its expert a slot gets is not the
+// same each time; nothing that is computed depends on it.
+__device__ __forceinline__ void expert_place(const PlaceArgs &a) {
+  __shared__ int counts[kExpertsMost], sums[2][256];
+  const int tid = threadIdx.x;
+  for (int e = tid; e < kExpertsMost; e += 256) counts[e] = 0;
   __syncthreads();
-  for (int s = threadIdx.x; s < a.slots; s += kPlaceThreads) {
+  for (int s = tid; s < a.slots; s += 256) {
     const int e = a.pick[s];
-    if (e >= 0 && e < a.experts) atomicAdd(&a.count[e], 1);
+    if (e >= 0 && e < a.experts) atomicAdd(&counts[e], 1);
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int place = 0, tile = 0;
-    for (int e = 0; e < a.experts; ++e) {
-      const int n = a.count[e];
-      a.count[e] = place;
-      for (int i = 0; i < n; i += a.tile) a.tiles[tile++] = Mx4Tile{e, place + i, min(a.tile, n - i)};
-      place += n;
-    }
-    *a.tile_count = tile;
+  int n[4], places = 0, tiles = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    n[i] = counts[4 * tid + i];
+    places += n[i];
+    tiles += (n[i] + a.tile - 1) / a.tile;
+  }
+  sums[0][tid] = places;
+  sums[1][tid] = tiles;
+  __syncthreads();
+  for (int d = 1; d < 256; d *= 2) {
+    const int p = tid >= d ? sums[0][tid - d] : 0, t = tid >= d ? sums[1][tid - d] : 0;
+    __syncthreads();
+    sums[0][tid] += p;
+    sums[1][tid] += t;
+    __syncthreads();
+  }
+  if (tid == 255) *a.tile_count = sums[1][255];
+  int place = sums[0][tid] - places, tile = sums[1][tid] - tiles;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    counts[4 * tid + i] = place;
+    for (int at = 0; at < n[i]; at += a.tile) a.tiles[tile++] = Mx4Tile{4 * tid + i, place + at, min(a.tile, n[i] - at)};
+    place += n[i];
   }
   __syncthreads();
-  for (int s = threadIdx.x; s < a.slots; s += kPlaceThreads) {
+  for (int s = tid; s < a.slots; s += 256) {
     const int e = a.pick[s];
-    int place = -1;
+    int at = -1;
     if (e >= 0 && e < a.experts) {
-      place = atomicAdd(&a.count[e], 1);
-      a.lane_of[place] = s / a.top;
+      at = atomicAdd(&counts[e], 1);
+      a.lane_of[at] = s / a.top;
     }
-    a.place_of[s] = place;
+    a.place_of[s] = at;
   }
 }
 
-// silu(x) = x / (1 + e^-x)
-__device__ __forceinline__ float silu_near(float x) {
-  if (!(x > -87.0f)) return x * 0.0f;
-  return x / (1.0f + exp_near(x > 87.0f ? -87.0f : -x));
+// The product of many lanes: WM x WN waves of 16 MT lanes x 16 NT rows, 128 columns a
+// step, both operands through LDS in two stages.
+//   * Stages are written only by global_load_lds, a step ahead.  A load to registers
+//     in the loop costs more than it brings: with such loads and these in flight the
+//     compiler waits for all of either.
+//   * Lanes' terms lie in the order in which they are read, sixteen bytes a wave lane
+//     side by side, so no bank meets twice; a row's four 16-byte pieces of codes are
+//     xored by a row key (tile_key) for the same end.
+//   * Scale bytes were put in the order of their reading by the launch before
+//     (mx4_prepare_kernel): as they lie, a byte a lane and row, they would take the
+//     cache as long as the codes do.
+template <int T, int MT, int NT, int WM, int WN>
+struct TileForm {
+  static_assert(NT % 4 == 0, "words of scale bytes");
+  static constexpr int kWaves = WM * WN;
+  static constexpr int kLanes = 16 * MT * WM;
+  static constexpr int kWaveRows = 16 * NT;
+  static constexpr int kRows = kWaveRows * WN;
+  static constexpr int kChunks = T == 0 ? 1 : TermForm<T == 0 ? 3 : T>::kChunks;  // of 1 KB, a tile of lanes
+  static constexpr int kLaneLoads = MT * WM * kChunks;              // DMA instructions of a step: lanes,
+  static constexpr int kRowLoads = NT * WN;                         // codes,
+  static constexpr int kScaleLoads = (kRows * 4 + 1023) / 1024;     // their scales,
+  static constexpr int kLaneScales = T == 0 ? (kLanes * 4 + 1023) / 1024 : 0;  // and microscaled lanes'
+  static constexpr int kAll = kLaneLoads + kRowLoads + kScaleLoads + kLaneScales;
+  static constexpr int kLoads = (kAll + kWaves - 1) / kWaves;       // of a wave
+  static constexpr int kRowsAt = kLaneLoads * 1024, kScalesAt = kRowsAt + kRowLoads * 1024;
+  static constexpr int kLaneScalesAt = kScalesAt + kScaleLoads * 1024;
+  static constexpr int kStage = kAll * 1024;
+  static constexpr int kOut = kWaves * 16 * (kWaveRows + 4) * 4;    // a tile of lanes' outputs of every wave
+  static constexpr int kGate = kWaves * 16 * MT * (kWaveRows / 2 + 4) * 4;  // all hidden values
+  static constexpr int most(int a, int b) { return a > b ? a : b; }
+  static constexpr int lds(bool gate) { return most(2 * kStage, gate ? kGate : kOut); }
+  static constexpr int kLds = lds(true);
+  static_assert(kLds <= 160 * 1024, "LDS");
+};
+
+// A row's sixteen-byte piece c of a step lies at c ^ key: sixteen rows' pieces then
+// meet sixteen slots of the 256 bytes that a cycle reads.
+__device__ __forceinline__ int tile_key(int row) { return (row >> 2) & 3; }
+
+// Row of tile j of a wave's block of 16 NT rows, of `rows` in all (clamped).
+template <int NT, bool PAIR>
+__device__ __forceinline__ int tile_row(int block, int j, int at, int rows) {
+  if (!PAIR) return min(block * 16 * NT + 16 * j + at, rows - 1);
+  // half the tiles rows of the gate, half the same rows of what it gates, behind all of the gate's
+  const int half = rows / 2, r = min(block * 8 * NT + 16 * (j % (NT / 2)) + at, half - 1);
+  return j < NT / 2 ? r : half + r;
 }
 
-// gate(g) * u of gate_up rows [place][2 inner] -> [place][inner]
-__global__ __launch_bounds__(256) void expert_gate_kernel(const float *both, int inner, int places, int silu, float *h) {
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long place = id / inner;
-  if (place >= places) return;
-  const int n = (int)(id - place * inner);
-  const float g = both[(size_t)place * 2 * inner + n], u = both[(size_t)place * 2 * inner + inner + n];
-  h[id] = (silu ? silu_near(g) : gelu_near(g)) * u;
+template <int NT, bool PAIR>
+__host__ __device__ __forceinline__ int tile_blocks(int rows) {
+  return PAIR ? (rows / 2 + 8 * NT - 1) / (8 * NT) : (rows + 16 * NT - 1) / (16 * NT);
 }
+
+// Scale bytes in the order a wave reads them: [block][step][wave lane][tile], zeros
+// behind a row's last group.
+struct PackArgs {
+  Mx4View w;
+  int rows, groups, experts, first_block;  // `rows` of each expert
+  uint8_t *dst;
+};
+
+template <int NT, bool PAIR>
+__device__ __forceinline__ void mx4_pack_scales(const PackArgs &a, long long id) {
+  const int steps = mx4_steps(a.groups), blocks = tile_blocks<NT, PAIR>(a.rows);
+  const int lane = (int)(id & 63);
+  const long long unit = id >> 6;
+  const int step = (int)(unit % steps);
+  const long long block = unit / steps;
+  const int e = (int)(block / blocks);
+  if (e >= a.experts) return;
+  const int g = 4 * step + (lane >> 4);
+  uint16_t out[NT / 2];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const size_t row = (size_t)e * a.rows + tile_row<NT, PAIR>((int)(block % blocks), j, lane & 15, a.rows);
+    const uint16_t b = g < a.groups ? a.w.scale[row * a.w.scale_stride + g] : 0;
+    out[j / 2] = j % 2 ? (uint16_t)(out[j / 2] | b << 8) : b;
+  }
+  uint16_t *dst = reinterpret_cast<uint16_t *>(a.dst) + (unit * 64 + lane) * (NT / 2);
+#pragma unroll
+  for (int i = 0; i < NT / 2; ++i) dst[i] = out[i];
+}
+
+// What products of many lanes need first, in one launch: lanes as terms, a sheet's scales
+// packed (as pairs of blocks for the experts' gate), then another's; of microscaled lanes
+// theirs, four tiles a block, in the first's place.  Experts' places in front (a
+// workgroup; place.experts 0: none).
+struct PrepareArgs {
+  const void *act;
+  long long act_stride;
+  int groups, lanes;
+  uint8_t *terms;
+  PlaceArgs place;
+  PackArgs pairs, rows;  // first_block: the workgroup they begin with
+  int lane_block;        // the terms' first, or the lane scales'
+  PackArgs lane_scales;
+};
+
+template <int T, int NT>
+__global__ __launch_bounds__(256) void mx4_prepare_kernel(PrepareArgs a) {
+  const int block = blockIdx.x;
+  if (block >= a.rows.first_block) {
+    mx4_pack_scales<NT, false>(a.rows, (long long)(block - a.rows.first_block) * 256 + threadIdx.x);
+  } else if (block >= a.pairs.first_block) {
+    mx4_pack_scales<NT, true>(a.pairs, (long long)(block - a.pairs.first_block) * 256 + threadIdx.x);
+  } else if (block >= a.lane_block) {
+    const long long id = (long long)(block - a.lane_block) * 256 + threadIdx.x;
+    if constexpr (T == 0)
+      mx4_pack_scales<4, false>(a.lane_scales, id);
+    else
+      mx4_terms_group<T, T == 3>(a.act, a.act_stride, a.groups, a.lanes, a.terms, id);
+  } else {
+    expert_place(a.place);
+  }
+}
+
+// What becomes of a tile's sums: rows of floats, or the gated products of row pairs (the
+// experts' hidden values) as terms for the product behind.
+enum { kOutF32 = 0, kOutBf16 = 1, kOutGate = 2 };
+
+template <int T, int MT, int NT, int WM, int WN, int OUT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
+  using F = TileForm<T, MT, NT, WM, WN>;
+  constexpr bool PAIR = OUT == kOutGate;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_x[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int part = lane >> 4, at = lane & 15, wm = wave / WN, wn = wave % WN;
+  int tile_x, tile_y;
+  xcd_tile(tile_x, tile_y);
+  int first = tile_y * F::kLanes, count = min(F::kLanes, g.lanes - first), expert = 0;
+  if (g.tiles) {
+    if (tile_y >= *g.tile_count) return;
+    const Mx4Tile t = g.tiles[tile_y];
+    first = t.first;
+    count = t.count;
+    expert = t.expert;
+  }
+  const size_t row0 = (size_t)expert * (size_t)g.rows;
+  const int blocks = tile_blocks<NT, PAIR>(g.rows);
+  const int block0 = tile_x * WN;  // blocks behind the last hold its rows, and are not stored
+  const int steps = mx4_steps(g.groups);
+
+  // ---- what this wave brings each step: sixteen bytes a lane, from src[i] + step * by[i] + min(step * walk[i] +
+  // plus[i], most).  By number: lanes' chunks (of first dwords, wave lane (part, at)'s sixteen bytes at its number;
+  // of last dwords two terms', eight bytes each, a lane's four groups side by side), rows' codes, packed scales.
+  // The last wave may bring one twice.  Codes walk to a row's last group at most.
+  const uint8_t *src[F::kLoads];
+  size_t by[F::kLoads];
+  uint32_t walk[F::kLoads], plus[F::kLoads];
+  const uint32_t most = 16u * (uint32_t)(g.groups - 1);
+#pragma unroll
+  for (int i = 0; i < F::kLoads; ++i) {
+    const int id = min(wave * F::kLoads + i, F::kAll - 1);
+    by[i] = walk[i] = plus[i] = 0;
+    if (id < F::kLaneLoads) {
+      const int c = id % F::kChunks, tile = id / F::kChunks;
+      const bool low = T == 0 || c < T;
+      const int place = first + min(16 * tile + (low ? at : (lane & 31) >> 1), count - 1);
+      const size_t from = (size_t)(g.lane_of ? g.lane_of[place] : place);
+      if constexpr (T == 0) {
+        src[i] = g.act.code + from * g.act.code_stride;
+        walk[i] = 64;
+        plus[i] = 16u * (uint32_t)part;
+      } else {
+        src[i] = g.terms + from * (F::kChunks * 64) + (low ? 64 * c + 16 * part : 64 * c + (lane >> 5) * 32 + (lane & 1) * 16);
+        by[i] = (size_t)g.term_lanes * (F::kChunks * 64);
+      }
+    } else if (id < F::kLaneLoads + F::kRowLoads) {
+      const int r = 16 * (id - F::kLaneLoads) + lane / 4;  // sixteen rows, four pieces each
+      const int block = block0 + r / F::kWaveRows, in = r % F::kWaveRows;
+      const size_t row = row0 + (size_t)tile_row<NT, PAIR>(block, in / 16, in % 16, g.rows);
+      src[i] = g.w.code + row * g.w.code_stride;
+      walk[i] = 64;
+      plus[i] = 16u * (uint32_t)((lane & 3) ^ tile_key(in));
+    } else if (id < F::kLaneLoads + F::kRowLoads + F::kScaleLoads) {
+      const int byte = (id - F::kLaneLoads - F::kRowLoads) * 1024 + lane * 16;  // of the blocks' 64 NT bytes each
+      const int block = min(block0 + min(byte / (64 * NT), WN - 1), blocks - 1);
+      src[i] = g.row_scales + ((size_t)expert * blocks + block) * (size_t)steps * (64 * NT) + byte % (64 * NT);
+      by[i] = 64 * NT;
+    } else {
+      const int byte = (id - F::kLaneLoads - F::kRowLoads - F::kScaleLoads) * 1024 + lane * 16;
+      const int block = min(first / 64 + byte / 256, (g.lanes - 1) / 64);
+      src[i] = reinterpret_cast<const uint8_t *>(g.lane_scales) + (size_t)block * steps * 256 + byte % 256;
+      by[i] = 256;
+    }
+  }
+  auto bring = [&](int step, int turn) {
+    uint8_t *dst = lds_x + (turn & 1) * F::kStage;
+#pragma unroll
+    for (int i = 0; i < F::kLoads; ++i) {
+      const uint8_t *from = src[i] + (size_t)step * by[i] + min((uint32_t)step * walk[i] + plus[i], most);
+      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)from,
+                                       (__attribute__((address_space(3))) void *)(dst + min(wave * F::kLoads + i, F::kAll - 1) * 1024),
+                                       16, 0, 0);
+    }
+  };
+
+  float4_t acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // Workgroups of neighbouring rows begin at other columns: rows are often a power of
+  // two bytes apart, and all at the same column would ask the same cache channels
+  int k = 2 * tile_x % steps;
+  bring(k, 0);
+  for (int s = 0; s < steps; ++s) {
+    const int k_next = k + 1 < steps ? k + 1 : 0;
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this step's stage is in, brought a step ago
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (s + 1 < steps) bring(k_next, s + 1);
+    const uint8_t *st = lds_x + (s & 1) * F::kStage;
+    // Lanes' terms behind the last group are zeros, and codes are finite; of microscaled lanes neither side's are
+    const uint32_t keep = T != 0 || 4 * k + part < g.groups ? 0xFFFFFFFFu : 0u;
+    int8v_t op[2][T == 0 ? 1 : T];
+    uint2_t scale[2];
+    auto read_lanes = [&](int i) {
+      const uint8_t *mine = st + (wm * MT + i) * F::kChunks * 1024;
+#pragma unroll
+      for (int t = 0; t < (T == 0 ? 1 : T); ++t) {
+        const uint4_t a = *reinterpret_cast<const uint4_t *>(mine + t * 1024 + lane * 16);
+        uint2_t b = {0, 0};
+        if constexpr (T != 0) b = *reinterpret_cast<const uint2_t *>(mine + T * 1024 + t * 512 + (4 * at + part) * 8);
+        op[i & 1][t] = int8v_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], 0, 0};
+      }
+      if constexpr (T != 0)
+        scale[i & 1] = *reinterpret_cast<const uint2_t *>(mine + T * 1024 + T * 512 + (4 * at + part) * 8);
+    };
+    int8v_t w[NT];
+    uint32_t ws[NT / 4];
+    read_lanes(0);
+#pragma unroll
+    for (int q = 0; q < NT / 4; ++q)
+      ws[q] = *reinterpret_cast<const uint32_t *>(st + F::kScalesAt + (wn * 64 + lane) * NT + 4 * q);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int r = 16 * j + at;
+      uint4_t c = *reinterpret_cast<const uint4_t *>(st + F::kRowsAt + (wn * F::kWaveRows + r) * 64 +
+                                                     16 * (part ^ tile_key(r)));
+      if (T == 0) c &= keep;
+      w[j] = int8v_t{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+    }
+    int ls = 0;
+    if constexpr (T == 0) {
+      static_assert(MT == 4 || T != 0, "a byte of the packed scales a tile");
+      ls = *reinterpret_cast<const int *>(st + F::kLaneScalesAt + wm * 256 + lane * 4);
+    }
+#define MX4_PRODUCT(I, J, A, FMT, OPSEL, SCALE)                                                                      \
+  switch (J % 4) {                                                                                                   \
+    case 0:                                                                                                          \
+      acc[I][J] =                                                                                                    \
+          __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 0, ws[J / 4], OPSEL, SCALE);  \
+      break;                                                                                                         \
+    case 1:                                                                                                          \
+      acc[I][J] =                                                                                                    \
+          __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 1, ws[J / 4], OPSEL, SCALE);  \
+      break;                                                                                                         \
+    case 2:                                                                                                          \
+      acc[I][J] =                                                                                                    \
+          __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 2, ws[J / 4], OPSEL, SCALE);  \
+      break;                                                                                                         \
+    default:                                                                                                         \
+      acc[I][J] =                                                                                                    \
+          __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 3, ws[J / 4], OPSEL, SCALE);  \
+  }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      // the next lanes' operands are on their way while these are multiplied
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + 1 < MT) read_lanes(i + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      // a term at a time over the row tiles: products that add to the same sums lie apart
+#pragma unroll
+      for (int t = 0; t < (T == 0 ? 1 : T); ++t)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          constexpr int kFmt = T == 0 ? 4 : 2;
+          const int a = T == 0 ? ls : (int)scale[i & 1][t / 4];
+          const int byte = T == 0 ? i : t % 4;
+          if (byte == 0) MX4_PRODUCT(i, j, op[i & 1][t], kFmt, 0, a)
+          if (byte == 1) MX4_PRODUCT(i, j, op[i & 1][t], kFmt, 1, a)
+          if (byte == 2) MX4_PRODUCT(i, j, op[i & 1][t], kFmt, 2, a)
+          if (byte == 3) MX4_PRODUCT(i, j, op[i & 1][t], kFmt, 3, a)
+        }
+    }
+#undef MX4_PRODUCT
+    k = k_next;
+  }
+  // every lane took part in the products: nothing of them may move behind a branch that some leave
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+  __syncthreads();
+
+  if constexpr (PAIR) {
+    // h = gate(g) u, both in this lane's registers; through LDS, so that a lane has the 32 values of a group.  The
+    // wave takes its own room, lanes by pitch
+    constexpr int kHalf = F::kWaveRows / 2, kPitch = kHalf + 4;
+    float *const turn = reinterpret_cast<float *>(lds_x) + wave * 16 * MT * kPitch;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT / 2; ++j) {
+        float4_t h;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          h[r] = (g.silu ? silu_near(acc[i][j][r]) : gelu_near(acc[i][j][r])) * acc[i][j + NT / 2][r];
+        *reinterpret_cast<float4_t *>(turn + (16 * i + at) * kPitch + 16 * j + 4 * part) = h;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // one wave's room, no barrier
+    const int inner_groups = g.rows / 2 / kMx4Group, group0 = (block0 + wn) * (kHalf / kMx4Group);
+    constexpr int kGroups = kHalf / kMx4Group;
+    for (int item = lane; item < 16 * MT * kGroups; item += 64) {
+      const int m = item / kGroups, group = group0 + item % kGroups;
+      const int place = 16 * wm * MT + m;
+      if (place >= count || group >= inner_groups) continue;
+      float x[32];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float4_t f = *reinterpret_cast<const float4_t *>(turn + m * kPitch + item % kGroups * 32 + 4 * q);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) x[4 * q + d] = f[d];
+      }
+      uint8_t *const h = static_cast<uint8_t *>(g.out);
+      const size_t to = (size_t)(first + place);
+      mx4_terms<T == 0 ? 3 : T>(x, h + term_at<T == 0 ? 3 : T>(to, group >> 2, (size_t)g.out_stride), group & 3);
+      if (group + 1 == inner_groups)  // the groups behind the last are zeros
+        for (int z = group + 1; z < 4 * mx4_steps(inner_groups); ++z) {
+          uint8_t *step = h + term_at<T == 0 ? 3 : T>(to, z >> 2, (size_t)g.out_stride);
+          for (int u = 0; u <= T; ++u) {
+            if (u < T) *reinterpret_cast<uint4_t *>(step + TermForm<T == 0 ? 3 : T>::low(u, z & 3)) = uint4_t{0, 0, 0, 0};
+            *reinterpret_cast<uint2_t *>(step + TermForm<T == 0 ? 3 : T>::high(u, z & 3)) = uint2_t{0, 0};
+          }
+        }
+    }
+    return;
+  }
+  // The weight is the first operand: this wave lane holds rows 4 part .. + 3 of lane
+  // `at`.  They cross LDS so that a lane's rows of the wave are stored in one go: four
+  // by four, sixteen lanes' lines would be written in halves, each to the same channel.
+  constexpr int kPitch = F::kWaveRows + 4;
+  float *const turn = reinterpret_cast<float *>(lds_x) + wave * 16 * kPitch;
+  const int n0 = (block0 + wn) * F::kWaveRows;
+  constexpr int kBytes = OUT == kOutBf16 ? 2 : 4;
+  const bool whole = g.out_stride % (16 / kBytes) == 0 && ((uintptr_t)g.out & 15u) == 0;
+  constexpr int kOf = 16 / kBytes;                 // outputs of a store
+  constexpr int kRowLanes = F::kWaveRows / kOf;    // wave lanes that store a lane's rows
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      *reinterpret_cast<float4_t *>(turn + at * kPitch + 16 * j + 4 * part) = acc[i][j];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // one wave's room, no barrier
+#pragma unroll
+    for (int r = 0; r < 16 * kRowLanes / 64; ++r) {
+      const int m = r * (64 / kRowLanes) + lane / kRowLanes, c = lane % kRowLanes * kOf;
+      float v[kOf];
+#pragma unroll
+      for (int q = 0; q < kOf / 4; ++q) {
+        const float4_t f = *reinterpret_cast<const float4_t *>(turn + m * kPitch + c + 4 * q);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) v[4 * q + d] = f[d];
+      }
+      const int n = n0 + c;
+      const int place = 16 * (wm * MT + i) + m;
+      if (place >= count) continue;
+      const size_t out = (size_t)(first + place) * (size_t)g.out_stride + n;
+      if (whole && n + kOf <= g.rows) {
+        uint4_t b;
+        if (OUT == kOutBf16) {
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            b[d] = float_bf16(v[(2 * d) % kOf]) | (uint32_t)float_bf16(v[(2 * d + 1) % kOf]) << 16;
+        } else {
+#pragma unroll
+          for (int d = 0; d < 4; ++d) b[d] = __builtin_bit_cast(uint32_t, v[d]);
+        }
+        *reinterpret_cast<uint4_t *>(static_cast<uint8_t *>(g.out) + out * kBytes) = b;
+      } else {
+#pragma unroll
+        for (int d = 0; d < kOf; ++d)
+          if (n + d < g.rows) {
+            if (OUT == kOutBf16)
+              static_cast<uint16_t *>(g.out)[out + d] = float_bf16(v[d]);
+            else
+              static_cast<float *>(g.out)[out + d] = v[d];
+          }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// ---- the experts' feed-forward ------------------------------------------------------
 
 // out[lane] = sum over its choices, in their order, of weight * row of the slot's place
 template <bool BF16>
@@ -452,13 +880,13 @@ extern "C" hipError_t igl_launch_mx4_read(const igl_mx4 *store, int row_first, i
 static size_t mx4_up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 static size_t terms_bytes(int lanes, int cols, int bf16) {
-  return mx4_up((size_t)lanes * (cols / kMx4Group) * (bf16 ? TermForm<3>::kBytes : TermForm<5>::kBytes));
+  return mx4_up((size_t)lanes * mx4_steps(cols / kMx4Group) * (bf16 ? TermForm<3>::kStep : TermForm<5>::kStep));
 }
 
-static hipError_t launch_terms(const void *act, int bf16, long long act_stride, int lanes, int cols, uint32_t *terms,
+static hipError_t launch_terms(const void *act, int bf16, long long act_stride, int lanes, int cols, uint8_t *terms,
                                hipStream_t stream) {
   const int groups = cols / kMx4Group;
-  const unsigned blocks = (unsigned)(((long long)lanes * groups + 255) / 256);
+  const unsigned blocks = (unsigned)(((long long)lanes * 4 * mx4_steps(groups) + 255) / 256);
   if (bf16)
     hipLaunchKernelGGL((mx4_terms_kernel<3, true>), dim3(blocks), dim3(256), 0, stream, act, act_stride, groups, lanes,
                        terms);
@@ -468,9 +896,54 @@ static hipError_t launch_terms(const void *act, int bf16, long long act_stride, 
   return hipGetLastError();
 }
 
-// tiles: lane tiles of the grid.  terms 0: microscaled lanes.
-static hipError_t launch_product(const Mx4Args &a, int terms, int out_bf16, int tiles, hipStream_t stream) {
-  const dim3 grid((a.rows + 63) / 64, tiles);
+// Bytes of packed scales of `experts` sheets of `rows`.
+template <int NT, bool PAIR>
+static size_t pack_bytes(int rows, int groups, int experts) {
+  return mx4_up((size_t)experts * tile_blocks<NT, PAIR>(rows) * mx4_steps(groups) * 64 * NT);
+}
+
+template <int NT, bool PAIR>
+static unsigned pack_blocks(int rows, int groups, int experts) {
+  return (unsigned)(((long long)experts * tile_blocks<NT, PAIR>(rows) * mx4_steps(groups) + 3) / 4);
+}
+
+// The launch before products of many lanes, what of it there is to do: `a` filled but for
+// the workgroups' numbers.
+template <int T, int NT>
+static hipError_t launch_prepare(PrepareArgs a, hipStream_t stream) {
+  long long block = a.place.experts ? 1 : 0;
+  a.lane_block = (int)block;
+  if (T == 0)
+    block += pack_blocks<4, false>(a.lane_scales.rows, a.lane_scales.groups, 1);
+  else
+    block += ((long long)a.lanes * 4 * mx4_steps(a.groups) + 255) / 256;
+  a.pairs.first_block = (int)block;
+  if (a.pairs.dst) block += pack_blocks<NT, true>(a.pairs.rows, a.pairs.groups, a.pairs.experts);
+  a.rows.first_block = (int)block;
+  block += pack_blocks<NT, false>(a.rows.rows, a.rows.groups, a.rows.experts);
+  hipLaunchKernelGGL((mx4_prepare_kernel<T, NT>), dim3((unsigned)block), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <int T, int MT, int NT, int WM, int WN, int OUT>
+static hipError_t launch_tile(const Mx4Args &a, int tiles, hipStream_t stream) {
+  using F = TileForm<T, MT, NT, WM, WN>;
+  static bool granted = false;  // the dynamic LDS a kernel asks for is granted once
+  if (!granted) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_tile_kernel<T, MT, NT, WM, WN, OUT>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, F::lds(OUT == kOutGate));
+    if (e != hipSuccess) return e;
+    granted = true;
+  }
+  const int blocks = tile_blocks<NT, OUT == kOutGate>(a.rows);
+  hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, WM, WN, OUT>), dim3((blocks + WN - 1) / WN, tiles), dim3(64 * F::kWaves),
+                     (size_t)F::lds(OUT == kOutGate), stream, a);
+  return hipGetLastError();
+}
+
+// A product of few lanes: tiles of sixteen.  terms 0: microscaled lanes.
+static hipError_t launch_wave(const Mx4Args &a, int terms, int out_bf16, hipStream_t stream) {
+  const dim3 grid((a.rows + 63) / 64, (a.lanes + 15) / 16);
   if (terms == 0 && out_bf16)
     hipLaunchKernelGGL((mx4_wave_kernel<0, true>), grid, dim3(256), 0, stream, a);
   else if (terms == 0)
@@ -486,30 +959,65 @@ static hipError_t launch_product(const Mx4Args &a, int terms, int out_bf16, int 
   return hipGetLastError();
 }
 
-extern "C" size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int act_bf16) {
-  (void)rows;
-  return terms_bytes(lanes, cols, act_bf16);
+// A product of many lanes: the launch that prepares it and the product.  `work` holds
+// mx4_many_bytes.
+template <int T, int MT, int NT, int WM, int WN>
+static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int out_bf16, uint8_t *work,
+                              hipStream_t stream) {
+  const size_t lanes_bytes =
+      T == 0 ? pack_bytes<4, false>(a.lanes, a.groups, 1) : terms_bytes(a.lanes, a.groups * kMx4Group, T == 3);
+  PrepareArgs p = {};
+  p.act = act;
+  p.act_stride = act_stride;
+  p.groups = a.groups;
+  p.lanes = a.lanes;
+  p.terms = work;
+  p.lane_scales = PackArgs{a.act, a.lanes, a.groups, 1, 0, work};
+  p.rows = PackArgs{a.w, a.rows, a.groups, 1, 0, work + lanes_bytes};
+  const hipError_t e = launch_prepare<T, NT>(p, stream);
+  if (e != hipSuccess) return e;
+  a.terms = work;
+  a.term_lanes = a.lanes;
+  a.lane_scales = reinterpret_cast<const uint32_t *>(work);
+  a.row_scales = work + lanes_bytes;
+  const int tiles = (a.lanes + 16 * MT * WM - 1) / (16 * MT * WM);
+  return out_bf16 ? launch_tile<T, MT, NT, WM, WN, kOutBf16>(a, tiles, stream)
+                  : launch_tile<T, MT, NT, WM, WN, kOutF32>(a, tiles, stream);
+}
+
+constexpr int kMx4Many = 64;  // lanes from which the tiles are taken
+
+// Enough for either form of a product: its lanes as terms, or their scales, and the
+// sheet's scales packed (eight tiles a block).
+extern "C" size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int terms) {
+  const int groups = cols / kMx4Group;
+  if (lanes < kMx4Many) return terms ? terms_bytes(lanes, cols, terms == 3) : 0;
+  const size_t sheet = pack_bytes<8, false>(rows, groups, 1);
+  return sheet + (terms ? terms_bytes(lanes, cols, terms == 3) : pack_bytes<4, false>(lanes, groups, 1));
 }
 
 extern "C" hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *act, int act_bf16, int act_stride,
                                              int lanes, void *out, int out_bf16, int out_stride, void *work,
                                              hipStream_t stream) {
-  const hipError_t e =
-      launch_terms(act, act_bf16, act_stride, lanes, sheet->col_count, static_cast<uint32_t *>(work), stream);
-  if (e != hipSuccess) return e;
   Mx4Args a = {};
   a.w = mx4_view(sheet, 0);
   a.rows = sheet->row_count;
   a.groups = sheet->col_count / kMx4Group;
-  a.terms = static_cast<const uint32_t *>(work);
+  a.terms = static_cast<const uint8_t *>(work);
+  a.term_lanes = lanes;
   a.lanes = lanes;
   a.out = out;
   a.out_stride = out_stride;
-  return launch_product(a, act_bf16 ? 3 : 5, out_bf16, (lanes + 15) / 16, stream);
+  uint8_t *const room = static_cast<uint8_t *>(work);
+  if (lanes >= kMx4Many)
+    return act_bf16 ? launch_many<3, 2, 4, 2, 4>(a, act, act_stride, out_bf16, room, stream)
+                    : launch_many<5, 2, 8, 2, 4>(a, act, act_stride, out_bf16, room, stream);
+  const hipError_t e = launch_terms(act, act_bf16, act_stride, lanes, sheet->col_count, room, stream);
+  return e != hipSuccess ? e : launch_wave(a, act_bf16 ? 3 : 5, out_bf16, stream);
 }
 
 extern "C" hipError_t igl_launch_mx4_mat_mx4(const igl_mx4 *sheet, const igl_mx4 *act, int lane_first, int lanes,
-                                             void *out, int out_bf16, int out_stride, hipStream_t stream) {
+                                             void *out, int out_bf16, int out_stride, void *work, hipStream_t stream) {
   Mx4Args a = {};
   a.w = mx4_view(sheet, 0);
   a.rows = sheet->row_count;
@@ -518,15 +1026,20 @@ extern "C" hipError_t igl_launch_mx4_mat_mx4(const igl_mx4 *sheet, const igl_mx4
   a.lanes = lanes;
   a.out = out;
   a.out_stride = out_stride;
-  return launch_product(a, 0, out_bf16, (lanes + 15) / 16, stream);
+  if (lanes >= kMx4Many)
+    return launch_many<0, 4, 4, 2, 4>(a, nullptr, 0, out_bf16, static_cast<uint8_t *>(work), stream);
+  return launch_wave(a, 0, out_bf16, stream);
 }
 
 namespace igl {
 
-// The places of a call's experts, its intermediate rows and their terms.
+// The places of a call's experts, its lanes' and hidden values' terms, packed scales, and
+// the rows that are joined.
 struct ExpertRoom {
-  size_t lane_of, place_of, tiles, tile_count, count, x, both, h, h_terms, rows, end;
+  size_t lane_of, place_of, tiles, tile_count, x, gate_up, down, h, rows, end;
 };
+
+constexpr int kExpertTile = 16;  // lanes of the smallest tile
 
 static int expert_tiles(int slots, int experts, int tile) {
   return slots / tile + (slots < experts ? slots : experts);
@@ -543,16 +1056,81 @@ static ExpertRoom expert_room(const igl_experts *x, int lanes, int top, int bf16
   };
   r.lane_of = take(slots * sizeof(int));
   r.place_of = take(slots * sizeof(int));
-  r.tiles = take((size_t)expert_tiles((int)slots, x->expert_count, 16) * sizeof(Mx4Tile));
+  r.tiles = take((size_t)expert_tiles((int)slots, x->expert_count, kExpertTile) * sizeof(Mx4Tile));
   r.tile_count = take(sizeof(int));
-  r.count = take((size_t)x->expert_count * sizeof(int));
   r.x = take(terms_bytes(lanes, x->hidden, bf16));
-  r.both = take(slots * 2 * x->inner * sizeof(float));
-  r.h = take(slots * x->inner * sizeof(float));
-  r.h_terms = take(terms_bytes((int)slots, x->inner, 0));
+  r.gate_up = take(pack_bytes<8, true>(2 * x->inner, x->hidden / kMx4Group, x->expert_count));
+  r.down = take(pack_bytes<8, false>(x->hidden, x->inner / kMx4Group, x->expert_count));
+  r.h = take(terms_bytes((int)slots, x->inner, bf16));
   r.rows = take(slots * x->hidden * sizeof(float));
   r.end = at;
   return r;
+}
+
+// What an experts' call is: its arguments and its room.
+struct ExpertCall {
+  const igl_experts *x;
+  const void *act;
+  int act_stride, lanes;
+  const int32_t *pick;
+  const float *weight;
+  int top;
+  void *out;
+  int out_bf16, out_stride;
+  uint8_t *base;
+  ExpertRoom room;
+};
+
+template <int T, int MT, int NT, int WM, int WN>
+static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
+  using F = TileForm<T, MT, NT, WM, WN>;
+  const igl_experts *x = c.x;
+  const ExpertRoom &r = c.room;
+  const int slots = c.lanes * c.top, tiles = expert_tiles(slots, x->expert_count, F::kLanes);
+  hipError_t e;
+  PrepareArgs p = {};
+  p.act = c.act;
+  p.act_stride = c.act_stride;
+  p.groups = x->hidden / kMx4Group;
+  p.lanes = c.lanes;
+  p.terms = c.base + r.x;
+  p.place = PlaceArgs{c.pick, slots, c.top, x->expert_count, F::kLanes, (int *)(c.base + r.lane_of),
+                      (int *)(c.base + r.place_of), (Mx4Tile *)(c.base + r.tiles), (int *)(c.base + r.tile_count)};
+  p.pairs = PackArgs{mx4_view(&x->gate_up, 0), 2 * x->inner, p.groups, x->expert_count, 0, c.base + r.gate_up};
+  p.rows = PackArgs{mx4_view(&x->down, 0), x->hidden, x->inner / kMx4Group, x->expert_count, 0, c.base + r.down};
+  if ((e = launch_prepare<T, NT>(p, stream)) != hipSuccess) return e;
+  Mx4Args a = {};
+  a.w = p.pairs.w;
+  a.rows = p.pairs.rows;
+  a.groups = p.groups;
+  a.terms = p.terms;
+  a.term_lanes = c.lanes;
+  a.tiles = p.place.tiles;
+  a.tile_count = p.place.tile_count;
+  a.lane_of = p.place.lane_of;
+  a.row_scales = p.pairs.dst;
+  a.out = c.base + r.h;
+  a.out_stride = slots;
+  a.silu = x->gate == IGL_GATE_SILU;
+  if ((e = launch_tile<T, MT, NT, WM, WN, kOutGate>(a, tiles, stream)) != hipSuccess) return e;
+  a.w = p.rows.w;
+  a.rows = p.rows.rows;
+  a.groups = p.rows.groups;
+  a.terms = c.base + r.h;
+  a.term_lanes = slots;
+  a.lane_of = nullptr;
+  a.row_scales = p.rows.dst;
+  a.out = c.base + r.rows;
+  a.out_stride = x->hidden;
+  if ((e = launch_tile<T, MT, NT, WM, WN, kOutF32>(a, tiles, stream)) != hipSuccess) return e;
+  const unsigned blocks = (unsigned)(((long long)c.lanes * x->hidden + 255) / 256);
+  if (c.out_bf16)
+    hipLaunchKernelGGL((expert_join_kernel<true>), dim3(blocks), dim3(256), 0, stream, (const float *)(c.base + r.rows),
+                       p.place.place_of, c.weight, c.top, x->hidden, c.lanes, c.out, c.out_stride);
+  else
+    hipLaunchKernelGGL((expert_join_kernel<false>), dim3(blocks), dim3(256), 0, stream, (const float *)(c.base + r.rows),
+                       p.place.place_of, c.weight, c.top, x->hidden, c.lanes, c.out, c.out_stride);
+  return hipGetLastError();
 }
 
 }  // namespace igl
@@ -564,47 +1142,10 @@ extern "C" size_t igl_experts_work_bytes(const igl_experts *x, int lanes, int to
 extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, int act_bf16, int act_stride, int lanes,
                                          const int32_t *pick, const float *weight, int top, void *out, int out_bf16,
                                          int out_stride, void *work, hipStream_t stream) {
-  const ExpertRoom r = expert_room(x, lanes, top, act_bf16);
-  uint8_t *base = static_cast<uint8_t *>(work);
-  const int slots = lanes * top, tiles = expert_tiles(slots, x->expert_count, 16);
-  hipError_t e;
-  PlaceArgs p = {pick, slots, top, x->expert_count, 16, (int *)(base + r.lane_of), (int *)(base + r.place_of),
-                 (Mx4Tile *)(base + r.tiles), (int *)(base + r.tile_count), (int *)(base + r.count)};
-  hipLaunchKernelGGL(expert_place_kernel, dim3(1), dim3(kPlaceThreads), 0, stream, p);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
-  if ((e = launch_terms(act, act_bf16, act_stride, lanes, x->hidden, (uint32_t *)(base + r.x), stream)) != hipSuccess)
-    return e;
-  Mx4Args a = {};
-  a.w = mx4_view(&x->gate_up, 0);
-  a.rows = 2 * x->inner;
-  a.groups = x->hidden / kMx4Group;
-  a.terms = (const uint32_t *)(base + r.x);
-  a.tiles = p.tiles;
-  a.tile_count = p.tile_count;
-  a.lane_of = p.lane_of;
-  a.out = base + r.both;
-  a.out_stride = 2 * x->inner;
-  if ((e = launch_product(a, act_bf16 ? 3 : 5, 0, tiles, stream)) != hipSuccess) return e;
-  hipLaunchKernelGGL(expert_gate_kernel, dim3((unsigned)(((long long)slots * x->inner + 255) / 256)), dim3(256), 0,
-                     stream, (const float *)(base + r.both), x->inner, slots, x->gate == IGL_GATE_SILU,
-                     (float *)(base + r.h));
-  if ((e = hipGetLastError()) != hipSuccess) return e;
-  if ((e = launch_terms(base + r.h, 0, x->inner, slots, x->inner, (uint32_t *)(base + r.h_terms), stream)) != hipSuccess)
-    return e;
-  a.w = mx4_view(&x->down, 0);
-  a.rows = x->hidden;
-  a.groups = x->inner / kMx4Group;
-  a.terms = (const uint32_t *)(base + r.h_terms);
-  a.lane_of = nullptr;
-  a.out = base + r.rows;
-  a.out_stride = x->hidden;
-  if ((e = launch_product(a, 5, 0, tiles, stream)) != hipSuccess) return e;
-  const unsigned blocks = (unsigned)(((long long)lanes * x->hidden + 255) / 256);
-  if (out_bf16)
-    hipLaunchKernelGGL((expert_join_kernel<true>), dim3(blocks), dim3(256), 0, stream, (const float *)(base + r.rows),
-                       p.place_of, weight, top, x->hidden, lanes, out, out_stride);
-  else
-    hipLaunchKernelGGL((expert_join_kernel<false>), dim3(blocks), dim3(256), 0, stream, (const float *)(base + r.rows),
-                       p.place_of, weight, top, x->hidden, lanes, out, out_stride);
-  return hipGetLastError();
+  const ExpertCall c = {x,   act,      act_stride, lanes, pick, weight, top,
+                        out, out_bf16, out_stride, static_cast<uint8_t *>(work), expert_room(x, lanes, top, act_bf16)};
+  const bool many = (long long)lanes * top >= 24LL * x->expert_count;
+  if (act_bf16)
+    return many ? experts_grouped<3, 2, 4, 2, 4>(c, stream) : experts_grouped<3, 1, 4, 1, 4>(c, stream);
+  return many ? experts_grouped<5, 2, 4, 2, 4>(c, stream) : experts_grouped<5, 1, 4, 1, 4>(c, stream);
 }

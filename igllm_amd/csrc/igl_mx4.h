@@ -168,8 +168,8 @@ struct TermForm {
 // The terms of a group.  s is 20 at least, so that s - 5 j stays a byte (five terms
 // then end at 2^-130, three at 2^-120); an infinity or a NaN makes the scale a NaN, so that
 // every output of its lane is one.
-template <int T>
-__device__ __forceinline__ void mx4_terms(float (&x)[32], uint8_t *step, int part) {
+template <int T, typename Put, typename Scales>
+__device__ __forceinline__ void mx4_cut(float (&x)[32], Put put, Scales scales) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 32; ++i) top = max(top, abs_bits(x[i]));
@@ -187,11 +187,7 @@ __device__ __forceinline__ void mx4_terms(float (&x)[32], uint8_t *step, int par
       odd[i] = x[2 * i + 1];
     }
     const uint6_t w = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, 1.0f);
-#pragma unroll
-    for (int i = 0; i < 1; ++i) {
-      *reinterpret_cast<uint4_t *>(step + TermForm<T>::low(t, part)) = uint4_t{w[0], w[1], w[2], w[3]};
-      *reinterpret_cast<uint2_t *>(step + TermForm<T>::high(t, part)) = uint2_t{w[4], w[5]};
-    }
+    put(t, w);
     if (t + 1 < T) {
       const float32_t back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, 32.0f);
 #pragma unroll
@@ -199,8 +195,33 @@ __device__ __forceinline__ void mx4_terms(float (&x)[32], uint8_t *step, int par
     }
   }
   if (none) s = 255;
-  *reinterpret_cast<uint2_t *>(step + TermForm<T>::high(T, part)) =
-      uint2_t{(uint32_t)s * 0x01010101u - 0x0F0A0500u, (uint32_t)(s - 20)};
+  scales(uint2_t{(uint32_t)s * 0x01010101u - 0x0F0A0500u, (uint32_t)(s - 20)});
+}
+
+// A group's terms into a step of its lane.
+template <int T>
+__device__ __forceinline__ void mx4_terms(float (&x)[32], uint8_t *step, int part) {
+  mx4_cut<T>(
+      x,
+      [&](int t, const uint6_t &w) {
+        *reinterpret_cast<uint4_t *>(step + TermForm<T>::low(t, part)) = uint4_t{w[0], w[1], w[2], w[3]};
+        *reinterpret_cast<uint2_t *>(step + TermForm<T>::high(t, part)) = uint2_t{w[4], w[5]};
+      },
+      [&](const uint2_t &s) { *reinterpret_cast<uint2_t *>(step + TermForm<T>::high(T, part)) = s; });
+}
+
+// And into a record of its own, a term behind the other.
+template <int T>
+__device__ __forceinline__ void mx4_terms_record(float (&x)[32], uint8_t *record) {
+  mx4_cut<T>(
+      x,
+      [&](int t, const uint6_t &w) {
+        uint2_t *to = reinterpret_cast<uint2_t *>(record + 24 * t);
+        to[0] = uint2_t{w[0], w[1]};
+        to[1] = uint2_t{w[2], w[3]};
+        to[2] = uint2_t{w[4], w[5]};
+      },
+      [&](const uint2_t &s) { *reinterpret_cast<uint2_t *>(record + 24 * T) = s; });
 }
 
 // The operand of term t of a group, and its scales.
@@ -250,6 +271,10 @@ __global__ __launch_bounds__(256) void mx4_terms_kernel(const void *act, long lo
 
 // ---- the product ------------------------------------------------------------------
 
+// What becomes of sums: rows of floats, or the gated products of row pairs (the experts'
+// hidden values; from tiles as terms for the product behind).
+enum { kOutF32 = 0, kOutBf16 = 1, kOutGate = 2 };
+
 // Rows of a microscaled weight; in a batch of experts expert e's rows begin at
 // row e * rows_each.
 struct Mx4View {
@@ -274,78 +299,18 @@ struct Mx4Args {
   int lanes;
   // grouped: the tiles, how many there are, and the lane of every place (NULL: the place)
   const Mx4Tile *tiles;
-  const int *tile_count;
+  int tile_count;
   const int *lane_of;
   const uint8_t *row_scales;    // packed (mx4_prepare_kernel), for the tile kernel
   const uint32_t *lane_scales;
   void *out;                // [lane or place][out_stride]; the experts' gate: terms of out_stride places
   int silu;                 // the experts' gate
+  // a few lanes' own floats, and a token's experts (lane_of: the picks)
+  const void *act_rows;
+  long long act_stride;
+  int experts, top;
   long long out_stride;
 };
-
-// The codes and scale byte of group g of a row; behind the row's last group zeros.
-__device__ __forceinline__ int8v_t mx4_group(const Mx4View &v, size_t row, int g, int groups, int &scale) {
-  if (g >= groups) {
-    scale = 0;
-    return int8v_t{0, 0, 0, 0, 0, 0, 0, 0};
-  }
-  const uint4_t c = *reinterpret_cast<const uint4_t *>(v.code + row * v.code_stride + 16 * (size_t)g);
-  scale = v.scale[row * v.scale_stride + g];
-  return int8v_t{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
-}
-
-// A wave takes 16 rows and 16 lanes, 128 columns a step: lane l of the wave holds
-// group l / 16 of row and lane l % 16.  T terms, 0: microscaled lanes.
-template <int T, bool OUT_BF16>
-__global__ __launch_bounds__(256) void mx4_wave_kernel(Mx4Args g) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n0 = (blockIdx.x * 4 + wave) * 16;
-  if (n0 >= g.rows) return;
-  int first = blockIdx.y * 16, count = min(16, g.lanes - first);
-  size_t row0 = 0;
-  if (g.tiles) {
-    if ((int)blockIdx.y >= *g.tile_count) return;
-    const Mx4Tile t = g.tiles[blockIdx.y];
-    first = t.first;
-    count = t.count;
-    row0 = (size_t)t.expert * (size_t)g.rows;
-  }
-  const int part = lane >> 4, at = lane & 15;
-  const size_t row = row0 + (size_t)min(n0 + at, g.rows - 1);
-  const int place = first + min(at, count - 1);
-  const size_t from = (size_t)(g.lane_of ? g.lane_of[place] : place);
-  float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int steps = mx4_steps(g.groups);
-  for (int s = 0; s < steps; ++s) {
-    int ws, as;
-    const int8v_t w = mx4_group(g.w, row, 4 * s + part, g.groups, ws);
-    if constexpr (T == 0) {
-      const int8v_t a = mx4_group(g.act, from, 4 * s + part, g.groups, as);
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 4, 4, 0, ws, 0, as);
-    } else {
-      const uint8_t *step = g.terms + term_at<T>(from, s, (size_t)g.term_lanes);
-      const uint2_t scales = term_scales<T>(step, part);
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        as = t < 4 ? (int)(scales[0] >> (8 * t)) : (int)scales[1];
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, term_operand<T>(step, t, part), acc, 4, 2, 0, ws,
-                                                               0, as);
-      }
-    }
-  }
-  // the weight is the first operand: this wave lane holds rows 4 (l / 16) .. + 3 of lane l % 16
-  if (at >= count) return;
-  const size_t out = (size_t)(first + at) * (size_t)g.out_stride;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int n = n0 + 4 * part + r;
-    if (n >= g.rows) continue;
-    if (OUT_BF16)
-      static_cast<uint16_t *>(g.out)[out + n] = float_bf16(acc[r]);
-    else
-      static_cast<float *>(g.out)[out + n] = acc[r];
-  }
-}
 
 // silu(x) = x / (1 + e^-x)
 __device__ __forceinline__ float silu_near(float x) {
@@ -356,65 +321,83 @@ __device__ __forceinline__ float silu_near(float x) {
 // ---- experts' places ----------------------------------------------------------------
 
 // Places: the slots (lane, choice) in the order of their experts; tiles: pieces of an
-// expert's places.  A slot whose expert is none (out of range) has no place.
-constexpr int kExpertsMost = 1024;
+// expert's places.  A slot whose expert is none (out of range) has no place.  Expert e's
+// tiles begin at tile (places before e) / tile + e: no more than that many lie before, and
+// every expert finds its own without the others.  Tiles left over have no places.
+constexpr int kPrepareThreads = 256;
+constexpr int kPlaceRound = 16;  // slots a lane has in flight
 
 struct PlaceArgs {
   const int32_t *pick;
   int slots, top, experts, tile;  // places a tile
   int *lane_of;                   // [slots] lane of a place
   int *place_of;                  // [slots] place of a slot, or -1
-  Mx4Tile *tiles;
-  int *tile_count;
+  Mx4Tile *tiles;                 // [slots / tile + experts]
 };
 
-// One workgroup of 256: counts, running sums of places and tiles over the experts (four a
-// thread), then the slots' numbers.  Which place of its expert a slot gets is not the
-// same each time; nothing that is computed depends on it.
-__device__ __forceinline__ void expert_place(const PlaceArgs &a) {
-  __shared__ int counts[kExpertsMost], sums[2][256];
-  const int tid = threadIdx.x;
-  for (int e = tid; e < kExpertsMost; e += 256) counts[e] = 0;
-  __syncthreads();
-  for (int s = tid; s < a.slots; s += 256) {
-    const int e = a.pick[s];
-    if (e >= 0 && e < a.experts) atomicAdd(&counts[e], 1);
-  }
-  __syncthreads();
-  int n[4], places = 0, tiles = 0;
+// A workgroup lists one expert's slots, in an order of their own that is always the same:
+// it reads every pick (from the L2 but once), counts its own and those of experts before,
+// and gives its own their numbers.  One workgroup for all of them, counting with atomics,
+// took 33 us for 16376 slots.
+__device__ __forceinline__ void expert_place(const PlaceArgs &a, int expert) {
+  __shared__ int sums[2][kPrepareThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kWaves = kPrepareThreads / 64;
+  const int each = (a.slots + kWaves - 1) / kWaves;
+  const int first = wave * each, end = min(first + each, a.slots);
+  auto round = [&](int s0, int (&e)[kPlaceRound]) {  // no branch, so that all are on their way at once
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    n[i] = counts[4 * tid + i];
-    places += n[i];
-    tiles += (n[i] + a.tile - 1) / a.tile;
-  }
-  sums[0][tid] = places;
-  sums[1][tid] = tiles;
-  __syncthreads();
-  for (int d = 1; d < 256; d *= 2) {
-    const int p = tid >= d ? sums[0][tid - d] : 0, t = tid >= d ? sums[1][tid - d] : 0;
-    __syncthreads();
-    sums[0][tid] += p;
-    sums[1][tid] += t;
-    __syncthreads();
-  }
-  if (tid == 255) *a.tile_count = sums[1][255];
-  int place = sums[0][tid] - places, tile = sums[1][tid] - tiles;
+    for (int i = 0; i < kPlaceRound; ++i) e[i] = a.pick[min(s0 + 64 * i + lane, a.slots - 1)];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    counts[4 * tid + i] = place;
-    for (int at = 0; at < n[i]; at += a.tile) a.tiles[tile++] = Mx4Tile{4 * tid + i, place + at, min(a.tile, n[i] - at)};
-    place += n[i];
-  }
-  __syncthreads();
-  for (int s = tid; s < a.slots; s += 256) {
-    const int e = a.pick[s];
-    int at = -1;
-    if (e >= 0 && e < a.experts) {
-      at = atomicAdd(&counts[e], 1);
-      a.lane_of[at] = s / a.top;
+    for (int i = 0; i < kPlaceRound; ++i) e[i] = s0 + 64 * i + lane < end ? e[i] : -1;
+  };
+  int mine = 0, before = 0;
+  for (int s0 = first; s0 < end; s0 += 64 * kPlaceRound) {
+    int e[kPlaceRound];
+    round(s0, e);
+#pragma unroll
+    for (int i = 0; i < kPlaceRound; ++i) {
+      mine += e[i] == expert;
+      before += (uint32_t)e[i] < (uint32_t)expert;
     }
-    a.place_of[s] = at;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    mine += __shfl_xor(mine, d);
+    before += __shfl_xor(before, d);
+  }
+  if (lane == 0) sums[0][wave] = mine, sums[1][wave] = before;
+  __syncthreads();
+  int base = 0, total = 0, next = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    base += sums[1][w];
+    total += sums[0][w];
+    if (w < wave) next += sums[0][w];
+  }
+  next += base;
+  for (int s0 = first; s0 < end; s0 += 64 * kPlaceRound) {
+    int e[kPlaceRound];
+    round(s0, e);
+#pragma unroll
+    for (int i = 0; i < kPlaceRound; ++i) {
+      const int s = s0 + 64 * i + lane;
+      const uint64_t own = __ballot(e[i] == expert);
+      const int place = next + __builtin_popcountll(own & ((1ull << lane) - 1));
+      next += __builtin_popcountll(own);
+      if (e[i] == expert) {
+        a.place_of[s] = place;
+        a.lane_of[place] = s / a.top;
+      }
+      if (expert == 0 && s < end && (uint32_t)e[i] >= (uint32_t)a.experts) a.place_of[s] = -1;
+    }
+  }
+  // this expert's tiles and those left over between it and the next's, or the end
+  const int tile0 = base / a.tile + expert;
+  const int tile1 = expert + 1 < a.experts ? (base + total) / a.tile + expert + 1 : a.slots / a.tile + a.experts;
+  for (int i = tile0 + (int)threadIdx.x; i < tile1; i += kPrepareThreads) {
+    const int from = (i - tile0) * a.tile;
+    a.tiles[i] = Mx4Tile{expert, base + min(from, total), max(0, min(a.tile, total - from))};
   }
 }
 
@@ -480,32 +463,75 @@ struct PackArgs {
   uint8_t *dst;
 };
 
+// Sixteen scale bytes of a row from group g on, zeros behind its last; nothing behind the
+// row is read.
+__device__ __forceinline__ uint4_t mx4_scales16(const uint8_t *row, int g, int groups) {
+  struct __attribute__((packed)) Word {
+    uint32_t w;
+  };
+  struct __attribute__((packed)) Words {
+    uint32_t w[4];
+  };
+  if (g + 16 <= groups) {
+    const Words b = *reinterpret_cast<const Words *>(row + g);
+    return uint4_t{b.w[0], b.w[1], b.w[2], b.w[3]};
+  }
+  uint4_t out = {0, 0, 0, 0};
+  if (groups >= 4) {  // words that end with the row, moved down to where they belong
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const Word *>(row + min(g + 4 * i, groups - 4))->w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int late = g + 4 * i - min(g + 4 * i, groups - 4);
+      out[i] = late < 4 ? w[i] >> (8 * late) : 0u;
+    }
+  } else if (g == 0) {
+    const uint32_t a = row[0], b = row[min(1, groups - 1)], c = row[groups - 1];
+    out[0] = a | (groups > 1 ? b << 8 : 0u) | (groups > 2 ? c << 16 : 0u);
+  }
+  return out;
+}
+
+// A thread takes row `at` of every tile of a block and sixteen groups, four steps: a turn of
+// four rows' bytes in registers for every four tiles.
 template <int NT, bool PAIR>
 __device__ __forceinline__ void mx4_pack_scales(const PackArgs &a, long long id) {
-  const int steps = mx4_steps(a.groups), blocks = tile_blocks<NT, PAIR>(a.rows);
-  const int lane = (int)(id & 63);
-  const long long unit = id >> 6;
-  const int step = (int)(unit % steps);
-  const long long block = unit / steps;
+  const int steps = mx4_steps(a.groups), blocks = tile_blocks<NT, PAIR>(a.rows), fours = (steps + 3) / 4;
+  const int at = (int)(id & 15);
+  const int four = (int)(id / 16 % fours);
+  const long long block = id / 16 / fours;
   const int e = (int)(block / blocks);
   if (e >= a.experts) return;
-  const int g = 4 * step + (lane >> 4);
-  uint16_t out[NT / 2];
+  uint4_t v[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    const size_t row = (size_t)e * a.rows + tile_row<NT, PAIR>((int)(block % blocks), j, lane & 15, a.rows);
-    const uint16_t b = g < a.groups ? a.w.scale[row * a.w.scale_stride + g] : 0;
-    out[j / 2] = j % 2 ? (uint16_t)(out[j / 2] | b << 8) : b;
+    const size_t row = (size_t)e * a.rows + tile_row<NT, PAIR>((int)(block % blocks), j, at, a.rows);
+    v[j] = mx4_scales16(a.w.scale + row * a.w.scale_stride, 16 * four, a.groups);
   }
-  uint16_t *dst = reinterpret_cast<uint16_t *>(a.dst) + (unit * 64 + lane) * (NT / 2);
 #pragma unroll
-  for (int i = 0; i < NT / 2; ++i) dst[i] = out[i];
+  for (int s = 0; s < 4; ++s) {
+    if (4 * four + s >= steps) break;
+    uint32_t *const dst =
+        reinterpret_cast<uint32_t *>(a.dst) + (((size_t)block * steps + 4 * four + s) * 64 + at) * (NT / 4);
+#pragma unroll
+    for (int q = 0; q < NT / 4; ++q) {
+      // bytes 0 .. 3 of four rows: pairs of rows, then pairs of pairs
+      const uint32_t r0 = v[4 * q][s], r1 = v[4 * q + 1][s], r2 = v[4 * q + 2][s], r3 = v[4 * q + 3][s];
+      const uint32_t lo01 = __builtin_amdgcn_perm(r1, r0, 0x05010400u), hi01 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
+      const uint32_t lo23 = __builtin_amdgcn_perm(r3, r2, 0x05010400u), hi23 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
+      dst[q] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+      dst[16 * (NT / 4) + q] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+      dst[32 * (NT / 4) + q] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+      dst[48 * (NT / 4) + q] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+    }
+  }
 }
 
 // What products of many lanes need first, in one launch: lanes as terms, a sheet's scales
 // packed (as pairs of blocks for the experts' gate), then another's; of microscaled lanes
 // theirs, four tiles a block, in the first's place.  Experts' places in front (a
-// workgroup; place.experts 0: none).
+// workgroup each; place.experts 0: none).
 struct PrepareArgs {
   const void *act;
   long long act_stride;
@@ -518,26 +544,23 @@ struct PrepareArgs {
 };
 
 template <int T, int NT>
-__global__ __launch_bounds__(256) void mx4_prepare_kernel(PrepareArgs a) {
+__global__ __launch_bounds__(kPrepareThreads) void mx4_prepare_kernel(PrepareArgs a) {
   const int block = blockIdx.x;
   if (block >= a.rows.first_block) {
-    mx4_pack_scales<NT, false>(a.rows, (long long)(block - a.rows.first_block) * 256 + threadIdx.x);
+    mx4_pack_scales<NT, false>(a.rows, (long long)(block - a.rows.first_block) * kPrepareThreads + threadIdx.x);
   } else if (block >= a.pairs.first_block) {
-    mx4_pack_scales<NT, true>(a.pairs, (long long)(block - a.pairs.first_block) * 256 + threadIdx.x);
+    mx4_pack_scales<NT, true>(a.pairs, (long long)(block - a.pairs.first_block) * kPrepareThreads + threadIdx.x);
   } else if (block >= a.lane_block) {
-    const long long id = (long long)(block - a.lane_block) * 256 + threadIdx.x;
+    const long long id = (long long)(block - a.lane_block) * kPrepareThreads + threadIdx.x;
     if constexpr (T == 0)
       mx4_pack_scales<4, false>(a.lane_scales, id);
     else
       mx4_terms_group<T, T == 3>(a.act, a.act_stride, a.groups, a.lanes, a.terms, id);
   } else {
-    expert_place(a.place);
+    expert_place(a.place, block);
   }
 }
 
-// What becomes of a tile's sums: rows of floats, or the gated products of row pairs (the
-// experts' hidden values) as terms for the product behind.
-enum { kOutF32 = 0, kOutBf16 = 1, kOutGate = 2 };
 
 template <int T, int MT, int NT, int WM, int WN, int OUT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
@@ -547,18 +570,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int part = lane >> 4, at = lane & 15, wm = wave / WN, wn = wave % WN;
-  int tile_x, tile_y;
-  xcd_tile(tile_x, tile_y);
-  int first = tile_y * F::kLanes, count = min(F::kLanes, g.lanes - first), expert = 0;
-  if (g.tiles) {
-    if (tile_y >= *g.tile_count) return;
+  const int blocks = tile_blocks<NT, PAIR>(g.rows);
+  int tile_x, tile_y, first, count, expert = 0;
+  if (!g.tiles) {
+    xcd_tile(tile_x, tile_y);
+    first = tile_y * F::kLanes;
+    count = min(F::kLanes, g.lanes - first);
+  } else {
+    // workgroups go to the eight XCDs in turn: each takes a run of tiles, all rows of one
+    // after another, so that its L2 serves a tile's lanes and its expert's rows again
+    const int gx = (blocks + WN - 1) / WN, total = gx * g.tile_count, id = (int)blockIdx.x;
+    const int run = (total + 7) / 8, at = (id & 7) * run + (id >> 3);
+    if (at >= total) return;
+    tile_x = at % gx;
+    tile_y = at / gx;
     const Mx4Tile t = g.tiles[tile_y];
     first = t.first;
     count = t.count;
     expert = t.expert;
+    if (count == 0) return;
   }
   const size_t row0 = (size_t)expert * (size_t)g.rows;
-  const int blocks = tile_blocks<NT, PAIR>(g.rows);
   const int block0 = tile_x * WN;  // blocks behind the last hold its rows, and are not stored
   const int steps = mx4_steps(g.groups);
 
@@ -623,6 +655,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
+  // A tile that an expert does not fill: waves without lanes only bring
+  const bool busy = 16 * wm * MT < count;
   // Workgroups of neighbouring rows begin at other columns: rows are often a power of
   // two bytes apart, and all at the same column would ask the same cache channels
   int k = 2 * tile_x % steps;
@@ -635,6 +669,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
     asm volatile("" ::: "memory");
     if (s + 1 < steps) bring(k_next, s + 1);
     const uint8_t *st = lds_x + (s & 1) * F::kStage;
+    if (!busy) {
+      k = k_next;
+      continue;
+    }
     // Lanes' terms behind the last group are zeros, and codes are finite; of microscaled lanes neither side's are
     const uint32_t keep = T != 0 || 4 * k + part < g.groups ? 0xFFFFFFFFu : 0u;
     int8v_t op[2][T == 0 ? 1 : T];
@@ -819,23 +857,349 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
 
 // ---- the experts' feed-forward ------------------------------------------------------
 
+// The codes and scale of group g of a row as loaded: behind its last group the last one's,
+// which `mx4_clear` makes zeros.
+struct Mx4Codes {
+  uint4_t code;
+  int scale;
+};
+
+__device__ __forceinline__ Mx4Codes mx4_load(const uint8_t *code, const uint8_t *scale, int g, int groups) {
+  const int at = min(g, groups - 1);
+  return Mx4Codes{*reinterpret_cast<const uint4_t *>(code + 16 * (size_t)at), scale[at]};
+}
+
+__device__ __forceinline__ int8v_t mx4_clear(const Mx4Codes &c, int g, int groups) {
+  const uint4_t k = g < groups ? c.code : uint4_t{0, 0, 0, 0};
+  return int8v_t{(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+}
+
+// The product of up to sixteen lanes, bound by the sheet's bytes: a workgroup takes 16 RT
+// rows and its four waves every fourth step, operands straight to registers, four steps'
+// codes in flight a wave; sums meet in LDS.  Lane l of a wave holds group l / 16 of row and
+// of lane l % 16.  T terms, 0: microscaled lanes.
+constexpr int kFewAhead = 4;
+
+template <int T, int RT, int OUT>
+__global__ __launch_bounds__(256) void mx4_few_kernel(Mx4Args g) {
+  __shared__ float4_t sums[3][RT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int part = lane >> 4, at = lane & 15;
+  const int n0 = blockIdx.x * 16 * RT, steps = mx4_steps(g.groups);
+  const int first = 16 * blockIdx.y, count = min(16, g.lanes - first);
+  const uint8_t *code[RT], *scale[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const size_t row = (size_t)min(n0 + 16 * r + at, g.rows - 1);
+    code[r] = g.w.code + row * g.w.code_stride;
+    scale[r] = g.w.scale + row * g.w.scale_stride;
+  }
+  const size_t from = (size_t)(first + min(at, count - 1));
+  float4_t acc[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) acc[r] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = wave; s0 < steps; s0 += 4 * kFewAhead) {
+    Mx4Codes w[kFewAhead][RT];
+#pragma unroll
+    for (int u = 0; u < kFewAhead; ++u)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) w[u][r] = mx4_load(code[r], scale[r], 4 * (s0 + 4 * u) + part, g.groups);
+#pragma unroll
+    for (int u = 0; u < kFewAhead; ++u) {
+      const int s = s0 + 4 * u;
+      if (s >= steps) break;
+      const int group = 4 * s + part;
+      if constexpr (T == 0) {
+        const Mx4Codes c = mx4_load(g.act.code + from * g.act.code_stride, g.act.scale + from * g.act.scale_stride, group,
+                                    g.groups);
+        const int8v_t a = mx4_clear(c, group, g.groups);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+          acc[r] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_clear(w[u][r], group, g.groups), a, acc[r], 4, 4, 0,
+                                                                    group < g.groups ? w[u][r].scale : 0, 0,
+                                                                    group < g.groups ? c.scale : 0);
+      } else {
+        // lanes' terms behind the last group are zeros, and codes are finite; their scales may not be
+        const uint8_t *step = g.terms + term_at<T == 0 ? 3 : T>(from, s, (size_t)g.term_lanes);
+        const uint2_t scales = term_scales<T == 0 ? 3 : T>(step, part);
+#pragma unroll
+        for (int q = 0; q < T; ++q) {
+          const int8v_t a = term_operand<T == 0 ? 3 : T>(step, q, part);
+          const int as = q < 4 ? (int)(scales[0] >> (8 * q)) : (int)scales[1];
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            acc[r] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_clear(w[u][r], group, g.groups), a, acc[r], 4, 2,
+                                                                      0, group < g.groups ? w[u][r].scale : 0, 0, as);
+        }
+      }
+    }
+  }
+  // every lane took part in the products: nothing of them may move behind a branch that some leave
+#pragma unroll
+  for (int r = 0; r < RT; ++r) asm volatile("" : "+v"(acc[r]));
+  if (wave > 0)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) sums[wave - 1][r][lane] = acc[r];
+  __syncthreads();
+  if (wave > 0 || at >= count) return;
+  const size_t out = (size_t)(first + at) * (size_t)g.out_stride;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    float4_t v = acc[r];
+#pragma unroll
+    for (int w = 0; w < 3; ++w) v += sums[w][r][lane];
+    const int n = n0 + 16 * r + 4 * part;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      if (n + d >= g.rows) continue;
+      if (OUT == kOutBf16)
+        static_cast<uint16_t *>(g.out)[out + n + d] = float_bf16(v[d]);
+      else
+        static_cast<float *>(g.out)[out + n + d] = v[d];
+    }
+  }
+}
+
+// ---- a few lanes of floats, cut where they are used -----------------------------------
+
+// A wave cuts the groups that its own steps need (first, first + stride, ..: `count` steps of
+// one row of `groups` groups) into LDS, [step][part] records of T terms and scales.
+template <int T>
+struct OwnTerms {
+  static constexpr int kRecord = 24 * T + 8;  // bytes: 128, 80
+};
+
+template <int T, bool BF16>
+__device__ __forceinline__ void own_terms(const void *row, int groups, int first, int stride, int count, int lane,
+                                          uint8_t *room) {
+  for (int i = lane; i < 4 * count; i += 64) {
+    const int g = 4 * (first + i / 4 * stride) + i % 4;
+    float x[32];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      if (g < groups) mx4_load8<BF16>(row, 32 * (size_t)g + 8 * e, part);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[8 * e + q] = part[q];
+    }
+    mx4_terms_record<T>(x, room + i * OwnTerms<T>::kRecord);
+  }
+}
+
+// Column c of an operand of single lanes: term c % T of lane c / T (columns behind the last
+// hold anything), from the lanes' records.
+template <int T>
+__device__ __forceinline__ int8v_t own_operand(const uint8_t *record, int t, int &scale) {
+  const uint2_t a = *reinterpret_cast<const uint2_t *>(record + 24 * t);
+  const uint2_t b = *reinterpret_cast<const uint2_t *>(record + 24 * t + 8);
+  const uint2_t c = *reinterpret_cast<const uint2_t *>(record + 24 * t + 16);
+  const uint2_t s = *reinterpret_cast<const uint2_t *>(record + 24 * T);
+  scale = t < 4 ? (int)(s[0] >> (8 * t)) : (int)s[1];
+  return int8v_t{(int)a[0], (int)a[1], (int)b[0], (int)b[1], (int)c[0], (int)c[1], 0, 0};
+}
+
+// One to three fp32 lanes (five bf16 ones), a token's step: a lane's terms are columns of
+// the one operand, so five terms cost one product, and a wave cuts the lanes itself while
+// its first codes are on their way: no launch before.  Sums of terms and waves in LDS.
+// kOutGate: blockIdx.y a slot of the experts: its expert's gate and up rows, the gated
+// products as floats.
+template <int T, int RT, int OUT, bool BF16>
+__global__ __launch_bounds__(256) void mx4_step_kernel(Mx4Args g) {
+  constexpr bool PAIR = OUT == kOutGate;
+  static_assert(!PAIR || RT == 2, "a tile of gate rows, and the rows they gate");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_x[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int part = lane >> 4, at = lane & 15;
+  const int steps = mx4_steps(g.groups), mine = (steps - wave + 3) / 4;
+  const int half = g.rows / 2, n0 = blockIdx.x * 16 * (PAIR ? 1 : RT);
+  int lanes = g.lanes;
+  size_t row0 = 0, from = 0;
+  if (PAIR) {
+    const int e = g.lane_of[blockIdx.y];  // the picks
+    if ((uint32_t)e >= (uint32_t)g.experts) return;
+    row0 = (size_t)e * (size_t)g.rows;
+    from = blockIdx.y / (uint32_t)g.top;
+    lanes = 1;
+  }
+  const uint8_t *code[RT], *scale[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const size_t row = row0 + (size_t)(PAIR ? r * half + min(n0 + at, half - 1) : min(n0 + 16 * r + at, g.rows - 1));
+    code[r] = g.w.code + row * g.w.code_stride;
+    scale[r] = g.w.scale + row * g.w.scale_stride;
+  }
+  Mx4Codes w[kFewAhead][RT];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kFewAhead; ++u)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) w[u][r] = mx4_load(code[r], scale[r], 4 * (wave + 4 * (i0 + u)) + part, g.groups);
+  };
+  load(0);
+  const int room_lane = 4 * ((steps + 3) / 4) * OwnTerms<T>::kRecord;  // of a lane, this wave's
+  uint8_t *const room = lds_x + wave * lanes * room_lane;
+  for (int m = 0; m < lanes; ++m)
+    own_terms<T, BF16>(static_cast<const uint8_t *>(g.act_rows) + (from + m) * (size_t)g.act_stride * (BF16 ? 2 : 4),
+                       g.groups, wave, 4, mine, lane, room + m * room_lane);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own, no barrier
+  const int column_lane = min(at / T, lanes - 1), column_term = at / T < lanes ? at % T : 0;
+  float4_t acc[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) acc[r] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < mine; i0 += kFewAhead) {
+    if (i0) load(i0);
+#pragma unroll
+    for (int u = 0; u < kFewAhead; ++u) {
+      if (i0 + u >= mine) break;
+      const int group = 4 * (wave + 4 * (i0 + u)) + part;
+      int as;
+      const int8v_t a =
+          own_operand<T>(room + column_lane * room_lane + (4 * (i0 + u) + part) * OwnTerms<T>::kRecord, column_term, as);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        acc[r] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_clear(w[u][r], group, g.groups), a, acc[r], 4, 2, 0,
+                                                                  group < g.groups ? w[u][r].scale : 0, 0, as);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) asm volatile("" : "+v"(acc[r]));  // as in mx4_few_kernel
+  __syncthreads();
+  // [wave][row][column]
+  float *const sums = reinterpret_cast<float *>(lds_x);
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) sums[((wave * RT + r) * 16 + 4 * part + d) * 17 + at] = acc[r][d];
+  __syncthreads();
+  auto total = [&](int r, int row, int m) {  // terms from the smallest on, waves in order
+    float v = 0.0f;
+#pragma unroll
+    for (int t = T - 1; t >= 0; --t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v += sums[((q * RT + r) * 16 + row) * 17 + m * T + t];
+    return v;
+  };
+  if (PAIR) {
+    if (threadIdx.x >= 16 || n0 + (int)threadIdx.x >= half) return;
+    const float gate = total(0, threadIdx.x, 0), up = total(RT - 1, threadIdx.x, 0);
+    static_cast<float *>(g.out)[(size_t)blockIdx.y * half + n0 + threadIdx.x] =
+        (g.silu ? silu_near(gate) : gelu_near(gate)) * up;
+    return;
+  }
+  for (int i = threadIdx.x; i < 16 * RT * lanes; i += 256) {
+    const int m = i / (16 * RT), n = i % (16 * RT);
+    if (n0 + n >= g.rows) continue;
+    const float v = total(n / 16, n % 16, m);
+    const size_t out = (size_t)m * (size_t)g.out_stride + n0 + n;
+    if (OUT == kOutBf16)
+      static_cast<uint16_t *>(g.out)[out] = float_bf16(v);
+    else
+      static_cast<float *>(g.out)[out] = v;
+  }
+}
+
+// The down products of a token's experts and their sum: blockIdx.y a lane, eight waves, each
+// every eighth of its choices (its hidden values cut by the wave), sixteen rows.
+template <int T, bool BF16>
+__global__ __launch_bounds__(512) void expert_step_kernel(Mx4Args g, const float *hidden, const float *weight, void *out) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_x[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int part = lane >> 4, at = lane & 15;
+  const int steps = mx4_steps(g.groups), n0 = blockIdx.x * 16;
+  uint8_t *const room = lds_x + wave * (4 * steps * OwnTerms<T>::kRecord);
+  float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j = wave; j < g.top; j += 8) {
+    const size_t slot = (size_t)blockIdx.y * (size_t)g.top + j;
+    const int e = g.lane_of[slot];
+    if ((uint32_t)e >= (uint32_t)g.experts) continue;
+    const size_t row = (size_t)e * (size_t)g.rows + (size_t)min(n0 + at, g.rows - 1);
+    const uint8_t *code = g.w.code + row * g.w.code_stride, *scale = g.w.scale + row * g.w.scale_stride;
+    constexpr int kAhead = 6;
+    Mx4Codes w[kAhead];
+    auto load = [&](int s0) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) w[u] = mx4_load(code, scale, 4 * (s0 + u) + part, g.groups);
+    };
+    load(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    own_terms<T, false>(hidden + slot * (size_t)(32 * g.groups), g.groups, 0, 1, steps, lane, room);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own, no barrier
+    float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < steps; s0 += kAhead) {
+      if (s0) load(s0);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s0 + u >= steps) break;
+        const int group = 4 * (s0 + u) + part;
+        int as;
+        const int8v_t a = own_operand<T>(room + (4 * (s0 + u) + part) * OwnTerms<T>::kRecord, at < T ? at : 0, as);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_clear(w[u], group, g.groups), a, acc, 4, 2, 0,
+                                                               group < g.groups ? w[u].scale : 0, 0, as);
+      }
+    }
+    asm volatile("" : "+v"(acc));
+    const float share = weight[slot];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) sum[d] = __builtin_fmaf(share, acc[d], sum[d]);
+  }
+  __syncthreads();
+  float *const sums = reinterpret_cast<float *>(lds_x);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) sums[(wave * 16 + 4 * part + d) * 17 + at] = sum[d];
+  __syncthreads();
+  if (threadIdx.x >= 16 || n0 + (int)threadIdx.x >= g.rows) return;
+  float v = 0.0f;
+#pragma unroll
+  for (int t = T - 1; t >= 0; --t)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += sums[(q * 16 + threadIdx.x) * 17 + t];
+  const size_t to = (size_t)blockIdx.y * (size_t)g.out_stride + n0 + threadIdx.x;
+  if (BF16)
+    static_cast<uint16_t *>(out)[to] = float_bf16(v);
+  else
+    static_cast<float *>(out)[to] = v;
+}
+
 // out[lane] = sum over its choices, in their order, of weight * row of the slot's place
 template <bool BF16>
 __global__ __launch_bounds__(256) void expert_join_kernel(const float *rows, const int *place_of, const float *weight,
                                                           int top, int hidden, int lanes, void *out, long long out_stride) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long lane = id / hidden;
+  const int quads = hidden / 4;
+  const long long lane = id / quads;
   if (lane >= lanes) return;
-  const int n = (int)(id - lane * hidden);
-  float sum = 0.0f;
-  for (int j = 0; j < top; ++j) {
-    const int place = place_of[lane * top + j];
-    if (place >= 0) sum = __builtin_fmaf(weight[lane * top + j], rows[(size_t)place * hidden + n], sum);
+  const int n = 4 * (int)(id - lane * quads);
+  float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j0 = 0; j0 < top; j0 += 8) {
+    float4_t v[8];
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {  // eight rows on their way at once
+      const int place = j0 + j < top ? place_of[lane * top + j0 + j] : -1;
+      w[j] = place >= 0 ? weight[lane * top + j0 + j] : 0.0f;
+      v[j] = place >= 0 ? __builtin_nontemporal_load(reinterpret_cast<const float4_t *>(rows + (size_t)place * hidden + n))
+                        : float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) sum[d] = __builtin_fmaf(w[j], v[j][d], sum[d]);
   }
-  if (BF16)
-    static_cast<uint16_t *>(out)[(size_t)lane * out_stride + n] = float_bf16(sum);
-  else
-    static_cast<float *>(out)[(size_t)lane * out_stride + n] = sum;
+  const size_t to = (size_t)lane * (size_t)out_stride + n;
+  struct __attribute__((packed)) Half4 {
+    uint16_t v[4];
+  };
+  if (BF16) {
+    Half4 h;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) h.v[d] = float_bf16(sum[d]);
+    *reinterpret_cast<Half4 *>(static_cast<uint16_t *>(out) + to) = h;
+  } else {
+    Mx4Quad f;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) f.v[d] = sum[d];
+    *reinterpret_cast<Mx4Quad *>(static_cast<float *>(out) + to) = f;
+  }
 }
 
 }  // namespace igl
@@ -904,24 +1268,25 @@ static size_t pack_bytes(int rows, int groups, int experts) {
 
 template <int NT, bool PAIR>
 static unsigned pack_blocks(int rows, int groups, int experts) {
-  return (unsigned)(((long long)experts * tile_blocks<NT, PAIR>(rows) * mx4_steps(groups) + 3) / 4);
+  const long long threads = (long long)experts * tile_blocks<NT, PAIR>(rows) * ((mx4_steps(groups) + 3) / 4) * 16;
+  return (unsigned)((threads + kPrepareThreads - 1) / kPrepareThreads);
 }
 
 // The launch before products of many lanes, what of it there is to do: `a` filled but for
 // the workgroups' numbers.
 template <int T, int NT>
 static hipError_t launch_prepare(PrepareArgs a, hipStream_t stream) {
-  long long block = a.place.experts ? 1 : 0;
+  long long block = a.place.experts;
   a.lane_block = (int)block;
   if (T == 0)
     block += pack_blocks<4, false>(a.lane_scales.rows, a.lane_scales.groups, 1);
   else
-    block += ((long long)a.lanes * 4 * mx4_steps(a.groups) + 255) / 256;
+    block += ((long long)a.lanes * 4 * mx4_steps(a.groups) + kPrepareThreads - 1) / kPrepareThreads;
   a.pairs.first_block = (int)block;
   if (a.pairs.dst) block += pack_blocks<NT, true>(a.pairs.rows, a.pairs.groups, a.pairs.experts);
   a.rows.first_block = (int)block;
   block += pack_blocks<NT, false>(a.rows.rows, a.rows.groups, a.rows.experts);
-  hipLaunchKernelGGL((mx4_prepare_kernel<T, NT>), dim3((unsigned)block), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((mx4_prepare_kernel<T, NT>), dim3((unsigned)block), dim3(kPrepareThreads), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -935,27 +1300,52 @@ static hipError_t launch_tile(const Mx4Args &a, int tiles, hipStream_t stream) {
     if (e != hipSuccess) return e;
     granted = true;
   }
-  const int blocks = tile_blocks<NT, OUT == kOutGate>(a.rows);
-  hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, WM, WN, OUT>), dim3((blocks + WN - 1) / WN, tiles), dim3(64 * F::kWaves),
+  const unsigned gx = (unsigned)((tile_blocks<NT, OUT == kOutGate>(a.rows) + WN - 1) / WN);
+  // grouped: one run of tiles for each of eight XCDs
+  const dim3 grid = a.tiles ? dim3((gx * (unsigned)tiles + 7) / 8 * 8) : dim3(gx, (unsigned)tiles);
+  hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, WM, WN, OUT>), grid, dim3(64 * F::kWaves),
                      (size_t)F::lds(OUT == kOutGate), stream, a);
   return hipGetLastError();
 }
 
-// A product of few lanes: tiles of sixteen.  terms 0: microscaled lanes.
-static hipError_t launch_wave(const Mx4Args &a, int terms, int out_bf16, hipStream_t stream) {
-  const dim3 grid((a.rows + 63) / 64, (a.lanes + 15) / 16);
-  if (terms == 0 && out_bf16)
-    hipLaunchKernelGGL((mx4_wave_kernel<0, true>), grid, dim3(256), 0, stream, a);
-  else if (terms == 0)
-    hipLaunchKernelGGL((mx4_wave_kernel<0, false>), grid, dim3(256), 0, stream, a);
-  else if (terms == 3 && out_bf16)
-    hipLaunchKernelGGL((mx4_wave_kernel<3, true>), grid, dim3(256), 0, stream, a);
-  else if (terms == 3)
-    hipLaunchKernelGGL((mx4_wave_kernel<3, false>), grid, dim3(256), 0, stream, a);
-  else if (out_bf16)
-    hipLaunchKernelGGL((mx4_wave_kernel<5, true>), grid, dim3(256), 0, stream, a);
+// A product of up to sixteen lanes a tile, its terms (if any) prepared: workgroups of 64 rows
+// where they still give every CU four, of 16 below.
+template <int T, int OUT>
+static hipError_t launch_few(const Mx4Args &a, hipStream_t stream) {
+  const int tiles = (a.lanes + 15) / 16;
+  if ((long long)a.rows * tiles >= 64 * 1024)
+    hipLaunchKernelGGL((mx4_few_kernel<T, 4, OUT>), dim3((a.rows + 63) / 64, tiles), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((mx4_wave_kernel<5, false>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((mx4_few_kernel<T, 1, OUT>), dim3((a.rows + 15) / 16, tiles), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+// LDS of a step's workgroup: every wave's records of its steps, or the sums.
+template <int T>
+static size_t step_lds(int groups, int lanes, int row_tiles, int waves, int stride) {
+  const size_t records = (size_t)waves * lanes * 4 * ((mx4_steps(groups) + stride - 1) / stride) * OwnTerms<T>::kRecord;
+  const size_t sums = (size_t)waves * row_tiles * 16 * 17 * sizeof(float);
+  return records > sums ? records : sums;
+}
+
+template <typename K>
+static hipError_t grant_lds(K kernel, size_t bytes, size_t &granted) {
+  if (bytes <= granted) return hipSuccess;
+  const hipError_t e =
+      hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == hipSuccess) granted = bytes;
+  return e;
+}
+
+constexpr size_t kStepLds = 64 * 1024;  // two workgroups a CU and more
+
+template <int T, int RT, int OUT, bool BF16>
+static hipError_t launch_step(const Mx4Args &a, dim3 grid, int lanes, hipStream_t stream) {
+  static size_t granted = 0;
+  const size_t lds = step_lds<T>(a.groups, lanes, RT, 4, 4);
+  const hipError_t e = grant_lds(&mx4_step_kernel<T, RT, OUT, BF16>, kStepLds, granted);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((mx4_step_kernel<T, RT, OUT, BF16>), grid, dim3(256), lds, stream, a);
   return hipGetLastError();
 }
 
@@ -1012,8 +1402,22 @@ extern "C" hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *a
   if (lanes >= kMx4Many)
     return act_bf16 ? launch_many<3, 2, 4, 2, 4>(a, act, act_stride, out_bf16, room, stream)
                     : launch_many<5, 2, 8, 2, 4>(a, act, act_stride, out_bf16, room, stream);
+  const bool single = act_bf16 ? lanes <= 5 && step_lds<3>(a.groups, lanes, 1, 4, 4) <= kStepLds
+                               : lanes <= 3 && step_lds<5>(a.groups, lanes, 1, 4, 4) <= kStepLds;
+  if (single) {
+    a.act_rows = act;
+    a.act_stride = act_stride;
+    const dim3 grid((a.rows + 15) / 16);
+    if (act_bf16)
+      return out_bf16 ? launch_step<3, 1, kOutBf16, true>(a, grid, lanes, stream)
+                      : launch_step<3, 1, kOutF32, true>(a, grid, lanes, stream);
+    return out_bf16 ? launch_step<5, 1, kOutBf16, false>(a, grid, lanes, stream)
+                    : launch_step<5, 1, kOutF32, false>(a, grid, lanes, stream);
+  }
   const hipError_t e = launch_terms(act, act_bf16, act_stride, lanes, sheet->col_count, room, stream);
-  return e != hipSuccess ? e : launch_wave(a, act_bf16 ? 3 : 5, out_bf16, stream);
+  if (e != hipSuccess) return e;
+  if (act_bf16) return out_bf16 ? launch_few<3, kOutBf16>(a, stream) : launch_few<3, kOutF32>(a, stream);
+  return out_bf16 ? launch_few<5, kOutBf16>(a, stream) : launch_few<5, kOutF32>(a, stream);
 }
 
 extern "C" hipError_t igl_launch_mx4_mat_mx4(const igl_mx4 *sheet, const igl_mx4 *act, int lane_first, int lanes,
@@ -1028,7 +1432,7 @@ extern "C" hipError_t igl_launch_mx4_mat_mx4(const igl_mx4 *sheet, const igl_mx4
   a.out_stride = out_stride;
   if (lanes >= kMx4Many)
     return launch_many<0, 4, 4, 2, 4>(a, nullptr, 0, out_bf16, static_cast<uint8_t *>(work), stream);
-  return launch_wave(a, 0, out_bf16, stream);
+  return out_bf16 ? launch_few<0, kOutBf16>(a, stream) : launch_few<0, kOutF32>(a, stream);
 }
 
 namespace igl {
@@ -1036,14 +1440,12 @@ namespace igl {
 // The places of a call's experts, its lanes' and hidden values' terms, packed scales, and
 // the rows that are joined.
 struct ExpertRoom {
-  size_t lane_of, place_of, tiles, tile_count, x, gate_up, down, h, rows, end;
+  size_t lane_of, place_of, tiles, x, gate_up, down, h, rows, end;
 };
 
 constexpr int kExpertTile = 16;  // lanes of the smallest tile
 
-static int expert_tiles(int slots, int experts, int tile) {
-  return slots / tile + (slots < experts ? slots : experts);
-}
+static int expert_tiles(int slots, int experts, int tile) { return slots / tile + experts; }
 
 static ExpertRoom expert_room(const igl_experts *x, int lanes, int top, int bf16) {
   const size_t slots = (size_t)lanes * top;
@@ -1057,11 +1459,10 @@ static ExpertRoom expert_room(const igl_experts *x, int lanes, int top, int bf16
   r.lane_of = take(slots * sizeof(int));
   r.place_of = take(slots * sizeof(int));
   r.tiles = take((size_t)expert_tiles((int)slots, x->expert_count, kExpertTile) * sizeof(Mx4Tile));
-  r.tile_count = take(sizeof(int));
   r.x = take(terms_bytes(lanes, x->hidden, bf16));
   r.gate_up = take(pack_bytes<8, true>(2 * x->inner, x->hidden / kMx4Group, x->expert_count));
   r.down = take(pack_bytes<8, false>(x->hidden, x->inner / kMx4Group, x->expert_count));
-  r.h = take(terms_bytes((int)slots, x->inner, bf16));
+  r.h = take(terms_bytes((int)slots, x->inner, 0));  // as floats (a token's step) they are no more
   r.rows = take(slots * x->hidden * sizeof(float));
   r.end = at;
   return r;
@@ -1095,7 +1496,7 @@ static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
   p.lanes = c.lanes;
   p.terms = c.base + r.x;
   p.place = PlaceArgs{c.pick, slots, c.top, x->expert_count, F::kLanes, (int *)(c.base + r.lane_of),
-                      (int *)(c.base + r.place_of), (Mx4Tile *)(c.base + r.tiles), (int *)(c.base + r.tile_count)};
+                      (int *)(c.base + r.place_of), (Mx4Tile *)(c.base + r.tiles)};
   p.pairs = PackArgs{mx4_view(&x->gate_up, 0), 2 * x->inner, p.groups, x->expert_count, 0, c.base + r.gate_up};
   p.rows = PackArgs{mx4_view(&x->down, 0), x->hidden, x->inner / kMx4Group, x->expert_count, 0, c.base + r.down};
   if ((e = launch_prepare<T, NT>(p, stream)) != hipSuccess) return e;
@@ -1106,7 +1507,7 @@ static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
   a.terms = p.terms;
   a.term_lanes = c.lanes;
   a.tiles = p.place.tiles;
-  a.tile_count = p.place.tile_count;
+  a.tile_count = tiles;
   a.lane_of = p.place.lane_of;
   a.row_scales = p.pairs.dst;
   a.out = c.base + r.h;
@@ -1123,13 +1524,51 @@ static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
   a.out = c.base + r.rows;
   a.out_stride = x->hidden;
   if ((e = launch_tile<T, MT, NT, WM, WN, kOutF32>(a, tiles, stream)) != hipSuccess) return e;
-  const unsigned blocks = (unsigned)(((long long)c.lanes * x->hidden + 255) / 256);
+  const unsigned blocks = (unsigned)(((long long)c.lanes * (x->hidden / 4) + 255) / 256);
   if (c.out_bf16)
     hipLaunchKernelGGL((expert_join_kernel<true>), dim3(blocks), dim3(256), 0, stream, (const float *)(c.base + r.rows),
                        p.place.place_of, c.weight, c.top, x->hidden, c.lanes, c.out, c.out_stride);
   else
     hipLaunchKernelGGL((expert_join_kernel<false>), dim3(blocks), dim3(256), 0, stream, (const float *)(c.base + r.rows),
                        p.place.place_of, c.weight, c.top, x->hidden, c.lanes, c.out, c.out_stride);
+  return hipGetLastError();
+}
+
+// A few lanes' experts, a slot at a time: gate and up, then down and the sum, two launches.
+template <int T, bool BF16>
+static hipError_t experts_step(const ExpertCall &c, hipStream_t stream) {
+  static size_t granted = 0;
+  const igl_experts *x = c.x;
+  Mx4Args a = {};
+  a.w = mx4_view(&x->gate_up, 0);
+  a.rows = 2 * x->inner;
+  a.groups = x->hidden / kMx4Group;
+  a.lanes = c.lanes;
+  a.lane_of = c.pick;
+  a.act_rows = c.act;
+  a.act_stride = c.act_stride;
+  a.experts = x->expert_count;
+  a.top = c.top;
+  a.silu = x->gate == IGL_GATE_SILU;
+  a.out = c.base + c.room.h;
+  hipError_t e = launch_step<T, 2, kOutGate, BF16>(a, dim3((x->inner + 15) / 16, c.lanes * c.top), 1, stream);
+  if (e != hipSuccess) return e;
+  a.w = mx4_view(&x->down, 0);
+  a.rows = x->hidden;
+  a.groups = x->inner / kMx4Group;
+  a.out_stride = c.out_stride;
+  const size_t lds = step_lds<T>(a.groups, 1, 1, 8, 1);
+  const dim3 grid((x->hidden + 15) / 16, c.lanes);
+  if (c.out_bf16) {
+    static size_t granted16 = 0;
+    if ((e = grant_lds(&expert_step_kernel<T, true>, kStepLds, granted16)) != hipSuccess) return e;
+    hipLaunchKernelGGL((expert_step_kernel<T, true>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
+                       c.weight, c.out);
+  } else {
+    if ((e = grant_lds(&expert_step_kernel<T, false>, kStepLds, granted)) != hipSuccess) return e;
+    hipLaunchKernelGGL((expert_step_kernel<T, false>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
+                       c.weight, c.out);
+  }
   return hipGetLastError();
 }
 
@@ -1144,6 +1583,12 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
                                          int out_stride, void *work, hipStream_t stream) {
   const ExpertCall c = {x,   act,      act_stride, lanes, pick, weight, top,
                         out, out_bf16, out_stride, static_cast<uint8_t *>(work), expert_room(x, lanes, top, act_bf16)};
+  const bool step = (long long)lanes * top <= 64 &&
+                    (act_bf16 ? step_lds<3>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
+                                    step_lds<3>(x->inner / kMx4Group, 1, 1, 8, 1) <= kStepLds
+                              : step_lds<5>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
+                                    step_lds<5>(x->inner / kMx4Group, 1, 1, 8, 1) <= kStepLds);
+  if (step) return act_bf16 ? experts_step<3, true>(c, stream) : experts_step<5, false>(c, stream);
   const bool many = (long long)lanes * top >= 24LL * x->expert_count;
   if (act_bf16)
     return many ? experts_grouped<3, 2, 4, 2, 4>(c, stream) : experts_grouped<3, 1, 4, 1, 4>(c, stream);

@@ -9,12 +9,14 @@
 // compared in double; without a bias and groups s rises with x, and x decides.
 #pragma once
 
+#include <type_traits>
+
 #include "igl_device.h"
 #include "igl_launch.h"
 
 namespace igl {
 
-constexpr int kRouteWaves = 4;  // lanes a workgroup, a wave each
+constexpr int kRouteWaves = 4;  // lanes of a batch a workgroup, a wave each
 
 struct RouteArgs {
   igl_route rule;
@@ -24,113 +26,229 @@ struct RouteArgs {
   const float *bias, *gain;
   int32_t *pick;
   float *weight;
+  uint32_t each_inverse;  // of a group's experts: e / each = e * each_inverse >> 20 for e < 1024
 };
 
-__device__ __forceinline__ double shfl_f64(double v, int from) { return __shfl(v, from); }
-
-// The larger choice, the lower index where equal.
-__device__ __forceinline__ bool route_before(double a, int ia, double b, int ib) {
-  return a > b || (a == b && ia < ib);
+// e^x in double: x = k ln 2 + r, |r| <= 0.35, the series of e^r to the thirteenth power
+// (what is left out is below 2^-57 of it), times 2^k.  x not above 1024; 0 far below.
+__device__ __forceinline__ double exp_f64(double x) {
+  const double k = __builtin_rint(x * 1.4426950408889634);
+  double r = __builtin_fma(k, -0.69314718036912382, x);  // ln 2 in two pieces, the first of 32 bits: k times it is exact
+  r = __builtin_fma(k, -1.9082149292705877e-10, r);
+  double p = 1.0 / 6227020800.0;
+  p = __builtin_fma(p, r, 1.0 / 479001600.0);
+  p = __builtin_fma(p, r, 1.0 / 39916800.0);
+  p = __builtin_fma(p, r, 1.0 / 3628800.0);
+  p = __builtin_fma(p, r, 1.0 / 362880.0);
+  p = __builtin_fma(p, r, 1.0 / 40320.0);
+  p = __builtin_fma(p, r, 1.0 / 5040.0);
+  p = __builtin_fma(p, r, 1.0 / 720.0);
+  p = __builtin_fma(p, r, 1.0 / 120.0);
+  p = __builtin_fma(p, r, 1.0 / 24.0);
+  p = __builtin_fma(p, r, 1.0 / 6.0);
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  return x > -1100.0 ? __builtin_ldexp(p, (int)fmax(k, -1100.0)) : 0.0;
 }
 
-// A wave a lane of the batch; wave lane l holds experts l, l + 64, .. (PER of them).
-// What may not be chosen has choice -infinity.
-template <int PER>
+// 1 / d, d in [1, infinity]: the hardware's estimate and two Newton steps.
+__device__ __forceinline__ double recip_f64(double d) {
+  double r = __builtin_amdgcn_rcp(d);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  return d < __builtin_inf() ? r : 0.0;
+}
+
+// A number's bits so that they order as it does, above 0 for all but a NaN.
+__device__ __forceinline__ uint64_t route_key(double c) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, c);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ uint32_t route_key(float c) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, c);
+  return u >> 31 ? ~u : u | 1u << 31;
+}
+
+// The largest of a wave's numbers, in every lane: a word at a time along the rows of a wave.
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  auto step = [&](int moved) { v = max(v, (uint32_t)moved); };
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));  // row_half_mirror
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));  // row_mirror
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, true));  // row_bcast:15
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, true));  // row_bcast:31
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// The lanes that hold the wave's largest key.
+__device__ __forceinline__ uint64_t route_best(uint32_t key, bool &any) {
+  const uint32_t top = wave_max_u32(key);
+  any = top > 0;
+  return __ballot(key == top);
+}
+__device__ __forceinline__ uint64_t route_best(uint64_t key, bool &any) {
+  const uint32_t high = (uint32_t)(key >> 32), top = wave_max_u32(high);
+  any = top > 0;
+  uint64_t at = __ballot(high == top);
+  if (at & (at - 1)) {  // upper words are seldom equal
+    const uint32_t low = high == top ? (uint32_t)key : 0u, rest = wave_max_u32(low);
+    at = __ballot(high == top && low == rest);
+  }
+  return at;
+}
+
+// A wave a lane of the batch; wave lane l holds experts PER l .. PER l + PER - 1, so that
+// of equal ones the lowest lane's is the lowest.  WIDE: choices are doubles (a bias, or
+// groups); else the logits.  What may not be chosen has key 0.
+template <int PER, bool WIDE>
 __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(RouteArgs a) {
-  __shared__ double choices[kRouteWaves][64 * PER];
-  __shared__ double scores[kRouteWaves][64];  // of groups
+  using Key = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
+  __shared__ double room[WIDE ? kRouteWaves : 1][WIDE ? 64 * PER : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long m = (long long)blockIdx.x * kRouteWaves + wave;
-  const bool here = m < a.lanes;
-  const int E = a.rule.expert_count;
-  const float *x = a.logits + (here ? m : 0) * a.logit_stride;
+  if (m >= a.lanes) return;  // a wave's own from here on, no barrier
+  const int E = a.rule.expert_count, first = PER * lane;
+  const float *x = a.logits + m * a.logit_stride;
   const double none = -__builtin_inf();
   float v[PER];
   float top = -__builtin_inff();
 #pragma unroll
+  for (int i = 0; i < PER; ++i) v[i] = x[min(first + i, E - 1)];
+#pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = lane + 64 * i;
-    v[i] = e < E ? x[e] : -__builtin_inff();
-    if (!(v[i] >= -3.402823466e38f)) v[i] = -__builtin_inff();  // a NaN is never chosen
-    if (v[i] > 3.402823466e38f) v[i] = 3.402823466e38f;
+    if (first + i >= E || !(v[i] >= -3.402823466e38f)) v[i] = -__builtin_inff();  // a NaN is never chosen
+    v[i] = fminf(v[i], 3.402823466e38f);
     top = fmaxf(top, v[i]);
   }
-  double s[PER], c[PER];
-  if (a.rule.score == IGL_ROUTE_SOFTMAX) {
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    double sum = 0.0;
+  const bool soft = a.rule.score == IGL_ROUTE_SOFTMAX;
+  double sum = 1.0;  // of the exponentials, where it is asked for
+  if (soft) {
+    const uint32_t key = wave_max_u32(route_key(top));  // at least minus infinity's
+    top = __builtin_bit_cast(float, key >> 31 ? key & 0x7FFFFFFFu : ~key);
+  }
+  // s before softmax's division; where the logits decide, only of the chosen
+  auto score = [&](float t) {
+    if (t == -__builtin_inff()) return 0.0;
+    return soft ? exp_f64((double)t - (double)top) : recip_f64(1.0 + exp_f64(fmin(-(double)t, 800.0)));
+  };
+  double s[WIDE ? PER : 1];
+  Key key[PER];
+  if (soft && (WIDE || !a.rule.renorm)) {
+    sum = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      s[i] = v[i] == -__builtin_inff() ? 0.0 : exp((double)v[i] - (double)top);
-      sum += s[i];
+      const double t = score(v[i]);
+      if constexpr (WIDE) s[i] = t;
+      sum += t;
     }
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = sum > 0.0 ? s[i] / sum : 0.0;
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    sum = sum > 0.0 ? sum : 1.0;
+  } else if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = score(v[i]);
+  }
+  if constexpr (WIDE) {
+    const double inverse = soft ? 1.0 / sum : 1.0;
+    double c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      s[i] *= inverse;
+      c[i] = v[i] == -__builtin_inff() ? none : s[i] + (a.bias ? (double)a.bias[min(first + i, E - 1)] : 0.0);
+      if (!(c[i] > none)) c[i] = none;  // and a bias that is a NaN
+    }
+    uint64_t kept = ~0ull;
+    if (a.rule.group_count > 1) {
+      const int each = E / a.rule.group_count;
+      double group_score = none;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) room[wave][first + i] = c[i];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const int lanes_each = each / PER;
+      if (each % PER == 0 && (lanes_each & (lanes_each - 1)) == 0) {
+        // a group is a run of lanes, a power of two: the two largest of each, merged
+        double most = none, second = none;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          second = fmax(second, fmin(most, c[i]));
+          most = fmax(most, c[i]);
+        }
+        for (int d = 1; d < lanes_each; d *= 2) {
+          const double other = __shfl_xor(most, d), other_second = __shfl_xor(second, d);
+          second = fmax(fmin(most, other), fmax(second, other_second));
+          most = fmax(most, other);
+        }
+        const double of_group = a.rule.group_best == 2 && second > none ? most + second : most;
+        group_score = __shfl(of_group, min(lane * lanes_each, 63));
+      } else if (lane < a.rule.group_count) {
+        double most = none, second = none;
+        for (int i = 0; i < each; ++i) {
+          const double t = room[wave][lane * each + i];
+          second = fmax(second, fmin(most, t));
+          most = fmax(most, t);
+        }
+        group_score = a.rule.group_best == 2 && second > none ? most + second : most;
+      }
+      if (lane >= a.rule.group_count) group_score = none;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      room[wave][lane] = group_score;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      // a group stays if fewer than group_top come before it
+      int ahead = 0;
+#pragma unroll 8
+      for (int q = 0; q < a.rule.group_count; ++q) {
+        const double other = room[wave][q];
+        ahead += other > group_score || (other == group_score && q < lane);
+      }
+      kept = __ballot(ahead < a.rule.group_top && group_score > none);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool in = a.rule.group_count == 1 || (kept >> ((uint32_t)(first + i) * a.each_inverse >> 20 & 63) & 1);
+      key[i] = in && c[i] > none ? route_key(c[i]) : 0;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = v[i] == -__builtin_inff() ? 0.0 : 1.0 / (1.0 + exp(-(double)v[i]));
-  }
-  const bool plain = !a.bias && a.rule.group_count == 1;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = lane + 64 * i;
-    c[i] = v[i] == -__builtin_inff() ? none : plain ? (double)v[i] : s[i] + (a.bias && e < E ? (double)a.bias[e] : 0.0);
-    if (!(c[i] > none)) c[i] = none;  // a bias that is a NaN
-    choices[wave][e] = c[i];
-  }
-  __syncthreads();
-  if (a.rule.group_count > 1) {
-    const int each = E / a.rule.group_count;
-    double score = none;
-    if (lane < a.rule.group_count) {
-      double first = none, second = none;
-      for (int i = 0; i < each; ++i) {
-        const double t = choices[wave][lane * each + i];
-        if (t > first) {
-          second = first;
-          first = t;
-        } else if (t > second) {
-          second = t;
-        }
-      }
-      score = a.rule.group_best == 2 && second > none ? first + second : first;
-    }
-    scores[wave][lane] = score;
-    __syncthreads();
-    // a group stays if fewer than group_top come before it
-    int ahead = 0;
-    for (int g = 0; g < a.rule.group_count; ++g) ahead += route_before(scores[wave][g], g, score, lane);
-    scores[wave][lane] = ahead < a.rule.group_top && score > none ? 1.0 : 0.0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = lane + 64 * i;
-      if (e < E && scores[wave][e / each] == 0.0) c[i] = none;
-    }
+    for (int i = 0; i < PER; ++i) key[i] = v[i] == -__builtin_inff() ? 0 : route_key(v[i]);
   }
   // the best, one at a time; wave lane j keeps the j-th's
   int mine = -1;
   double share = 0.0, total = 0.0;
   for (int j = 0; j < a.rule.top; ++j) {
-    double best = none, score = 0.0;
-    int at = 0x7FFFFFFF;
+    Key best = key[0];
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < PER; ++i)
+      if (key[i] > best) best = key[i], at = i;
+    bool any;
+    const int from = __builtin_ctzll(route_best(best, any));
+    if (!any) break;
+    const int slot = __builtin_amdgcn_readlane(at, from);
+    double taken = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (c[i] > best) best = c[i], at = lane + 64 * i, score = s[i];
-    for (int d = 32; d; d >>= 1) {
-      const double other = __shfl_xor(best, d), other_score = __shfl_xor(score, d);
-      const int other_at = __shfl_xor(at, d);
-      if (route_before(other, other_at, best, at)) best = other, at = other_at, score = other_score;
+      if (i == slot) {
+        if constexpr (WIDE) taken = s[i];
+        if (lane == from) key[i] = 0;
+      }
+    if constexpr (WIDE) {
+      const uint64_t bits = __builtin_bit_cast(uint64_t, taken);
+      const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, from);
+      const uint32_t high = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), from);
+      taken = __builtin_bit_cast(double, (uint64_t)high << 32 | low);
+      total += taken;
     }
-    if (!(best > none)) break;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 64 * i == at) c[i] = none;
-    total += score;
-    if (lane == j) mine = at, share = score;
+    if (lane == j) mine = PER * from + slot, share = taken;
   }
-  if (!here || lane >= a.rule.top) return;
+  if constexpr (!WIDE) {
+    if (mine >= 0) share = score(fminf(x[mine], 3.402823466e38f)) / sum;
+    total = share;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+  }
+  if (lane >= a.rule.top) return;
   if (a.rule.renorm) share = total > 0.0 ? share / total : 0.0;
   share *= (double)a.rule.gain_scale;
   if (a.gain && mine >= 0) share *= (double)a.gain[mine];
@@ -138,23 +256,28 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(RouteArgs a) {
   a.weight[m * a.rule.top + lane] = mine >= 0 ? (float)share : 0.0f;
 }
 
+template <int PER>
+static hipError_t launch_route(const RouteArgs &a, hipStream_t stream) {
+  const dim3 grid((unsigned)((a.lanes + kRouteWaves - 1) / kRouteWaves)), block(64 * kRouteWaves);
+  if (a.bias || a.rule.group_count > 1)
+    hipLaunchKernelGGL((route_kernel<PER, true>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((route_kernel<PER, false>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
 }  // namespace igl
 
 extern "C" hipError_t igl_launch_route(const igl_route *rule, const float *logits, int logit_stride, int lanes,
                                        const float *bias, const float *gain, int32_t *pick, float *weight,
                                        hipStream_t stream) {
-  const igl::RouteArgs a = {*rule, logits, logit_stride, lanes, bias, gain, pick, weight};
-  const dim3 grid((unsigned)((lanes + igl::kRouteWaves - 1) / igl::kRouteWaves)), block(64 * igl::kRouteWaves);
+  const int each = rule->expert_count / rule->group_count;
+  const igl::RouteArgs a = {*rule, logits, logit_stride, lanes, bias, gain, pick, weight,
+                            (uint32_t)(((1 << 20) + each - 1) / each)};
   const int per = (rule->expert_count + 63) / 64;
-  if (per <= 1)
-    hipLaunchKernelGGL((igl::route_kernel<1>), grid, block, 0, stream, a);
-  else if (per <= 2)
-    hipLaunchKernelGGL((igl::route_kernel<2>), grid, block, 0, stream, a);
-  else if (per <= 4)
-    hipLaunchKernelGGL((igl::route_kernel<4>), grid, block, 0, stream, a);
-  else if (per <= 8)
-    hipLaunchKernelGGL((igl::route_kernel<8>), grid, block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((igl::route_kernel<16>), grid, block, 0, stream, a);
-  return hipGetLastError();
+  return per <= 1   ? igl::launch_route<1>(a, stream)
+         : per <= 2 ? igl::launch_route<2>(a, stream)
+         : per <= 4 ? igl::launch_route<4>(a, stream)
+         : per <= 8 ? igl::launch_route<8>(a, stream)
+                    : igl::launch_route<16>(a, stream);
 }

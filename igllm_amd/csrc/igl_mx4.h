@@ -304,6 +304,8 @@ struct Mx4Args {
   const uint8_t *row_scales;    // packed (mx4_prepare_kernel), for the tile kernel
   const uint32_t *lane_scales;
   void *out;                // [lane or place][out_stride]; the experts' gate: terms of out_stride places
+  int slice;                // steps of a slice of the columns (blockIdx.z), whose sums lie slice_out outputs apart
+  size_t slice_out;
   int silu;                 // the experts' gate
   // a few lanes' own floats, and a token's experts (lane_of: the picks)
   const void *act_rows;
@@ -402,8 +404,8 @@ __device__ __forceinline__ void expert_place(const PlaceArgs &a, int expert) {
 }
 
 // The product of many lanes: WM x WN waves of 16 MT lanes x 16 NT rows, 128 columns a
-// step, both operands through LDS in two stages.
-//   * Stages are written only by global_load_lds, a step ahead.  A load to registers
+// step, both operands through LDS in ST stages.
+//   * Stages are written only by global_load_lds, ST - 1 steps ahead.  A load to registers
 //     in the loop costs more than it brings: with such loads and these in flight the
 //     compiler waits for all of either.
 //   * Lanes' terms lie in the order in which they are read, sixteen bytes a wave lane
@@ -412,9 +414,9 @@ __device__ __forceinline__ void expert_place(const PlaceArgs &a, int expert) {
 //   * Scale bytes were put in the order of their reading by the launch before
 //     (mx4_prepare_kernel): as they lie, a byte a lane and row, they would take the
 //     cache as long as the codes do.
-template <int T, int MT, int NT, int WM, int WN>
+template <int T, int MT, int NT, int WM, int WN, int ST>
 struct TileForm {
-  static_assert(NT % 4 == 0, "words of scale bytes");
+  static_assert(NT % 4 == 0 && ST >= 2, "words of scale bytes");
   static constexpr int kWaves = WM * WN;
   static constexpr int kLanes = 16 * MT * WM;
   static constexpr int kWaveRows = 16 * NT;
@@ -432,7 +434,7 @@ struct TileForm {
   static constexpr int kOut = kWaves * 16 * (kWaveRows + 4) * 4;    // a tile of lanes' outputs of every wave
   static constexpr int kGate = kWaves * 16 * MT * (kWaveRows / 2 + 4) * 4;  // all hidden values
   static constexpr int most(int a, int b) { return a > b ? a : b; }
-  static constexpr int lds(bool gate) { return most(2 * kStage, gate ? kGate : kOut); }
+  static constexpr int lds(bool gate) { return most(ST * kStage, gate ? kGate : kOut); }
   static constexpr int kLds = lds(true);
   static_assert(kLds <= 160 * 1024, "LDS");
 };
@@ -562,9 +564,9 @@ __global__ __launch_bounds__(kPrepareThreads) void mx4_prepare_kernel(PrepareArg
 }
 
 
-template <int T, int MT, int NT, int WM, int WN, int OUT>
+template <int T, int MT, int NT, int WM, int WN, int ST, int OUT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
-  using F = TileForm<T, MT, NT, WM, WN>;
+  using F = TileForm<T, MT, NT, WM, WN, ST>;
   constexpr bool PAIR = OUT == kOutGate;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_x[];
   const int lane = threadIdx.x & 63;
@@ -639,7 +641,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
     }
   }
   auto bring = [&](int step, int turn) {
-    uint8_t *dst = lds_x + (turn & 1) * F::kStage;
+    uint8_t *dst = lds_x + turn % ST * F::kStage;
 #pragma unroll
     for (int i = 0; i < F::kLoads; ++i) {
       const uint8_t *from = src[i] + (size_t)step * by[i] + min((uint32_t)step * walk[i] + plus[i], most);
@@ -659,16 +661,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
   const bool busy = 16 * wm * MT < count;
   // Workgroups of neighbouring rows begin at other columns: rows are often a power of
   // two bytes apart, and all at the same column would ask the same cache channels
-  int k = 2 * tile_x % steps;
-  bring(k, 0);
-  for (int s = 0; s < steps; ++s) {
-    const int k_next = k + 1 < steps ? k + 1 : 0;
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this step's stage is in, brought a step ago
+  const int k_first = blockIdx.z * g.slice, k_end = min(k_first + g.slice, steps), k_count = k_end - k_first;
+  int k = k_first + 2 * tile_x % k_count, k_ahead = k;
+  auto bring_next = [&](int turn) {
+    bring(k_ahead, turn);
+    k_ahead = k_ahead + 1 < k_end ? k_ahead + 1 : k_first;
+  };
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s)
+    if (s < k_count) bring_next(s);
+  for (int s = 0; s < k_count; ++s) {
+    const int k_next = k + 1 < k_end ? k + 1 : k_first;
+    // lgkmcnt(0), and of this wave's loads all but the ST - 2 stages behind this step's
+    constexpr int kBehind = (ST - 2) * F::kLoads;
+    static_assert(kBehind < 64, "vmcnt");
+    if (ST > 2 && s + ST - 2 < k_count)
+      __builtin_amdgcn_s_waitcnt((kBehind & 15) | (kBehind >> 4) << 14 | 0x0070);
+    else
+      __builtin_amdgcn_s_waitcnt(0x0070);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + 1 < steps) bring(k_next, s + 1);
-    const uint8_t *st = lds_x + (s & 1) * F::kStage;
+    if (s + ST - 1 < k_count) bring_next(s + ST - 1);
+    const uint8_t *st = lds_x + s % ST * F::kStage;
     if (!busy) {
       k = k_next;
       continue;
@@ -828,7 +843,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
       const int n = n0 + c;
       const int place = 16 * (wm * MT + i) + m;
       if (place >= count) continue;
-      const size_t out = (size_t)(first + place) * (size_t)g.out_stride + n;
+      const size_t out = (size_t)blockIdx.z * g.slice_out + (size_t)(first + place) * (size_t)g.out_stride + n;
       if (whole && n + kOf <= g.rows) {
         uint4_t b;
         if (OUT == kOutBf16) {
@@ -1290,22 +1305,41 @@ static hipError_t launch_prepare(PrepareArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int T, int MT, int NT, int WM, int WN, int OUT>
-static hipError_t launch_tile(const Mx4Args &a, int tiles, hipStream_t stream) {
-  using F = TileForm<T, MT, NT, WM, WN>;
+template <int T, int MT, int NT, int WM, int WN, int ST, int OUT>
+static hipError_t launch_tile(Mx4Args a, int tiles, int slices, hipStream_t stream) {
+  using F = TileForm<T, MT, NT, WM, WN, ST>;
   static bool granted = false;  // the dynamic LDS a kernel asks for is granted once
   if (!granted) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_tile_kernel<T, MT, NT, WM, WN, OUT>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_tile_kernel<T, MT, NT, WM, WN, ST, OUT>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, F::lds(OUT == kOutGate));
     if (e != hipSuccess) return e;
     granted = true;
   }
   const unsigned gx = (unsigned)((tile_blocks<NT, OUT == kOutGate>(a.rows) + WN - 1) / WN);
   // grouped: one run of tiles for each of eight XCDs
-  const dim3 grid = a.tiles ? dim3((gx * (unsigned)tiles + 7) / 8 * 8) : dim3(gx, (unsigned)tiles);
-  hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, WM, WN, OUT>), grid, dim3(64 * F::kWaves),
+  const dim3 grid = a.tiles ? dim3((gx * (unsigned)tiles + 7) / 8 * 8) : dim3(gx, (unsigned)tiles, (unsigned)slices);
+  const int steps = mx4_steps(a.groups);
+  a.slice = (steps + slices - 1) / slices;
+  hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, WM, WN, ST, OUT>), grid, dim3(64 * F::kWaves),
                      (size_t)F::lds(OUT == kOutGate), stream, a);
   return hipGetLastError();
+}
+
+// Slices' sums added in their order.
+template <bool BF16>
+__global__ __launch_bounds__(256) void mx4_fold_kernel(const float *sums, int slices, size_t slice_out, int rows, void *out,
+                                                       long long out_stride) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= rows) return;
+  const float *from = sums + (size_t)blockIdx.y * rows + n;
+  float v = 0.0f;
+#pragma unroll 8
+  for (int z = 0; z < slices; ++z) v += from[(size_t)z * slice_out];
+  const size_t to = (size_t)blockIdx.y * (size_t)out_stride + n;
+  if (BF16)
+    static_cast<uint16_t *>(out)[to] = float_bf16(v);
+  else
+    static_cast<float *>(out)[to] = v;
 }
 
 // A product of up to sixteen lanes a tile, its terms (if any) prepared: workgroups of 64 rows
@@ -1337,7 +1371,7 @@ static hipError_t grant_lds(K kernel, size_t bytes, size_t &granted) {
   return e;
 }
 
-constexpr size_t kStepLds = 64 * 1024;  // two workgroups a CU and more
+constexpr size_t kStepLds = 100 * 1024;
 
 template <int T, int RT, int OUT, bool BF16>
 static hipError_t launch_step(const Mx4Args &a, dim3 grid, int lanes, hipStream_t stream) {
@@ -1349,11 +1383,26 @@ static hipError_t launch_step(const Mx4Args &a, dim3 grid, int lanes, hipStream_
   return hipGetLastError();
 }
 
-// A product of many lanes: the launch that prepares it and the product.  `work` holds
-// mx4_many_bytes.
-template <int T, int MT, int NT, int WM, int WN>
-static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int out_bf16, uint8_t *work,
+// Tiles of a product, and slices of its columns: twice as many as long as the tiles give
+// fewer than 160 CUs a workgroup, a slice has two steps and the sums stay within 16 MiB.
+static long long mx4_tiles(int rows, int lanes, int tile_lanes, int tile_rows) {
+  return (long long)((lanes + tile_lanes - 1) / tile_lanes) * ((rows + tile_rows - 1) / tile_rows);
+}
+
+static int mx4_slices(int rows, int groups, int lanes, int tile_lanes, int tile_rows) {
+  const long long tiles = mx4_tiles(rows, lanes, tile_lanes, tile_rows);
+  const int steps = mx4_steps(groups);
+  int slices = 1;
+  while (tiles * slices < 160 && steps >= 4 * slices && 2LL * slices * lanes * rows <= 1 << 22) slices *= 2;
+  const int each = (steps + slices - 1) / slices;
+  return (steps + each - 1) / each;  // none empty
+}
+
+// A product of many lanes: the launch that prepares it and the product.
+template <int T, int MT, int NT, int WM, int WN, int ST>
+static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int out_bf16, uint8_t *work, bool slice,
                               hipStream_t stream) {
+  using F = TileForm<T, MT, NT, WM, WN, ST>;
   const size_t lanes_bytes =
       T == 0 ? pack_bytes<4, false>(a.lanes, a.groups, 1) : terms_bytes(a.lanes, a.groups * kMx4Group, T == 3);
   PrepareArgs p = {};
@@ -1370,20 +1419,50 @@ static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int ou
   a.term_lanes = a.lanes;
   a.lane_scales = reinterpret_cast<const uint32_t *>(work);
   a.row_scales = work + lanes_bytes;
-  const int tiles = (a.lanes + 16 * MT * WM - 1) / (16 * MT * WM);
-  return out_bf16 ? launch_tile<T, MT, NT, WM, WN, kOutBf16>(a, tiles, stream)
-                  : launch_tile<T, MT, NT, WM, WN, kOutF32>(a, tiles, stream);
+  const int tiles = (a.lanes + F::kLanes - 1) / F::kLanes;
+  const int slices = slice ? mx4_slices(a.rows, a.groups, a.lanes, F::kLanes, F::kRows) : 1;
+  if (slices == 1)
+    return out_bf16 ? launch_tile<T, MT, NT, WM, WN, ST, kOutBf16>(a, tiles, 1, stream)
+                    : launch_tile<T, MT, NT, WM, WN, ST, kOutF32>(a, tiles, 1, stream);
+  Mx4Args b = a;
+  b.out = work + lanes_bytes + pack_bytes<NT, false>(a.rows, a.groups, 1);
+  b.out_stride = a.rows;
+  b.slice_out = (size_t)a.lanes * a.rows;
+  const hipError_t f = launch_tile<T, MT, NT, WM, WN, ST, kOutF32>(b, tiles, slices, stream);
+  if (f != hipSuccess) return f;
+  const dim3 grid((a.rows + 255) / 256, a.lanes);
+  if (out_bf16)
+    hipLaunchKernelGGL((mx4_fold_kernel<true>), grid, dim3(256), 0, stream, (const float *)b.out, slices, b.slice_out,
+                       a.rows, a.out, a.out_stride);
+  else
+    hipLaunchKernelGGL((mx4_fold_kernel<false>), grid, dim3(256), 0, stream, (const float *)b.out, slices, b.slice_out,
+                       a.rows, a.out, a.out_stride);
+  return hipGetLastError();
 }
 
-constexpr int kMx4Many = 64;  // lanes from which the tiles are taken
+// Which kernels a product of `lanes` takes (terms 0: microscaled lanes).
+enum { kFormFew = 0, kFormHead, kFormSmall, kFormLarge };
 
-// Enough for either form of a product: its lanes as terms, or their scales, and the
-// sheet's scales packed (eight tiles a block).
+static int mx4_form(int rows, int groups, int lanes, int terms) {
+  const int steps = mx4_steps(groups);
+  if (lanes <= 16 && terms != 0 && rows >= 65536) return kFormHead;
+  if ((long long)lanes * steps < (terms == 5 ? 192 : terms == 3 ? 640 : 2048)) return kFormFew;
+  const long long large = terms == 5   ? mx4_tiles(rows, lanes, 64, 512)
+                          : terms == 3 ? mx4_tiles(rows, lanes, 64, 256)
+                                       : mx4_tiles(rows, lanes, 128, 256);
+  return large >= 192 ? kFormLarge : kFormSmall;
+}
+
+// Enough for any form of a product: its lanes as terms, or their scales, the sheet's scales
+// packed (eight tiles a block at most), and slices' sums.
 extern "C" size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int terms) {
-  const int groups = cols / kMx4Group;
-  if (lanes < kMx4Many) return terms ? terms_bytes(lanes, cols, terms == 3) : 0;
-  const size_t sheet = pack_bytes<8, false>(rows, groups, 1);
-  return sheet + (terms ? terms_bytes(lanes, cols, terms == 3) : pack_bytes<4, false>(lanes, groups, 1));
+  const int groups = cols / kMx4Group, form = mx4_form(rows, groups, lanes, terms);
+  const size_t of_lanes = terms ? terms_bytes(lanes, cols, terms == 3) : pack_bytes<4, false>(lanes, groups, 1);
+  if (form == kFormFew) return terms ? of_lanes : 0;
+  const int slices =
+      form == kFormSmall ? terms ? mx4_slices(rows, groups, lanes, 32, 256) : mx4_slices(rows, groups, lanes, 64, 256) : 1;
+  return of_lanes + pack_bytes<8, false>(rows, groups, 1) +
+         (slices > 1 ? mx4_up((size_t)slices * lanes * rows * sizeof(float)) : 0);
 }
 
 extern "C" hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *act, int act_bf16, int act_stride,
@@ -1399,9 +1478,6 @@ extern "C" hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *a
   a.out = out;
   a.out_stride = out_stride;
   uint8_t *const room = static_cast<uint8_t *>(work);
-  if (lanes >= kMx4Many)
-    return act_bf16 ? launch_many<3, 2, 4, 2, 4>(a, act, act_stride, out_bf16, room, stream)
-                    : launch_many<5, 2, 8, 2, 4>(a, act, act_stride, out_bf16, room, stream);
   const bool single = act_bf16 ? lanes <= 5 && step_lds<3>(a.groups, lanes, 1, 4, 4) <= kStepLds
                                : lanes <= 3 && step_lds<5>(a.groups, lanes, 1, 4, 4) <= kStepLds;
   if (single) {
@@ -1414,6 +1490,16 @@ extern "C" hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *a
     return out_bf16 ? launch_step<5, 1, kOutBf16, false>(a, grid, lanes, stream)
                     : launch_step<5, 1, kOutF32, false>(a, grid, lanes, stream);
   }
+  const int form = mx4_form(a.rows, a.groups, lanes, act_bf16 ? 3 : 5);
+  if (form == kFormHead)
+    return act_bf16 ? launch_many<3, 1, 4, 1, 4, 3>(a, act, act_stride, out_bf16, room, false, stream)
+                    : launch_many<5, 1, 4, 1, 4, 3>(a, act, act_stride, out_bf16, room, false, stream);
+  if (form == kFormSmall)
+    return act_bf16 ? launch_many<3, 1, 4, 2, 4, 3>(a, act, act_stride, out_bf16, room, true, stream)
+                    : launch_many<5, 1, 4, 2, 4, 3>(a, act, act_stride, out_bf16, room, true, stream);
+  if (form == kFormLarge)
+    return act_bf16 ? launch_many<3, 2, 4, 2, 4, 2>(a, act, act_stride, out_bf16, room, false, stream)
+                    : launch_many<5, 2, 8, 2, 4, 2>(a, act, act_stride, out_bf16, room, false, stream);
   const hipError_t e = launch_terms(act, act_bf16, act_stride, lanes, sheet->col_count, room, stream);
   if (e != hipSuccess) return e;
   if (act_bf16) return out_bf16 ? launch_few<3, kOutBf16>(a, stream) : launch_few<3, kOutF32>(a, stream);
@@ -1430,8 +1516,11 @@ extern "C" hipError_t igl_launch_mx4_mat_mx4(const igl_mx4 *sheet, const igl_mx4
   a.lanes = lanes;
   a.out = out;
   a.out_stride = out_stride;
-  if (lanes >= kMx4Many)
-    return launch_many<0, 4, 4, 2, 4>(a, nullptr, 0, out_bf16, static_cast<uint8_t *>(work), stream);
+  const int form = mx4_form(a.rows, a.groups, lanes, 0);
+  if (form == kFormSmall)
+    return launch_many<0, 4, 4, 1, 4, 3>(a, nullptr, 0, out_bf16, static_cast<uint8_t *>(work), true, stream);
+  if (form == kFormLarge)
+    return launch_many<0, 4, 4, 2, 4, 2>(a, nullptr, 0, out_bf16, static_cast<uint8_t *>(work), false, stream);
   return out_bf16 ? launch_few<0, kOutBf16>(a, stream) : launch_few<0, kOutF32>(a, stream);
 }
 
@@ -1482,9 +1571,9 @@ struct ExpertCall {
   ExpertRoom room;
 };
 
-template <int T, int MT, int NT, int WM, int WN>
+template <int T, int MT, int NT, int WM, int WN, int ST>
 static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
-  using F = TileForm<T, MT, NT, WM, WN>;
+  using F = TileForm<T, MT, NT, WM, WN, ST>;
   const igl_experts *x = c.x;
   const ExpertRoom &r = c.room;
   const int slots = c.lanes * c.top, tiles = expert_tiles(slots, x->expert_count, F::kLanes);
@@ -1513,7 +1602,7 @@ static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
   a.out = c.base + r.h;
   a.out_stride = slots;
   a.silu = x->gate == IGL_GATE_SILU;
-  if ((e = launch_tile<T, MT, NT, WM, WN, kOutGate>(a, tiles, stream)) != hipSuccess) return e;
+  if ((e = launch_tile<T, MT, NT, WM, WN, ST, kOutGate>(a, tiles, 1, stream)) != hipSuccess) return e;
   a.w = p.rows.w;
   a.rows = p.rows.rows;
   a.groups = p.rows.groups;
@@ -1523,7 +1612,7 @@ static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
   a.row_scales = p.rows.dst;
   a.out = c.base + r.rows;
   a.out_stride = x->hidden;
-  if ((e = launch_tile<T, MT, NT, WM, WN, kOutF32>(a, tiles, stream)) != hipSuccess) return e;
+  if ((e = launch_tile<T, MT, NT, WM, WN, ST, kOutF32>(a, tiles, 1, stream)) != hipSuccess) return e;
   const unsigned blocks = (unsigned)(((long long)c.lanes * (x->hidden / 4) + 255) / 256);
   if (c.out_bf16)
     hipLaunchKernelGGL((expert_join_kernel<true>), dim3(blocks), dim3(256), 0, stream, (const float *)(c.base + r.rows),
@@ -1583,7 +1672,9 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
                                          int out_stride, void *work, hipStream_t stream) {
   const ExpertCall c = {x,   act,      act_stride, lanes, pick, weight, top,
                         out, out_bf16, out_stride, static_cast<uint8_t *>(work), expert_room(x, lanes, top, act_bf16)};
-  const bool step = (long long)lanes * top <= 64 &&
+  // a slot at a time reads an expert's weights for each; by experts takes two launches more
+  const int slots = lanes * top;
+  const bool step = slots <= 64 && slots <= 32 + x->expert_count / 4 &&
                     (act_bf16 ? step_lds<3>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
                                     step_lds<3>(x->inner / kMx4Group, 1, 1, 8, 1) <= kStepLds
                               : step_lds<5>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
@@ -1591,6 +1682,6 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
   if (step) return act_bf16 ? experts_step<3, true>(c, stream) : experts_step<5, false>(c, stream);
   const bool many = (long long)lanes * top >= 24LL * x->expert_count;
   if (act_bf16)
-    return many ? experts_grouped<3, 2, 4, 2, 4>(c, stream) : experts_grouped<3, 1, 4, 1, 4>(c, stream);
-  return many ? experts_grouped<5, 2, 4, 2, 4>(c, stream) : experts_grouped<5, 1, 4, 1, 4>(c, stream);
+    return many ? experts_grouped<3, 2, 4, 2, 4, 2>(c, stream) : experts_grouped<3, 1, 4, 1, 4, 3>(c, stream);
+  return many ? experts_grouped<5, 2, 4, 2, 4, 2>(c, stream) : experts_grouped<5, 1, 4, 1, 4, 3>(c, stream);
 }

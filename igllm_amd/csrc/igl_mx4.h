@@ -152,18 +152,25 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(const uint8_t *code, size
 
 // ---- lanes of floats as terms ---------------------------------------------------
 
-// Four groups of a lane (a step of a product) in T terms of six dwords: the first four
-// dwords of every term and group (64 bytes a term), then the last two (32 bytes a
-// term), then the scales as if a term's last two: the bytes of the first four terms (s,
-// s - 5, ..) and of the fifth.  An operand is then sixteen bytes and eight, each read
-// in place, and a step of a lane is one block.
+// Four groups of a lane (a step of a product) in T terms of six dwords, as pieces of 64
+// bytes, sixteen a group: the first four dwords of every term, then the last two, two terms'
+// side by side; the scales as if a term's last two: the bytes of the first four terms
+// (s, s - 5, ..) and of the fifth.  Two pieces of a lane lie side by side, a step's lanes
+// behind each other, then the next two pieces (the fifth of three terms by itself): a
+// cache looks up a line of 128 bytes as fast as half of one, and at that rate the tiles of
+// a product are brought.
 template <int T>
 struct TermForm {
   static constexpr int kStep = T * 96 + 32;  // bytes: 320, 512
-  static constexpr int kChunks = kStep / 64; // of sixteen bytes a group
-  static constexpr int low(int t, int part) { return 64 * t + 16 * part; }
-  static constexpr int high(int t, int part) { return 64 * T + 32 * t + 8 * part; }
+  static constexpr int kChunks = kStep / 64; // pieces
 };
+
+// Where group `part` of piece c begins in a step of `lanes` lanes.
+template <int T>
+__device__ __forceinline__ size_t term_piece(size_t lane, size_t lanes, int c, int part) {
+  constexpr int kChunks = TermForm<T>::kChunks;
+  return (size_t)(c / 2) * lanes * 128 + (c + 1 < kChunks || c % 2 ? lane * 128 + 64 * (c % 2) : lane * 64) + 16 * part;
+}
 
 // The terms of a group.  s is 20 at least, so that s - 5 j stays a byte (five terms
 // then end at 2^-130, three at 2^-120); an infinity or a NaN makes the scale a NaN, so that
@@ -198,16 +205,21 @@ __device__ __forceinline__ void mx4_cut(float (&x)[32], Put put, Scales scales) 
   scales(uint2_t{(uint32_t)s * 0x01010101u - 0x0F0A0500u, (uint32_t)(s - 20)});
 }
 
-// A group's terms into a step of its lane.
+// A group's terms into its step.
 template <int T>
-__device__ __forceinline__ void mx4_terms(float (&x)[32], uint8_t *step, int part) {
+__device__ __forceinline__ void mx4_terms(float (&x)[32], uint8_t *step, size_t lane, size_t lanes, int part) {
+  uint2_t high[T + 1];
   mx4_cut<T>(
       x,
       [&](int t, const uint6_t &w) {
-        *reinterpret_cast<uint4_t *>(step + TermForm<T>::low(t, part)) = uint4_t{w[0], w[1], w[2], w[3]};
-        *reinterpret_cast<uint2_t *>(step + TermForm<T>::high(t, part)) = uint2_t{w[4], w[5]};
+        *reinterpret_cast<uint4_t *>(step + term_piece<T>(lane, lanes, t, part)) = uint4_t{w[0], w[1], w[2], w[3]};
+        high[t] = uint2_t{w[4], w[5]};
       },
-      [&](const uint2_t &s) { *reinterpret_cast<uint2_t *>(step + TermForm<T>::high(T, part)) = s; });
+      [&](const uint2_t &s) { high[T] = s; });
+#pragma unroll
+  for (int t = 0; t <= T; t += 2)
+    *reinterpret_cast<uint4_t *>(step + term_piece<T>(lane, lanes, T + t / 2, part)) =
+        uint4_t{high[t][0], high[t][1], high[t + 1][0], high[t + 1][1]};
 }
 
 // And into a record of its own, a term behind the other.
@@ -226,21 +238,15 @@ __device__ __forceinline__ void mx4_terms_record(float (&x)[32], uint8_t *record
 
 // The operand of term t of a group, and its scales.
 template <int T>
-__device__ __forceinline__ int8v_t term_operand(const uint8_t *step, int t, int part) {
-  const uint4_t a = *reinterpret_cast<const uint4_t *>(step + TermForm<T>::low(t, part));
-  const uint2_t b = *reinterpret_cast<const uint2_t *>(step + TermForm<T>::high(t, part));
+__device__ __forceinline__ int8v_t term_operand(const uint8_t *step, size_t lane, size_t lanes, int t, int part) {
+  const uint4_t a = *reinterpret_cast<const uint4_t *>(step + term_piece<T>(lane, lanes, t, part));
+  const uint2_t b = *reinterpret_cast<const uint2_t *>(step + term_piece<T>(lane, lanes, T + t / 2, part) + 8 * (t % 2));
   return int8v_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], 0, 0};
 }
 
 template <int T>
-__device__ __forceinline__ uint2_t term_scales(const uint8_t *step, int part) {
-  return *reinterpret_cast<const uint2_t *>(step + TermForm<T>::high(T, part));
-}
-
-// Steps lie by step, then by lane, so that sixteen lanes of a product are one block.
-template <int T>
-__device__ __forceinline__ size_t term_at(size_t lane, int step, size_t lanes) {
-  return ((size_t)step * lanes + lane) * TermForm<T>::kStep;
+__device__ __forceinline__ uint2_t term_scales(const uint8_t *step, size_t lane, size_t lanes, int part) {
+  return *reinterpret_cast<const uint2_t *>(step + term_piece<T>(lane, lanes, T + T / 2, part) + 8);
 }
 
 // A thread for group id of the lanes' groups: floats to its terms.
@@ -260,7 +266,7 @@ __device__ __forceinline__ void mx4_terms_group(const void *act, long long act_s
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[8 * e + i] = part[i];
   }
-  mx4_terms<T>(x, terms + term_at<T>((size_t)lane, g >> 2, (size_t)lanes), g & 3);
+  mx4_terms<T>(x, terms + (size_t)(g >> 2) * (size_t)lanes * TermForm<T>::kStep, (size_t)lane, (size_t)lanes, g & 3);
 }
 
 template <int T, bool BF16>
@@ -408,9 +414,8 @@ __device__ __forceinline__ void expert_place(const PlaceArgs &a, int expert) {
 //   * Stages are written only by global_load_lds, ST - 1 steps ahead.  A load to registers
 //     in the loop costs more than it brings: with such loads and these in flight the
 //     compiler waits for all of either.
-//   * Lanes' terms lie in the order in which they are read, sixteen bytes a wave lane
-//     side by side, so no bank meets twice; a row's four 16-byte pieces of codes are
-//     xored by a row key (tile_key) for the same end.
+//   * The 16-byte pieces of a row's codes and of a lane's terms are xored by a key of the
+//     row (tile_key, pair_key), so that no bank meets twice.
 //   * Scale bytes were put in the order of their reading by the launch before
 //     (mx4_prepare_kernel): as they lie, a byte a lane and row, they would take the
 //     cache as long as the codes do.
@@ -433,15 +438,23 @@ struct TileForm {
   static constexpr int kStage = kAll * 1024;
   static constexpr int kOut = kWaves * 16 * (kWaveRows + 4) * 4;    // a tile of lanes' outputs of every wave
   static constexpr int kGate = kWaves * 16 * MT * (kWaveRows / 2 + 4) * 4;  // all hidden values
+  static constexpr __host__ __device__ bool pair(int c) { return T != 0 && (c + 1 < kChunks || c % 2); }  // as in term_piece
   static constexpr int most(int a, int b) { return a > b ? a : b; }
   static constexpr int lds(bool gate) { return most(ST * kStage, gate ? kGate : kOut); }
+  static constexpr bool kAhead = MT * NT < 32;  // two lane tiles' operands in registers
+  static constexpr bool kSpread = !kAhead;
   static constexpr int kLds = lds(true);
   static_assert(kLds <= 160 * 1024, "LDS");
 };
 
-// A row's sixteen-byte piece c of a step lies at c ^ key: sixteen rows' pieces then
-// meet sixteen slots of the 256 bytes that a cycle reads.
-__device__ __forceinline__ int tile_key(int row) { return (row >> 2) & 3; }
+// A row's sixteen-byte piece c of a step lies at c ^ key, so that lanes that are read
+// together meet all banks: these are not sixteen in a row but 0-3, 12-15 and 20-27, and
+// 4-11, 16-19 and 28-31 (keys 0, 1, 2, 3 cost four cycles more a read, by the counter of
+// bank conflicts).
+__device__ __forceinline__ int tile_key(int row) { return 0x78 >> (row >> 1 & 6) & 3; }
+
+// The same of a lane's two pieces of terms, 128 bytes.
+__device__ __forceinline__ int pair_key(int lane) { return lane >> 1 & 7; }
 
 // Row of tile j of a wave's block of 16 NT rows, of `rows` in all (clamped).
 template <int NT, bool PAIR>
@@ -564,6 +577,11 @@ __global__ __launch_bounds__(kPrepareThreads) void mx4_prepare_kernel(PrepareArg
 }
 
 
+template <bool V>
+struct Choice {
+  static constexpr bool value = V;
+};
+
 template <int T, int MT, int NT, int WM, int WN, int ST, int OUT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
   using F = TileForm<T, MT, NT, WM, WN, ST>;
@@ -596,59 +614,74 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
   const int block0 = tile_x * WN;  // blocks behind the last hold its rows, and are not stored
   const int steps = mx4_steps(g.groups);
 
-  // ---- what this wave brings each step: sixteen bytes a lane, from src[i] + step * by[i] + min(step * walk[i] +
-  // plus[i], most).  By number: lanes' chunks (of first dwords, wave lane (part, at)'s sixteen bytes at its number;
-  // of last dwords two terms', eight bytes each, a lane's four groups side by side), rows' codes, packed scales.
-  // The last wave may bring one twice.  Codes walk to a row's last group at most.
-  const uint8_t *src[F::kLoads];
-  size_t by[F::kLoads];
-  uint32_t walk[F::kLoads], plus[F::kLoads];
-  const uint32_t most = 16u * (uint32_t)(g.groups - 1);
+  // ---- what this wave brings each step: sixteen bytes a lane, from base[i] + step * by[i] + off[i], and of codes
+  // (walks[i] all ones) a step's piece, to a row's last at most.  By number: lanes' chunks (wave lane (part, at)'s sixteen bytes at its number), rows' codes, packed
+  // scales.  The last wave may bring one twice.  What is the wave's is uniform and what is a lane's fits 32 bits
+  // (sixteen rows' codes, all lanes' terms), so that a load takes two or three instructions of the lanes'.
+  const uint8_t *base[F::kLoads];
+  uint32_t by[F::kLoads], off[F::kLoads], walks[F::kLoads];
+  int from[F::kLoads];  // the lanes, all on their way at once
+#pragma unroll
+  for (int i = 0; i < F::kLoads; ++i) {
+    const int c = (wave * F::kLoads + i) % F::kChunks, of = 16 * ((wave * F::kLoads + i) / F::kChunks);
+    from[i] = first + min(of + (F::pair(c) ? 8 * (c % 2) + lane / 8 : lane / 4), count - 1);
+  }
+  if (g.lane_of) {
+#pragma unroll
+    for (int i = 0; i < F::kLoads; ++i) from[i] = g.lane_of[from[i]];
+  }
+  // of a step's four pieces of a row this lane's; behind the last group the last (all codes are finite)
+  const int piece = (lane & 3) ^ tile_key(lane >> 2), last_step = (g.groups - 1) >> 2;
 #pragma unroll
   for (int i = 0; i < F::kLoads; ++i) {
     const int id = min(wave * F::kLoads + i, F::kAll - 1);
-    by[i] = walk[i] = plus[i] = 0;
+    walks[i] = 0;
+    by[i] = 0;
     if (id < F::kLaneLoads) {
-      const int c = id % F::kChunks, tile = id / F::kChunks;
-      const bool low = T == 0 || c < T;
-      const int place = first + min(16 * tile + (low ? at : (lane & 31) >> 1), count - 1);
-      const size_t from = (size_t)(g.lane_of ? g.lane_of[place] : place);
+      const int c = id % F::kChunks;
       if constexpr (T == 0) {
-        src[i] = g.act.code + from * g.act.code_stride;
-        walk[i] = 64;
-        plus[i] = 16u * (uint32_t)part;
+        const int low = first + min(16 * (id / F::kChunks), count - 1);
+        base[i] = g.act.code + (size_t)low * g.act.code_stride;
+        off[i] = (uint32_t)(from[i] - low) * (uint32_t)g.act.code_stride;
+        by[i] = 64;
+        walks[i] = ~0u;
       } else {
-        src[i] = g.terms + from * (F::kChunks * 64) + (low ? 64 * c + 16 * part : 64 * c + (lane >> 5) * 32 + (lane & 1) * 16);
-        by[i] = (size_t)g.term_lanes * (F::kChunks * 64);
+        // two pieces of eight lanes, or one of sixteen
+        const int in = 8 * (c % 2) + lane / 8;
+        base[i] = g.terms + (size_t)(c / 2) * (size_t)g.term_lanes * 128;
+        off[i] = F::pair(c) ? (uint32_t)from[i] * 128 + 16 * ((lane & 7) ^ pair_key(in))
+                            : (uint32_t)from[i] * 64 + 16 * ((lane & 3) ^ tile_key(lane >> 2));
+        by[i] = (uint32_t)g.term_lanes * (F::kChunks * 64);
       }
     } else if (id < F::kLaneLoads + F::kRowLoads) {
-      const int r = 16 * (id - F::kLaneLoads) + lane / 4;  // sixteen rows, four pieces each
-      const int block = block0 + r / F::kWaveRows, in = r % F::kWaveRows;
-      const size_t row = row0 + (size_t)tile_row<NT, PAIR>(block, in / 16, in % 16, g.rows);
-      src[i] = g.w.code + row * g.w.code_stride;
-      walk[i] = 64;
-      plus[i] = 16u * (uint32_t)((lane & 3) ^ tile_key(in));
+      const int r = 16 * (id - F::kLaneLoads);  // sixteen rows, four pieces each
+      const int block = block0 + r / F::kWaveRows, j = r % F::kWaveRows / 16;
+      const int low = tile_row<NT, PAIR>(block, j, 0, g.rows), row = tile_row<NT, PAIR>(block, j, lane / 4, g.rows);
+      base[i] = g.w.code + (row0 + (size_t)low) * g.w.code_stride;
+      off[i] = (uint32_t)(row - low) * (uint32_t)g.w.code_stride;
+      by[i] = 64;
+      walks[i] = ~0u;
     } else if (id < F::kLaneLoads + F::kRowLoads + F::kScaleLoads) {
       const int byte = (id - F::kLaneLoads - F::kRowLoads) * 1024 + lane * 16;  // of the blocks' 64 NT bytes each
       const int block = min(block0 + min(byte / (64 * NT), WN - 1), blocks - 1);
-      src[i] = g.row_scales + ((size_t)expert * blocks + block) * (size_t)steps * (64 * NT) + byte % (64 * NT);
+      base[i] = g.row_scales + (size_t)expert * blocks * (size_t)steps * (64 * NT);
+      off[i] = (uint32_t)block * (uint32_t)(steps * (64 * NT)) + byte % (64 * NT);
       by[i] = 64 * NT;
     } else {
       const int byte = (id - F::kLaneLoads - F::kRowLoads - F::kScaleLoads) * 1024 + lane * 16;
       const int block = min(first / 64 + byte / 256, (g.lanes - 1) / 64);
-      src[i] = reinterpret_cast<const uint8_t *>(g.lane_scales) + (size_t)block * steps * 256 + byte % 256;
+      base[i] = reinterpret_cast<const uint8_t *>(g.lane_scales);
+      off[i] = (uint32_t)block * (uint32_t)(steps * 256) + byte % 256;
       by[i] = 256;
     }
   }
-  auto bring = [&](int step, int turn) {
-    uint8_t *dst = lds_x + turn % ST * F::kStage;
-#pragma unroll
-    for (int i = 0; i < F::kLoads; ++i) {
-      const uint8_t *from = src[i] + (size_t)step * by[i] + min((uint32_t)step * walk[i] + plus[i], most);
-      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)from,
-                                       (__attribute__((address_space(3))) void *)(dst + min(wave * F::kLoads + i, F::kAll - 1) * 1024),
-                                       16, 0, 0);
-    }
+  auto bring = [&](int step, int turn, int i) {
+    uint8_t *dst = lds_x + turn % ST * F::kStage + min(wave * F::kLoads + i, F::kAll - 1) * 1024;
+    const uint8_t *const at_step = base[i] + (size_t)min((uint32_t)step, (uint32_t)last_step | ~walks[i]) * by[i];
+    const int most = g.groups - 1 - 4 * min(step, last_step);  // of a step's pieces
+    const uint32_t more = 16u * (uint32_t)min(piece, most) & walks[i];
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)(at_step + (off[i] + more)),
+                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
   };
 
   float4_t acc[MT][NT];
@@ -663,46 +696,53 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
   // two bytes apart, and all at the same column would ask the same cache channels
   const int k_first = blockIdx.z * g.slice, k_end = min(k_first + g.slice, steps), k_count = k_end - k_first;
   int k = k_first + 2 * tile_x % k_count, k_ahead = k;
-  auto bring_next = [&](int turn) {
-    bring(k_ahead, turn);
-    k_ahead = k_ahead + 1 < k_end ? k_ahead + 1 : k_first;
-  };
+  auto next = [&](int at) { return at + 1 < k_end ? at + 1 : k_first; };
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s)
-    if (s < k_count) bring_next(s);
-  for (int s = 0; s < k_count; ++s) {
-    const int k_next = k + 1 < k_end ? k + 1 : k_first;
+    if (s < k_count) {
+#pragma unroll
+      for (int i = 0; i < F::kLoads; ++i) bring(k_ahead, s, i);
+      k_ahead = next(k_ahead);
+    }
+  // A step; its stage `ST - 1` ahead is brought a load after every few products (all at once,
+  // loads hold the wave up while they are taken, and the matrix cores wait)
+  auto step = [&](int s, auto ahead) {
+    constexpr bool kBring = decltype(ahead)::value;
     // lgkmcnt(0), and of this wave's loads all but the ST - 2 stages behind this step's
     constexpr int kBehind = (ST - 2) * F::kLoads;
     static_assert(kBehind < 64, "vmcnt");
-    if (ST > 2 && s + ST - 2 < k_count)
+    if (ST > 2 && (kBring || s + ST - 2 < k_count))
       __builtin_amdgcn_s_waitcnt((kBehind & 15) | (kBehind >> 4) << 14 | 0x0070);
     else
       __builtin_amdgcn_s_waitcnt(0x0070);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + ST - 1 < k_count) bring_next(s + ST - 1);
     const uint8_t *st = lds_x + s % ST * F::kStage;
-    if (!busy) {
-      k = k_next;
-      continue;
+    if (kBring && (!F::kSpread || !busy)) {
+#pragma unroll
+      for (int i = 0; i < F::kLoads; ++i) bring(k_ahead, s + ST - 1, i);
     }
+    if (!busy) return;
     // Lanes' terms behind the last group are zeros, and codes are finite; of microscaled lanes neither side's are
     const uint32_t keep = T != 0 || 4 * k + part < g.groups ? 0xFFFFFFFFu : 0u;
-    int8v_t op[2][T == 0 ? 1 : T];
-    uint2_t scale[2];
+    constexpr int kOps = F::kAhead ? 2 : 1;
+    int8v_t op[kOps][T == 0 ? 1 : T];
+    uint2_t scale[kOps];
     auto read_lanes = [&](int i) {
       const uint8_t *mine = st + (wm * MT + i) * F::kChunks * 1024;
+      uint4_t piece[F::kChunks];
+#pragma unroll
+      for (int c = 0; c < F::kChunks; ++c)
+        piece[c] = *reinterpret_cast<const uint4_t *>(
+            F::pair(c) ? mine + c / 2 * 2048 + at * 128 + 16 * ((4 * (c % 2) + part) ^ pair_key(at))
+                       : mine + c * 1024 + at * 64 + 16 * (part ^ tile_key(at)));
 #pragma unroll
       for (int t = 0; t < (T == 0 ? 1 : T); ++t) {
-        const uint4_t a = *reinterpret_cast<const uint4_t *>(mine + t * 1024 + lane * 16);
-        uint2_t b = {0, 0};
-        if constexpr (T != 0) b = *reinterpret_cast<const uint2_t *>(mine + T * 1024 + t * 512 + (4 * at + part) * 8);
-        op[i & 1][t] = int8v_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], 0, 0};
+        const uint4_t a = piece[t], b = T == 0 ? uint4_t{0, 0, 0, 0} : piece[T == 0 ? 0 : T + t / 2];
+        op[i % kOps][t] = int8v_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[2 * (t % 2)], (int)b[2 * (t % 2) + 1], 0, 0};
       }
-      if constexpr (T != 0)
-        scale[i & 1] = *reinterpret_cast<const uint2_t *>(mine + T * 1024 + T * 512 + (4 * at + part) * 8);
+      if constexpr (T != 0) scale[i % kOps] = uint2_t{piece[F::kChunks - 1][2], piece[F::kChunks - 1][3]};
     };
     int8v_t w[NT];
     uint32_t ws[NT / 4];
@@ -745,24 +785,44 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
     for (int i = 0; i < MT; ++i) {
       // the next lanes' operands are on their way while these are multiplied
       __builtin_amdgcn_sched_barrier(0);
-      if (i + 1 < MT) read_lanes(i + 1);
+      if (F::kAhead && i + 1 < MT) read_lanes(i + 1);
+      if (!F::kAhead && i > 0) read_lanes(i);
       __builtin_amdgcn_sched_barrier(0);
       // a term at a time over the row tiles: products that add to the same sums lie apart
 #pragma unroll
-      for (int t = 0; t < (T == 0 ? 1 : T); ++t)
+      for (int t = 0; t < (T == 0 ? 1 : T); ++t) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           constexpr int kFmt = T == 0 ? 4 : 2;
-          const int a = T == 0 ? ls : (int)scale[i & 1][t / 4];
+          const int a = T == 0 ? ls : (int)scale[i % kOps][t / 4];
           const int byte = T == 0 ? i : t % 4;
-          if (byte == 0) MX4_PRODUCT(i, j, op[i & 1][t], kFmt, 0, a)
-          if (byte == 1) MX4_PRODUCT(i, j, op[i & 1][t], kFmt, 1, a)
-          if (byte == 2) MX4_PRODUCT(i, j, op[i & 1][t], kFmt, 2, a)
-          if (byte == 3) MX4_PRODUCT(i, j, op[i & 1][t], kFmt, 3, a)
+          if (byte == 0) MX4_PRODUCT(i, j, op[i % kOps][t], kFmt, 0, a)
+          if (byte == 1) MX4_PRODUCT(i, j, op[i % kOps][t], kFmt, 1, a)
+          if (byte == 2) MX4_PRODUCT(i, j, op[i % kOps][t], kFmt, 2, a)
+          if (byte == 3) MX4_PRODUCT(i, j, op[i % kOps][t], kFmt, 3, a)
         }
+        constexpr int kRuns = MT * (T == 0 ? 1 : T), kEach = (F::kLoads + kRuns - 1) / kRuns;
+        if (kBring && F::kSpread) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int u = 0; u < kEach; ++u)
+            if ((i * (T == 0 ? 1 : T) + t) * kEach + u < F::kLoads)
+              bring(k_ahead, s + ST - 1, (i * (T == 0 ? 1 : T) + t) * kEach + u);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
     }
 #undef MX4_PRODUCT
-    k = k_next;
+  };
+  int s = 0;
+  for (; s < k_count - (ST - 1); ++s) {
+    step(s, Choice<true>());
+    k = next(k);
+    k_ahead = next(k_ahead);
+  }
+  for (; s < k_count; ++s) {
+    step(s, Choice<false>());
+    k = next(k);
   }
   // every lane took part in the products: nothing of them may move behind a branch that some leave
 #pragma unroll
@@ -801,16 +861,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
         for (int d = 0; d < 4; ++d) x[4 * q + d] = f[d];
       }
       uint8_t *const h = static_cast<uint8_t *>(g.out);
-      const size_t to = (size_t)(first + place);
-      mx4_terms<T == 0 ? 3 : T>(x, h + term_at<T == 0 ? 3 : T>(to, group >> 2, (size_t)g.out_stride), group & 3);
+      const size_t to = (size_t)(first + place), of = (size_t)g.out_stride;
+      constexpr int kTerms = T == 0 ? 3 : T;
+      auto step = [&](int group) { return h + (size_t)(group >> 2) * of * TermForm<kTerms>::kStep; };
+      mx4_terms<kTerms>(x, step(group), to, of, group & 3);
       if (group + 1 == inner_groups)  // the groups behind the last are zeros
-        for (int z = group + 1; z < 4 * mx4_steps(inner_groups); ++z) {
-          uint8_t *step = h + term_at<T == 0 ? 3 : T>(to, z >> 2, (size_t)g.out_stride);
-          for (int u = 0; u <= T; ++u) {
-            if (u < T) *reinterpret_cast<uint4_t *>(step + TermForm<T == 0 ? 3 : T>::low(u, z & 3)) = uint4_t{0, 0, 0, 0};
-            *reinterpret_cast<uint2_t *>(step + TermForm<T == 0 ? 3 : T>::high(u, z & 3)) = uint2_t{0, 0};
-          }
-        }
+        for (int z = group + 1; z < 4 * mx4_steps(inner_groups); ++z)
+          for (int c = 0; c < TermForm<kTerms>::kChunks; ++c)
+            *reinterpret_cast<uint4_t *>(step(z) + term_piece<kTerms>(to, of, c, z & 3)) = uint4_t{0, 0, 0, 0};
     }
     return;
   }
@@ -935,11 +993,13 @@ __global__ __launch_bounds__(256) void mx4_few_kernel(Mx4Args g) {
                                                                     group < g.groups ? c.scale : 0);
       } else {
         // lanes' terms behind the last group are zeros, and codes are finite; their scales may not be
-        const uint8_t *step = g.terms + term_at<T == 0 ? 3 : T>(from, s, (size_t)g.term_lanes);
-        const uint2_t scales = term_scales<T == 0 ? 3 : T>(step, part);
+        constexpr int kTerms = T == 0 ? 3 : T;
+        const size_t of = (size_t)g.term_lanes;
+        const uint8_t *step = g.terms + (size_t)s * of * TermForm<kTerms>::kStep;
+        const uint2_t scales = term_scales<kTerms>(step, from, of, part);
 #pragma unroll
         for (int q = 0; q < T; ++q) {
-          const int8v_t a = term_operand<T == 0 ? 3 : T>(step, q, part);
+          const int8v_t a = term_operand<kTerms>(step, from, of, q, part);
           const int as = q < 4 ? (int)(scales[0] >> (8 * q)) : (int)scales[1];
 #pragma unroll
           for (int r = 0; r < RT; ++r)
@@ -1393,7 +1453,8 @@ static int mx4_slices(int rows, int groups, int lanes, int tile_lanes, int tile_
   const long long tiles = mx4_tiles(rows, lanes, tile_lanes, tile_rows);
   const int steps = mx4_steps(groups);
   int slices = 1;
-  while (tiles * slices < 160 && steps >= 4 * slices && 2LL * slices * lanes * rows <= 1 << 22) slices *= 2;
+  while (tiles * slices < 160 && steps >= 4 * slices && 100000LL * steps >= (long long)slices * slices * lanes * rows)
+    slices *= 2;
   const int each = (steps + slices - 1) / slices;
   return (steps + each - 1) / each;  // none empty
 }
@@ -1441,15 +1502,16 @@ static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int ou
 }
 
 // Which kernels a product of `lanes` takes (terms 0: microscaled lanes).
-enum { kFormFew = 0, kFormHead, kFormSmall, kFormLarge };
+enum { kFormFew = 0, kFormHead, kFormSmall, kFormLarge, kFormWhole };
 
 static int mx4_form(int rows, int groups, int lanes, int terms) {
   const int steps = mx4_steps(groups);
   if (lanes <= 16 && terms != 0 && rows >= 65536) return kFormHead;
-  if ((long long)lanes * steps < (terms == 5 ? 192 : terms == 3 ? 640 : 2048)) return kFormFew;
+  if ((long long)lanes * steps < (terms == 5 ? 192 : terms == 3 ? 640 : 1200)) return kFormFew;
   const long long large = terms == 5   ? mx4_tiles(rows, lanes, 64, 512)
                           : terms == 3 ? mx4_tiles(rows, lanes, 64, 256)
                                        : mx4_tiles(rows, lanes, 128, 256);
+  if (terms == 3 && mx4_tiles(rows, lanes, 128, 512) >= 192) return kFormWhole;
   return large >= 192 ? kFormLarge : kFormSmall;
 }
 
@@ -1500,6 +1562,7 @@ extern "C" hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *a
   if (form == kFormLarge)
     return act_bf16 ? launch_many<3, 2, 4, 2, 4, 2>(a, act, act_stride, out_bf16, room, false, stream)
                     : launch_many<5, 2, 8, 2, 4, 2>(a, act, act_stride, out_bf16, room, false, stream);
+  if (form == kFormWhole) return launch_many<3, 4, 8, 2, 4, 2>(a, act, act_stride, out_bf16, room, false, stream);
   const hipError_t e = launch_terms(act, act_bf16, act_stride, lanes, sheet->col_count, room, stream);
   if (e != hipSuccess) return e;
   if (act_bf16) return out_bf16 ? launch_few<3, kOutBf16>(a, stream) : launch_few<3, kOutF32>(a, stream);
@@ -1680,8 +1743,13 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
                               : step_lds<5>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
                                     step_lds<5>(x->inner / kMx4Group, 1, 1, 8, 1) <= kStepLds);
   if (step) return act_bf16 ? experts_step<3, true>(c, stream) : experts_step<5, false>(c, stream);
-  const bool many = (long long)lanes * top >= 24LL * x->expert_count;
-  if (act_bf16)
-    return many ? experts_grouped<3, 2, 4, 2, 4, 2>(c, stream) : experts_grouped<3, 1, 4, 1, 4, 3>(c, stream);
-  return many ? experts_grouped<5, 2, 4, 2, 4, 2>(c, stream) : experts_grouped<5, 1, 4, 1, 4, 3>(c, stream);
+  const long long each = (long long)slots / x->expert_count;
+  if (act_bf16) {
+    if (each >= 40) return experts_grouped<3, 2, 4, 2, 4, 2>(c, stream);
+    if (each >= 12) return experts_grouped<3, 1, 4, 2, 4, 2>(c, stream);
+    return experts_grouped<3, 1, 4, 1, 4, 3>(c, stream);
+  }
+  if (each >= 40) return experts_grouped<5, 2, 8, 2, 4, 2>(c, stream);
+  if (each >= 12) return experts_grouped<5, 1, 4, 2, 4, 2>(c, stream);
+  return experts_grouped<5, 1, 4, 1, 4, 3>(c, stream);
 }

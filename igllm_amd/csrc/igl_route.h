@@ -30,8 +30,10 @@ struct RouteArgs {
 };
 
 // e^x in double: x = k ln 2 + r, |r| <= 0.35, the series of e^r to the thirteenth power
-// (what is left out is below 2^-57 of it), times 2^k.  x not above 1024; 0 far below.
+// (what is left out is below 2^-57 of it), times 2^k.  x not above 1024; 0 far below, and of
+// a NaN.  No branch: a wave has its experts' exponentials on their way side by side.
 __device__ __forceinline__ double exp_f64(double x) {
+  x = fmax(x, -1100.0);
   const double k = __builtin_rint(x * 1.4426950408889634);
   double r = __builtin_fma(k, -0.69314718036912382, x);  // ln 2 in two pieces, the first of 32 bits: k times it is exact
   r = __builtin_fma(k, -1.9082149292705877e-10, r);
@@ -49,7 +51,7 @@ __device__ __forceinline__ double exp_f64(double x) {
   p = __builtin_fma(p, r, 0.5);
   p = __builtin_fma(p, r, 1.0);
   p = __builtin_fma(p, r, 1.0);
-  return x > -1100.0 ? __builtin_ldexp(p, (int)fmax(k, -1100.0)) : 0.0;
+  return __builtin_ldexp(p, (int)k);
 }
 
 // 1 / d, d in [1, infinity]: the hardware's estimate and two Newton steps.
@@ -128,18 +130,16 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(RouteArgs a) {
     const uint32_t key = wave_max_u32(route_key(top));  // at least minus infinity's
     top = __builtin_bit_cast(float, key >> 31 ? key & 0x7FFFFFFFu : ~key);
   }
-  // s before softmax's division; where the logits decide, only of the chosen
-  auto score = [&](float t) {
-    if (t == -__builtin_inff()) return 0.0;
-    return soft ? exp_f64((double)t - (double)top) : recip_f64(1.0 + exp_f64(fmin(-(double)t, 800.0)));
-  };
+  // s before softmax's division, 0 of minus infinity; where the logits decide, only of the chosen
+  auto share_of = [&](float t) { return exp_f64((double)t - (double)top); };
+  auto sigmoid = [&](float t) { return recip_f64(1.0 + exp_f64(fmin(-(double)t, 800.0))); };
   double s[WIDE ? PER : 1];
   Key key[PER];
   if (soft && (WIDE || !a.rule.renorm)) {
     sum = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const double t = score(v[i]);
+      const double t = share_of(v[i]);
       if constexpr (WIDE) s[i] = t;
       sum += t;
     }
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(RouteArgs a) {
     sum = sum > 0.0 ? sum : 1.0;
   } else if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = score(v[i]);
+    for (int i = 0; i < PER; ++i) s[i] = sigmoid(v[i]);
   }
   if constexpr (WIDE) {
     const double inverse = soft ? 1.0 / sum : 1.0;
@@ -243,7 +243,10 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(RouteArgs a) {
     if (lane == j) mine = PER * from + slot, share = taken;
   }
   if constexpr (!WIDE) {
-    if (mine >= 0) share = score(fminf(x[mine], 3.402823466e38f)) / sum;
+    if (mine >= 0) {
+      const float t = fminf(x[mine], 3.402823466e38f);
+      share = soft ? share_of(t) / sum : sigmoid(t);
+    }
     total = share;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
@@ -254,6 +257,192 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(RouteArgs a) {
   if (a.gain && mine >= 0) share *= (double)a.gain[mine];
   a.pick[m * a.rule.top + lane] = mine;
   a.weight[m * a.rule.top + lane] = mine >= 0 ? (float)share : 0.0f;
+}
+
+// The largest, or least, of each row of sixteen wave lanes, in all of them.
+__device__ __forceinline__ uint32_t row_max_u32(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t row_min_u32(uint32_t v) { return ~row_max_u32(~v); }
+
+// Many lanes of a batch: four a wave, sixteen wave lanes each, so that a round of the choice
+// serves four.  Wave lane l of a row holds experts 64 q + 4 l + 0 .. 3, a quad each
+// of PER / 4.  E a multiple of four, sixteen choices and groups at most.
+template <int PER, bool WIDE>
+__global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteArgs a) {
+  using Key = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
+  __shared__ double room[WIDE ? kRouteWaves : 1][WIDE ? 64 * PER : 1];  // choices, then scores, of four rows
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, row = lane >> 4;
+  const long long m0 = ((long long)blockIdx.x * kRouteWaves + wave) * 4;
+  if (m0 >= a.lanes) return;  // a wave's own from here on, no barrier
+  const long long m = min(m0 + row, (long long)a.lanes - 1);
+  const int E = a.rule.expert_count;
+  const float *x = a.logits + m * a.logit_stride;
+  const double none = -__builtin_inf();
+  struct __attribute__((packed)) Quad {
+    float v[4];
+  };
+  auto load = [&](const float *from, float (&to)[PER]) {
+#pragma unroll
+    for (int q = 0; q < PER / 4; ++q) {
+      const Quad f = *reinterpret_cast<const Quad *>(from + min(64 * q + 4 * l, E - 4));
+#pragma unroll
+      for (int d = 0; d < 4; ++d) to[4 * q + d] = f.v[d];
+    }
+  };
+  auto expert = [&](int i) { return 64 * (i / 4) + 4 * l + i % 4; };
+  float v[PER], bias[WIDE ? PER : 4] = {};
+  load(x, v);
+  if constexpr (WIDE)
+    if (a.bias) load(a.bias, bias);
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (expert(i) >= E || !(v[i] >= -3.402823466e38f)) v[i] = -__builtin_inff();  // a NaN is never chosen
+    v[i] = fminf(v[i], 3.402823466e38f);
+    top = fmaxf(top, v[i]);
+  }
+  const bool soft = a.rule.score == IGL_ROUTE_SOFTMAX;
+  if (soft) {
+    const uint32_t key = row_max_u32(route_key(top));
+    top = __builtin_bit_cast(float, key >> 31 ? key & 0x7FFFFFFFu : ~key);
+  }
+  auto share_of = [&](float t) { return exp_f64((double)t - (double)top); };
+  auto sigmoid = [&](float t) { return recip_f64(1.0 + exp_f64(fmin(-(double)t, 800.0))); };
+  double s[WIDE ? PER : 1], sum = 1.0;
+  Key key[PER];
+  if (soft && (WIDE || !a.rule.renorm)) {
+    double of_all = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const double t = share_of(v[i]);
+      if constexpr (WIDE) s[i] = t;
+      of_all += t;
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) of_all += __shfl_xor(of_all, d);
+    sum = of_all > 0.0 ? of_all : 1.0;
+  } else if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = sigmoid(v[i]);
+  }
+  if constexpr (WIDE) {
+    double *const mine = room[wave] + row * 16 * PER;
+    const double inverse = 1.0 / sum;
+    double c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      s[i] *= inverse;
+      c[i] = v[i] == -__builtin_inff() ? none : s[i] + (double)bias[i];
+      if (!(c[i] > none)) c[i] = none;  // and a bias that is a NaN
+    }
+    uint32_t kept = ~0u;
+    if (a.rule.group_count > 1) {
+      const int G = a.rule.group_count, each = E / G;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) mine[expert(i)] = c[i];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      // a group's two largest, by `split` wave lanes, which begin at different experts
+      const int split = G <= 2 ? 8 : G <= 4 ? 4 : G <= 8 ? 2 : 1;
+      const int group = l / split, part = l % split, n = (each - part + split - 1) / split;
+      double most = none, second = none;
+      if (group < G && n > 0) {
+        int at = lane % n;
+        for (int i = 0; i < n; ++i) {
+          const double t = mine[group * each + part + split * at];
+          at = at + 1 < n ? at + 1 : 0;
+          second = fmax(second, fmin(most, t));
+          most = fmax(most, t);
+        }
+      }
+      for (int d = 1; d < split; d *= 2) {
+        const double other = __shfl_xor(most, d), other_second = __shfl_xor(second, d);
+        second = fmax(fmin(most, other), fmax(second, other_second));
+        most = fmax(most, other);
+      }
+      double score_of = a.rule.group_best == 2 && second > none ? most + second : most;
+      score_of = __shfl(score_of, 16 * row + min(l * split, 15));
+      if (l >= G) score_of = none;
+      // a group stays if fewer than group_top come before it
+      int ahead = 0;
+      for (int q = 0; q < G; ++q) {
+        const double other = __shfl(score_of, 16 * row + q);
+        ahead += other > score_of || (other == score_of && q < l);
+      }
+      kept = (uint32_t)(__ballot(ahead < a.rule.group_top && score_of > none) >> (16 * row)) & 0xFFFFu;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine[expert(i)] = s[i];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool in = a.rule.group_count == 1 || (kept >> ((uint32_t)expert(i) * a.each_inverse >> 20 & 31) & 1);
+      key[i] = in && c[i] > none ? route_key(c[i]) : 0;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = v[i] == -__builtin_inff() ? 0 : route_key(v[i]);
+  }
+  // the best, one at a time, by upper words; wave lane j of a row keeps the j-th's
+  auto high = [](Key k) { return WIDE ? (uint32_t)((uint64_t)k >> 32) : (uint32_t)k; };
+  int chosen = -1;
+  for (int j = 0; j < a.rule.top; ++j) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) word = max(word, high(key[i]));
+    const uint32_t most = row_max_u32(word);
+    uint32_t at = ~0u;
+    int holders = 0;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; --i) {
+      const bool holds = high(key[i]) == most;
+      at = holds ? 64 * (i / 4) + i % 4 : at;
+      if (WIDE) holders += __builtin_popcountll(__ballot(holds));
+    }
+    if (WIDE && holders > 4) {  // upper words are seldom equal
+      uint32_t low = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) low = max(low, high(key[i]) == most ? (uint32_t)key[i] : 0u);
+      const uint32_t rest = row_max_u32(low);
+      at = ~0u;
+#pragma unroll
+      for (int i = PER - 1; i >= 0; --i) at = high(key[i]) == most && (uint32_t)key[i] == rest ? 64 * (i / 4) + i % 4 : at;
+    }
+    const int e = (int)row_min_u32(at != ~0u ? at + 4 * l : ~0u);  // of equal ones the lowest
+    if (__ballot(most > 0) == 0) break;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (e - 4 * l == 64 * (i / 4) + i % 4) key[i] = 0;
+    if (l == j && most > 0) chosen = e;
+  }
+  double share = 0.0, total;
+  if (chosen >= 0) {
+    const float t = fminf(x[chosen], 3.402823466e38f);
+    share = WIDE ? room[wave][WIDE ? row * 16 * PER + chosen : 0] : soft ? share_of(t) / sum : sigmoid(t);
+  }
+  total = share;
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) total += __shfl_xor(total, d);
+  if (l >= a.rule.top || m0 + row >= a.lanes) return;
+  if (a.rule.renorm) share = total > 0.0 ? share / total : 0.0;
+  share *= (double)a.rule.gain_scale;
+  if (a.gain && chosen >= 0) share *= (double)a.gain[chosen];
+  a.pick[m * a.rule.top + l] = chosen;
+  a.weight[m * a.rule.top + l] = chosen >= 0 ? (float)share : 0.0f;
+}
+
+template <int PER>
+static hipError_t launch_route_rows(const RouteArgs &a, hipStream_t stream) {
+  const dim3 grid((unsigned)((a.lanes + 4 * kRouteWaves - 1) / (4 * kRouteWaves))), block(64 * kRouteWaves);
+  if (a.bias || a.rule.group_count > 1)
+    hipLaunchKernelGGL((route_rows_kernel<PER, true>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((route_rows_kernel<PER, false>), grid, block, 0, stream, a);
+  return hipGetLastError();
 }
 
 template <int PER>
@@ -274,6 +463,10 @@ extern "C" hipError_t igl_launch_route(const igl_route *rule, const float *logit
   const int each = rule->expert_count / rule->group_count;
   const igl::RouteArgs a = {*rule, logits, logit_stride, lanes, bias, gain, pick, weight,
                             (uint32_t)(((1 << 20) + each - 1) / each)};
+  if (lanes >= 2048 && rule->expert_count % 4 == 0 && rule->expert_count <= 256 && rule->top <= 16 && rule->group_count <= 16)
+    return rule->expert_count <= 64    ? igl::launch_route_rows<4>(a, stream)
+           : rule->expert_count <= 128 ? igl::launch_route_rows<8>(a, stream)
+                                       : igl::launch_route_rows<16>(a, stream);
   const int per = (rule->expert_count + 63) / 64;
   return per <= 1   ? igl::launch_route<1>(a, stream)
          : per <= 2 ? igl::launch_route<2>(a, stream)

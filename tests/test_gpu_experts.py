@@ -69,9 +69,26 @@ def test_route(backend, r, count, lanes, biased):
     check_route(backend, logits, r, bias, gain, lanes % 2)
 
 
-@pytest.mark.parametrize("r,count", RULES)
+# four lanes of a batch a wave: up to 256 experts, a multiple of four, and sixteen choices and groups
+MANY = RULES + [({"top": 16, "score": "sigmoid", "groups": 16, "kept": 9, "best": 2}, 256), ({"top": 1, "score": "sigmoid"}, 4),
+                ({"top": 7, "score": "softmax", "groups": 7, "kept": 3, "best": 2}, 84),
+                ({"top": 9, "score": "softmax", "groups": 2, "kept": 1, "best": 1, "renorm": 0}, 20)]
+
+
+@pytest.mark.parametrize("r,count", MANY)
 @pytest.mark.parametrize("biased", [False, True])
-def test_route_of_equal_and_of_no_numbers(backend, r, count, biased):
+def test_route_of_many_lanes(backend, r, count, biased):
+    rng = np.random.default_rng(count + 1)
+    logits = (1.5 * rng.normal(size=(2051, count))).astype(np.float32)
+    bias = (0.1 * rng.normal(size=count)).astype(np.float32) if biased else None
+    gain = rng.uniform(0.5, 2, size=count).astype(np.float32) if biased else None
+    check_route(backend, logits, r, bias, gain, 1)
+
+
+@pytest.mark.parametrize("r,count", MANY)
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("times", [1, 35])
+def test_route_of_equal_and_of_no_numbers(backend, r, count, biased, times):
     """Equal scores, masked experts, infinities and NaN: few values, many ties."""
     rng = np.random.default_rng(count)
     logits = rng.integers(-2, 3, size=(60, count)).astype(np.float32)
@@ -91,7 +108,7 @@ def test_route_of_equal_and_of_no_numbers(backend, r, count, biased):
         bias[rng.random(count) < 0.1] = np.nan
     if r["score"] == "softmax":  # sums of unequal scores can be equal in one order of adding and not in another
         logits = np.where(np.isfinite(logits) & (logits > -3e38), 0, logits).astype(np.float32) if biased or r.get("groups", 1) > 1 else logits
-    check_route(backend, logits, r, bias)
+    check_route(backend, np.tile(logits, (times, 1)), r, bias)
 
 
 def test_route_next_to_each_other(backend):
@@ -99,7 +116,8 @@ def test_route_next_to_each_other(backend):
     rng = np.random.default_rng(4)
     base = rng.uniform(0.5, 1.5, size=(100, 1)).astype(np.float32)
     logits = (base.view(np.int32) + rng.permuted(np.tile(np.arange(48, dtype=np.int32), (100, 1)), axis=1)).view(np.float32)
-    for score in ("softmax", "sigmoid"):
+    for score, times in (("softmax", 1), ("sigmoid", 1), ("softmax", 21), ("sigmoid", 21)):
+        logits = np.tile(logits[:100], (times, 1))
         check_route(backend, logits, {"top": 8, "score": score})
         bias = (np.float32(0.125).view(np.int32) + rng.permutation(48).astype(np.int32)).view(np.float32)
         check_route(backend, logits, {"top": 8, "score": score}, bias)

@@ -969,8 +969,8 @@ static int mx4_good(const igl_mx4 *s) {
          s->code_stride >= (size_t)s->col_count / 2 && s->scale_stride >= (size_t)s->col_count / 32;
 }
 
-/* Kernels count a wave's rows (128) in 32 bits. */
-static int mx4_wide(const igl_mx4 *s) { return s->code_stride > (size_t)1 << 24; }
+/* Products count the bytes of sixteen rows in 32 bits, and have 256 threads for them. */
+static int mx4_wide(const igl_mx4 *s) { return s->code_stride > (size_t)1 << 24 || s->row_count > 1 << 27; }
 
 static int mx4_span_good(const igl_mx4 *s, int first, int count) {
   return mx4_good(s) && first >= 0 && count >= 1 && first <= s->row_count - count;

@@ -167,7 +167,7 @@ struct TermForm {
 
 // Where group `part` of piece c begins in a step of `lanes` lanes.
 template <int T>
-__device__ __forceinline__ size_t term_piece(size_t lane, size_t lanes, int c, int part) {
+__host__ __device__ __forceinline__ size_t term_piece(size_t lane, size_t lanes, int c, int part) {
   constexpr int kChunks = TermForm<T>::kChunks;
   return (size_t)(c / 2) * lanes * 128 + (c + 1 < kChunks || c % 2 ? lane * 128 + 64 * (c % 2) : lane * 64) + 16 * part;
 }
@@ -451,10 +451,10 @@ struct TileForm {
 // together meet all banks: these are not sixteen in a row but 0-3, 12-15 and 20-27, and
 // 4-11, 16-19 and 28-31 (keys 0, 1, 2, 3 cost four cycles more a read, by the counter of
 // bank conflicts).
-__device__ __forceinline__ int tile_key(int row) { return 0x78 >> (row >> 1 & 6) & 3; }
+__host__ __device__ __forceinline__ int tile_key(int row) { return 0x78 >> (row >> 1 & 6) & 3; }
 
 // The same of a lane's two pieces of terms, 128 bytes.
-__device__ __forceinline__ int pair_key(int lane) { return lane >> 1 & 7; }
+__host__ __device__ __forceinline__ int pair_key(int lane) { return lane >> 1 & 7; }
 
 // Row of tile j of a wave's block of 16 NT rows, of `rows` in all (clamped).
 template <int NT, bool PAIR>
@@ -663,15 +663,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
       walks[i] = ~0u;
     } else if (id < F::kLaneLoads + F::kRowLoads + F::kScaleLoads) {
       const int byte = (id - F::kLaneLoads - F::kRowLoads) * 1024 + lane * 16;  // of the blocks' 64 NT bytes each
-      const int block = min(block0 + min(byte / (64 * NT), WN - 1), blocks - 1);
-      base[i] = g.row_scales + (size_t)expert * blocks * (size_t)steps * (64 * NT);
-      off[i] = (uint32_t)block * (uint32_t)(steps * (64 * NT)) + byte % (64 * NT);
+      const int low = min(block0, blocks - 1), block = min(block0 + min(byte / (64 * NT), WN - 1), blocks - 1);
+      base[i] = g.row_scales + ((size_t)expert * blocks + low) * (size_t)steps * (64 * NT);
+      off[i] = (uint32_t)(block - low) * (uint32_t)(steps * (64 * NT)) + byte % (64 * NT);
       by[i] = 64 * NT;
     } else {
       const int byte = (id - F::kLaneLoads - F::kRowLoads - F::kScaleLoads) * 1024 + lane * 16;
-      const int block = min(first / 64 + byte / 256, (g.lanes - 1) / 64);
-      base[i] = reinterpret_cast<const uint8_t *>(g.lane_scales);
-      off[i] = (uint32_t)block * (uint32_t)(steps * 256) + byte % 256;
+      const int low = first / 64, block = min(low + byte / 256, (g.lanes - 1) / 64);
+      base[i] = reinterpret_cast<const uint8_t *>(g.lane_scales) + (size_t)low * (size_t)steps * 256;
+      off[i] = (uint32_t)(block - low) * (uint32_t)(steps * 256) + byte % 256;
       by[i] = 256;
     }
   }
@@ -1474,19 +1474,23 @@ static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int ou
   p.terms = work;
   p.lane_scales = PackArgs{a.act, a.lanes, a.groups, 1, 0, work};
   p.rows = PackArgs{a.w, a.rows, a.groups, 1, 0, work + lanes_bytes};
+  const size_t sums = lanes_bytes + pack_bytes<NT, false>(a.rows, a.groups, 1);
+  const int tiles = (a.lanes + F::kLanes - 1) / F::kLanes;
+  const int slices = slice ? mx4_slices(a.rows, a.groups, a.lanes, F::kLanes, F::kRows) : 1;
+  if (sums + (slices > 1 ? (size_t)slices * a.lanes * a.rows * sizeof(float) : 0) >
+      igl_mx4_work_bytes(a.rows, a.groups * kMx4Group, a.lanes, T))
+    return hipErrorInvalidValue;
   const hipError_t e = launch_prepare<T, NT>(p, stream);
   if (e != hipSuccess) return e;
   a.terms = work;
   a.term_lanes = a.lanes;
   a.lane_scales = reinterpret_cast<const uint32_t *>(work);
   a.row_scales = work + lanes_bytes;
-  const int tiles = (a.lanes + F::kLanes - 1) / F::kLanes;
-  const int slices = slice ? mx4_slices(a.rows, a.groups, a.lanes, F::kLanes, F::kRows) : 1;
   if (slices == 1)
     return out_bf16 ? launch_tile<T, MT, NT, WM, WN, ST, kOutBf16>(a, tiles, 1, stream)
                     : launch_tile<T, MT, NT, WM, WN, ST, kOutF32>(a, tiles, 1, stream);
   Mx4Args b = a;
-  b.out = work + lanes_bytes + pack_bytes<NT, false>(a.rows, a.groups, 1);
+  b.out = work + sums;
   b.out_stride = a.rows;
   b.slice_out = (size_t)a.lanes * a.rows;
   const hipError_t f = launch_tile<T, MT, NT, WM, WN, ST, kOutF32>(b, tiles, slices, stream);

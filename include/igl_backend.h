@@ -334,16 +334,16 @@ int igl_mx4_lay_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row
 int igl_mx4_read_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row_count,
                      void *dst_dev, int dst_type, int dst_stride);
 /* igl_mat_mat_dev for a microscaled sheet: out[m] = sheet x[m], lanes of act_type to
- * lanes of out_type (F32 or BF16), sums in 32 bits.  F32 lanes are taken to 2^-24
- * and BF16 lanes to 2^-14 of the largest of their 32 values (a bf16 output has 2^-8);
+ * lanes of out_type (F32 or BF16), sums in 32 bits.  F32 lanes are taken to
+ * 2^-23.9 and BF16 lanes to 2^-13.9 of the largest of their 32 values (a bf16 output has 2^-8);
  * neither finer than 2^-130 and 2^-120.  A lane with an infinity or a NaN has NaN
- * outputs.  Lanes are cut into terms in the desk's workspace, which grows
- * to lanes * col_count * 4 bytes (2.5 for BF16): call it once before recording. */
+ * outputs.  out and act do not overlap.  Sheets of code_stride up to 2^24 and 2^27 rows,
+ * 1048560 lanes.  The desk's workspace grows with the call's lanes and, from a few of
+ * them on, with the sheet: make the calls of a recording once before it. */
 int igl_mx4_mat_mat_dev(igl_desk *desk, const igl_mx4 *sheet, const void *act_dev, int act_type,
                         int act_stride, int lane_count, void *out_dev, int out_type,
                         int out_stride);
-/* The same for lanes that are microscaled rows, act's lane_first .. + lane_count - 1;
- * no workspace. */
+/* The same for lanes that are microscaled rows, act's lane_first .. + lane_count - 1. */
 int igl_mx4_mat_mx4_dev(igl_desk *desk, const igl_mx4 *sheet, const igl_mx4 *act, int lane_first,
                         int lane_count, void *out_dev, int out_type, int out_stride);
 
@@ -392,8 +392,10 @@ typedef struct igl_experts {
 /* out[m] = sum_j weight[m][j] down_e(gate(gate_e x[m]) * up_e x[m]), e = pick[m][j], j
  * in rising order: igl_route_dev's picks and weights, [lane_count][top].  A pick
  * outside 0 .. expert_count - 1 takes no expert; a lane without one is zero.  Lanes and
- * their precision as igl_mx4_mat_mat_dev's.  The desk's workspace grows with the
- * call's size: call it once before recording. */
+ * their precision as igl_mx4_mat_mat_dev's; out and act do not overlap.  1024 experts
+ * at most and 64 a lane, lane_count * top times hidden, or inner, below 2^32 - 2048, and
+ * lane_count * top / 16 + expert_count below 65536.  The desk's workspace grows with
+ * the call's size: make the calls of a recording once before it. */
 int igl_experts_dev(igl_desk *desk, const igl_experts *experts, const void *act_dev, int act_type,
                     int act_stride, int lane_count, const int32_t *pick_dev,
                     const float *weight_dev, int top, void *out_dev, int out_type, int out_stride);

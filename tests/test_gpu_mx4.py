@@ -4,8 +4,10 @@ products, against their definitions in 64 bits (mx4_oracle).
 Codes and scales are decided exactly: every byte equal, bytes of other rows and
 between rows untouched.  A read value is exact.
 
-Bar of a product, from the arithmetic.  A lane's group is held to e = 2^-24 (fp32
-lanes) or 2^-14 (bf16 lanes) of its largest value, so an output is off by
+Bar of a product, from the arithmetic.  A lane's group is held to e = 2^-23 / 1.875
+(fp32 lanes) or 2^-13 / 1.875 (bf16 lanes) of its largest value: the largest lies
+above 1.875 of its scale, and what five terms leave is at most half the widest step,
+1/8, of the last, 2^-20 of the first's (test_mx4_terms); so an output is off by
 e * sum |w| top(group); the sums are fp32 adds, sixteen an instruction and an
 instruction for every 128 columns and term, each off by 2^-24 of what it holds,
 at most 1.1 sum |w x| (the terms together are no larger than x by a sixteenth).
@@ -23,7 +25,7 @@ pytestmark = pytest.mark.gpu
 
 F32, BF16 = native.IGL_STORE_F32, native.IGL_STORE_BF16
 TERMS = {F32: 5, BF16: 3}
-HELD = {F32: 2.0 ** -24, BF16: 2.0 ** -14}
+HELD = {F32: 2.0 ** -23 / 1.875, BF16: 2.0 ** -13 / 1.875}
 
 
 class At:
@@ -149,7 +151,9 @@ def bar(x, w, kind, out_kind, want):
 SHAPES = [(1, 16, 32), (1, 1, 64), (1, 6144, 1536), (2, 50, 96), (3, 33, 128), (4, 200, 160), (5, 1000, 2080),
           (6, 77, 8192), (7, 130, 544), (8, 64, 256), (13, 17, 1536), (16, 48, 384), (17, 47, 416), (31, 300, 224),
           (37, 257, 8192), (63, 129, 704), (64, 256, 512), (65, 100, 1056), (100, 520, 768), (129, 1030, 96),
-          (300, 1537, 1536), (517, 272, 320), (1000, 300, 2048)]
+          (300, 1537, 1536), (517, 272, 320), (1000, 300, 2048),
+          # a head; tiles of many lanes and rows, the last of either not full
+          (4, 65552, 96), (16, 65601, 288), (500, 6150, 64), (1000, 6201, 96), (1540, 7690, 160)]
 
 
 @pytest.mark.parametrize("lanes,rows,cols", SHAPES)
@@ -345,6 +349,46 @@ def test_quantised_round_trip_of_what_was_read(backend):
         values.append(mx.values(code.reshape(rows, -1), scale.reshape(rows, -1)))
     assert np.array_equal(*values)
     close(a, b, x, back)
+
+
+@pytest.mark.parametrize("lanes", [1, 5, 40])
+def test_rows_past_32_bits(backend, lanes):
+    """Rows 16 MiB apart, the last beyond 4 GiB, of a sheet, of lanes and of outputs."""
+    rows, cols, far = 272, 96, 1 << 24
+    rng = np.random.default_rng(lanes)
+    w, a = sheet(rng, rows, cols), sheet(rng, rows, cols)
+    code, scale = backend.alloc(rows * far), backend.upload(w[1])
+    for n in range(rows):
+        code.put(w[0][n], n * far)
+    held = backend.mx4(rows, cols, code, scale, far, cols // 32)
+    x, wv = mx.bf16(rng.normal(size=(rows, cols))), mx.values(*w)
+    at = rows - lanes  # the last rows
+    # the sheet's, and as microscaled lanes
+    act, out = put(backend, x[:lanes], F32), backend.alloc(4 * lanes * rows)
+    backend.mx4_mat_mat_dev(held, act, F32, cols, lanes, out, F32, rows)
+    want = x[:lanes].astype(np.float64) @ wv.T
+    assert (np.abs(get(out, (lanes, rows), F32) - want) <= bar(x[:lanes], wv, F32, F32, want)).all()
+    other = hold(backend, *a)
+    backend.mx4_mat_mx4_dev(other, held, at, lanes, out, F32, rows)
+    av = mx.values(*a)
+    want = wv[at:] @ av.T
+    assert (np.abs(get(out, (lanes, rows), F32) - want) <= bar(wv[at:], av, None, F32, want)).all()
+    # laid and read there
+    backend.mx4_lay_dev(held, at, lanes, act, F32, cols)
+    back = backend.alloc(4 * lanes * cols)
+    backend.mx4_read_dev(held, at, lanes, back, F32, cols)
+    laid = mx.quantise(x[:lanes])
+    assert np.array_equal(get(back, (lanes, cols), F32), mx.values(mx.pack(laid[0]), laid[1]).astype(np.float32))
+    close(out, back, act, scale)
+    # lanes and outputs as far apart: the same memory, as floats
+    wide = far // 4
+    for n in range(rows):
+        code.put(x[n], n * far)
+    backend.mx4_mat_mat_dev(other, At(code, at * far), F32, wide, lanes, At(code, at * far + (1 << 20)), F32, wide)
+    want = x[at:].astype(np.float64) @ av.T
+    got = np.stack([code.get(np.float32, rows, (at + m) * far + (1 << 20)) for m in range(lanes)])
+    assert (np.abs(got - want) <= bar(x[at:], av, F32, F32, want)).all()
+    close(code, other)
 
 
 def test_unaligned_lanes(backend):

@@ -1173,6 +1173,155 @@ __global__ __launch_bounds__(256) void mx4_step_kernel(Mx4Args g) {
   }
 }
 
+// Up to sixteen lanes of floats of a sheet of many rows (a vocabulary), bound by its bytes:
+// workgroups that stay, a wave sixteen rows at a time, the next rows' codes and scales on
+// their way to registers while these are multiplied.  Lanes' terms are columns of
+// operands (five lanes of fp32 two), cut by the workgroup and kept in LDS as they are
+// read; sums cross LDS to be added and stored.
+constexpr int kHeadWaves = 8;
+constexpr int kHeadSteps = 4;  // of a piece: sixteen scales of a row
+constexpr int kHeadAhead = 6;  // pieces of a wave on their way
+
+template <int T>
+struct HeadForm {
+  static constexpr int kImage = 64 * 28;  // bytes of an operand: sixteen a wave lane, eight, a scale
+  static int operands(int lanes) { return (lanes * T + 15) / 16; }
+  static size_t sums(int lanes) { return (size_t)kHeadWaves * 16 * (16 * operands(lanes) + 1) * sizeof(float); }
+  static size_t lds(int groups, int lanes) { return (size_t)operands(lanes) * mx4_steps(groups) * kImage + sums(lanes); }
+};
+
+// A piece of sixteen rows: codes, a group a wave lane and step, and the scales of its row.
+struct HeadPiece {
+  uint4_t code[kHeadSteps], scale;
+};
+
+template <int T, int OPERANDS, int OUT, bool BF16>
+__global__ __launch_bounds__(64 * kHeadWaves, 2) void mx4_head_kernel(Mx4Args g) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_x[];
+  constexpr int kImage = HeadForm<T>::kImage, kPitch = 16 * OPERANDS + 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int part = lane >> 4, at = lane & 15;
+  const int steps = mx4_steps(g.groups), pieces = (steps + kHeadSteps - 1) / kHeadSteps;
+  const int blocks = (g.rows + 15) / 16, stride = gridDim.x * kHeadWaves;
+  float *const sums = reinterpret_cast<float *>(lds_x + (size_t)OPERANDS * steps * kImage) + wave * 16 * kPitch;
+  HeadPiece ring[kHeadAhead];
+  auto load = [&](HeadPiece &r, int block, int piece) {  // no branch: what lies behind is a row's last, and cleared
+    const size_t row = (size_t)min(16 * block + at, g.rows - 1);
+    const uint8_t *code = g.w.code + row * g.w.code_stride, *scale = g.w.scale + row * g.w.scale_stride;
+#pragma unroll
+    for (int s = 0; s < kHeadSteps; ++s)
+      r.code[s] =
+          *reinterpret_cast<const uint4_t *>(code + 16 * (size_t)min(4 * (piece * kHeadSteps + s) + part, g.groups - 1));
+    struct __attribute__((packed)) Words {
+      uint32_t w[4];
+    };
+    const Words b = *reinterpret_cast<const Words *>(scale + min(16 * piece, g.groups - 16));
+    r.scale = uint4_t{b.w[0], b.w[1], b.w[2], b.w[3]};
+  };
+  int block = blockIdx.x * kHeadWaves + wave;
+  int ahead = block, ahead_piece = 0, piece = 0;
+  auto load_next = [&](HeadPiece &r) {
+    load(r, min(ahead, blocks - 1), ahead_piece);
+    if (++ahead_piece == pieces) ahead_piece = 0, ahead += stride;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeadAhead; ++i) load_next(ring[i]);
+  // the lanes' operands; columns that no term has hold anything
+  for (int i = threadIdx.x; i < g.lanes * 4 * steps; i += 64 * kHeadWaves) {
+    const int m = i / (4 * steps), group = i - m * 4 * steps;
+    const void *row = static_cast<const uint8_t *>(g.act_rows) + (size_t)m * (size_t)g.act_stride * (BF16 ? 2 : 4);
+    float x[32];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      if (group < g.groups) mx4_load8<BF16>(row, 32 * (size_t)group + 8 * e, v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[8 * e + q] = v[q];
+    }
+    auto image = [&](int t) { return lds_x + (size_t)((m * T + t) / 16 * steps + group / 4) * kImage; };
+    auto slot = [&](int t) { return group % 4 * 16 + (m * T + t) % 16; };
+    mx4_cut<T>(
+        x,
+        [&](int t, const uint6_t &w) {
+          *reinterpret_cast<uint4_t *>(image(t) + 16 * slot(t)) = uint4_t{w[0], w[1], w[2], w[3]};
+          *reinterpret_cast<uint2_t *>(image(t) + 1024 + 8 * slot(t)) = uint2_t{w[4], w[5]};
+        },
+        [&](const uint2_t &s) {
+#pragma unroll
+          for (int t = 0; t < T; ++t)
+            *reinterpret_cast<uint32_t *>(image(t) + 1536 + 4 * slot(t)) = t < 4 ? s[0] >> (8 * t) : s[1];
+        });
+  }
+  __syncthreads();
+  float4_t acc[OPERANDS];
+  auto multiply = [&](HeadPiece &r, int piece) {
+    // a row's last sixteen scales, where its last piece has fewer, moved down to where they belong
+    int late = 16 * piece - min(16 * piece, g.groups - 16);
+    if (late) {
+      for (; late >= 4; late -= 4) r.scale = uint4_t{r.scale[1], r.scale[2], r.scale[3], 0u};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        r.scale[i] = (uint32_t)(((uint64_t)(i < 3 ? r.scale[i + 1] : 0u) << 32 | r.scale[i]) >> (8 * late));
+    }
+#pragma unroll
+    for (int s = 0; s < kHeadSteps; ++s) {
+      const int step = piece * kHeadSteps + s;
+      if (step >= steps) break;
+      const bool in = 4 * step + part < g.groups;
+      const uint4_t c = in ? r.code[s] : uint4_t{0, 0, 0, 0};
+      const int8v_t w = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+      const int ws = (int)(r.scale[s] >> (8 * part));  // zeros behind the last
+#pragma unroll
+      for (int q = 0; q < OPERANDS; ++q) {
+        const uint8_t *image = lds_x + (size_t)(q * steps + step) * kImage;
+        const uint4_t a = *reinterpret_cast<const uint4_t *>(image + 16 * lane);
+        const uint2_t b = *reinterpret_cast<const uint2_t *>(image + 1024 + 8 * lane);
+        const int as = *reinterpret_cast<const int *>(image + 1536 + 4 * lane);
+        const int8v_t op = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], 0, 0};
+        acc[q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, op, acc[q], 4, 2, 0, ws, 0, as);
+      }
+    }
+  };
+  auto store = [&](int of) {
+#pragma unroll
+    for (int q = 0; q < OPERANDS; ++q) {
+      asm volatile("" : "+v"(acc[q]));  // every lane took part in the products, as in mx4_few_kernel
+#pragma unroll
+      for (int d = 0; d < 4; ++d) sums[(4 * part + d) * kPitch + 16 * q + at] = acc[q][d];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own, no barrier
+    for (int i = lane; i < 16 * g.lanes; i += 64) {
+      const int m = i / 16, n = 16 * of + i % 16;
+      float v = 0.0f;
+#pragma unroll
+      for (int t = T - 1; t >= 0; --t) v += sums[i % 16 * kPitch + m * T + t];
+      if (n >= g.rows) continue;
+      const size_t out = (size_t)m * (size_t)g.out_stride + n;
+      if (OUT == kOutBf16)
+        static_cast<uint16_t *>(g.out)[out] = float_bf16(v);
+      else
+        static_cast<float *>(g.out)[out] = v;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  while (block < blocks) {
+#pragma unroll
+    for (int i = 0; i < kHeadAhead; ++i) {
+      if (block >= blocks) break;
+      if (piece == 0)
+#pragma unroll
+        for (int q = 0; q < OPERANDS; ++q) acc[q] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      multiply(ring[i], piece);
+      load_next(ring[i]);
+      if (++piece == pieces) {
+        store(block);
+        piece = 0;
+        block += stride;
+      }
+    }
+  }
+}
+
 // The down products of a token's experts and their sum: blockIdx.y a lane, eight waves, each
 // every eighth of its choices (its hidden values cut by the wave), sixteen rows.
 template <int T, bool BF16>
@@ -1443,6 +1592,24 @@ static hipError_t launch_step(const Mx4Args &a, dim3 grid, int lanes, hipStream_
   return hipGetLastError();
 }
 
+constexpr size_t kHeadLds = 156 * 1024;
+
+template <int T, int OPERANDS, bool BF16>
+static hipError_t launch_head(const Mx4Args &a, int out_bf16, hipStream_t stream) {
+  static size_t granted = 0, granted16 = 0;
+  const dim3 grid(min(256, ((a.rows + 15) / 16 + kHeadWaves - 1) / kHeadWaves)), block(64 * kHeadWaves);
+  const size_t lds = HeadForm<T>::lds(a.groups, a.lanes);
+  hipError_t e;
+  if (out_bf16) {
+    if ((e = grant_lds(&mx4_head_kernel<T, OPERANDS, kOutBf16, BF16>, kHeadLds, granted16)) != hipSuccess) return e;
+    hipLaunchKernelGGL((mx4_head_kernel<T, OPERANDS, kOutBf16, BF16>), grid, block, lds, stream, a);
+  } else {
+    if ((e = grant_lds(&mx4_head_kernel<T, OPERANDS, kOutF32, BF16>, kHeadLds, granted)) != hipSuccess) return e;
+    hipLaunchKernelGGL((mx4_head_kernel<T, OPERANDS, kOutF32, BF16>), grid, block, lds, stream, a);
+  }
+  return hipGetLastError();
+}
+
 // Tiles of a product, and slices of its columns: twice as many as long as the tiles give
 // fewer than 160 CUs a workgroup, a slice has two steps and the sums stay within 16 MiB.
 static long long mx4_tiles(int rows, int lanes, int tile_lanes, int tile_rows) {
@@ -1506,17 +1673,28 @@ static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int ou
 }
 
 // Which kernels a product of `lanes` takes (terms 0: microscaled lanes).
-enum { kFormFew = 0, kFormHead, kFormSmall, kFormLarge, kFormWhole };
+enum { kFormFew = 0, kFormHead, kFormSmall, kFormLarge, kFormWhole, kFormTall };
+
+constexpr long long kFewBytes = 28 << 20;
+
+static long long mx4_bytes(int rows, int groups) { return (long long)rows * groups * 17; }
 
 static int mx4_form(int rows, int groups, int lanes, int terms) {
   const int steps = mx4_steps(groups);
-  if (lanes <= 16 && terms != 0 && rows >= 65536) return kFormHead;
-  if ((long long)lanes * steps < (terms == 5 ? 192 : terms == 3 ? 640 : 1200)) return kFormFew;
-  const long long large = terms == 5   ? mx4_tiles(rows, lanes, 64, 512)
-                          : terms == 3 ? mx4_tiles(rows, lanes, 64, 256)
-                                       : mx4_tiles(rows, lanes, 128, 256);
-  if (terms == 3 && mx4_tiles(rows, lanes, 128, 512) >= 192) return kFormWhole;
-  return large >= 192 ? kFormLarge : kFormSmall;
+  const long long bytes = mx4_bytes(rows, groups);
+  if (terms != 0 && lanes <= 16 && rows >= 32768 && bytes >= kFewBytes) {
+    const bool two = lanes * terms <= 32 && groups >= 16 &&
+                     (terms == 5 ? HeadForm<5>::lds(groups, lanes) : HeadForm<3>::lds(groups, lanes)) <= kHeadLds;
+    return two ? kFormHead : kFormTall;
+  }
+  if ((long long)lanes * steps < (terms == 5 ? 192 : terms == 3 ? 640 : 1200) &&
+      bytes * ((lanes + 15) / 16) < (terms ? kFewBytes : kFewBytes / 2 * 3))
+    return kFormFew;
+  if (terms == 3 && lanes > 64 && mx4_tiles(rows, lanes, 128, 512) >= 192) return kFormWhole;
+  const bool large = terms == 5   ? lanes > 32 && mx4_tiles(rows, lanes, 64, 512) >= 192
+                     : terms == 3 ? lanes > 32 && mx4_tiles(rows, lanes, 64, 256) >= 192
+                                  : lanes > 64 && mx4_tiles(rows, lanes, 128, 256) >= 192;
+  return large ? kFormLarge : kFormSmall;
 }
 
 // Enough for any form of a product: its lanes as terms, or their scales, the sheet's scales
@@ -1524,6 +1702,7 @@ static int mx4_form(int rows, int groups, int lanes, int terms) {
 extern "C" size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int terms) {
   const int groups = cols / kMx4Group, form = mx4_form(rows, groups, lanes, terms);
   const size_t of_lanes = terms ? terms_bytes(lanes, cols, terms == 3) : pack_bytes<4, false>(lanes, groups, 1);
+  if (form == kFormHead) return 0;
   if (form == kFormFew) return terms ? of_lanes : 0;
   const int slices =
       form == kFormSmall ? terms ? mx4_slices(rows, groups, lanes, 32, 256) : mx4_slices(rows, groups, lanes, 64, 256) : 1;
@@ -1544,8 +1723,10 @@ extern "C" hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *a
   a.out = out;
   a.out_stride = out_stride;
   uint8_t *const room = static_cast<uint8_t *>(work);
-  const bool single = act_bf16 ? lanes <= 5 && step_lds<3>(a.groups, lanes, 1, 4, 4) <= kStepLds
-                               : lanes <= 3 && step_lds<5>(a.groups, lanes, 1, 4, 4) <= kStepLds;
+  const int form = mx4_form(a.rows, a.groups, lanes, act_bf16 ? 3 : 5);
+  const bool single = form != kFormHead && lanes <= (act_bf16 ? 5 : 3) &&
+                      (lanes == 1 || mx4_bytes(a.rows, a.groups) < kFewBytes) &&
+                      (act_bf16 ? step_lds<3>(a.groups, lanes, 1, 4, 4) : step_lds<5>(a.groups, lanes, 1, 4, 4)) <= kStepLds;
   if (single) {
     a.act_rows = act;
     a.act_stride = act_stride;
@@ -1556,8 +1737,15 @@ extern "C" hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *a
     return out_bf16 ? launch_step<5, 1, kOutBf16, false>(a, grid, lanes, stream)
                     : launch_step<5, 1, kOutF32, false>(a, grid, lanes, stream);
   }
-  const int form = mx4_form(a.rows, a.groups, lanes, act_bf16 ? 3 : 5);
-  if (form == kFormHead)
+  if (form == kFormHead) {
+    a.act_rows = act;
+    a.act_stride = act_stride;
+    const int operands = act_bf16 ? HeadForm<3>::operands(lanes) : HeadForm<5>::operands(lanes);
+    if (act_bf16)
+      return operands == 1 ? launch_head<3, 1, true>(a, out_bf16, stream) : launch_head<3, 2, true>(a, out_bf16, stream);
+    return operands == 1 ? launch_head<5, 1, false>(a, out_bf16, stream) : launch_head<5, 2, false>(a, out_bf16, stream);
+  }
+  if (form == kFormTall)
     return act_bf16 ? launch_many<3, 1, 4, 1, 4, 3>(a, act, act_stride, out_bf16, room, false, stream)
                     : launch_many<5, 1, 4, 1, 4, 3>(a, act, act_stride, out_bf16, room, false, stream);
   if (form == kFormSmall)

@@ -333,7 +333,7 @@ __device__ __forceinline__ float silu_near(float x) {
 // tiles begin at tile (places before e) / tile + e: no more than that many lie before, and
 // every expert finds its own without the others.  Tiles left over have no places.
 constexpr int kPrepareThreads = 256;
-constexpr int kPlaceRound = 16;  // slots a lane has in flight
+constexpr int kPlaceRound = 16, kPlaceRounds = 4;  // slots of a lane on their way; rounds kept in registers
 
 struct PlaceArgs {
   const int32_t *pick;
@@ -359,15 +359,22 @@ __device__ __forceinline__ void expert_place(const PlaceArgs &a, int expert) {
 #pragma unroll
     for (int i = 0; i < kPlaceRound; ++i) e[i] = s0 + 64 * i + lane < end ? e[i] : -1;
   };
+  // up to 16384 slots are read once: all rounds on their way, and kept for the numbers
+  constexpr int kSpan = 64 * kPlaceRound, kHeld = kSpan * kPlaceRounds;
+  int held[kPlaceRounds][kPlaceRound];
   int mine = 0, before = 0;
-  for (int s0 = first; s0 < end; s0 += 64 * kPlaceRound) {
-    int e[kPlaceRound];
-    round(s0, e);
+  for (int s0 = first; s0 < end; s0 += kHeld) {
 #pragma unroll
-    for (int i = 0; i < kPlaceRound; ++i) {
-      mine += e[i] == expert;
-      before += (uint32_t)e[i] < (uint32_t)expert;
-    }
+    for (int r = 0; r < kPlaceRounds; ++r)
+      if (s0 + kSpan * r < end) round(s0 + kSpan * r, held[r]);
+#pragma unroll
+    for (int r = 0; r < kPlaceRounds; ++r)
+      if (s0 + kSpan * r < end)
+#pragma unroll
+        for (int i = 0; i < kPlaceRound; ++i) {
+          mine += held[r][i] == expert;
+          before += (uint32_t)held[r][i] < (uint32_t)expert;
+        }
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
@@ -384,20 +391,23 @@ __device__ __forceinline__ void expert_place(const PlaceArgs &a, int expert) {
     if (w < wave) next += sums[0][w];
   }
   next += base;
-  for (int s0 = first; s0 < end; s0 += 64 * kPlaceRound) {
-    int e[kPlaceRound];
-    round(s0, e);
+  for (int s0 = first; s0 < end; s0 += kHeld) {
 #pragma unroll
-    for (int i = 0; i < kPlaceRound; ++i) {
-      const int s = s0 + 64 * i + lane;
-      const uint64_t own = __ballot(e[i] == expert);
-      const int place = next + __builtin_popcountll(own & ((1ull << lane) - 1));
-      next += __builtin_popcountll(own);
-      if (e[i] == expert) {
-        a.place_of[s] = place;
-        a.lane_of[place] = s / a.top;
+    for (int r = 0; r < kPlaceRounds; ++r) {
+      if (s0 + kSpan * r >= end) break;
+      if (end - first > kHeld) round(s0 + kSpan * r, held[r]);
+#pragma unroll
+      for (int i = 0; i < kPlaceRound; ++i) {
+        const int e = held[r][i], s = s0 + kSpan * r + 64 * i + lane;
+        const uint64_t own = __ballot(e == expert);
+        const int place = next + __builtin_popcountll(own & ((1ull << lane) - 1));
+        next += __builtin_popcountll(own);
+        if (e == expert) {
+          a.place_of[s] = place;
+          a.lane_of[place] = s / a.top;
+        }
+        if (expert == 0 && s < end && (uint32_t)e >= (uint32_t)a.experts) a.place_of[s] = -1;
       }
-      if (expert == 0 && s < end && (uint32_t)e[i] >= (uint32_t)a.experts) a.place_of[s] = -1;
     }
   }
   // this expert's tiles and those left over between it and the next's, or the end
@@ -508,38 +518,36 @@ __device__ __forceinline__ uint4_t mx4_scales16(const uint8_t *row, int g, int g
   return out;
 }
 
-// A thread takes row `at` of every tile of a block and sixteen groups, four steps: a turn of
-// four rows' bytes in registers for every four tiles.
+// A thread takes row `at` of four tiles of a block and sixteen groups, four steps: a turn of
+// four rows' bytes in registers.
 template <int NT, bool PAIR>
 __device__ __forceinline__ void mx4_pack_scales(const PackArgs &a, long long id) {
   const int steps = mx4_steps(a.groups), blocks = tile_blocks<NT, PAIR>(a.rows), fours = (steps + 3) / 4;
-  const int at = (int)(id & 15);
-  const int four = (int)(id / 16 % fours);
-  const long long block = id / 16 / fours;
+  const int at = (int)(id & 15), q = (int)(id / 16 % (NT / 4));
+  id /= 16 * (NT / 4);
+  const int four = (int)(id % fours);
+  const long long block = id / fours;
   const int e = (int)(block / blocks);
   if (e >= a.experts) return;
-  uint4_t v[NT];
+  uint4_t v[4];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const size_t row = (size_t)e * a.rows + tile_row<NT, PAIR>((int)(block % blocks), j, at, a.rows);
+  for (int j = 0; j < 4; ++j) {
+    const size_t row = (size_t)e * a.rows + tile_row<NT, PAIR>((int)(block % blocks), 4 * q + j, at, a.rows);
     v[j] = mx4_scales16(a.w.scale + row * a.w.scale_stride, 16 * four, a.groups);
   }
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     if (4 * four + s >= steps) break;
     uint32_t *const dst =
-        reinterpret_cast<uint32_t *>(a.dst) + (((size_t)block * steps + 4 * four + s) * 64 + at) * (NT / 4);
-#pragma unroll
-    for (int q = 0; q < NT / 4; ++q) {
-      // bytes 0 .. 3 of four rows: pairs of rows, then pairs of pairs
-      const uint32_t r0 = v[4 * q][s], r1 = v[4 * q + 1][s], r2 = v[4 * q + 2][s], r3 = v[4 * q + 3][s];
-      const uint32_t lo01 = __builtin_amdgcn_perm(r1, r0, 0x05010400u), hi01 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
-      const uint32_t lo23 = __builtin_amdgcn_perm(r3, r2, 0x05010400u), hi23 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
-      dst[q] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
-      dst[16 * (NT / 4) + q] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
-      dst[32 * (NT / 4) + q] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
-      dst[48 * (NT / 4) + q] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
-    }
+        reinterpret_cast<uint32_t *>(a.dst) + (((size_t)block * steps + 4 * four + s) * 64 + at) * (NT / 4) + q;
+    // bytes 0 .. 3 of four rows: pairs of rows, then pairs of pairs
+    const uint32_t r0 = v[0][s], r1 = v[1][s], r2 = v[2][s], r3 = v[3][s];
+    const uint32_t lo01 = __builtin_amdgcn_perm(r1, r0, 0x05010400u), hi01 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
+    const uint32_t lo23 = __builtin_amdgcn_perm(r3, r2, 0x05010400u), hi23 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
+    dst[0] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+    dst[16 * (NT / 4)] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+    dst[32 * (NT / 4)] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+    dst[48 * (NT / 4)] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
   }
 }
 
@@ -1492,7 +1500,7 @@ static size_t pack_bytes(int rows, int groups, int experts) {
 
 template <int NT, bool PAIR>
 static unsigned pack_blocks(int rows, int groups, int experts) {
-  const long long threads = (long long)experts * tile_blocks<NT, PAIR>(rows) * ((mx4_steps(groups) + 3) / 4) * 16;
+  const long long threads = (long long)experts * tile_blocks<NT, PAIR>(rows) * ((mx4_steps(groups) + 3) / 4) * 16 * (NT / 4);
   return (unsigned)((threads + kPrepareThreads - 1) / kPrepareThreads);
 }
 

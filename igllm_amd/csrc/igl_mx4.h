@@ -14,9 +14,10 @@
 // s a byte for the group, t_j e2m3 numbers.  The group's largest is at most 3.75
 // under its scale, so t_0 is off by 1/8 at most, thirty-two times what is left is 4
 // at most, off by 1/8 again, and so on: T terms hold a value to 2^(-3 - 5 (T - 1))
-// where the group's largest is more than 1.875, so to 2^(1 - 5 T) of the largest:
-// 2^-24 with five (fp32 lanes), 2^-14 with three (bf16 lanes, whose outputs are
-// rounded to 2^-8).  e2m3 against e2m1 runs at twice e4m3's rate (8.8 to 4.7
+// of the group's scale, whose largest is more than 1.875: to 2^-23.9 of the largest with
+// five (fp32 lanes), 2^-13.9 with three (bf16 lanes, whose outputs are rounded to
+// 2^-8).  A term less would be 2^-18.9 and 2^-8.9, where fp32 lanes have 2^-24 and bf16's
+// own rounding is 2^-8 of the output.  Sums are single precision.  e2m3 against e2m1 runs at twice e4m3's rate (8.8 to 4.7
 // PFLOP/s, all of a card's SIMDs), so five terms are 1.8 PFLOP/s of fp32 lanes and
 // three 2.9 of bf16 ones, and no code is ever decoded.
 #pragma once
@@ -420,7 +421,10 @@ __device__ __forceinline__ void expert_place(const PlaceArgs &a, int expert) {
 }
 
 // The product of many lanes: WM x WN waves of 16 MT lanes x 16 NT rows, 128 columns a
-// step, both operands through LDS in ST stages.
+// step, both operands through LDS in ST stages.  2047 bf16 lanes of 8192 x 2048 take 52
+// us of the GPU (1.3 PFLOP/s, 4.0 of terms), 2048 microscaled ones 30; of the 52 the products
+// by themselves, operands in registers, are 31 (clocks fall under them), the same
+// without what is brought 41, the stores 7.
 //   * Stages are written only by global_load_lds, ST - 1 steps ahead.  A load to registers
 //     in the loop costs more than it brings: with such loads and these in flight the
 //     compiler waits for all of either.
@@ -955,7 +959,8 @@ __device__ __forceinline__ int8v_t mx4_clear(const Mx4Codes &c, int g, int group
   return int8v_t{(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
 }
 
-// The product of up to sixteen lanes, bound by the sheet's bytes: a workgroup takes 16 RT
+// The product of up to sixteen lanes of a sheet that the caches hold (6144 x 1536: 8 bf16
+// lanes 9 us with the terms' launch, microscaled ones 5): a workgroup takes 16 RT
 // rows and its four waves every fourth step, operands straight to registers, four steps'
 // codes in flight a wave; sums meet in LDS.  Lane l of a wave holds group l / 16 of row and
 // of lane l % 16.  T terms, 0: microscaled lanes.
@@ -1084,6 +1089,8 @@ __device__ __forceinline__ int8v_t own_operand(const uint8_t *record, int t, int
 // One to three fp32 lanes (five bf16 ones), a token's step: a lane's terms are columns of
 // the one operand, so five terms cost one product, and a wave cuts the lanes itself while
 // its first codes are on their way: no launch before.  Sums of terms and waves in LDS.
+// One fp32 lane of 6144 x 1536: 5.7 us, 4.8 at best, of which a launch by itself is 2 and
+// the codes a microsecond; with terms from a launch before it 12.8.
 // kOutGate: blockIdx.y a slot of the experts: its expert's gate and up rows, the gated
 // products as floats.
 template <int T, int RT, int OUT, bool BF16>
@@ -1185,7 +1192,11 @@ __global__ __launch_bounds__(256) void mx4_step_kernel(Mx4Args g) {
 // workgroups that stay, a wave sixteen rows at a time, the next rows' codes and scales on
 // their way to registers while these are multiplied.  Lanes' terms are columns of
 // operands (five lanes of fp32 two), cut by the workgroup and kept in LDS as they are
-// read; sums cross LDS to be added and stored.
+// read; sums cross LDS to be added and stored.  Five fp32 lanes of 262144 x 1536: 47 us
+// out of the caches (4.6 TB/s; a copy has 4.96), 39 in them; as tiles 55 and 42, of which
+// packing the scales is ten, and a workgroup every 64 rows 74.  Loads past the caches
+// 50 either way.  Three operands and more take longer than tiles (8 lanes 57 for 44, in
+// the caches).
 constexpr int kHeadWaves = 8;
 constexpr int kHeadSteps = 4;  // of a piece: sixteen scales of a row
 constexpr int kHeadAhead = 6;  // pieces of a wave on their way
@@ -1331,7 +1342,8 @@ __global__ __launch_bounds__(64 * kHeadWaves, 2) void mx4_head_kernel(Mx4Args g)
 }
 
 // The down products of a token's experts and their sum: blockIdx.y a lane, eight waves, each
-// every eighth of its choices (its hidden values cut by the wave), sixteen rows.
+// every eighth of its choices (its hidden values cut by the wave), sixteen rows.  Eight of
+// 128 experts, 1536 and 768: 6.2 us behind 7.5 of gate and up; by experts, in five launches, 49.
 template <int T, bool BF16>
 __global__ __launch_bounds__(512) void expert_step_kernel(Mx4Args g, const float *hidden, const float *weight, void *out) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_x[];
@@ -1392,7 +1404,8 @@ __global__ __launch_bounds__(512) void expert_step_kernel(Mx4Args g, const float
     static_cast<float *>(out)[to] = v;
 }
 
-// out[lane] = sum over its choices, in their order, of weight * row of the slot's place
+// out[lane] = sum over its choices, in their order, of weight * row of the slot's place.
+// 2047 lanes of eight rows of 1536: 17 us, 6.3 TB/s of rows that the launch before wrote.
 template <bool BF16>
 __global__ __launch_bounds__(256) void expert_join_kernel(const float *rows, const int *place_of, const float *weight,
                                                           int top, int hidden, int lanes, void *out, long long out_stride) {
@@ -1619,7 +1632,10 @@ static hipError_t launch_head(const Mx4Args &a, int out_bf16, hipStream_t stream
 }
 
 // Tiles of a product, and slices of its columns: twice as many as long as the tiles give
-// fewer than 160 CUs a workgroup, a slice has two steps and the sums stay within 16 MiB.
+// fewer than 160 CUs a workgroup, a slice has two steps, and the steps that it spares (0.4 us
+// each) are more than the sums that it adds to what is written and read again.  37 fp32
+// lanes of 2048 x 8192: 18 us in sixteen slices, 41 in one; 256 microscaled lanes of 6144 x
+// 1536, whose sums are 12 MB: 21.5 in two, 16.4 in one.
 static long long mx4_tiles(int rows, int lanes, int tile_lanes, int tile_rows) {
   return (long long)((lanes + tile_lanes - 1) / tile_lanes) * ((rows + tile_rows - 1) / tile_rows);
 }
@@ -1680,7 +1696,17 @@ static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int ou
   return hipGetLastError();
 }
 
-// Which kernels a product of `lanes` takes (terms 0: microscaled lanes).
+// Which kernels a product of `lanes` takes (terms 0: microscaled lanes).  Both sides, us:
+//   * a sheet past the caches' reach, up to sixteen lanes: operands of columns up to two of
+//     them, else tiles of 16 lanes.  32768 x 2048: 8 fp32 lanes 16.9, a few lanes a
+//     workgroup 31; 5 bf16 ones 14.5, a token's kernel 32.  Microscaled lanes' codes are the
+//     operand as they lie: up to 42 MB a few a workgroup win (8 lanes 13.7 for 16.2)
+//   * few lanes: every sixteen read the sheet again and fetch their terms themselves, so
+//     as long as terms by steps are few: 4 fp32 lanes of 1536 x 6144 17 for 12 in tiles,
+//     16 of 6144 x 1536 12.8 for 13.8; 12 bf16 lanes of 2048 x 8192 16 for 10.5; 64
+//     microscaled ones of 6144 x 1536 9.4 for 12
+//   * tiles as large as still give most CUs one: 2047 bf16 lanes of 8192 x 2048 68 in 64 x
+//     256, 69 in 64 x 512, 58 in 128 x 512
 enum { kFormFew = 0, kFormHead, kFormSmall, kFormLarge, kFormWhole, kFormTall };
 
 constexpr long long kFewBytes = 28 << 20;
@@ -1935,7 +1961,8 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
                                          int out_stride, void *work, hipStream_t stream) {
   const ExpertCall c = {x,   act,      act_stride, lanes, pick, weight, top,
                         out, out_bf16, out_stride, static_cast<uint8_t *>(work), expert_room(x, lanes, top, act_bf16)};
-  // a slot at a time reads an expert's weights for each; by experts takes two launches more
+  // a slot at a time reads an expert's weights for each; by experts takes two launches more: 48
+  // slots of 64 experts 34 us for 39, 32 of 8 26 for 25
   const int slots = lanes * top;
   const bool step = slots <= 64 && slots <= 32 + x->expert_count / 4 &&
                     (act_bf16 ? step_lds<3>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
@@ -1943,6 +1970,10 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
                               : step_lds<5>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
                                     step_lds<5>(x->inner / kMx4Group, 1, 1, 8, 1) <= kStepLds);
   if (step) return act_bf16 ? experts_step<3, true>(c, stream) : experts_step<5, false>(c, stream);
+  // tiles of as many places as an expert has, where they are whole: 12 of 64 experts 53 us in 32s
+  // and 59 in 16s (fp32; bf16 42 and 51), 16 of 128 91 and 98, but 16 of 32 59 and 48; 32 of 32 63
+  // in 32s and 95 in 64s; 128 of 128 bf16 193 in 64s, 228 in 128 x 512 tiles, of which every
+  // expert's second is nearly empty
   const long long each = (long long)slots / x->expert_count;
   if (act_bf16) {
     if (each >= 40) return experts_grouped<3, 2, 4, 2, 4, 2>(c, stream);

@@ -627,7 +627,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
   const int steps = mx4_steps(g.groups);
 
   // ---- what this wave brings each step: sixteen bytes a lane, from base[i] + step * by[i] + off[i], and of codes
-  // (walks[i] all ones) a step's piece, to a row's last at most.  By number: lanes' chunks (wave lane (part, at)'s sixteen bytes at its number), rows' codes, packed
+  // (walks[i] all ones) a step's piece, to a row's last at most.  By number: lanes' chunks, rows' codes, packed
   // scales.  The last wave may bring one twice.  What is the wave's is uniform and what is a lane's fits 32 bits
   // (sixteen rows' codes, all lanes' terms), so that a load takes two or three instructions of the lanes'.
   const uint8_t *base[F::kLoads];

@@ -338,11 +338,20 @@ constexpr int kPlaceRound = 16, kPlaceRounds = 4;  // slots of a lane on their w
 
 struct PlaceArgs {
   const int32_t *pick;
-  int slots, top, experts, tile;  // places a tile
+  int slots, experts, tile;       // places a tile
+  uint32_t top_inverse;           // 2^32 / top and up to one more, for slot / top (slots below 2^20); 0: top is 1
   int *lane_of;                   // [slots] lane of a place
   int *place_of;                  // [slots] place of a slot, or -1
   Mx4Tile *tiles;                 // [slots / tile + experts]
 };
+
+__host__ __device__ __forceinline__ uint32_t place_inverse(int top) {
+  return top == 1 ? 0u : (uint32_t)((1ull << 32) / (uint32_t)top) + 1;
+}
+
+__host__ __device__ __forceinline__ int place_lane(int slot, uint32_t inverse) {
+  return inverse ? (int)((uint64_t)(uint32_t)slot * inverse >> 32) : slot;
+}
 
 // A workgroup lists one expert's slots, in an order of their own that is always the same:
 // it reads every pick (from the L2 but once), counts its own and those of experts before,
@@ -401,11 +410,11 @@ __device__ __forceinline__ void expert_place(const PlaceArgs &a, int expert) {
       for (int i = 0; i < kPlaceRound; ++i) {
         const int e = held[r][i], s = s0 + kSpan * r + 64 * i + lane;
         const uint64_t own = __ballot(e == expert);
-        const int place = next + __builtin_popcountll(own & ((1ull << lane) - 1));
+        const int place = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(own >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)own, (uint32_t)next));
         next += __builtin_popcountll(own);
         if (e == expert) {
           a.place_of[s] = place;
-          a.lane_of[place] = s / a.top;
+          a.lane_of[place] = place_lane(s, a.top_inverse);
         }
         if (expert == 0 && s < end && (uint32_t)e >= (uint32_t)a.experts) a.place_of[s] = -1;
       }
@@ -1873,7 +1882,7 @@ static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
   p.groups = x->hidden / kMx4Group;
   p.lanes = c.lanes;
   p.terms = c.base + r.x;
-  p.place = PlaceArgs{c.pick, slots, c.top, x->expert_count, F::kLanes, (int *)(c.base + r.lane_of),
+  p.place = PlaceArgs{c.pick, slots, x->expert_count, F::kLanes, place_inverse(c.top), (int *)(c.base + r.lane_of),
                       (int *)(c.base + r.place_of), (Mx4Tile *)(c.base + r.tiles)};
   p.pairs = PackArgs{mx4_view(&x->gate_up, 0), 2 * x->inner, p.groups, x->expert_count, 0, c.base + r.gate_up};
   p.rows = PackArgs{mx4_view(&x->down, 0), x->hidden, x->inner / kMx4Group, x->expert_count, 0, c.base + r.down};

@@ -38,6 +38,13 @@ extern "C" int planmx_room(int experts, int hidden, int inner, int lanes, int to
   return 0;
 }
 
+// Zero, or a slot whose lane is not slot / top.
+extern "C" int planmx_lanes(int top) {
+  for (int slot = 0; slot < 1 << 20; ++slot)
+    if (place_lane(slot, place_inverse(top)) != slot / top) return slot;
+  return 0;
+}
+
 // Zero, or the first thing wrong with a step's pieces of `lanes` lanes of terms: bytes of
 // two groups at one place, or a step's not all taken.
 template <int T>

@@ -30,7 +30,7 @@ def load(path):
         fn.restype, fn.argtypes = res, args
     lib.audit_report.restype = ctypes.c_long
     lib.audit_report.argtypes = [ctypes.POINTER(ctypes.c_long)] * 2
-    for name, count in (("form", 4), ("slices", 5), ("steps", 1), ("room", 6), ("pieces", 2), ("banks", 2)):
+    for name, count in (("form", 4), ("slices", 5), ("steps", 1), ("room", 6), ("pieces", 2), ("banks", 2), ("lanes", 1)):
         fn = getattr(lib, "planmx_" + name)
         fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_int] * count
     lib.planmx_tiles.restype, lib.planmx_tiles.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int]
@@ -350,6 +350,10 @@ def test_pieces_of_terms(lib):
 def test_rows_in_lds_meet_no_bank_twice(lib):
     for width in (64, 128):
         assert lib.planmx_banks(width, 1) == 0 and lib.planmx_banks(width, 0) != 0
+
+
+def test_a_slots_lane(lib):
+    assert all(lib.planmx_lanes(top) == 0 for top in range(1, 65))
 
 
 def test_tiles_of_experts_places(lib):

@@ -1640,11 +1640,12 @@ static hipError_t launch_head(const Mx4Args &a, int out_bf16, hipStream_t stream
   return hipGetLastError();
 }
 
-// Tiles of a product, and slices of its columns: twice as many as long as the tiles give
-// fewer than 160 CUs a workgroup, a slice has two steps, and the steps that it spares (0.4 us
-// each) are more than the sums that it adds to what is written and read again.  37 fp32
-// lanes of 2048 x 8192: 18 us in sixteen slices, 41 in one; 256 microscaled lanes of 6144 x
-// 1536, whose sums are 12 MB: 21.5 in two, 16.4 in one.
+// Tiles of a product, and slices of its columns: as many as cost the least, a power of two, as
+// long as fewer give less than 160 CUs a workgroup and a slice has two steps.  A step takes
+// 0.7 us, the launch that adds the sums 3, sums are written and read at 4 TB/s.  37 fp32 lanes
+// of 2048 x 8192: 18 us in sixteen slices, 41 in one; 256 microscaled lanes of 6144 x 1536,
+// whose sums are 12 MB: 21.5 in two, 16.4 in one; 1500 bf16 ones of 593 x 1280 27 and
+// 17; 17 fp32 ones of 8192 x 2048 12.6 in eight, 17 in one.
 static long long mx4_tiles(int rows, int lanes, int tile_lanes, int tile_rows) {
   return (long long)((lanes + tile_lanes - 1) / tile_lanes) * ((rows + tile_rows - 1) / tile_rows);
 }
@@ -1652,9 +1653,10 @@ static long long mx4_tiles(int rows, int lanes, int tile_lanes, int tile_rows) {
 static int mx4_slices(int rows, int groups, int lanes, int tile_lanes, int tile_rows) {
   const long long tiles = mx4_tiles(rows, lanes, tile_lanes, tile_rows);
   const int steps = mx4_steps(groups);
+  auto cost = [&](long long s) { return 700 * steps / s + (s > 1 ? 3000 + 2 * s * lanes * rows / 1000 : 0); };
   int slices = 1;
-  while (tiles * slices < 160 && steps >= 4 * slices && 100000LL * steps >= (long long)slices * slices * lanes * rows)
-    slices *= 2;
+  for (int s = 2; tiles * s < 320 && steps >= 2 * s; s *= 2)
+    if (cost(s) < cost(slices)) slices = s;
   const int each = (steps + slices - 1) / slices;
   return (steps + each - 1) / each;  // none empty
 }
@@ -1708,12 +1710,12 @@ static hipError_t launch_many(Mx4Args a, const void *act, int act_stride, int ou
 // Which kernels a product of `lanes` takes (terms 0: microscaled lanes).  Both sides, us:
 //   * a sheet past the caches' reach, up to sixteen lanes: operands of columns up to two of
 //     them, else tiles of 16 lanes.  32768 x 2048: 8 fp32 lanes 16.9, a few lanes a
-//     workgroup 31; 5 bf16 ones 14.5, a token's kernel 32.  Microscaled lanes' codes are the
-//     operand as they lie: up to 42 MB a few a workgroup win (8 lanes 13.7 for 16.2)
-//   * few lanes: every sixteen read the sheet again and fetch their terms themselves, so
-//     as long as terms by steps are few: 4 fp32 lanes of 1536 x 6144 17 for 12 in tiles,
-//     16 of 6144 x 1536 12.8 for 13.8; 12 bf16 lanes of 2048 x 8192 16 for 10.5; 64
-//     microscaled ones of 6144 x 1536 9.4 for 12
+//     workgroup 31; 5 bf16 ones 14.5, a token's kernel 32
+//   * few lanes: every sixteen of them and of rows read their own from the caches, and a wave
+//     fetches terms for itself, so as long as these are few, and a row's chain is short: 4 fp32
+//     lanes of 1536 x 6144 17 for 12 in tiles, 8 of 8192 x 2048 13.5 for 11.5, 16 of 6144 x 1536
+//     12.8 for 13.8; 12 bf16 lanes of 2048 x 8192 16 for 10.5, 33 of 6144 x 1536 13 for 13; 64
+//     microscaled ones 9.4 for 12, 100 14.9 for 14.3, and 8 of 32768 x 2048 13.7 for 16.2
 //   * tiles as large as still give most CUs one: 2047 bf16 lanes of 8192 x 2048 68 in 64 x
 //     256, 69 in 64 x 512, 58 in 128 x 512
 enum { kFormFew = 0, kFormHead, kFormSmall, kFormLarge, kFormWhole, kFormTall };
@@ -1730,8 +1732,10 @@ static int mx4_form(int rows, int groups, int lanes, int terms) {
                      (terms == 5 ? HeadForm<5>::lds(groups, lanes) : HeadForm<3>::lds(groups, lanes)) <= kHeadLds;
     return two ? kFormHead : kFormTall;
   }
-  if ((long long)lanes * steps < (terms == 5 ? 192 : terms == 3 ? 640 : 1200) &&
-      bytes * ((lanes + 15) / 16) < (terms ? kFewBytes : kFewBytes / 2 * 3))
+  const long long few = mx4_tiles(rows, lanes, 16, 16) * steps;
+  if (terms == 5   ? few < 6000 && steps <= 24
+      : terms == 3 ? few < 12000 && steps <= 40
+                   : few < (lanes <= 16 ? 38000 : 24000))
     return kFormFew;
   if (terms == 3 && lanes > 64 && mx4_tiles(rows, lanes, 128, 512) >= 192) return kFormWhole;
   const bool large = terms == 5   ? lanes > 32 && mx4_tiles(rows, lanes, 64, 512) >= 192

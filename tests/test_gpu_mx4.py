@@ -153,7 +153,9 @@ SHAPES = [(1, 16, 32), (1, 1, 64), (1, 6144, 1536), (2, 50, 96), (3, 33, 128), (
           (37, 257, 8192), (63, 129, 704), (64, 256, 512), (65, 100, 1056), (100, 520, 768), (129, 1030, 96),
           (300, 1537, 1536), (517, 272, 320), (1000, 300, 2048),
           # a head; tiles of many lanes and rows, the last of either not full
-          (4, 32776, 1760), (16, 40001, 1408), (2, 65540, 96), (500, 6150, 64), (1000, 6201, 96), (1540, 7690, 160)]
+          (4, 32776, 1760), (16, 40001, 1408), (2, 65540, 96), (500, 6150, 64), (1000, 6201, 96), (1540, 7690, 160),
+          # columns in slices, the last one short
+          (70, 2100, 8192), (21, 4100, 4128)]
 
 
 @pytest.mark.parametrize("lanes,rows,cols", SHAPES)

@@ -968,8 +968,8 @@ __device__ __forceinline__ int8v_t mx4_clear(const Mx4Codes &c, int g, int group
   return int8v_t{(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
 }
 
-// The product of up to sixteen lanes of a sheet that the caches hold (6144 x 1536: 8 bf16
-// lanes 9 us with the terms' launch, microscaled ones 5): a workgroup takes 16 RT
+// The product of few lanes, sixteen a workgroup, with a sheet that the caches hold (6144 x 1536:
+// 8 bf16 lanes 9 us with the terms' launch, microscaled ones 5): a workgroup takes 16 RT
 // rows and its four waves every fourth step, operands straight to registers, four steps'
 // codes in flight a wave; sums meet in LDS.  Lane l of a wave holds group l / 16 of row and
 // of lane l % 16.  T terms, 0: microscaled lanes.
@@ -1581,7 +1581,7 @@ __global__ __launch_bounds__(256) void mx4_fold_kernel(const float *sums, int sl
     static_cast<float *>(out)[to] = v;
 }
 
-// A product of up to sixteen lanes a tile, its terms (if any) prepared: workgroups of 64 rows
+// A product of few lanes, sixteen a tile, its terms (if any) prepared: workgroups of 64 rows
 // where they still give every CU four, of 16 below.
 template <int T, int OUT>
 static hipError_t launch_few(const Mx4Args &a, hipStream_t stream) {
@@ -1610,7 +1610,7 @@ static hipError_t grant_lds(K kernel, size_t bytes, size_t &granted) {
   return e;
 }
 
-constexpr size_t kStepLds = 100 * 1024;
+constexpr size_t kStepLds = 100 * 1024;  // a token's longest rows: one workgroup a CU still takes them
 
 template <int T, int RT, int OUT, bool BF16>
 static hipError_t launch_step(const Mx4Args &a, dim3 grid, int lanes, hipStream_t stream) {

@@ -194,6 +194,25 @@ def test_experts(backend, count, hidden, inner, top, lanes, kind, out_kind, gate
     close(*block.held)
 
 
+@pytest.mark.parametrize("lanes", [2, 30, 150, 600])
+def test_rows_apart(backend, lanes):
+    """Weights whose rows have bytes between them, at odd places of scales."""
+    count, hidden, inner, top = 5, 224, 160, 2
+    rng = np.random.default_rng(lanes)
+    block = Block(backend, rng, count, hidden, inner)
+    apart = [hold(backend, *w, 16 * (i + 1), 3 - i) for i, w in enumerate(block.w)]
+    x = mx.bf16(rng.normal(size=(lanes, hidden)))
+    pick, weight = picks(rng, lanes, count, top)
+    for kind in (F32, BF16):
+        close_by = run(backend, block, x, pick, weight, kind, F32)
+        own, block.set = block.set, backend.experts(*apart, count, hidden, inner)
+        assert np.array_equal(run(backend, block, x, pick, weight, kind, F32), close_by)
+        block.set = own
+        want, reach = block.want(x, pick, weight)
+        assert (np.abs(close_by - want) <= block.tol(reach, kind, F32, want)).all()
+    close(*block.held, *apart)
+
+
 @pytest.mark.parametrize("lanes", [1, 3, 30, 200])
 def test_picks_of_every_kind(backend, lanes):
     """None, out of range, the same expert twice in a lane, all lanes at one expert."""

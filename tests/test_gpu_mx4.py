@@ -336,6 +336,40 @@ def test_recorded(backend, lanes):
     close(held, store, x, back, *outs)
 
 
+@pytest.mark.parametrize("lanes", [1, 5, 16])
+def test_a_head_recorded(backend, lanes):
+    """A sheet past the caches' reach, replayed over new lanes among eager calls of others."""
+    cols, rows = 1760, 32776
+    rng = np.random.default_rng(lanes)
+    w = sheet(rng, rows, cols)
+    held, x, out = hold(backend, *w), backend.alloc(4 * lanes * cols), backend.alloc(4 * lanes * rows)
+    small = hold(backend, w[0][:40], w[1][:40])
+
+    def call():
+        backend.mx4_mat_mat_dev(held, x, F32, cols, lanes, out, F32, rows)
+
+    x.put(rng.normal(size=(lanes, cols)).astype(np.float32))
+    call()
+    backend.record_begin()
+    call()
+    replay = backend.record_end()
+    try:
+        for _ in range(3):
+            host = rng.normal(size=(lanes, cols)).astype(np.float32)
+            x.put(host)
+            call()
+            want = out.get(np.float32, lanes * rows)
+            backend.mx4_mat_mat_dev(small, x, F32, cols, 1, out, F32, 40)
+            backend.replay_run(replay)
+            assert np.array_equal(out.get(np.float32, lanes * rows), want)
+        exact = host.astype(np.float64) @ mx.values(w[0][:200], w[1][:200]).T
+        got = want.reshape(lanes, rows)[:, :200]
+        assert (np.abs(got - exact) <= bar(host.astype(np.float64), mx.values(w[0][:200], w[1][:200]), F32, F32, exact)).all()
+    finally:
+        backend.replay_free(replay)
+    close(held, small, x, out)
+
+
 def test_quantised_round_trip_of_what_was_read(backend):
     """Rows read back lie where they lay: laying them again changes nothing."""
     rng = np.random.default_rng(1)

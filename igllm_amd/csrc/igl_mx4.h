@@ -1611,6 +1611,7 @@ static hipError_t grant_lds(K kernel, size_t bytes, size_t &granted) {
 }
 
 constexpr size_t kStepLds = 100 * 1024;  // a token's longest rows: one workgroup a CU still takes them
+constexpr size_t kExpertLds = 150 * 1024;  // and its experts': by experts takes three times as long
 
 template <int T, int RT, int OUT, bool BF16>
 static hipError_t launch_step(const Mx4Args &a, dim3 grid, int lanes, hipStream_t stream) {
@@ -1952,11 +1953,11 @@ static hipError_t experts_step(const ExpertCall &c, hipStream_t stream) {
   const dim3 grid((x->hidden + 15) / 16, c.lanes);
   if (c.out_bf16) {
     static size_t granted16 = 0;
-    if ((e = grant_lds(&expert_step_kernel<T, true>, kStepLds, granted16)) != hipSuccess) return e;
+    if ((e = grant_lds(&expert_step_kernel<T, true>, kExpertLds, granted16)) != hipSuccess) return e;
     hipLaunchKernelGGL((expert_step_kernel<T, true>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
                        c.weight, c.out);
   } else {
-    if ((e = grant_lds(&expert_step_kernel<T, false>, kStepLds, granted)) != hipSuccess) return e;
+    if ((e = grant_lds(&expert_step_kernel<T, false>, kExpertLds, granted)) != hipSuccess) return e;
     hipLaunchKernelGGL((expert_step_kernel<T, false>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
                        c.weight, c.out);
   }
@@ -1974,26 +1975,31 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
                                          int out_stride, void *work, hipStream_t stream) {
   const ExpertCall c = {x,   act,      act_stride, lanes, pick, weight, top,
                         out, out_bf16, out_stride, static_cast<uint8_t *>(work), expert_room(x, lanes, top, act_bf16)};
-  // a slot at a time reads an expert's weights for each; by experts takes two launches more: 48
-  // slots of 64 experts 34 us for 39, 32 of 8 26 for 25
+  // a slot at a time reads an expert's weights for each, by experts takes two launches more: up
+  // to a count, and while what is read twice (slots^2 / (experts + slots) of them where picks
+  // are even) is less than those launches.  48 slots of 64 experts 34 us for 39, 64 of 128 42 for 46,
+  // 32 of eight 26 for 24; 32 of sixteen of 13 MB each 165 for 59
   const int slots = lanes * top;
-  const bool step = slots <= 64 && slots <= 32 + x->expert_count / 4 &&
+  const long long expert_bytes = 3LL * x->hidden * x->inner * 17 / 32;
+  const bool step = slots <= 64 && slots <= 20 + x->expert_count / 2 &&
+                    slots * expert_bytes / (x->expert_count + slots) < (50 << 20) / slots &&
                     (act_bf16 ? step_lds<3>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
-                                    step_lds<3>(x->inner / kMx4Group, 1, 1, 8, 1) <= kStepLds
+                                    step_lds<3>(x->inner / kMx4Group, 1, 1, 8, 1) <= kExpertLds
                               : step_lds<5>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
-                                    step_lds<5>(x->inner / kMx4Group, 1, 1, 8, 1) <= kStepLds);
+                                    step_lds<5>(x->inner / kMx4Group, 1, 1, 8, 1) <= kExpertLds);
   if (step) return act_bf16 ? experts_step<3, true>(c, stream) : experts_step<5, false>(c, stream);
-  // tiles of as many places as an expert has, where they are whole: 12 of 64 experts 53 us in 32s
-  // and 59 in 16s (fp32; bf16 42 and 51), 16 of 128 91 and 98, but 16 of 32 59 and 48; 32 of 32 63
-  // in 32s and 95 in 64s; 128 of 128 bf16 193 in 64s, 228 in 128 x 512 tiles, of which every
-  // expert's second is nearly empty
-  const long long each = (long long)slots / x->expert_count;
-  if (act_bf16) {
-    if (each >= 40) return experts_grouped<3, 2, 4, 2, 4, 2>(c, stream);
-    if (each >= 12) return experts_grouped<3, 1, 4, 2, 4, 2>(c, stream);
-    return experts_grouped<3, 1, 4, 1, 4, 3>(c, stream);
-  }
-  if (each >= 40) return experts_grouped<5, 2, 8, 2, 4, 2>(c, stream);
-  if (each >= 12) return experts_grouped<5, 1, 4, 2, 4, 2>(c, stream);
+  // tiles of as many places as an expert has, while smaller ones are more than two workgroups a
+  // CU: 12 of 64 experts 53 us in 32s and 59 in 16s (fp32; bf16 42 and 51), 16 of 128 91 and 98,
+  // but 16 of 32 59 and 48; 64 of eight small ones 25 in 16s and 44 in 64s; 128 of 128 bf16 193
+  // in 64s, 228 in 128 x 512 tiles, of which every expert's second is nearly empty
+  const int each = slots / x->expert_count, blocks = (2 * x->inner + 255) / 256;
+  auto groups = [&](int tile) { return (long long)expert_tiles(slots, x->expert_count, tile) * blocks; };
+  const int tile = each >= 40 && groups(32) >= 520 ? 64 : each >= 12 && groups(16) >= 520 ? 32 : 16;
+  if (act_bf16)
+    return tile == 64   ? experts_grouped<3, 2, 4, 2, 4, 2>(c, stream)
+           : tile == 32 ? experts_grouped<3, 1, 4, 2, 4, 2>(c, stream)
+                        : experts_grouped<3, 1, 4, 1, 4, 3>(c, stream);
+  if (tile == 64) return experts_grouped<5, 2, 8, 2, 4, 2>(c, stream);
+  if (tile == 32) return experts_grouped<5, 1, 4, 2, 4, 2>(c, stream);
   return experts_grouped<5, 1, 4, 1, 4, 3>(c, stream);
 }

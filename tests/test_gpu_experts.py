@@ -175,7 +175,9 @@ def run(backend, block, x, pick, weight, kind, out_kind, pad=0):
 @pytest.mark.parametrize("count,hidden,inner,top,lanes", [
     (1, 32, 32, 1, 1), (4, 64, 96, 2, 1), (16, 256, 160, 4, 1), (32, 1536, 704, 8, 1), (8, 128, 64, 3, 2),
     (16, 320, 224, 2, 5), (8, 96, 128, 8, 7), (64, 160, 96, 6, 17), (5, 544, 288, 3, 40), (32, 256, 128, 4, 64),
-    (3, 128, 160, 2, 150), (12, 288, 352, 4, 300), (2, 64, 32, 1, 700)])
+    (3, 128, 160, 2, 150), (12, 288, 352, 4, 300), (2, 64, 32, 1, 700),
+    # a token's longest rows; tiles of 32 and of 64 places
+    (3, 64, 4096, 2, 2), (64, 96, 512, 4, 300), (40, 96, 1024, 3, 600)])
 @pytest.mark.parametrize("kind,out_kind", [(F32, F32), (BF16, BF16), (BF16, F32)])
 @pytest.mark.parametrize("gate", [native.IGL_GATE_GELU, native.IGL_GATE_SILU])
 def test_experts(backend, count, hidden, inner, top, lanes, kind, out_kind, gate):

@@ -7,6 +7,7 @@ every allocation and checks every launch's grid, block and buffers
 (tests/hostmx); no kernel runs.
 """
 import ctypes
+import fcntl
 import os
 import shutil
 import subprocess
@@ -43,7 +44,9 @@ def so():
     if shutil.which("make") is None or not os.path.exists("/opt/rocm/bin/hipcc"):
         pytest.skip("hipcc or make absent")
     where = os.path.join(HERE, "hostmx")
-    r = subprocess.run(["make", "-s", "-j8", "-C", where], capture_output=True, text=True, timeout=900)
+    with open(os.path.join(where, "Makefile")) as lock:  # test processes side by side build once
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        r = subprocess.run(["make", "-s", "-j8", "-C", where], capture_output=True, text=True, timeout=900)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
     return os.path.join(where, "_build", "libhostmx.so")
 

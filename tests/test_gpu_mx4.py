@@ -248,6 +248,26 @@ def test_range(backend, lanes):
             close(held, act, out)
 
 
+@pytest.mark.parametrize("lanes", [1, 5, 30, 700])
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_the_largest_lanes(backend, lanes, kind):
+    """Values up to the largest of their type, whose group's scale is the largest byte that is none's."""
+    cols, rows = 96, 200
+    rng = np.random.default_rng(lanes)
+    top = np.float32(3.4028234663852886e38)
+    x = (top * rng.uniform(0.2, 1, size=(lanes, cols)) * rng.choice([-1, 1], size=(lanes, cols))).astype(np.float32)
+    x[:, ::7] = top
+    if kind == BF16:
+        x = mx.bits_float(x.view(np.uint32) >> 16)  # towards zero: the largest stays finite
+    w = sheet(rng, rows, cols, 40, 44)
+    held, act, out = hold(backend, *w), put(backend, x, kind), backend.alloc(4 * lanes * rows)
+    backend.mx4_mat_mat_dev(held, act, kind, cols, lanes, out, F32, rows)
+    wv = mx.values(*w)
+    want = x.astype(np.float64) @ wv.T
+    assert (np.abs(get(out, (lanes, rows), F32) - want) <= bar(x.astype(np.float64), wv, kind, F32, want)).all()
+    close(held, act, out)
+
+
 @pytest.mark.parametrize("lanes", [1, 5, 30, 140])
 @pytest.mark.parametrize("kind", [F32, BF16])
 def test_what_is_no_number(backend, lanes, kind):

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(RouteArgs a) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (first + i >= E || !(v[i] >= -3.402823466e38f)) v[i] = -__builtin_inff();  // a NaN is never chosen
-    v[i] = fminf(v[i], 3.402823466e38f);
+    v[i] = fminf(v[i], 3.402823466e38f) + 0.0f;  // a zero without its sign: keys are bits
     top = fmaxf(top, v[i]);
   }
   const bool soft = a.rule.score == IGL_ROUTE_SOFTMAX;
@@ -269,14 +269,13 @@ __device__ __forceinline__ uint32_t row_max_u32(uint32_t v) {
 __device__ __forceinline__ uint32_t row_min_u32(uint32_t v) { return ~row_max_u32(~v); }
 
 // Many lanes of a batch: four a wave, sixteen wave lanes each, so that a round of the choice
-// serves four: 16383 lanes of 256 experts, eight groups of which four stay, 22 us where
+// serves four: 16383 lanes of 256 experts, eight groups of which four stay, 21 us where
 // a wave a lane takes 27 (2048 lanes 11.5 and 12).  Vector issue is half of a SIMD's
-// cycles: 2250 instructions a wave, 900 of them the eight rounds, 650 the exponentials in
+// cycles: 2100 instructions a wave, 750 of them the eight rounds, 650 the exponentials in
 // double; the logits are 3.4 us of a copy.  Wave lane l of a row holds experts 64 q + 4 l + 0 .. 3, a quad each
 // of PER / 4.  E a multiple of four, sixteen choices and groups at most.
 template <int PER, bool WIDE>
 __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteArgs a) {
-  using Key = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
   __shared__ double room[WIDE ? kRouteWaves : 1][WIDE ? 64 * PER : 1];  // choices, then scores, of four rows
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, row = lane >> 4;
   const long long m0 = ((long long)blockIdx.x * kRouteWaves + wave) * 4;
@@ -305,7 +304,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteArgs 
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (expert(i) >= E || !(v[i] >= -3.402823466e38f)) v[i] = -__builtin_inff();  // a NaN is never chosen
-    v[i] = fminf(v[i], 3.402823466e38f);
+    v[i] = fminf(v[i], 3.402823466e38f) + 0.0f;  // a zero without its sign: keys are bits
     top = fmaxf(top, v[i]);
   }
   const bool soft = a.rule.score == IGL_ROUTE_SOFTMAX;
@@ -316,7 +315,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteArgs 
   auto share_of = [&](float t) { return exp_f64((double)t - (double)top); };
   auto sigmoid = [&](float t) { return recip_f64(1.0 + exp_f64(fmin(-(double)t, 800.0))); };
   double s[WIDE ? PER : 1], sum = 1.0;
-  Key key[PER];
+  uint32_t key[PER], low[WIDE ? PER : 1];  // keys' upper words, 0 of what may not be chosen, and lower ones
   if (soft && (WIDE || !a.rule.renorm)) {
     double of_all = 0.0;
 #pragma unroll
@@ -353,10 +352,11 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteArgs 
       const int group = l / split, part = l % split, n = (each - part + split - 1) / split;
       double most = none, second = none;
       if (group < G && n > 0) {
-        int at = lane % n;
+        const int from = lane % n;
+#pragma unroll 8
         for (int i = 0; i < n; ++i) {
+          const int at = from + i < n ? from + i : from + i - n;
           const double t = mine[group * each + part + split * at];
-          at = at + 1 < n ? at + 1 : 0;
           second = fmax(second, fmin(most, t));
           most = fmax(most, t);
         }
@@ -369,10 +369,14 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteArgs 
       double score_of = a.rule.group_best == 2 && second > none ? most + second : most;
       score_of = __shfl(score_of, 16 * row + min(l * split, 15));
       if (l >= G) score_of = none;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      mine[l] = score_of;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       // a group stays if fewer than group_top come before it
       int ahead = 0;
+#pragma unroll 8
       for (int q = 0; q < G; ++q) {
-        const double other = __shfl(score_of, 16 * row + q);
+        const double other = mine[q];
         ahead += other > score_of || (other == score_of && q < l);
       }
       kept = (uint32_t)(__ballot(ahead < a.rule.group_top && score_of > none) >> (16 * row)) & 0xFFFFu;
@@ -383,7 +387,9 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteArgs 
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const bool in = a.rule.group_count == 1 || (kept >> ((uint32_t)expert(i) * a.each_inverse >> 20 & 31) & 1);
-      key[i] = in && c[i] > none ? route_key(c[i]) : 0;
+      const uint64_t k = route_key(c[i]);
+      key[i] = in && c[i] > none ? (uint32_t)(k >> 32) : 0;
+      low[i] = (uint32_t)k;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   } else {
@@ -391,29 +397,28 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(RouteArgs 
     for (int i = 0; i < PER; ++i) key[i] = v[i] == -__builtin_inff() ? 0 : route_key(v[i]);
   }
   // the best, one at a time, by upper words; wave lane j of a row keeps the j-th's
-  auto high = [](Key k) { return WIDE ? (uint32_t)((uint64_t)k >> 32) : (uint32_t)k; };
   int chosen = -1;
   for (int j = 0; j < a.rule.top; ++j) {
     uint32_t word = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) word = max(word, high(key[i]));
+    for (int i = 0; i < PER; ++i) word = max(word, key[i]);
     const uint32_t most = row_max_u32(word);
     uint32_t at = ~0u;
     int holders = 0;
 #pragma unroll
     for (int i = PER - 1; i >= 0; --i) {
-      const bool holds = high(key[i]) == most;
+      const bool holds = key[i] == most;
       at = holds ? 64 * (i / 4) + i % 4 : at;
       if (WIDE) holders += __builtin_popcountll(__ballot(holds));
     }
     if (WIDE && holders > 4) {  // upper words are seldom equal
-      uint32_t low = 0;
+      uint32_t rest = 0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) low = max(low, high(key[i]) == most ? (uint32_t)key[i] : 0u);
-      const uint32_t rest = row_max_u32(low);
+      for (int i = 0; i < PER; ++i) rest = max(rest, key[i] == most ? low[WIDE ? i : 0] : 0u);
+      rest = row_max_u32(rest);
       at = ~0u;
 #pragma unroll
-      for (int i = PER - 1; i >= 0; --i) at = high(key[i]) == most && (uint32_t)key[i] == rest ? 64 * (i / 4) + i % 4 : at;
+      for (int i = PER - 1; i >= 0; --i) at = key[i] == most && low[WIDE ? i : 0] == rest ? 64 * (i / 4) + i % 4 : at;
     }
     const int e = (int)row_min_u32(at != ~0u ? at + 4 * l : ~0u);  // of equal ones the lowest
     if (__ballot(most > 0) == 0) break;

@@ -111,6 +111,18 @@ def test_route_of_equal_and_of_no_numbers(backend, r, count, biased, times):
     check_route(backend, np.tile(logits, (times, 1)), r, bias)
 
 
+@pytest.mark.parametrize("lanes", [3, 2100])
+@pytest.mark.parametrize("count", [9, 64, 200])
+def test_route_of_zeros_of_both_signs(backend, count, lanes):
+    """Equal numbers, the lowest index first."""
+    rng = np.random.default_rng(count)
+    logits = np.where(rng.random((lanes, count)) < 0.5, np.float32(-0.0), np.float32(0.0))
+    bias = np.where(rng.random(count) < 0.5, np.float32(-0.0), np.float32(0.0))
+    for score in ("softmax", "sigmoid"):
+        check_route(backend, logits, {"top": 5, "score": score})
+        check_route(backend, logits, {"top": 5, "score": score}, bias)
+
+
 def test_route_next_to_each_other(backend):
     """Logits and biases one float apart fall as the reals do."""
     rng = np.random.default_rng(4)

@@ -282,6 +282,9 @@ __global__ __launch_bounds__(256) void mx4_terms_kernel(const void *act, long lo
 // hidden values; from tiles as terms for the product behind).
 enum { kOutF32 = 0, kOutBf16 = 1, kOutGate = 2 };
 
+// Hidden values are formed in single precision whatever the lanes' type, and keep it.
+constexpr int kHiddenTerms = 5;
+
 // Rows of a microscaled weight; in a batch of experts expert e's rows begin at
 // row e * rows_each.
 struct Mx4View {
@@ -883,13 +886,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
       }
       uint8_t *const h = static_cast<uint8_t *>(g.out);
       const size_t to = (size_t)(first + place), of = (size_t)g.out_stride;
-      constexpr int kTerms = T == 0 ? 3 : T;
-      auto step = [&](int group) { return h + (size_t)(group >> 2) * of * TermForm<kTerms>::kStep; };
-      mx4_terms<kTerms>(x, step(group), to, of, group & 3);
+      auto step = [&](int group) { return h + (size_t)(group >> 2) * of * TermForm<kHiddenTerms>::kStep; };
+      mx4_terms<kHiddenTerms>(x, step(group), to, of, group & 3);
       if (group + 1 == inner_groups)  // the groups behind the last are zeros
         for (int z = group + 1; z < 4 * mx4_steps(inner_groups); ++z)
-          for (int c = 0; c < TermForm<kTerms>::kChunks; ++c)
-            *reinterpret_cast<uint4_t *>(step(z) + term_piece<kTerms>(to, of, c, z & 3)) = uint4_t{0, 0, 0, 0};
+          for (int c = 0; c < TermForm<kHiddenTerms>::kChunks; ++c)
+            *reinterpret_cast<uint4_t *>(step(z) + term_piece<kHiddenTerms>(to, of, c, z & 3)) = uint4_t{0, 0, 0, 0};
     }
     return;
   }
@@ -1353,8 +1355,9 @@ __global__ __launch_bounds__(64 * kHeadWaves, 2) void mx4_head_kernel(Mx4Args g)
 // The down products of a token's experts and their sum: blockIdx.y a lane, eight waves, each
 // every eighth of its choices (its hidden values cut by the wave), sixteen rows.  Eight of
 // 128 experts, 1536 and 768: 6.2 us behind 7.5 of gate and up; by experts, in five launches, 49.
-template <int T, bool BF16>
+template <bool BF16>
 __global__ __launch_bounds__(512) void expert_step_kernel(Mx4Args g, const float *hidden, const float *weight, void *out) {
+  constexpr int T = kHiddenTerms;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_x[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int part = lane >> 4, at = lane & 15;
@@ -1915,7 +1918,7 @@ static hipError_t experts_grouped(const ExpertCall &c, hipStream_t stream) {
   a.row_scales = p.rows.dst;
   a.out = c.base + r.rows;
   a.out_stride = x->hidden;
-  if ((e = launch_tile<T, MT, NT, WM, WN, ST, kOutF32>(a, tiles, 1, stream)) != hipSuccess) return e;
+  if ((e = launch_tile<kHiddenTerms, MT, NT, WM, WN, ST, kOutF32>(a, tiles, 1, stream)) != hipSuccess) return e;
   const unsigned blocks = (unsigned)(((long long)c.lanes * (x->hidden / 4) + 255) / 256);
   if (c.out_bf16)
     hipLaunchKernelGGL((expert_join_kernel<true>), dim3(blocks), dim3(256), 0, stream, (const float *)(c.base + r.rows),
@@ -1949,16 +1952,16 @@ static hipError_t experts_step(const ExpertCall &c, hipStream_t stream) {
   a.rows = x->hidden;
   a.groups = x->inner / kMx4Group;
   a.out_stride = c.out_stride;
-  const size_t lds = step_lds<T>(a.groups, 1, 1, 8, 1);
+  const size_t lds = step_lds<kHiddenTerms>(a.groups, 1, 1, 8, 1);
   const dim3 grid((x->hidden + 15) / 16, c.lanes);
   if (c.out_bf16) {
     static size_t granted16 = 0;
-    if ((e = grant_lds(&expert_step_kernel<T, true>, kExpertLds, granted16)) != hipSuccess) return e;
-    hipLaunchKernelGGL((expert_step_kernel<T, true>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
+    if ((e = grant_lds(&expert_step_kernel<true>, kExpertLds, granted16)) != hipSuccess) return e;
+    hipLaunchKernelGGL((expert_step_kernel<true>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
                        c.weight, c.out);
   } else {
-    if ((e = grant_lds(&expert_step_kernel<T, false>, kExpertLds, granted)) != hipSuccess) return e;
-    hipLaunchKernelGGL((expert_step_kernel<T, false>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
+    if ((e = grant_lds(&expert_step_kernel<false>, kExpertLds, granted)) != hipSuccess) return e;
+    hipLaunchKernelGGL((expert_step_kernel<false>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
                        c.weight, c.out);
   }
   return hipGetLastError();
@@ -1983,10 +1986,9 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
   const long long expert_bytes = 3LL * x->hidden * x->inner * 17 / 32;
   const bool step = slots <= 64 && slots <= 20 + x->expert_count / 2 &&
                     slots * expert_bytes / (x->expert_count + slots) < (50 << 20) / slots &&
-                    (act_bf16 ? step_lds<3>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
-                                    step_lds<3>(x->inner / kMx4Group, 1, 1, 8, 1) <= kExpertLds
-                              : step_lds<5>(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
-                                    step_lds<5>(x->inner / kMx4Group, 1, 1, 8, 1) <= kExpertLds);
+                    (act_bf16 ? step_lds<3>(x->hidden / kMx4Group, 1, 2, 4, 4)
+                              : step_lds<5>(x->hidden / kMx4Group, 1, 2, 4, 4)) <= kStepLds &&
+                    step_lds<kHiddenTerms>(x->inner / kMx4Group, 1, 1, 8, 1) <= kExpertLds;
   if (step) return act_bf16 ? experts_step<3, true>(c, stream) : experts_step<5, false>(c, stream);
   // tiles of as many places as an expert has, while smaller ones are more than two workgroups a
   // CU: 12 of 64 experts 53 us in 32s and 59 in 16s (fp32; bf16 42 and 51), 16 of 128 91 and 98,

@@ -392,7 +392,8 @@ typedef struct igl_experts {
 /* out[m] = sum_j weight[m][j] down_e(gate(gate_e x[m]) * up_e x[m]), e = pick[m][j], j
  * in rising order: igl_route_dev's picks and weights, [lane_count][top].  A pick
  * outside 0 .. expert_count - 1 takes no expert; a lane without one is zero.  Lanes and
- * their precision as igl_mx4_mat_mat_dev's; out and act do not overlap.  1024 experts
+ * their precision as igl_mx4_mat_mat_dev's, hidden values that of F32 lanes whatever
+ * the lanes' type; out and act do not overlap.  1024 experts
  * at most and 64 a lane, lane_count * top times hidden, or inner, below 2^32 - 2048, and
  * lane_count * top / 16 + expert_count below 65536.  The desk's workspace grows with
  * the call's size: make the calls of a recording once before it. */

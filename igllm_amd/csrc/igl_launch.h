@@ -255,8 +255,8 @@ hipError_t igl_launch_mx4_lay(const igl_mx4 *store, int row_first, int rows, con
                               int src_stride, hipStream_t stream);
 hipError_t igl_launch_mx4_read(const igl_mx4 *store, int row_first, int rows, void *dst, int bf16,
                                int dst_stride, hipStream_t stream);
-/* terms: 5 and 3 for lanes of floats and bf16, 0 for microscaled ones. */
-size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int terms);
+/* kind: 5 for lanes of floats, 3 of bf16, 0 microscaled ones. */
+size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int kind);
 hipError_t igl_launch_mx4_mat_mat(const igl_mx4 *sheet, const void *act, int act_bf16, int act_stride,
                                   int lanes, void *out, int out_bf16, int out_stride, void *work,
                                   hipStream_t stream);

@@ -334,10 +334,10 @@ int igl_mx4_lay_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row
 int igl_mx4_read_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row_count,
                      void *dst_dev, int dst_type, int dst_stride);
 /* igl_mat_mat_dev for a microscaled sheet: out[m] = sheet x[m], lanes of act_type to
- * lanes of out_type (F32 or BF16), sums in 32 bits.  F32 lanes are taken to
- * 2^-23.9 and BF16 lanes to 2^-13.9 of the largest of their 32 values (a bf16 output has 2^-8);
- * neither finer than 2^-130 and 2^-120.  A lane with an infinity or a NaN has NaN
- * outputs.  out and act do not overlap.  Sheets of code_stride up to 2^24 and 2^27 rows,
+ * lanes of out_type (F32 or BF16), sums in 32 bits.  Lanes are taken to 2^-23.9 of
+ * the largest of their 32 values, and not finer than 2^-130: an F32 value of 2^-n of that
+ * largest has 24 - n digits, a BF16 one keeps its eight down to 2^-16 (in calls of many
+ * lanes all are exact).  A lane with an infinity or a NaN has NaN outputs.  out and act do not overlap.  Sheets of code_stride up to 2^24 and 2^27 rows,
  * 1048560 lanes.  The desk's workspace grows with the call's lanes and, from a few of
  * them on, with the sheet: make the calls of a recording once before it. */
 int igl_mx4_mat_mat_dev(igl_desk *desk, const igl_mx4 *sheet, const void *act_dev, int act_type,

@@ -1821,15 +1821,21 @@ static int mx4_form(int rows, int groups, int lanes, int kind) {
   return large ? kFormLarge : kFormSmall;
 }
 
-// Enough for any form of a product: its lanes as terms, or their scales, the sheet's scales
-// packed (eight tiles a block at most), and slices' sums.
+// A token's step: its kernel cuts the lanes itself.
+static bool mx4_single(int rows, int groups, int lanes, int form, int kind) {
+  return kind != kMx4Lanes && form != kFormHead && lanes <= 3 && (lanes == 1 || mx4_bytes(rows, groups) < kFewBytes) &&
+         step_lds(groups, lanes, 1, 4, 4) <= kStepLds;
+}
+
+// What a product's form uses: its lanes as terms, or their scales, the sheet's scales packed (eight
+// tiles a block at most), and slices' sums; a token's step and a head nothing.
 extern "C" size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int kind) {
   const int groups = cols / kMx4Group, form = mx4_form(rows, groups, lanes, kind);
   const bool plain = kind == kBf16Lanes && (form == kFormLarge || form == kFormWhole);
   const size_t of_lanes = kind == kMx4Lanes ? pack_bytes<4, false>(lanes, groups, 1)
                           : plain           ? terms_bytes<kPlain>(lanes, cols)
                                             : terms_bytes<kTerms>(lanes, cols);
-  if (form == kFormHead) return 0;
+  if (form == kFormHead || mx4_single(rows, groups, lanes, form, kind)) return 0;
   if (form == kFormFew) return kind == kMx4Lanes ? 0 : of_lanes;
   const int slices = form == kFormSmall ? mx4_slices(rows, groups, lanes, kind == kMx4Lanes ? 64 : 32, 256) : 1;
   return of_lanes + pack_bytes<8, false>(rows, groups, 1) +
@@ -1839,12 +1845,11 @@ extern "C" size_t igl_mx4_work_bytes(int rows, int cols, int lanes, int kind) {
 // A product of lanes of floats, by its form.
 template <bool BF16>
 static hipError_t launch_floats(Mx4Args a, const void *act, int act_stride, int out_bf16, uint8_t *room, hipStream_t stream) {
-  const int form = mx4_form(a.rows, a.groups, a.lanes, BF16 ? kBf16Lanes : kF32Lanes);
-  const bool single = form != kFormHead && a.lanes <= 3 && (a.lanes == 1 || mx4_bytes(a.rows, a.groups) < kFewBytes) &&
-                      step_lds(a.groups, a.lanes, 1, 4, 4) <= kStepLds;
+  constexpr int kKind = BF16 ? kBf16Lanes : kF32Lanes;
+  const int form = mx4_form(a.rows, a.groups, a.lanes, kKind);
   a.act_rows = act;
   a.act_stride = act_stride;
-  if (single) {
+  if (mx4_single(a.rows, a.groups, a.lanes, form, kKind)) {
     const dim3 grid((a.rows + 15) / 16);
     return out_bf16 ? launch_step<1, kOutBf16, BF16>(a, grid, a.lanes, stream)
                     : launch_step<1, kOutF32, BF16>(a, grid, a.lanes, stream);
@@ -1927,10 +1932,22 @@ static ExpertRoom expert_room(const igl_experts *x, int lanes, int top, int /* o
   r.x = take(terms_bytes<kTerms>(lanes, x->hidden));
   r.gate_up = take(pack_bytes<8, true>(2 * x->inner, x->hidden / kMx4Group, x->expert_count));
   r.down = take(pack_bytes<8, false>(x->hidden, x->inner / kMx4Group, x->expert_count));
-  r.h = take(terms_bytes<kTerms>((int)slots, x->inner));  // as floats (a token's step) they are no more
+  r.h = take(terms_bytes<kTerms>((int)slots, x->inner));
   r.rows = take(slots * x->hidden * sizeof(float));
   r.end = at;
   return r;
+}
+
+// Whether a call's slots are taken one by one.  That reads an expert's weights for each, by
+// experts takes two launches more: up to a count, and while what is read twice (slots^2 /
+// (experts + slots) of them where picks are even) is less than those launches.  48 slots of 64
+// experts 34 us for 39, 64 of 128 42 for 46, 32 of eight 26 for 24; 32 of sixteen of 13 MB
+// each 165 for 59
+static bool expert_steps(const igl_experts *x, int slots) {
+  const long long expert_bytes = 3LL * x->hidden * x->inner * 17 / 32;
+  return slots <= 64 && slots <= 20 + x->expert_count / 2 &&
+         slots * expert_bytes / (x->expert_count + slots) < (50 << 20) / slots &&
+         step_lds(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds && step_lds(x->inner / kMx4Group, 1, 1, 8, 1) <= kExpertLds;
 }
 
 // What an experts' call is: its arguments and its room.
@@ -2015,7 +2032,7 @@ static hipError_t experts_step(const ExpertCall &c, hipStream_t stream) {
   a.experts = x->expert_count;
   a.top = c.top;
   a.silu = x->gate == IGL_GATE_SILU;
-  a.out = c.base + c.room.h;
+  a.out = c.base;  // hidden values as floats, all it keeps
   hipError_t e = launch_step<2, kOutGate, BF16>(a, dim3((x->inner + 15) / 16, c.lanes * c.top), 1, stream);
   if (e != hipSuccess) return e;
   a.w = mx4_view(&x->down, 0);
@@ -2027,11 +2044,11 @@ static hipError_t experts_step(const ExpertCall &c, hipStream_t stream) {
   if (c.out_bf16) {
     static size_t granted16 = 0;
     if ((e = grant_lds(&expert_step_kernel<true>, kExpertLds, granted16)) != hipSuccess) return e;
-    hipLaunchKernelGGL((expert_step_kernel<true>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
+    hipLaunchKernelGGL((expert_step_kernel<true>), grid, dim3(512), lds, stream, a, (const float *)c.base,
                        c.weight, c.out);
   } else {
     if ((e = grant_lds(&expert_step_kernel<false>, kExpertLds, granted)) != hipSuccess) return e;
-    hipLaunchKernelGGL((expert_step_kernel<false>), grid, dim3(512), lds, stream, a, (const float *)(c.base + c.room.h),
+    hipLaunchKernelGGL((expert_step_kernel<false>), grid, dim3(512), lds, stream, a, (const float *)c.base,
                        c.weight, c.out);
   }
   return hipGetLastError();
@@ -2040,7 +2057,8 @@ static hipError_t experts_step(const ExpertCall &c, hipStream_t stream) {
 }  // namespace igl
 
 extern "C" size_t igl_experts_work_bytes(const igl_experts *x, int lanes, int top, int act_bf16) {
-  return expert_room(x, lanes, top, act_bf16).end;
+  return expert_steps(x, lanes * top) ? mx4_up((size_t)lanes * top * x->inner * sizeof(float))
+                                      : expert_room(x, lanes, top, act_bf16).end;
 }
 
 extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, int act_bf16, int act_stride, int lanes,
@@ -2048,17 +2066,8 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
                                          int out_stride, void *work, hipStream_t stream) {
   const ExpertCall c = {x,   act,      act_stride, lanes, pick, weight, top,
                         out, out_bf16, out_stride, static_cast<uint8_t *>(work), expert_room(x, lanes, top, act_bf16)};
-  // a slot at a time reads an expert's weights for each, by experts takes two launches more: up
-  // to a count, and while what is read twice (slots^2 / (experts + slots) of them where picks
-  // are even) is less than those launches.  48 slots of 64 experts 34 us for 39, 64 of 128 42 for 46,
-  // 32 of eight 26 for 24; 32 of sixteen of 13 MB each 165 for 59
   const int slots = lanes * top;
-  const long long expert_bytes = 3LL * x->hidden * x->inner * 17 / 32;
-  const bool step = slots <= 64 && slots <= 20 + x->expert_count / 2 &&
-                    slots * expert_bytes / (x->expert_count + slots) < (50 << 20) / slots &&
-                    step_lds(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds &&
-                    step_lds(x->inner / kMx4Group, 1, 1, 8, 1) <= kExpertLds;
-  if (step) return act_bf16 ? experts_step<true>(c, stream) : experts_step<false>(c, stream);
+  if (expert_steps(x, slots)) return act_bf16 ? experts_step<true>(c, stream) : experts_step<false>(c, stream);
   // tiles of as many places as an expert has, while smaller ones are more than two workgroups a
   // CU: 12 of 64 experts 44 us in 32s and 51 in 16s, 16 of 128 79 and 84, but 16 of 32 48 and 44;
   // 64 of eight small ones 24 in 16s and 26 in 32s.  In 64s, of which an expert's last is nearly

@@ -6,7 +6,8 @@
 //     the chosen are the largest c among them, the lowest index first where equal
 //     w = s of the chosen (over their sum), times the rule's gain and the expert's
 // A choice next to another's must fall as the reals' does, so scores are formed and
-// compared in double; without a bias and groups s rises with x, and x decides.
+// compared in double.  Without a bias and groups s rises with x, and x decides, also where
+// scores are one double (sigmoid's 1 of logits above 37).
 #pragma once
 
 #include <type_traits>

@@ -371,10 +371,13 @@ typedef struct igl_route {
  * the group_top groups of the largest group scores stay; the `top` largest choices in
  * falling order, the lowest index first where equal.  A weight is the chosen s (over
  * the sum of the lane's with renorm; zero where that is zero), times gain_scale and
- * gain_dev[e] (may be NULL).  Choices are formed and compared in 64 bits.  An expert
- * whose logit is minus infinity or a NaN, or whose choice is, is never chosen; a lane
- * with too few has -1 and weight 0 in the places left over.  A logit of plus infinity
- * counts as the largest float. */
+ * gain_dev[e] (may be NULL).  Without a bias and groups the logits are compared, whose
+ * order is the scores'.  Else choices are formed and compared in 64 bits, and scores that
+ * are one number there (sigmoid's of all logits above 37, softmax's of logits 746 and more
+ * below the lane's largest) are equal: a bias of zeros may choose otherwise than none.
+ * An expert whose logit is minus infinity or a NaN, or whose choice is, is never chosen;
+ * a lane with too few has -1 and weight 0 in the places left over.  A logit of plus
+ * infinity counts as the largest float. */
 int igl_route_dev(igl_desk *desk, const igl_route *rule, const float *logit_dev, int logit_stride,
                   int lane_count, const float *bias_dev, const float *gain_dev, int32_t *pick_dev,
                   float *weight_dev);

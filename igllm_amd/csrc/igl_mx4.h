@@ -118,8 +118,8 @@ __global__ __launch_bounds__(256) void mx4_lay_kernel(const void *src, long long
   if ((at & 3) == 0) scale[(size_t)row * scale_stride + (at >> 2)] = (uint8_t)byte;
 }
 
-// Eight values a thread.  A level times its power of two is exact (a NaN scale gives NaN); rounded to bf16
-// none is lost either, but below 2^-126, where bf16's digits end.
+// Eight values a thread.  A level times its power of two is exact (a NaN scale gives NaN) below 2^128; rounded to
+// bf16 none is lost either, but below 2^-126, where bf16's digits end.
 template <bool BF16>
 __global__ __launch_bounds__(256) void mx4_read_kernel(const uint8_t *code, size_t code_stride, const uint8_t *scale,
                                                        size_t scale_stride, int eighths, int rows, void *dst,

@@ -326,20 +326,23 @@ typedef struct igl_mx4 {
 /* Rows of floats (IGL_STORE_F32 or IGL_STORE_BF16, src_stride values apart) into
  * rows row_first .. + row_count - 1: a group's power of two is two below its largest
  * magnitude's (2^-127 at least), a value's code the nearest level, ties to the even
- * code, 6 at most.  A group with an infinity or a NaN gets scale 255 and codes 0. */
+ * code, 6 at most.  A group with an infinity or a NaN gets scale 255 and codes 0.  Up to
+ * 2^35 - 2048 values a call, as for reading. */
 int igl_mx4_lay_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row_count,
                     const void *src_dev, int src_type, int src_stride);
 /* Rows as floats again: level * 2^(b - 127), exactly but where F32 or BF16 has no
- * such small number. */
+ * such small number, or no such large one (2^128 and more are infinite). */
 int igl_mx4_read_dev(igl_desk *desk, const igl_mx4 *store, int row_first, int row_count,
                      void *dst_dev, int dst_type, int dst_stride);
 /* igl_mat_mat_dev for a microscaled sheet: out[m] = sheet x[m], lanes of act_type to
  * lanes of out_type (F32 or BF16), sums in 32 bits.  Lanes are taken to 2^-23.9 of
  * the largest of their 32 values, and not finer than 2^-130: an F32 value of 2^-n of that
  * largest has 24 - n digits, a BF16 one keeps its eight down to 2^-16 (in calls of many
- * lanes all are exact).  A lane with an infinity or a NaN has NaN outputs.  out and act do not overlap.  Sheets of code_stride up to 2^24 and 2^27 rows,
- * 1048560 lanes.  The desk's workspace grows with the call's lanes and, from a few of
- * them on, with the sheet: make the calls of a recording once before it. */
+ * lanes all are exact).  A lane with an infinity or a NaN has NaN outputs.  Values of a
+ * sheet from 2^128 on may count as infinite, and sums from 2^127 on, on their way too.
+ * out and act do not overlap.  Sheets of code_stride up to 2^24 and 2^27 rows, 1048560
+ * lanes and 2^35 - 2048 of their values.  The desk's workspace grows with the call's lanes
+ * and, from a few of them on, with the sheet: make the calls of a recording once before it. */
 int igl_mx4_mat_mat_dev(igl_desk *desk, const igl_mx4 *sheet, const void *act_dev, int act_type,
                         int act_stride, int lane_count, void *out_dev, int out_type,
                         int out_stride);

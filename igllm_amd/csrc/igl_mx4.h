@@ -1950,6 +1950,18 @@ static bool expert_steps(const igl_experts *x, int slots) {
          step_lds(x->hidden / kMx4Group, 1, 2, 4, 4) <= kStepLds && step_lds(x->inner / kMx4Group, 1, 1, 8, 1) <= kExpertLds;
 }
 
+// Tiles of as many places as an expert has, while smaller ones are more than two workgroups a
+// CU: 12 of 64 experts 44 us in 32s and 51 in 16s, 16 of 128 79 and 84, but 16 of 32 48 and 44;
+// 64 of eight small ones 24 in 16s and 26 in 32s.  In 64s, of which an expert's last is nearly
+// empty, bf16 lanes win from 60 on (62 of 16 70 and 76 in 32s, 64 of 128 150 and 154; 56 of 64
+// 85 and 76), fp32 ones, whose tiles of 64 leave a CU one workgroup, from 250 (125 of 32 140 and 116,
+// 256 of 128 472 and 483)
+static int expert_tile(const igl_experts *x, int slots, int bf16) {
+  const int each = slots / x->expert_count, blocks = (2 * x->inner + 255) / 256;
+  auto groups = [&](int tile) { return (long long)expert_tiles(slots, x->expert_count, tile) * blocks; };
+  return each >= (bf16 ? 60 : 250) && groups(32) >= 520 ? 64 : each >= 12 && groups(16) >= 520 ? 32 : 16;
+}
+
 // What an experts' call is: its arguments and its room.
 struct ExpertCall {
   const igl_experts *x;
@@ -2068,15 +2080,7 @@ extern "C" hipError_t igl_launch_experts(const igl_experts *x, const void *act, 
                         out, out_bf16, out_stride, static_cast<uint8_t *>(work), expert_room(x, lanes, top, act_bf16)};
   const int slots = lanes * top;
   if (expert_steps(x, slots)) return act_bf16 ? experts_step<true>(c, stream) : experts_step<false>(c, stream);
-  // tiles of as many places as an expert has, while smaller ones are more than two workgroups a
-  // CU: 12 of 64 experts 44 us in 32s and 51 in 16s, 16 of 128 79 and 84, but 16 of 32 48 and 44;
-  // 64 of eight small ones 24 in 16s and 26 in 32s.  In 64s, of which an expert's last is nearly
-  // empty, bf16 lanes win from 60 on (62 of 16 70 and 76 in 32s, 64 of 128 150 and 154; 56 of 64
-  // 85 and 76), fp32 ones, whose tiles of 64 leave a CU one workgroup, from 250 (125 of 32 140 and 116,
-  // 256 of 128 472 and 483)
-  const int each = slots / x->expert_count, blocks = (2 * x->inner + 255) / 256;
-  auto groups = [&](int tile) { return (long long)expert_tiles(slots, x->expert_count, tile) * blocks; };
-  const int tile = each >= (act_bf16 ? 60 : 250) && groups(32) >= 520 ? 64 : each >= 12 && groups(16) >= 520 ? 32 : 16;
+  const int tile = expert_tile(x, slots, act_bf16);
   if (act_bf16)
     return tile == 64   ? experts_grouped<kPlain, 2, 4, 2, 4, 2, true>(c, stream)
            : tile == 32 ? experts_grouped<kTerms, 1, 4, 2, 4, 2, true>(c, stream)

@@ -38,6 +38,20 @@ extern "C" int planmx_room(int experts, int hidden, int inner, int lanes, int to
   return 0;
 }
 
+// The places of a call's tiles of experts, or zero where slots are taken one by one.
+extern "C" int planmx_experts(int experts, int hidden, int inner, int lanes, int top, int bf16) {
+  igl_experts x = {};
+  x.expert_count = experts;
+  x.hidden = hidden;
+  x.inner = inner;
+  return expert_steps(&x, lanes * top) ? 0 : expert_tile(&x, lanes * top, bf16);
+}
+
+// Whether a product is a token's step.
+extern "C" int planmx_single(int rows, int cols, int lanes, int kind) {
+  return mx4_single(rows, cols / kMx4Group, lanes, mx4_form(rows, cols / kMx4Group, lanes, kind), kind);
+}
+
 // Zero, or a slot whose lane is not slot / top.
 extern "C" int planmx_lanes(int top) {
   for (int slot = 0; slot < 1 << 20; ++slot)

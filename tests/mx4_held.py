@@ -45,6 +45,23 @@ FORMS = [(1, 416, 416, STEP, STEP, FEW), (3, 1000, 96, STEP, STEP, FEW), (5, 300
          (300, 1537, 544, SMALL, SMALL, FEW), (513, 4100, 288, SMALL, SMALL, SMALL), (500, 6150, 416, SMALL, LARGE, SMALL),
          (1540, 7690, 160, LARGE, WHOLE, LARGE), (2050, 8190, 416, LARGE, WHOLE, LARGE)]
 
+# of rows that lie apart (bytes; None: as far as reaches past 4 GiB)
+FAR = [(5, 32776, 1760, HEAD, HEAD, FEW), (16, 32776, 1760, TALL, TALL, FEW), (70, 2400, 4128, SMALL, SMALL, SMALL),
+       (300, 1537, 544, SMALL, SMALL, FEW), (500, 6150, 416, SMALL, LARGE, SMALL), (1540, 7690, 160, LARGE, WHOLE, LARGE),
+       (21, 272, 3232, SMALL, SMALL, FEW), (3, 272, 3232, STEP, STEP, FEW)]
+STRIDES = [None] * 6 + [1 << 24] * 2
+
+# Experts' blocks that pass values through: (lanes, hidden, inner), and the places of their tiles (0: a token's step)
+BLOCKS = [(1, 512, 512, 0), (5, 96, 96, 0), (40, 512, 512, 16), (600, 2048, 2048, 32), (1200, 2048, 2048, 64)]
+UPS = [(1, 512, 256, 0), (5, 64, 32, 0), (40, 512, 256, 16), (600, 4096, 2048, 32), (1200, 4096, 2048, 64)]
+# of many slots: (experts, hidden, inner, choices, lanes, places for fp32 lanes, for bf16 ones)
+SLOTS = [(6, 64, 32, 6, 520, 16, 16), (16, 64, 32, 8, 2048, 64, 64), (16, 32, 32, 8, 2049, 64, 64), (16, 64, 32, 8, 4096, 64, 64),
+         (130, 32, 64, 5, 3300, 32, 64), (4, 32, 32, 1, 20000, 64, 64), (3, 96, 2080, 2, 2500, 64, 64),
+         (40, 32, 1056, 4, 1500, 32, 64), (200, 32, 32, 64, 1100, 64, 64)]
+# of many choices
+CHOICES = [(64, 160, 96, 9, 1, 0, 0), (90, 320, 64, 64, 1, 0, 0), (128, 96, 160, 16, 4, 0, 0), (40, 64, 224, 17, 2, 0, 0),
+           (40, 64, 96, 20, 37, 16, 16), (70, 96, 32, 64, 50, 16, 16)]
+
 
 def wide_lanes(lanes, cols, bf16, spread=3.0):
     """Lanes whose groups span many binades."""

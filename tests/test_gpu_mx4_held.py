@@ -11,7 +11,7 @@ from test_gpu_mx4 import BF16, F32, close, get, hold, put, sheet
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("lanes,width", [(1, 512), (5, 96), (40, 512), (600, 2048), (1200, 2048)])  # a step; tiles of 16, 32, 64
+@pytest.mark.parametrize("lanes,width", [b[:2] for b in held.BLOCKS])
 @pytest.mark.parametrize("kind", [F32, BF16])
 @pytest.mark.parametrize("gate", [native.IGL_GATE_GELU, native.IGL_GATE_SILU])
 def test_hidden_values(backend, lanes, width, kind, gate):
@@ -54,7 +54,7 @@ def test_microscaled_values(backend, case):
     close(rows_held, act, out)
 
 
-@pytest.mark.parametrize("lanes,width", [(1, 512), (5, 64), (40, 512), (600, 4096), (1200, 4096)])  # a step; tiles of 16, 32, 64
+@pytest.mark.parametrize("lanes,width", [b[:2] for b in held.UPS])
 @pytest.mark.parametrize("kind", [F32, BF16])
 def test_up_values(backend, lanes, width, kind):
     """What the experts' up products pass through."""

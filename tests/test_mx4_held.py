@@ -51,13 +51,20 @@ def test_outliers():
         assert (off <= 2.0 ** -16 * np.abs(x[:, rest]).sum(1)).all() == (terms == 5)
 
 
-@pytest.mark.parametrize("case", held.FORMS)
+@pytest.mark.parametrize("case", held.FORMS + held.FAR)
 def test_forms(lib, case):  # noqa: F811
     """Which form every case takes, so that a change of the rule cannot leave one without tests."""
     lanes, rows, cols = case[:3]
     for kind, form in zip((5, 3, 0), case[3:]):
-        got = lib.planmx_form(rows, cols, lanes, kind)
-        assert got == form if form >= 0 else (lanes <= 3 and got != held.HEAD and rows * cols // 32 * 17 < 28 << 20)
+        single = lib.planmx_single(rows, cols, lanes, kind)
+        assert single if form == held.STEP else not single and lib.planmx_form(rows, cols, lanes, kind) == form
+
+
+def test_experts_forms(lib):  # noqa: F811
+    for lanes, hidden, inner, places in held.BLOCKS + held.UPS:
+        assert {lib.planmx_experts(1, hidden, inner, lanes, 1, bf16) for bf16 in (0, 1)} == {places}
+    for case in held.SLOTS + held.CHOICES:
+        assert [lib.planmx_experts(*case[:3], case[4], case[3], bf16) for bf16 in (0, 1)] == list(case[5:]), case
 
 
 def test_every_form_is_there(lib):  # noqa: F811

@@ -400,10 +400,10 @@ typedef struct igl_experts {
  * calls of other lane counts a lane's sums may be added in another order.  A pick
  * outside 0 .. expert_count - 1 takes no expert; a lane without one is zero.  Lanes and
  * their precision as igl_mx4_mat_mat_dev's, hidden values that of F32 lanes whatever
- * the lanes' type; out and act do not overlap.  1024 experts at most and 64 a lane,
- * lane_count * top times hidden, or inner, up to 2^32 - 2048, and lane_count * top / 16 +
- * expert_count below 65536.  The desk's workspace grows with the call's size: make the
- * calls of a recording once before it. */
+ * the lanes' type (one past the largest float makes its lane's outputs NaN); out and act
+ * do not overlap.  1024 experts at most and 64 a lane, lane_count * top times hidden, or
+ * inner, up to 2^32 - 2048, and lane_count * top / 16 + expert_count below 65536.  The
+ * desk's workspace grows with the call's size: make the calls of a recording once before it. */
 int igl_experts_dev(igl_desk *desk, const igl_experts *experts, const void *act_dev, int act_type,
                     int act_stride, int lane_count, const int32_t *pick_dev,
                     const float *weight_dev, int top, void *out_dev, int out_type, int out_stride);

@@ -252,3 +252,93 @@ def test_many_choices(backend, count, hidden, inner, top, lanes, kind):
         want, reach = block.want(x, pick, weight)
         assert (np.abs(got - want) <= block.tol(reach, F32, out_kind, want)).all()
     close(*block.held)
+
+
+BLOCKS = pytest.mark.parametrize("count,hidden,inner,top,lanes", [(16, 96, 160, 4, 1), (8, 224, 96, 3, 37), (5, 64, 2080, 2, 800)])
+
+
+@BLOCKS
+@pytest.mark.parametrize("kind,out_kind", [(F32, F32), (BF16, BF16), (BF16, F32), (F32, BF16)])
+def test_experts_at_odd_addresses(backend, count, hidden, inner, top, lanes, kind, out_kind):
+    """Lanes and outputs at the least alignment of their types, rows of odd strides; nothing else written."""
+    rng = np.random.default_rng(lanes)
+    block = Block(backend, rng, count, hidden, inner)
+    wide, far = hidden + 3, hidden + 1
+    x = mx.bf16(rng.normal(size=(lanes, hidden)))
+    host = np.full((lanes, wide), 9.0, np.float32)
+    host[:, :hidden] = x
+    pick, weight = picks(rng, lanes, count, top)
+    p, w = backend.upload(pick), backend.upload(weight.astype(np.float32))
+    size, out_size = (2 if kind == BF16 else 4), (2 if out_kind == BF16 else 4)
+    act = backend.alloc(size * (lanes * wide + 8))
+    want, reach = block.want(x, pick, weight.astype(np.float32))
+    for shift in (1, 3):
+        act.put(mx.bf16_bits(host) if kind == BF16 else host, shift * size)
+        out = put(backend, np.full(lanes * far + 16, 7.5, np.float32), out_kind)
+        backend.experts_dev(block.set, At(act, shift * size), kind, wide, lanes, p, w, top, At(out, shift * out_size), out_kind, far)
+        raw = get(out, (lanes * far + 16,), out_kind)
+        got = raw[shift:shift + lanes * far].reshape(lanes, far)
+        assert (raw[:shift] == 7.5).all() and (raw[shift + lanes * far:] == 7.5).all() and (got[:, hidden:] == 7.5).all()
+        assert (np.abs(got[:, :hidden] - want) <= block.tol(reach, F32, out_kind, want)).all()
+        close(out)
+    close(*block.held, act, p, w)
+
+
+@BLOCKS
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_two_recordings(backend, count, hidden, inner, top, lanes, kind):
+    """An experts' call and a product, recorded apart over one workspace and replayed in turns over new lanes."""
+    rng = np.random.default_rng(lanes + 1)
+    block, w = Block(backend, rng, count, hidden, inner), sheet(rng, 2500, hidden)
+    rows_held, act = hold(backend, *w), Lanes(backend, lanes, hidden, kind)
+    out, sums = backend.alloc(4 * lanes * hidden), backend.alloc(4 * lanes * 2500)
+    pick, weight = picks(rng, lanes, count, top)
+    p, q = backend.upload(pick), backend.upload(weight.astype(np.float32))
+    calls = (lambda: backend.experts_dev(block.set, act.buf, kind, hidden, lanes, p, q, top, out, F32, hidden),
+             lambda: act.product(rows_held, 2500, sums))
+    act.new(rng)
+    for call in calls:
+        call()
+    replays = []
+    for call in calls:
+        backend.record_begin()
+        call()
+        replays.append(backend.record_end())
+    try:
+        for _ in range(3):
+            x = act.new(rng)
+            for call in calls:
+                call()
+            want = get(out, (lanes, hidden), F32), get(sums, (lanes, 2500), F32)
+            exact, reach = block.want(x, pick, weight.astype(np.float32))
+            assert (np.abs(want[0] - exact) <= block.tol(reach, F32, F32, exact)).all()
+            out.put(np.zeros(lanes * hidden, np.float32))
+            sums.put(np.zeros(lanes * 2500, np.float32))
+            for replay in replays[::-1]:
+                backend.replay_run(replay)
+            backend.sync()
+            assert np.array_equal(get(out, (lanes, hidden), F32), want[0]) and np.array_equal(get(sums, (lanes, 2500), F32), want[1])
+    finally:
+        for replay in replays:
+            backend.replay_free(replay)
+    close(*block.held, rows_held, act.buf, out, sums, p, q)
+
+
+@BLOCKS
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_experts_of_no_numbers(backend, count, hidden, inner, top, lanes, kind):
+    """A lane with an infinity or a NaN has NaN outputs, and so has one whose hidden values pass the largest float; the
+    others have theirs."""
+    rng = np.random.default_rng(lanes + 2)
+    block = Block(backend, rng, count, hidden, inner)
+    x = mx.bf16(rng.normal(size=(lanes, hidden)))
+    pick, weight = picks(rng, lanes, count, top)
+    want, reach = block.want(x, pick, weight)
+    bad = np.arange(0, lanes, 4)
+    x[bad[::3], hidden // 2], x[bad[1::3], 0] = np.inf, np.nan
+    x[bad[2::3]] = mx.bf16(1e30 * x[bad[2::3]])
+    got = run(backend, block, x, pick, weight, kind, F32)
+    good = np.setdiff1d(np.arange(lanes), bad)
+    assert np.isnan(got[bad]).all()
+    assert (np.abs(got - want) <= block.tol(reach, F32, F32, want))[good].all()
+    close(*block.held)

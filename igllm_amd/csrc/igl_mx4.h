@@ -793,7 +793,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
       for (int i = 0; i < F::kLoads; ++i) bring(k_ahead, s + ST - 1, i);
     }
     if (!busy) return;
-    // What the loads ahead take their turns with: after every `runs`-th part of the products
+    // A share of the loads ahead, behind the run-th of `runs` parts of the products
     auto spread = [&](int run, auto runs) {
       constexpr int kEach = (F::kLoads + decltype(runs)::value - 1) / decltype(runs)::value;
       if (kBring && F::kSpread) {
@@ -878,23 +878,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(Mx4Args g) {
         ls = *reinterpret_cast<const int *>(st + F::kLaneScalesAt + wm * 256 + lane * 4);
       }
 #define MX4_PRODUCT(I, J, A, FMT, OPSEL, SCALE)                                                                      \
-    switch (J % 4) {                                                                                                   \
-      case 0:                                                                                                          \
-        acc[I][J] =                                                                                                    \
-            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 0, ws[J / 4], OPSEL, SCALE);  \
-        break;                                                                                                         \
-      case 1:                                                                                                          \
-        acc[I][J] =                                                                                                    \
-            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 1, ws[J / 4], OPSEL, SCALE);  \
-        break;                                                                                                         \
-      case 2:                                                                                                          \
-        acc[I][J] =                                                                                                    \
-            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 2, ws[J / 4], OPSEL, SCALE);  \
-        break;                                                                                                         \
-      default:                                                                                                         \
-        acc[I][J] =                                                                                                    \
-            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 3, ws[J / 4], OPSEL, SCALE);  \
-    }
+  switch (J % 4) {                                                                                                   \
+    case 0:                                                                                                          \
+      acc[I][J] =                                                                                                    \
+          __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 0, ws[J / 4], OPSEL, SCALE);  \
+      break;                                                                                                         \
+    case 1:                                                                                                          \
+      acc[I][J] =                                                                                                    \
+          __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 1, ws[J / 4], OPSEL, SCALE);  \
+      break;                                                                                                         \
+    case 2:                                                                                                          \
+      acc[I][J] =                                                                                                    \
+          __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 2, ws[J / 4], OPSEL, SCALE);  \
+      break;                                                                                                         \
+    default:                                                                                                         \
+      acc[I][J] =                                                                                                    \
+          __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[J], A, acc[I][J], 4, FMT, 3, ws[J / 4], OPSEL, SCALE);  \
+  }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         // the next lanes' operands are on their way while these are multiplied
